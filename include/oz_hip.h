@@ -345,6 +345,126 @@ int oz1_recon_block_f64(oz_dev* dev, const int32_t* P, int M, int N, int ldp, lo
                         const oz1_recon_dev* r, int first, int last, float* limbs, long long limb_stride, int ldl,
                         const int32_t* dA, const int32_t* dB, double* out, int ldo);
 
+/* ==== Operators around a product (no counterpart in the reference) =============================
+ * What a program that trains a network, or answers with one, runs beside its products: a product with
+ * its epilogue and its gradients, embeddings and their gradient, and the optimizer's step. Operands
+ * stay in device memory; every call is stream-ordered on the handle, allocates nothing, and gives the
+ * same bits for the same inputs. A workspace (16-byte aligned, its size asked for first; 0 means none is
+ * needed) holds intermediates of the call only. Leading dimensions count elements. Sums, activations and
+ * states are computed in FP32. Outputs must not overlap inputs unless said so.
+ */
+enum oz_type { OZ_BF16 = 0, OZ_F16 = 1, OZ_F32 = 2 };
+/* GELU is its tanh form, z/2 (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))); SILU is z / (1 + exp(-z)). */
+enum oz_act { OZ_ACT_NONE = 0, OZ_ACT_RELU = 1, OZ_ACT_GELU = 2, OZ_ACT_SILU = 3 };
+
+/* ---- product with bias, activation and residual ------------------------------------------------
+ * Y = act(X W^T + bias) + residual, X: M x K, W: N x K (a row for each output), Y: M x N, row-major,
+ * products on the BF16 or FP16 matrix cores, sums in FP32, each output rounded once. Z, when not null,
+ * receives X W^T + bias (what oz_linear_grad takes). bias (N values) and residual (M x N) may be null.
+ * M may be 0 (nothing is done), and 1 (one token) to 2^31 - 1; N and K from 1. Any leading dimension
+ * from the row length up to 2^22 (0: the row length) and any alignment to the type's own size is taken; operands at 16-byte
+ * boundaries with rows of a multiple of 8 values are read in place, other ones of larger products are
+ * laid out in the workspace first. residual may be Y itself (the same leading dimension). */
+typedef struct oz_linear_desc {
+    int M, N, K;
+    int type;   /* oz_type of X, W, bias and Z: OZ_BF16 or OZ_F16 */
+    int y_type; /* oz_type of Y and residual: type or OZ_F32 */
+    int act;    /* oz_act */
+    long long ldx, ldw, ldy, ldr, ldz;
+} oz_linear_desc;
+/* Bytes of workspace, or a negative oz_status where the descriptor is refused. */
+long long oz_linear_workspace(oz_dev* dev, const oz_linear_desc* d);
+int oz_linear(oz_dev* dev, const oz_linear_desc* d, const void* X, const void* W, const void* bias,
+              const void* residual, void* Y, void* Z, void* work, size_t bytes);
+
+/* Gradients of oz_linear from dY (M x N, `type`): with dZ = dY act'(Z),
+ *   dX (M x K, `type`) = dZ W,  dW (N x K, dw_type) = dZ^T X,  dbias (N, dw_type) = sum over the rows of dZ.
+ * dX, dW and dbias may each be null; the gradient of the residual is dY. Z may be null for OZ_ACT_NONE
+ * (it is not read then); X may be null without dW, W without dX. The products take dZ rounded to
+ * `type`, what the matrix cores read; dbias sums it unrounded. accumulate: dW and dbias are added to what
+ * is there (gradients of several batches). M = 0: dW and dbias are sums of nothing. */
+typedef struct oz_linear_grad_desc {
+    int M, N, K;
+    int type;       /* oz_type of dY, X, W, Z and dX: OZ_BF16 or OZ_F16 */
+    int dw_type;    /* oz_type of dW and dbias: type or OZ_F32 */
+    int act;        /* oz_act */
+    int accumulate; /* 0 or 1 */
+    long long lddy, ldx, ldw, ldz, lddx, lddw;
+} oz_linear_grad_desc;
+long long oz_linear_grad_workspace(oz_dev* dev, const oz_linear_grad_desc* d);
+int oz_linear_grad(oz_dev* dev, const oz_linear_grad_desc* d, const void* dY, const void* X, const void* W,
+                   const void* Z, void* dX, void* dW, void* dbias, void* work, size_t bytes);
+
+/* ---- embedding -----------------------------------------------------------------------------------
+ * out[t] = scale * table[ids[t]] for T tokens: rows of D values, each product rounded once. A token
+ * outside 0..vocab-1 gives a row of zeros and ORs 1 into *flags (a device word, 4-byte aligned, that the
+ * caller clears; may be null). T may be 0; the ids are int32 or int64. */
+typedef struct oz_embedding_desc {
+    long long T, vocab, D; /* T and vocab up to 2^31 - 1 */
+    int type;              /* oz_type of the table, out and dOut: any */
+    int grad_type;         /* oz_type of dTable: type or OZ_F32 */
+    int id_bits;           /* 32 or 64 */
+    int accumulate;        /* 1: the gradient is added to what dTable holds */
+    long long padding;     /* a token without a gradient, or -1 */
+    long long ldt, ldo;    /* leading dimensions of table and dTable, of out and dOut */
+    float scale;
+} oz_embedding_desc;
+int oz_embedding(oz_dev* dev, const oz_embedding_desc* d, const void* table, const void* ids, void* out, uint32_t* flags);
+/* dTable[v] = scale * (sum of dOut[t] over the tokens t with ids[t] = v, in FP32), 0 where there is none;
+ * the padding token's rows and tokens outside the vocabulary are left out (the latter OR 1 into *flags).
+ * The tokens are sorted, and equal ones summed in an order that depends on ids alone. */
+long long oz_embedding_grad_workspace(oz_dev* dev, const oz_embedding_desc* d);
+int oz_embedding_grad(oz_dev* dev, const oz_embedding_desc* d, const void* dOut, const void* ids, void* dTable,
+                      uint32_t* flags, void* work, size_t bytes);
+
+/* ---- AdamW over many tensors ---------------------------------------------------------------------
+ * One step of every value p with gradient g, in FP32 and in this order of operations:
+ *   g' = g grad_scale
+ *   m' = beta1 m + (1 - beta1) g'
+ *   v' = beta2 v + ((1 - beta2) g') g'
+ *   p' = p (1 - lr weight_decay) - (m' / (sqrt(v') / sqrt(1 - beta2^step) + eps)) lr / (1 - beta1^step)
+ * (the factors that the options alone give are computed in FP64 and rounded to FP32). With a master, p is the FP32 master
+ * and param receives p' rounded; without, p is param itself. States in 32 bits: m and v are FP32.
+ * States in 8 bits: OZ_ADAMW_BLOCK values in a row (the tensor's last block may be shorter) share a
+ * scale byte E, meaning 2^(E - 127): m is kept as e4m3 (OCP) bytes of m / scale, v as e4m3 bytes of
+ * sqrt(v) / scale; E is the least with which all finite values of the block are at most 448 in size.
+ * They are rounded to one of their two neighbours at random, up with the probability of the distance from
+ * the lower one (rounded to the nearest, a state that changes by less than half a step a call would never
+ * change), and sqrt(v) > 0 never to 0. The random bits of value i of a tensor are h = mix(q xor
+ * seed), q = OZ_ADAMW_BLOCK * (the blocks of all tensors before it) + i modulo 2^32, with mix(x):
+ * x ^= x >> 16, x *= 0x7FEB352D, x ^= x >> 15, x *= 0x846CA68B, x ^= x >> 16; m takes (h mod 2^16 + 1/2) /
+ * 2^16, v (h div 2^16 + 1/2) / 2^16 as the number in [0, 1) below which a distance rounds up. A value
+ * that is not finite is kept as NaN. All-zero states are those of a first step. */
+#define OZ_ADAMW_BLOCK 64
+typedef struct oz_adamw_tensor {
+    long long n; /* values; may be 0 */
+    void* param;
+    const void* grad;
+    float* master;              /* or null; must be null where param_type is OZ_F32 */
+    void *m, *v;                /* float, or uint8_t with states in 8 bits */
+    uint8_t *m_scale, *v_scale; /* ceil(n / OZ_ADAMW_BLOCK) bytes each; null with states in 32 bits */
+    int param_type, grad_type;  /* oz_type */
+    float weight_decay;
+} oz_adamw_tensor;
+/* The plan of a list of tensors (host array): the list and the division of its values over the
+ * workgroups, copied into device memory of oz_adamw_plan_bytes bytes (16-byte aligned), which the caller
+ * keeps unchanged as long as it steps with the plan. Returns when the copy is done. state_bits: 32 or 8. */
+typedef struct oz_adamw_plan {
+    const void* memory;
+    long long chunks; /* workgroups of a step */
+    int count, state_bits;
+} oz_adamw_plan;
+long long oz_adamw_plan_bytes(const oz_adamw_tensor* tensors, int count);
+int oz_adamw_make_plan(oz_dev* dev, const oz_adamw_tensor* tensors, int count, int state_bits, void* memory,
+                       size_t bytes, oz_adamw_plan* plan);
+typedef struct oz_adamw_options {
+    double lr, beta1, beta2, eps;
+    long long step;          /* from 1 */
+    uint32_t seed;           /* of the random bits; another one for each step */
+    const float* grad_scale; /* one device value that every gradient is multiplied by, or null */
+} oz_adamw_options;
+int oz_adamw_step(oz_dev* dev, const oz_adamw_plan* plan, const oz_adamw_options* o);
+
 #ifdef __cplusplus
 }
 #endif

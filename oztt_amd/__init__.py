@@ -140,6 +140,8 @@ def hip() -> ctypes.CDLL:
     if _hip is None:
         _hip = _load("liboz_hip.so")
         _hip.oz_last_error.restype = ctypes.c_char_p
+        for name in ("oz_linear_workspace", "oz_linear_grad_workspace", "oz_embedding_grad_workspace", "oz_adamw_plan_bytes"):
+            getattr(_hip, name).restype = ctypes.c_longlong
     return _hip
 
 

@@ -49,6 +49,9 @@ HIP_SOURCES = {
     "oz2_pass.hip": [],
     "oz2_noalloc.hip": [],
     "oz_rules.hip": [],
+    "oz_linear.hip": [],
+    "oz_embedding.hip": [],
+    "oz_adamw.hip": [],
 }
 HOST_FLAGS = ["-std=c++20", "-O2", "-fPIC", "-ffp-contract=off", "-fno-fast-math", "-fopenmp",
               "-Wall", "-Wextra", f"-I{INCLUDE}", f"-I{CSRC / 'host'}"]

@@ -92,6 +92,81 @@ def crt_desc(moduli, b: int, nd: int) -> CrtDesc:
     return d
 
 
+# ---- operators around a product ------------------------------------------------------------------
+
+TYPES = {"bf16": 0, "f16": 1, "f32": 2}
+ACTS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+ADAMW_BLOCK = 64
+
+
+def _number(names: dict, name) -> int:
+    if name not in names:
+        raise ValueError(f"{name!r} is none of {', '.join(names)}")
+    return names[name]
+
+
+class LinearDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("M", "N", "K", "type", "y_type", "act")] + \
+               [(n, ctypes.c_longlong) for n in ("ldx", "ldw", "ldy", "ldr", "ldz")]
+
+
+class LinearGradDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("M", "N", "K", "type", "dw_type", "act", "accumulate")] + \
+               [(n, ctypes.c_longlong) for n in ("lddy", "ldx", "ldw", "ldz", "lddx", "lddw")]
+
+
+class EmbeddingDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_longlong) for n in ("T", "vocab", "D")] + \
+               [(n, ctypes.c_int) for n in ("type", "grad_type", "id_bits", "accumulate")] + \
+               [(n, ctypes.c_longlong) for n in ("padding", "ldt", "ldo")] + [("scale", ctypes.c_float)]
+
+
+class AdamwTensor(ctypes.Structure):
+    _fields_ = [("n", ctypes.c_longlong)] + \
+               [(n, ctypes.c_void_p) for n in ("param", "grad", "master", "m", "v", "m_scale", "v_scale")] + \
+               [("param_type", ctypes.c_int), ("grad_type", ctypes.c_int), ("weight_decay", ctypes.c_float)]
+
+
+class AdamwPlan(ctypes.Structure):
+    _fields_ = [("memory", ctypes.c_void_p), ("chunks", ctypes.c_longlong), ("count", ctypes.c_int), ("state_bits", ctypes.c_int)]
+
+
+class AdamwOptions(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps")] + \
+               [("step", ctypes.c_longlong), ("seed", ctypes.c_uint32), ("grad_scale", ctypes.c_void_p)]
+
+
+def linear_desc(M, N, K, type="bf16", act="none", y_type=None, ldx=0, ldw=0, ldy=0, ldr=0, ldz=0) -> LinearDesc:
+    """Sizes and types of Device.linear; y_type None: `type`, a leading dimension of 0: the row length."""
+    t = _number(TYPES, type)
+    return LinearDesc(M, N, K, t, t if y_type is None else _number(TYPES, y_type), _number(ACTS, act), ldx, ldw, ldy, ldr, ldz)
+
+
+def linear_grad_desc(M, N, K, type="bf16", act="none", dw_type=None, accumulate=False, lddy=0, ldx=0, ldw=0, ldz=0,
+                     lddx=0, lddw=0) -> LinearGradDesc:
+    t = _number(TYPES, type)
+    return LinearGradDesc(M, N, K, t, t if dw_type is None else _number(TYPES, dw_type), _number(ACTS, act),
+                          int(accumulate), lddy, ldx, ldw, ldz, lddx, lddw)
+
+
+def embedding_desc(T, vocab, D, type="bf16", id_bits=64, scale=1.0, grad_type=None, accumulate=False, padding=-1, ldt=0,
+                   ldo=0) -> EmbeddingDesc:
+    t = _number(TYPES, type)
+    return EmbeddingDesc(T, vocab, D, t, t if grad_type is None else _number(TYPES, grad_type), id_bits, int(accumulate),
+                         padding, ldt, ldo, scale)
+
+
+def adamw_tensor(n, param, grad, m, v, master=0, m_scale=0, v_scale=0, param_type="f32", grad_type="f32",
+                 weight_decay=0.0) -> AdamwTensor:
+    """One tensor of n values; arrays by their device addresses, 0 for none."""
+    return AdamwTensor(n, param, grad, master, m, v, m_scale, v_scale, _number(TYPES, param_type),
+                       _number(TYPES, grad_type), weight_decay)
+
+
+def _at(buf) -> ctypes.c_void_p:
+    return buf.ptr if buf is not None else ctypes.c_void_p()
+
+
 class Buffer:
     def __init__(self, dev: "Device", nbytes: int):
         self.dev, self.nbytes = dev, int(nbytes)
@@ -273,6 +348,60 @@ class Device:
         tm = (ctypes.c_ubyte * OZ2_MAXOUT)(*[int(x) for x in term_modulus])
         self._check(hip().oz2_crt_terms_f64(self.h, W.ptr, M, N, ldw, ctypes.c_longlong(sW), nterms, tm,
                                                ctypes.byref(desc), dA.ptr, dB.ptr, out.ptr, ldo), "oz2_crt_terms_f64")
+
+    # ---- operators around a product ------------------------------------------------------------
+    def _bytes(self, n: int, what: str) -> int:
+        if n < 0:
+            self._check(int(n), what)
+        return int(n)
+
+    def linear_workspace(self, desc: LinearDesc) -> int:
+        return self._bytes(hip().oz_linear_workspace(self.h, ctypes.byref(desc)), "oz_linear_workspace")
+
+    def linear(self, desc: LinearDesc, X: Buffer, W: Buffer, Y: Buffer, bias=None, residual=None, Z=None, work=None, work_bytes=0):
+        """Y = act(X W^T + bias) + residual; Z, where given, receives X W^T + bias."""
+        self._check(hip().oz_linear(self.h, ctypes.byref(desc), X.ptr, W.ptr, _at(bias), _at(residual), Y.ptr, _at(Z),
+                                    _at(work), ctypes.c_size_t(work_bytes)), "oz_linear")
+
+    def linear_grad_workspace(self, desc: LinearGradDesc) -> int:
+        return self._bytes(hip().oz_linear_grad_workspace(self.h, ctypes.byref(desc)), "oz_linear_grad_workspace")
+
+    def linear_grad(self, desc: LinearGradDesc, dY: Buffer, X, W, Z=None, dX=None, dW=None, dbias=None, work=None, work_bytes=0):
+        """dX, dW and dbias, those that are given, from dY and linear()'s X, W and Z."""
+        self._check(hip().oz_linear_grad(self.h, ctypes.byref(desc), dY.ptr, _at(X), _at(W), _at(Z), _at(dX), _at(dW),
+                                         _at(dbias), _at(work), ctypes.c_size_t(work_bytes)), "oz_linear_grad")
+
+    def embedding(self, desc: EmbeddingDesc, table: Buffer, ids: Buffer, out: Buffer, flags=None):
+        """out[t] = scale table[ids[t]]; a token outside the vocabulary gives zeros and sets bit 0 of flags."""
+        self._check(hip().oz_embedding(self.h, ctypes.byref(desc), table.ptr, ids.ptr, out.ptr, _at(flags)), "oz_embedding")
+
+    def embedding_grad_workspace(self, desc: EmbeddingDesc) -> int:
+        return self._bytes(hip().oz_embedding_grad_workspace(self.h, ctypes.byref(desc)), "oz_embedding_grad_workspace")
+
+    def embedding_grad(self, desc: EmbeddingDesc, dout: Buffer, ids: Buffer, dtable: Buffer, flags=None, work=None, work_bytes=0):
+        """dtable[v] = scale (sum of dout[t] over the tokens t that are v)."""
+        self._check(hip().oz_embedding_grad(self.h, ctypes.byref(desc), dout.ptr, ids.ptr, dtable.ptr, _at(flags), _at(work),
+                                            ctypes.c_size_t(work_bytes)), "oz_embedding_grad")
+
+    def adamw_plan_bytes(self, tensors) -> int:
+        arr = (AdamwTensor * max(len(tensors), 1))(*tensors)
+        return self._bytes(hip().oz_adamw_plan_bytes(arr, len(tensors)), "oz_adamw_plan_bytes")
+
+    def adamw_plan(self, tensors, state_bits: int, memory: Buffer = None) -> AdamwPlan:
+        """The plan of a list of adamw_tensor()s, in `memory` (adamw_plan_bytes; allocated here if none is
+        given), which lives as long as the plan."""
+        arr = (AdamwTensor * max(len(tensors), 1))(*tensors)
+        nbytes = self.adamw_plan_bytes(tensors)
+        memory = memory if memory is not None else self.alloc(nbytes)
+        plan = AdamwPlan()
+        self._check(hip().oz_adamw_make_plan(self.h, arr, len(tensors), state_bits, memory.ptr, ctypes.c_size_t(nbytes),
+                                             ctypes.byref(plan)), "oz_adamw_make_plan")
+        plan.buffer = memory
+        return plan
+
+    def adamw_step(self, plan: AdamwPlan, lr, beta1=0.9, beta2=0.999, eps=1e-8, step=1, seed=0, grad_scale=None):
+        o = AdamwOptions(lr, beta1, beta2, eps, step, seed, _at(grad_scale))
+        self._check(hip().oz_adamw_step(self.h, ctypes.byref(plan), ctypes.byref(o)), "oz_adamw_step")
 
     def crt(self, C: Buffer, M, N, ldc, sC, desc: CrtDesc, dA: Buffer, dB: Buffer, out: Buffer, ldo):
         self._check(hip().oz2_crt_f64(self.h, C.ptr, M, N, ldc, ctypes.c_longlong(sC), ctypes.byref(desc), dA.ptr,

@@ -1,0 +1,265 @@
+"""oz_adamw_step against the same sequence of FP32 operations (bit for bit) and the formula in 64 bits."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from oztt_amd import device as ozd
+from oztt_amd.device import E4M3
+from tests.operator_cases import DTYPE, Ptr, generator
+
+pytestmark = pytest.mark.gpu
+
+BLOCK = ozd.ADAMW_BLOCK
+F = np.float32
+
+
+def mix(x):
+    x = x.astype(np.uint32)
+    with np.errstate(over="ignore"):
+        x = (x ^ (x >> np.uint32(16))) * np.uint32(0x7FEB352D)
+        x = (x ^ (x >> np.uint32(15))) * np.uint32(0x846CA68B)
+    return x ^ (x >> np.uint32(16))
+
+
+def encode(x, u, root):
+    """Bytes and scale bytes of the values x (FP32), by exact arithmetic in 64 bits."""
+    n = len(x)
+    blocks = -(-n // BLOCK)
+    full = np.zeros(blocks * BLOCK)
+    full[:n] = np.where(np.isfinite(x), np.abs(x.astype(np.float64)), 0)
+    top = full.reshape(blocks, BLOCK).max(1)
+    e = np.full(blocks, -127)
+    with np.errstate(divide="ignore"):
+        some = top > 0
+        e[some] = np.maximum(np.ceil(np.log2(top[some] / 448)).astype(int), -127)
+    for b in range(blocks):  # the logarithm decides nothing by itself
+        while e[b] > -127 and top[b] <= 448 * 2.0 ** (e[b] - 1):
+            e[b] -= 1
+        while top[b] > 448 * 2.0 ** e[b]:
+            e[b] += 1
+    y = np.abs(x.astype(np.float64)) / np.repeat(2.0**e, BLOCK)[:n]
+    y = np.where(np.isfinite(x), y, 0)
+    exp = np.where(y > 0, np.maximum(np.frexp(y)[1] - 1, -6), -6)
+    t = y * 2.0 ** (3 - exp)
+    # the sum is rounded to FP32 as the kernel's is
+    code = 8 * (exp + 6) + np.floor((t.astype(F) + u.astype(F)).astype(F)).astype(int)
+    if root:
+        code = np.where(y > 0, np.maximum(code, 1), code)
+    code = np.where(np.isfinite(x), code, 127) | np.where(x < 0, 128, 0)
+    return code.astype(np.uint8), (e + 127).astype(np.uint8)
+
+
+def decode(code, scale):
+    return E4M3[code].astype(F) * np.repeat(2.0 ** (scale.astype(np.float64) - 127), BLOCK)[: len(code)].astype(F)
+
+
+def expected(t, o, bits, first_block):
+    """One tensor's step in FP32, operation by operation."""
+    with np.errstate(all="ignore"):
+        g = t["grad"].astype(F) * F(o["grad_scale"])
+        p = (t["master"] if t["master"] is not None else t["param"]).astype(F)
+        if bits == 32:
+            m, v = t["m"], t["v"]
+        else:
+            m, r = decode(t["m"], t["m_scale"]), decode(t["v"], t["v_scale"])
+            v = r * r
+        b1, b2, lr, step = o["beta1"], o["beta2"], o["lr"], o["step"]
+        m = F(b1) * m + F(1 - b1) * g
+        v = F(b2) * v + (F(1 - b2) * g) * g
+        r = np.sqrt(v)
+        keep = F(1) - F(lr) * F(t["decay"])
+        p = p * keep - (m / (r * F(1 / np.sqrt(1 - b2**step)) + F(o["eps"]))) * F(lr / (1 - b1**step))
+    out = {"p": p}
+    if bits == 32:
+        return {**out, "m": m, "v": v}
+    h = mix((first_block * BLOCK + np.arange(len(p))).astype(np.uint64).astype(np.uint32) ^ np.uint32(o["seed"]))
+    out["m"], out["m_scale"] = encode(m, ((h & np.uint32(0xFFFF)).astype(F) + F(0.5)) * F(2.0**-16), False)
+    out["v"], out["v_scale"] = encode(r, ((h >> np.uint32(16)).astype(F) + F(0.5)) * F(2.0**-16), True)
+    return out
+
+
+def same(got, want, what):
+    got, want = np.ascontiguousarray(got), np.ascontiguousarray(want)
+    kind = {1: np.uint8, 2: np.uint16, 4: np.uint32}[got.itemsize]
+    differ = got.view(kind) != want.view(kind)
+    if got.dtype.kind == "f":
+        differ &= ~(np.isnan(got) & np.isnan(want))
+    assert not differ.any(), (what, int(differ.sum()), int(np.argmax(differ)), got[np.argmax(differ)], want[np.argmax(differ)])
+
+
+class Tensor:
+    """A tensor of n values at `shift` values behind an aligned address, with something around it."""
+
+    def __init__(self, n, param, grad, master, bits, shift, decay, seed, special=False):
+        g = generator(seed)
+        rnd = lambda: torch.randn(n, device="cuda:0", generator=g)  # noqa: E731
+        size = torch.exp(2 * torch.randn(-(-max(n, 1) // BLOCK), device="cuda:0", generator=g)).repeat_interleave(BLOCK)[:n]
+        x = {"param": (rnd() * 0.05).to(DTYPE[param]), "grad": (rnd() * size).to(DTYPE[grad])}
+        if special and n:
+            bad = torch.tensor([float("inf"), float("-inf"), float("nan"), 0.0, -0.0, 1e-30, 3e38], device="cuda:0").to(DTYPE[grad])
+            at = torch.arange(0, n, 37, device="cuda:0")
+            x["grad"][at] = bad[torch.arange(len(at), device="cuda:0") % len(bad)]
+            x["grad"][n // 2 : n // 2 + 130] = 0
+        x["master"] = x["param"].float() + 1e-6 * rnd() if master else None
+        m, r = rnd() * size * 0.3, (rnd().abs() * 0.5 + 0.01) * size
+        if special and n:
+            m[n // 2 : n // 2 + 130] = 0
+            r[n // 2 : n // 2 + 130] = 0
+            m[: n // 8] *= 1e-38
+            r[: n // 8] *= 1e-38
+        if bits == 32:
+            x["m"], x["v"] = m, r * r
+            x["m_scale"] = x["v_scale"] = None
+        else:
+            half = np.full(n, 0.5, dtype=F)
+            for k, s, root in (("m", m, False), ("v", r, True)):
+                code, scale = encode(s.cpu().numpy(), half, root)
+                x[k], x[k + "_scale"] = torch.from_numpy(code).cuda(), torch.from_numpy(scale).cuda()
+        self.n, self.param, self.grad, self.decay = n, param, grad, decay
+        self.before = {k: None if v is None else v.float().cpu().numpy() if v.dtype == torch.bfloat16 else v.cpu().numpy() for k, v in x.items()}
+        self.before["decay"] = decay
+        self.base, self.t = {}, {}
+        for k, v in x.items():
+            if v is None:
+                continue
+            s = 0 if k.endswith("scale") else shift
+            self.base[k] = torch.full((v.numel() + s + 16,), 77, dtype=v.dtype, device="cuda:0")
+            self.t[k] = self.base[k][s : s + v.numel()]
+            self.t[k].copy_(v)
+
+    def entry(self):
+        a = lambda k: self.t[k].data_ptr() if k in self.t else 0  # noqa: E731
+        return ozd.adamw_tensor(self.n, a("param"), a("grad"), a("m"), a("v"), a("master"), a("m_scale"), a("v_scale"), self.param, self.grad, self.decay)
+
+    def check(self, want, what):
+        p = want["p"]
+        if "master" in self.t:
+            same(self.t["master"].cpu().numpy(), p, what + " master")
+        low = torch.from_numpy(p).to(DTYPE[self.param])
+        got = self.t["param"].cpu()
+        if self.param != "f32":
+            low, got = low.view(torch.int16), got.view(torch.int16)
+            nan = torch.from_numpy(np.isnan(p))
+            assert torch.equal(low[~nan], got[~nan]), what
+        else:
+            same(got.numpy(), p, what + " param")
+        for k in ("m", "v", "m_scale", "v_scale"):
+            if k in self.t:
+                same(self.t[k].cpu().numpy(), want[k], f"{what} {k}")
+        for k, b in self.base.items():
+            self.t[k].fill_(77)
+            assert bool((b == 77).all()), (what, k, "around")
+
+
+def step(dev, tensors, bits, **o):
+    o = {"lr": 1e-3, "beta1": 0.9, "beta2": 0.99, "eps": 1e-8, "step": 3, "seed": 12345, "grad_scale": 1.0, **o}
+    plan = dev.adamw_plan([t.entry() for t in tensors], bits)
+    scale = torch.tensor([o["grad_scale"]], device="cuda:0")
+    torch.cuda.synchronize()
+    dev.adamw_step(plan, o["lr"], o["beta1"], o["beta2"], o["eps"], o["step"], o["seed"], Ptr(scale) if o["grad_scale"] != 1.0 else None)
+    dev.sync()
+    block = 0
+    for k, t in enumerate(tensors):
+        t.check(expected(t.before, o, bits, block), f"tensor {k} of {t.n}")
+        block += -(-t.n // BLOCK)
+
+
+SIZES = [1, 0, 7, 8, 9, 63, 64, 65, 511, 2047, 2048, 2049, 8191, 8192, 8193, 0, 20000]
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("param,grad,master", [("f32", "f32", False), ("bf16", "bf16", True), ("bf16", "f32", False), ("f16", "f16", True), ("f32", "bf16", False)])
+@pytest.mark.parametrize("shift", [0, 1, 8])
+def test_step(dev, bits, param, grad, master, shift):
+    print("adamw", bits, param, grad, master, shift, flush=True)
+    step(dev, [Tensor(n, param, grad, master, bits, shift, 0.1 * (k % 2), k + 1) for k, n in enumerate(SIZES)], bits)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_mixed_types_and_options(dev, bits):
+    kinds = [("f32", "f32", False), ("bf16", "f32", True), ("f16", "bf16", True), ("bf16", "bf16", False)]
+    for o in ({"step": 1}, {"grad_scale": 0.25, "beta1": 0.0}, {"lr": 0.0}, {"step": 10**6, "beta2": 0.999, "seed": 2**32 - 1}):
+        step(dev, [Tensor(n, *kinds[k % 4], bits, k % 3, 0.05 * k, k + 50) for k, n in enumerate((100, 64, 5000, 3, 12289))], bits, **o)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("grad", ["f32", "bf16"])
+def test_infinities_and_zeros(dev, bits, grad):
+    """Gradients that are not finite, all-zero blocks, values near both ends of FP32."""
+    step(dev, [Tensor(n, "f32", grad, False, bits, 0, 0.1, n, special=True) for n in (5000, 64, 1000)], bits)
+
+
+def test_many_tensors(dev):
+    step(dev, [Tensor(1 + 37 * k % 500, "f32", "f32", False, 8, 0, 0.0, k) for k in range(300)], 8)
+
+
+def test_no_tensors(dev):
+    for tensors in ([], [ozd.adamw_tensor(0, 0, 0, 0, 0)]):
+        dev.adamw_step(dev.adamw_plan(tensors, 32), 1e-3)
+    dev.sync()
+
+
+def run_steps(dev, bits, steps, beta2=0.999):
+    """A quadratic's minimum by AdamW, and the same in 64 bits; returns both parameters and the states' values."""
+    n = 4096
+    g = generator(3)
+    target = torch.randn(n, device="cuda:0", generator=g)
+    p = torch.zeros(n, device="cuda:0")
+    grad = torch.zeros(n, device="cuda:0")
+    st = lambda k: torch.zeros(k, dtype=torch.float32 if bits == 32 else torch.uint8, device="cuda:0")  # noqa: E731
+    m, v, ms, vs = st(n), st(n), st(n // BLOCK), st(n // BLOCK)
+    z = lambda t: t.data_ptr() if bits == 8 else 0  # noqa: E731
+    plan = dev.adamw_plan([ozd.adamw_tensor(n, p.data_ptr(), grad.data_ptr(), m.data_ptr(), v.data_ptr(), 0, z(ms), z(vs))], bits)
+    P, M, V, T = (torch.zeros(n, dtype=torch.float64, device="cuda:0") for _ in range(3)), None, None, target.double()
+    P, M, V = P
+    for k in range(1, steps + 1):
+        grad.copy_(p - target)
+        torch.cuda.synchronize()
+        dev.adamw_step(plan, 0.02, 0.9, beta2, 1e-8, k, k)
+        dev.sync()
+        G = P - T
+        M = 0.9 * M + 0.1 * G
+        V = beta2 * V + (1 - beta2) * G * G
+        P = P - 0.02 * (M / (1 - 0.9**k)) / ((V / (1 - beta2**k)).sqrt() + 1e-8)
+    if bits == 8:
+        v = torch.from_numpy(decode(v.cpu().numpy(), vs.cpu().numpy())).cuda() ** 2
+    return p.double(), P, v.double(), V, T
+
+
+def test_against_64_bits(dev):
+    """100 steps of a quadratic: with a relative error of about 2^-22 a step in the states, which the update turns into
+    at most lr 2^-22 a step, and p's own rounding of 2^-24 |p|, 1e-5 bounds the parameters."""
+    p, P, v, V, _ = run_steps(dev, 32, 100)
+    assert float((p - P).abs().max()) <= 1e-5
+    assert float(((v - V).abs() / V).max()) <= 100 * 2.0**-21
+
+
+def test_8bit_states_follow(dev):
+    """The same with states in 8 bits, beta2 = 0.999: a second moment that shrinks by 0.1% a step would stay where it is if
+    its root were rounded to the nearest of neighbours 6 to 12% apart; rounded at random its mean follows. Over
+    4096 values the mean of v / V is off by less than the states' own spread (each root has a relative error of
+    about 12%/sqrt(12) a step, of which some 1/2 lasts: below 1.15 in the mean of squares), and the minimum is
+    reached as with 32 bits."""
+    p, P, v, V, T = run_steps(dev, 8, 400)
+    assert 0.8 <= float((v.sum() / V.sum())) <= 1.25
+    start = float((T**2).sum())
+    assert float(((p - T) ** 2).sum()) <= 1e-2 * start and float(((P - T) ** 2).sum()) <= 1e-2 * start
+
+
+def test_refusals_name_what_is_wrong(dev):
+    x = torch.zeros(4096, device="cuda:0")
+    a = x.data_ptr()
+    for what, tensor, bits in (("arrays", ozd.adamw_tensor(8, a, 0, a, a), 32), ("arrays", ozd.adamw_tensor(8, a, a, a, a), 8),
+                               ("arrays", ozd.adamw_tensor(8, a, a, a, a, m_scale=a, v_scale=a), 32), ("size", ozd.adamw_tensor(-1, a, a, a, a), 32),
+                               ("types", ozd.adamw_tensor(8, a, a, a, a, master=a), 32), ("address", ozd.adamw_tensor(8, a + 2, a, a, a), 32),
+                               ("weight decay", ozd.adamw_tensor(8, a, a, a, a, weight_decay=float("nan")), 32), ("16 bits", ozd.adamw_tensor(8, a, a, a, a), 16)):
+        with pytest.raises(RuntimeError, match=what if what != "size" else "status -1"):
+            dev.adamw_plan([tensor], bits)
+    plan = dev.adamw_plan([ozd.adamw_tensor(8, a, a + 256, a + 512, a + 1024)], 32)
+    for o in ({"lr": -1.0}, {"lr": float("nan")}, {"lr": 1.0, "beta1": 1.0}, {"lr": 1.0, "step": 0}, {"lr": 1.0, "eps": float("inf")}):
+        with pytest.raises(RuntimeError, match="oz_adamw_step"):
+            dev.adamw_step(plan, **o)
+    dev.sync()
+    assert not x.any()
