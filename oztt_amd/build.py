@@ -50,6 +50,8 @@ HIP_SOURCES = {
     "oz2_noalloc.hip": [],
     "oz_rules.hip": [],
     "oz_linear.hip": [],
+    "oz_linear_rows.hip": [],
+    "oz_linear_tiles.hip": [],
     "oz_embedding.hip": [],
     "oz_adamw.hip": [],
 }

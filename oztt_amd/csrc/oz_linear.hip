@@ -11,6 +11,7 @@
 namespace {
 
 using namespace ozt;
+using namespace ozl;
 
 // Any sizes, strides and alignment: 64 x 64 outputs by 4 waves of 32 x 32, operands element by element
 // through LDS, 32 of c at a time. Elements outside are zeros.
@@ -63,41 +64,217 @@ __global__ void __launch_bounds__(256) product_any_kernel(const ozl::Product a) 
         }
 }
 
-// dZ = dY act'(Z), rounded for the products (left out where dz is null), and dbias: 64 columns by a workgroup,
-// 4 of its waves a row each.
+// dZ = dY act'(Z), rounded for the products (left out where dz is null), and the sums of its columns over `rows` rows each
+// (left out where parts is null): 8 columns a lane, 256 by 8 rows at a time by a workgroup. One pass over dY and Z.
+// VEC: rows of whole 16-byte pieces.
+template <bool VEC>
 __global__ void __launch_bounds__(256) act_grad_kernel(const void* __restrict__ dY, const void* __restrict__ Z,
-                                                       void* __restrict__ dz, void* __restrict__ dbias, int type,
-                                                       int dw_type, int act, int accumulate, long long M, int N,
-                                                       long long lddy, long long ldz) {
-    const int col = blockIdx.x * 64 + (threadIdx.x & 63);
-    float sum = 0.0f;
-    if (col < N)
-        for (long long m = threadIdx.x >> 6; m < M; m += 4) {
-            float d = load(dY, type, m * lddy + col);
-            if (act != OZ_ACT_NONE) d *= act_grad(load(Z, type, m * ldz + col), act);
-            if (dz) store(dz, type, m * N + col, d);
-            sum += d;
+                                                       void* __restrict__ dz, float* __restrict__ parts, int type, int act,
+                                                       long long M, int N, long long lddy, long long ldz, long long lddz,
+                                                       int rows, int strips) {
+    const int strip = blockIdx.x % strips, chunk = blockIdx.x / strips;
+    const int col = strip * 256 + 8 * (threadIdx.x & 31), r = threadIdx.x >> 5;
+    const long long end = (long long)(chunk + 1) * rows < M ? (long long)(chunk + 1) * rows : M;
+    float sum[8] = {};
+    if (col < N) {
+        auto get = [&](const void* p, long long at, float* x) {
+            if (VEC) {
+                load8(p, type, at, x);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[k] = col + k < N ? load(p, type, at + k) : 0.0f;
+            }
+        };
+#pragma unroll 4
+        for (long long m = (long long)chunk * rows + r; m < end; m += 8) {
+            float d[8], z[8];
+            get(dY, m * lddy + col, d);
+            if (act != OZ_ACT_NONE) {
+                get(Z, m * ldz + col, z);
+#pragma unroll
+                for (int k = 0; k < 8; k++) d[k] *= act_grad(z[k], act);
+            }
+            if (dz) store8(dz, type, m * lddz + col, d);
+#pragma unroll
+            for (int k = 0; k < 8; k++) sum[k] += d[k];
         }
-    __shared__ float part[256];
-    part[threadIdx.x] = sum;
-    __syncthreads();
-    if (threadIdx.x < 64 && col < N && dbias) {
-        sum = (part[threadIdx.x] + part[64 + threadIdx.x]) + (part[128 + threadIdx.x] + part[192 + threadIdx.x]);
-        if (accumulate) sum += load(dbias, dw_type, col);
-        store(dbias, dw_type, col, sum);
     }
+    if (!parts) return;
+    __shared__ float part[8][256];
+#pragma unroll
+    for (int k = 0; k < 8; k++) part[r][8 * (threadIdx.x & 31) + k] = sum[k];
+    __syncthreads();
+    const int c = strip * 256 + threadIdx.x;
+    if (c < N) {
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; k++) s += part[k][threadIdx.x];
+        parts[(long long)chunk * N + c] = s;
+    }
+}
+
+// dbias from the chunks' sums, 16 chunks at a time by 16 lanes: lane k of a column sums chunks k, k + 16, ..., then the lanes.
+__global__ void __launch_bounds__(256) bias_grad_kernel(const float* __restrict__ parts, void* __restrict__ dbias, int dw_type,
+                                                        int accumulate, int chunks, int N) {
+    const int col = blockIdx.x * 16 + (threadIdx.x & 15), k = threadIdx.x >> 4;
+    __shared__ float part[16][16];
+    float s = 0.0f;
+    if (col < N)
+        for (int c = k; c < chunks; c += 16) s += parts[(long long)c * N + col];
+    part[k][threadIdx.x & 15] = s;
+    __syncthreads();
+    if (k == 0 && col < N) {
+#pragma unroll
+        for (int j = 1; j < 16; j++) s += part[j][threadIdx.x & 15];
+        if (accumulate) s += load(dbias, dw_type, col);
+        store(dbias, dw_type, col, s);
+    }
+}
+
+// Operands whose rows are not whole 16-byte pieces, laid out so: rows x cols values at src to rows of `ldd` values, zeros
+// behind the last one. Two operands by one launch, 8 values a thread.
+struct Layout {
+    const uint16_t* src;
+    uint16_t* dst;
+    long long rows, cols, ld, ldd;
+};
+__global__ void __launch_bounds__(256) lay_out_kernel(Layout a, Layout b, long long pieces_a, long long pieces_b) {
+    long long i = 256ll * blockIdx.x + threadIdx.x;
+    const bool first = i < pieces_a;
+    if (!first) i -= pieces_a;
+    if (!first && i >= pieces_b) return;
+    const Layout& l = first ? a : b;
+    const long long across = l.ldd / 8, row = i / across, col = 8 * (i % across);
+    const uint16_t* from = l.src + row * l.ld + col;
+    union {
+        uint16_t v[8];
+        u32x4 w;
+    } x;
+    if (col + 8 <= l.cols) {
+        __builtin_memcpy(&x, from, 16);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; k++) x.v[k] = col + k < l.cols ? from[k] : 0;
+    }
+    *reinterpret_cast<u32x4*>(l.dst + row * l.ldd + col) = x.w;
 }
 
 constexpr long long kMaxTiles = 1ll << 23;  // workgroups of 256 threads in one launch
 
-int launch_product(oz_dev* dev, int type, const ozl::Product& a) {
-    if (!a.nq || !a.np) return OZ_OK;
+// Whether rows are whole 16-byte pieces.
+bool whole_rows(const void* p, long long ld) { return !((uintptr_t)p & 15) && ld % 8 == 0; }
+
+bool vec(const Epilogue& e) {
+    return (!e.Y || whole_rows(e.Y, e.ldy)) && (!e.Z || whole_rows(e.Z, e.ldz)) && whole_rows(e.bias, 0) &&
+           (!e.residual || whole_rows(e.residual, e.ldr));
+}
+
+size_t up(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
+
+constexpr int kFewRows = 16;
+
+// How a product runs, from its sizes alone.
+struct Route {
+    bool few;       // oz_linear_rows.hip
+    Tile tile;
+    int splits;
+    size_t parts;   // bytes of the ranges' sums
+};
+
+// Estimated us of a tile's launch with its c cut into `splits` ranges: whole rounds of workgroups over the CUs and the
+// last, partly filled one, and the join's launch and traffic (8 bytes an output and range at 4 TB/s).
+float estimate(const Shape& t, int cus, long long nq, long long np, long long C, int splits) {
+    const long long tiles = (nq + t.q - 1) / t.q * ((np + t.p - 1) / t.p) * splits, slots = (long long)cus * t.per_cu;
+    const float stages = (float)(((C + 63) / 64 + splits - 1) / splits);
+    const long long rest = tiles % slots;
+    float us = (float)(tiles / slots) * (t.fixed + stages * t.full);
+    if (rest) us += t.fixed + stages * (rest <= cus ? t.alone : t.full);
+    if (splits > 1) us += 3.0f + (float)splits * (float)nq * (float)np * 8.0f / 4e6f;
+    return us;
+}
+
+// Few rows: their own kernel, c in ranges where the rows of W are too few to keep all CUs reading (2 workgroups a CU,
+// each range long enough for its 8 waves). 1 row, N = K = 2048: 6.4 us in one range, 7.7 in four; K = 8192: 18.4 and 10.3.
+// More: the tile and ranges with the least estimate. 1000 x 704 x 1504: 9.4 us by 64 x 64, 17 by 128 x 128; 2048 x 4096 x
+// 4096: 66 by 128 x 128, 74 by 256 x 256 in two ranges, 101 by 64 x 64; 256 x 1024 x 8192: 15.5 by 64 x 64 in 4 ranges, 38 in one.
+Route route_of(int cus, long long nq, long long np, long long C, bool contiguous, bool aligned) {
+    Route r{};
+    r.splits = 1;
+    if (contiguous && (nq <= kFewRows || (!aligned && nq <= 64))) {
+        r.few = true;
+        const long long groups = (np + 31) / 32;
+        while (r.splits < 8 && groups * r.splits * 2 <= 2 * cus && C / (r.splits * 2) >= 2048) r.splits *= 2;
+    } else {
+        float best = 0.0f;
+        for (int t = 0; t < TILES; t++)
+            for (int s = 1; s <= 16; s *= 2) {
+                if (s > 1 && (C + 63) / 64 / s < 4) break;
+                const float us = estimate(shape_of((Tile)t), cus, nq, np, C, s);
+                if (best == 0.0f || us < best) best = us, r.tile = (Tile)t, r.splits = s;
+            }
+    }
+    if (r.splits > 1) r.parts = up(4 * (size_t)r.splits * nq * ((np + 7) / 8 * 8));
+    return r;
+}
+
+int launch_any(oz_dev* dev, int type, const Product& a) {
     const long long tiles = (long long)oz::ceil_div(a.np, 64) * oz::ceil_div(a.nq, 64);
     if (tiles > kMaxTiles) return oz::fail(dev, OZ_ERR_ARG, "a product of %lld x %lld outputs is too large", a.nq, a.np);
     const dim3 grid((unsigned)tiles);
     if (type == OZ_BF16) hipLaunchKernelGGL(product_any_kernel<OZ_BF16>, grid, dim3(256), 0, dev->stream, a);
     else hipLaunchKernelGGL(product_any_kernel<OZ_F16>, grid, dim3(256), 0, dev->stream, a);
     return oz::launch_check(dev, "product_any_kernel");
+}
+
+// Bytes of an operand's copy of whole rows: n rows along c, or C rows along n.
+size_t copy_bytes(long long n, long long C, bool major) { return up(2 * (size_t)(major ? C : n) * (((major ? n : C) + 7) / 8 * 8)); }
+
+// Workspace of a product whose operands need copies or not.
+size_t product_bytes(int cus, long long nq, long long np, long long C, bool q_major, bool p_major, bool copy_q, bool copy_p) {
+    if (!nq || !np || !C) return 0;
+    const Route r = route_of(cus, nq, np, C, !q_major && !p_major, !copy_q && !copy_p);
+    if (r.few) return r.parts;
+    return r.parts + (copy_q ? copy_bytes(nq, C, q_major) : 0) + (copy_p ? copy_bytes(np, C, p_major) : 0);
+}
+
+// Runs a product in `bytes` bytes of workspace. Operands whose rows are not whole are laid out in it; where that has no room (the
+// sizes are asked for by leading dimensions, operands may be at odd addresses besides) the element by element kernel runs.
+int launch_product(oz_dev* dev, int type, Product a, void* work, size_t bytes) {
+    if (!a.nq || !a.np) return OZ_OK;
+    a.epi.vec = vec(a.epi);
+    a.splits = 1;
+    if (!a.C) return launch_any(dev, type, a);
+    const bool copy_q = !whole_rows(a.Q, a.ldq), copy_p = !whole_rows(a.P, a.ldp);
+    const Route r = route_of(dev->cus, a.nq, a.np, a.C, !a.q_major && !a.p_major, !copy_q && !copy_p);
+    const size_t need = product_bytes(dev->cus, a.nq, a.np, a.C, a.q_major, a.p_major, copy_q, copy_p);
+    if (need > bytes) return launch_any(dev, type, a);
+    char* at = static_cast<char*>(work);
+    a.splits = r.splits;
+    a.parts = reinterpret_cast<float*>(at);
+    a.ldparts = (a.np + 7) / 8 * 8;
+    at += r.parts;
+    if (r.few) return launch_few_rows(dev, type, a);
+    const long long tiles = (long long)oz::ceil_div(a.np, shape_of(r.tile).p) * oz::ceil_div(a.nq, shape_of(r.tile).q) * r.splits;
+    if (tiles > kMaxTiles) return oz::fail(dev, OZ_ERR_ARG, "a product of %lld x %lld outputs is too large", a.nq, a.np);
+    if (copy_q || copy_p) {
+        Layout l[2] = {};
+        long long pieces[2] = {};
+        auto lay = [&](const void*& p, long long& ld, long long n, bool major, int i) {
+            const long long rows = major ? a.C : n, cols = major ? n : a.C, ldd = (cols + 7) / 8 * 8;
+            l[i] = Layout{static_cast<const uint16_t*>(p), reinterpret_cast<uint16_t*>(at), rows, cols, ld, ldd};
+            pieces[i] = rows * (ldd / 8);
+            p = at;
+            ld = ldd;
+            at += copy_bytes(n, a.C, major);
+        };
+        if (copy_q) lay(a.Q, a.ldq, a.nq, a.q_major, 0);
+        if (copy_p) lay(a.P, a.ldp, a.np, a.p_major, 1);
+        const long long groups = (pieces[0] + pieces[1] + 255) / 256;
+        if (groups > kMaxTiles) return oz::fail(dev, OZ_ERR_ARG, "operands of %lld and %lld rows are too large to lay out", l[0].rows, l[1].rows);
+        hipLaunchKernelGGL(lay_out_kernel, dim3((unsigned)groups), dim3(256), 0, dev->stream, l[0], l[1], pieces[0], pieces[1]);
+        if (int st = oz::launch_check(dev, "lay_out_kernel")) return st;
+    }
+    return launch_tile(dev, type, r.tile, a);
 }
 
 constexpr long long kMaxLd = 1ll << 22;  // offsets inside a tile's operands are 32-bit
@@ -132,11 +309,35 @@ const char* refuse(const oz_linear_grad_desc* d) {
     return nullptr;
 }
 
+bool misaligned16(const void* p) { return ((uintptr_t)p & 15) != 0; }
 bool misaligned(const void* p, int type) { return ((uintptr_t)p & (size_of(type) - 1)) != 0; }
 
-size_t dz_bytes(const oz_linear_grad_desc* d) {
-    return d->act == OZ_ACT_NONE ? 0 : ((size_t)d->M * d->N * 2 + 255) & ~(size_t)255;
+// Workspace of the gradients: dZ where it is not dY (or dY's rows are not whole), the columns' sums, and the larger of the
+// products' own.
+struct GradWork {
+    bool make_dz;
+    long long lddz;
+    int rows, chunks;  // of M for the columns' sums
+    size_t dz, sums, product, bytes;
+};
+GradWork grad_work(int cus, const oz_linear_grad_desc* d, bool whole_dy) {
+    GradWork w{};
+    w.make_dz = d->act != OZ_ACT_NONE || !whole_dy;
+    w.lddz = (d->N + 7) / 8 * 8;
+    w.dz = w.make_dz ? up(2 * (size_t)d->M * w.lddz) : 0;
+    // enough workgroups of 256 columns to fill the chip twice, 16 to 256 rows each
+    const long long strips = (d->N + 255) / 256;
+    long long rows = (long long)d->M * strips / (4 * cus);
+    w.rows = (int)std::min(256ll, std::max(16ll, (rows + 7) / 8 * 8));
+    w.chunks = (int)std::max(1ll, ((long long)d->M + w.rows - 1) / w.rows);
+    w.sums = up(4 * (size_t)w.chunks * d->N);
+    w.product = std::max(product_bytes(cus, d->M, d->K, d->N, false, true, false, or_row(d->ldw, d->K) % 8 != 0),
+                         product_bytes(cus, d->N, d->K, d->M, true, true, false, or_row(d->ldx, d->K) % 8 != 0));
+    w.bytes = w.dz + w.sums + w.product;
+    return w;
 }
+
+int cus_of(const oz_dev* dev) { return dev && dev->cus > 0 ? dev->cus : 256; }
 
 }  // namespace
 
@@ -144,7 +345,7 @@ extern "C" {
 
 long long oz_linear_workspace(oz_dev* dev, const oz_linear_desc* d) {
     if (const char* e = refuse(d)) return oz::fail(dev, OZ_ERR_ARG, "oz_linear: %s", e);
-    return 0;
+    return (long long)product_bytes(cus_of(dev), d->M, d->N, d->K, false, false, or_row(d->ldx, d->K) % 8 != 0, or_row(d->ldw, d->K) % 8 != 0);
 }
 
 int oz_linear(oz_dev* dev, const oz_linear_desc* d, const void* X, const void* W, const void* bias,
@@ -158,16 +359,18 @@ int oz_linear(oz_dev* dev, const oz_linear_desc* d, const void* X, const void* W
         return oz::fail(dev, OZ_ERR_ARG, "oz_linear: residual is Y with another leading dimension");
     if (int st = oz::use(dev)) return st;
     if (d->M == 0) return OZ_OK;
-    (void)work, (void)bytes;
+    if (misaligned16(work)) return oz::fail(dev, OZ_ERR_ARG, "oz_linear: workspace not 16-byte aligned");
+    const size_t need = (size_t)oz_linear_workspace(dev, d);
+    if (need && (!work || bytes < need)) return oz::fail(dev, OZ_ERR_ARG, "oz_linear: workspace of %zu bytes, %zu needed", bytes, need);
     ozl::Product p{};
     p.Q = X, p.P = W, p.nq = d->M, p.np = d->N, p.C = d->K, p.ldq = or_row(d->ldx, d->K), p.ldp = or_row(d->ldw, d->K);
-    p.epi = {Y, or_row(d->ldy, d->N), d->y_type, Z, or_row(d->ldz, d->N), bias, residual, or_row(d->ldr, d->N), d->act, 0};
-    return launch_product(dev, d->type, p);
+    p.epi = {Y, or_row(d->ldy, d->N), d->y_type, Z, or_row(d->ldz, d->N), bias, residual, or_row(d->ldr, d->N), d->act};
+    return launch_product(dev, d->type, p, work, work ? bytes : 0);
 }
 
 long long oz_linear_grad_workspace(oz_dev* dev, const oz_linear_grad_desc* d) {
     if (const char* e = refuse(d)) return oz::fail(dev, OZ_ERR_ARG, "oz_linear_grad: %s", e);
-    return (long long)dz_bytes(d);
+    return (long long)grad_work(cus_of(dev), d, or_row(d->lddy, d->N) % 8 == 0).bytes;
 }
 
 int oz_linear_grad(oz_dev* dev, const oz_linear_grad_desc* d, const void* dY, const void* X, const void* W,
@@ -179,31 +382,53 @@ int oz_linear_grad(oz_dev* dev, const oz_linear_grad_desc* d, const void* dY, co
     if (misaligned(dY, d->type) || misaligned(X, d->type) || misaligned(W, d->type) || misaligned(Z, d->type) ||
         misaligned(dX, d->type) || misaligned(dW, d->dw_type) || misaligned(dbias, d->dw_type))
         return oz::fail(dev, OZ_ERR_ARG, "oz_linear_grad: operands at addresses that their types do not allow");
-    const size_t need = dz_bytes(d);
-    if (need && (!work || bytes < need || ((uintptr_t)work & 15)))
-        return oz::fail(dev, OZ_ERR_ARG, "oz_linear_grad: workspace of %zu bytes, %zu needed (16-byte aligned)", bytes, need);
+    const size_t least = grad_work(cus_of(dev), d, or_row(d->lddy, d->N) % 8 == 0).bytes;
+    if (!work || bytes < least || misaligned16(work))
+        return oz::fail(dev, OZ_ERR_ARG, "oz_linear_grad: workspace of %zu bytes, %zu needed (16-byte aligned)", bytes, least);
     if (int st = oz::use(dev)) return st;
+    const long long lddy = or_row(d->lddy, d->N), ldz = or_row(d->ldz, d->N);
+    GradWork w = grad_work(cus_of(dev), d, whole_rows(dY, lddy));
+    if (w.bytes > bytes) w.make_dz = false, w.dz = 0;  // dY at an odd address without room for a copy
+    char* at = static_cast<char*>(work);
     const void* dz = dY;
-    long long lddz = or_row(d->lddy, d->N);
+    long long lddz = lddy;
     const bool products = d->M > 0 && (dX || dW);
-    if ((curved && products) || dbias) {
-        if (curved) dz = work, lddz = d->N;
-        hipLaunchKernelGGL(act_grad_kernel, dim3(oz::ceil_div(d->N, 64)), dim3(256), 0, dev->stream, dY, Z,
-                           curved && products ? work : nullptr, dbias, d->type, d->dw_type, d->act, d->accumulate,
-                           (long long)d->M, d->N, or_row(d->lddy, d->N), or_row(d->ldz, d->N));
-        if (int st = oz::launch_check(dev, "act_grad_kernel")) return st;
+    if ((w.make_dz && products) || dbias) {
+        void* make = w.make_dz && products ? at : nullptr;
+        if (make) dz = make, lddz = w.lddz;
+        float* sums = dbias ? reinterpret_cast<float*>(at + w.dz) : nullptr;
+        const int strips = (int)oz::ceil_div(d->N, 256), chunks = d->M ? w.chunks : 0;
+        const bool wide = d->N % 8 == 0 && whole_rows(dY, lddy) && (!curved || whole_rows(Z, ldz));
+        if ((long long)strips * w.chunks > kMaxTiles) return oz::fail(dev, OZ_ERR_ARG, "oz_linear_grad: %d x %d outputs are too many", d->M, d->N);
+        if (chunks) {
+            const dim3 grid((unsigned)(strips * chunks));
+            if (wide)
+                hipLaunchKernelGGL(act_grad_kernel<true>, grid, dim3(256), 0, dev->stream, dY, Z, make, sums, d->type, d->act,
+                                   (long long)d->M, d->N, lddy, ldz, w.lddz, w.rows, strips);
+            else
+                hipLaunchKernelGGL(act_grad_kernel<false>, grid, dim3(256), 0, dev->stream, dY, Z, make, sums, d->type, d->act,
+                                   (long long)d->M, d->N, lddy, ldz, w.lddz, w.rows, strips);
+            if (int st = oz::launch_check(dev, "act_grad_kernel")) return st;
+        }
+        if (dbias) {
+            hipLaunchKernelGGL(bias_grad_kernel, dim3(oz::ceil_div(d->N, 16)), dim3(256), 0, dev->stream, sums, dbias, d->dw_type,
+                               d->accumulate, chunks, d->N);
+            if (int st = oz::launch_check(dev, "bias_grad_kernel")) return st;
+        }
     }
+    char* room = at + w.dz + w.sums;
+    const size_t left = bytes - w.dz - w.sums;
     if (dX && d->M > 0) {
         ozl::Product p{};
         p.Q = dz, p.P = W, p.nq = d->M, p.np = d->K, p.C = d->N, p.ldq = lddz, p.ldp = or_row(d->ldw, d->K), p.p_major = 1;
-        p.epi = {dX, or_row(d->lddx, d->K), d->type, nullptr, 0, nullptr, nullptr, 0, OZ_ACT_NONE, 0};
-        if (int st = launch_product(dev, d->type, p)) return st;
+        p.epi = {dX, or_row(d->lddx, d->K), d->type, nullptr, 0, nullptr, nullptr, 0, OZ_ACT_NONE};
+        if (int st = launch_product(dev, d->type, p, room, left)) return st;
     }
     if (dW) {
         ozl::Product p{};
         p.Q = dz, p.P = X, p.nq = d->N, p.np = d->K, p.C = d->M, p.ldq = lddz, p.ldp = or_row(d->ldx, d->K), p.q_major = p.p_major = 1;
-        p.epi = {dW, or_row(d->lddw, d->K), d->dw_type, nullptr, 0, nullptr, nullptr, 0, OZ_ACT_NONE, d->accumulate};
-        if (int st = launch_product(dev, d->type, p)) return st;
+        p.epi = {dW, or_row(d->lddw, d->K), d->dw_type, nullptr, 0, nullptr, d->accumulate ? dW : nullptr, or_row(d->lddw, d->K), OZ_ACT_NONE};
+        if (int st = launch_product(dev, d->type, p, room, left)) return st;
     }
     return OZ_OK;
 }

@@ -2,9 +2,11 @@
 #pragma once
 #include "oz_types.hpp"
 
+struct oz_dev;
+
 namespace ozl {
 
-// v = sum + bias[p]; Z(q, p) = v; Y(q, p) = act(v) + residual(q, p), or added to Y with accumulate.
+// v = sum + bias[p]; Z(q, p) = v; Y(q, p) = act(v) + residual(q, p). The residual may be Y itself.
 struct Epilogue {
     void* Y;
     long long ldy;
@@ -14,16 +16,20 @@ struct Epilogue {
     const void* bias;
     const void* residual;
     long long ldr;
-    int act, accumulate;
+    int act;
+    int vec;  // every array at 16 bytes, rows of a multiple of 8 values
 };
 
 // C(q, p) = sum over c < C of Q(q, c) P(p, c), q < nq, p < np. Q(q, c) is at q ldq + c, or at c ldq + q where
-// q_major; P alike.
+// q_major; P alike. With splits > 1 range s of c goes to parts + s nq ldparts as FP32, for join_kernel.
 struct Product {
     const void *Q, *P;
     long long nq, np, C, ldq, ldp;
     int q_major, p_major;
     Epilogue epi;
+    float* parts;
+    long long ldparts;
+    int splits;
 };
 
 // One value. bias, Z in the operands' type, residual and Y in y_type.
@@ -32,8 +38,55 @@ __device__ __forceinline__ void finish(const Epilogue& e, int type, long long q,
     if (e.Z) ozt::store(e.Z, type, q * e.ldz + p, v);
     v = ozt::act(v, e.act);
     if (e.residual) v += ozt::load(e.residual, e.y_type, q * e.ldr + p);
-    if (e.accumulate) v += ozt::load(e.Y, e.y_type, q * e.ldy + p);
     ozt::store(e.Y, e.y_type, q * e.ldy + p, v);
 }
+
+// Eight values in a row from p on, p a multiple of 8.
+template <int TYPE>
+__device__ __forceinline__ void finish8(const Epilogue& e, long long np, long long q, long long p, float* v) {
+    if (e.vec && p + 8 <= np) {
+        float x[8];
+        if (e.bias) {
+            ozt::load8(e.bias, TYPE, p, x);
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] += x[k];
+        }
+        if (e.Z) ozt::store8(e.Z, TYPE, q * e.ldz + p, v);
+        if (e.act != OZ_ACT_NONE)
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = ozt::act(v[k], e.act);
+        if (e.residual) {
+            ozt::load8(e.residual, e.y_type, q * e.ldr + p, x);
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] += x[k];
+        }
+        ozt::store8(e.Y, e.y_type, q * e.ldy + p, v);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (p + k < np) finish(e, TYPE, q, p + k, v[k]);
+    }
+}
+
+// Tiles of an aligned product, rows x columns of outputs.
+enum Tile { T256, T128, T64, T64X32, T32, TILES };
+struct Shape {
+    int q, p;            // outputs
+    int per_cu;          // workgroups that a CU holds (LDS)
+    float alone, full;   // us for a stage of 64 values of c: one workgroup on a CU, per_cu of them
+    float fixed;         // us from the first copy to the first product, and from the last to the outputs
+};
+// Measured on 256 CUs, BF16: alone from 256 tiles of K = 512, 1024 and 2048, full from 512.
+inline const Shape& shape_of(Tile t) {
+    static const Shape shapes[TILES] = {
+        {256, 256, 1, 1.5f, 1.5f, 10.0f}, {128, 128, 2, 0.58f, 0.93f, 5.6f}, {64, 64, 2, 0.22f, 0.35f, 3.7f},
+        {64, 32, 2, 0.21f, 0.29f, 3.7f},  {32, 32, 2, 0.18f, 0.22f, 3.4f}};
+    return shapes[t];
+}
+int launch_tile(oz_dev* dev, int type, Tile tile, const Product& a);
+// At most 64 rows of Q, operands along c at any address; splits as in Product.
+int launch_few_rows(oz_dev* dev, int type, const Product& a);
+// Joins the ranges of c in order.
+int launch_join(oz_dev* dev, int type, const Product& a);
 
 }  // namespace ozl

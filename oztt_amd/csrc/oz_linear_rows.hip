@@ -1,0 +1,134 @@
+// Products of few rows (an answering program's tokens): Y = act(X W^T + bias) + residual with M <= 64.
+//
+// The weights are read once and used M times, so the time is theirs: the waves stream them straight into registers, with
+// no LDS and no barrier on the way, as one operand of the matrix instructions (16 rows of W x 32 values of c; M = 1 wastes
+// 15 of their 16 columns, and there are still 20 times more than the weights' bandwidth could feed), the rows of X, which
+// all workgroups share, come from the L2. A workgroup has 16 NB rows of W and deals c out to its 8 waves, 64 or 128 at a time,
+// so that together they read 1 or 2 KB of each row in a piece; the waves' sums are joined in LDS, in order. Few rows of
+// W (N small): ranges of c go to several workgroups, joined by a second launch.
+#include "oz_internal.hpp"
+#include "oz_linear.hpp"
+
+namespace {
+
+using namespace ozl;
+using namespace ozt;
+
+constexpr int WAVES = 8;
+
+// Eight values from p on. !ALIGNED: at any even address (the hardware's loads allow it).
+template <class T8, bool ALIGNED>
+__device__ __forceinline__ T8 load_chunk(const void* p) {
+    T8 v;
+    if constexpr (ALIGNED) v = *static_cast<const T8*>(p);
+    else __builtin_memcpy(&v, p, 16);
+    return v;
+}
+
+template <int TYPE, int MB, int NB, bool ALIGNED>
+__global__ void __launch_bounds__(64 * WAVES, 4) few_rows_kernel(const Product a, int blocks_p) {
+    typedef typename Half<TYPE>::t T;
+    typedef typename Half<TYPE>::x8 T8;
+    constexpr int F = MB == 1 ? 4 : 2, UNIT = 32 * F;  // values of c that a wave takes at a time
+    __shared__ f32x4 sums[WAVES][NB * MB][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int split = blockIdx.x / blocks_p;
+    const long long p0 = 16ll * NB * (blockIdx.x - split * blocks_p);
+    const int r = lane & 15, g = lane >> 4;
+    // rows beyond an operand's last are its last one again; their sums are not used
+    const T *pw[NB], *px[MB];
+#pragma unroll
+    for (int n = 0; n < NB; n++) pw[n] = static_cast<const T*>(a.P) + (p0 + 16 * n + r < a.np ? p0 + 16 * n + r : a.np - 1) * a.ldp + 8 * g;
+#pragma unroll
+    for (int m = 0; m < MB; m++) px[m] = static_cast<const T*>(a.Q) + (16 * m + r < a.nq ? 16 * m + r : a.nq - 1) * a.ldq + 8 * g;
+    const int units = (int)(a.C / UNIT);  // whole ones; what is left behind them goes to one wave of the last range
+    const int u0 = (int)((long long)units * split / a.splits), u1 = (int)((long long)units * (split + 1) / a.splits);
+    f32x4 acc[NB][MB] = {};
+    T8 w[2][NB][F], x[2][MB][F];
+    auto ask = [&](int b, int u) {
+        if (u < u1) {
+#pragma unroll
+            for (int n = 0; n < NB; n++)
+#pragma unroll
+                for (int f = 0; f < F; f++) w[b][n][f] = load_chunk<T8, ALIGNED>(pw[n] + (long long)u * UNIT + 32 * f);
+#pragma unroll
+            for (int m = 0; m < MB; m++)
+#pragma unroll
+                for (int f = 0; f < F; f++) x[b][m][f] = load_chunk<T8, ALIGNED>(px[m] + (long long)u * UNIT + 32 * f);
+        }
+    };
+    auto multiply = [&](int b) {
+#pragma unroll
+        for (int f = 0; f < F; f++)
+#pragma unroll
+            for (int n = 0; n < NB; n++)
+#pragma unroll
+                for (int m = 0; m < MB; m++) acc[n][m] = Half<TYPE>::mfma(w[b][n][f], x[b][m][f], acc[n][m]);
+    };
+    int u = u0 + wave;
+    ask(0, u);
+    for (; u < u1; u += 2 * WAVES) {
+        ask(1, u + WAVES);
+        multiply(0);
+        ask(0, u + 2 * WAVES);
+        if (u + WAVES < u1) multiply(1);
+    }
+    if (split == a.splits - 1 && wave == WAVES - 1 && a.C % UNIT) {
+        for (long long c = (long long)units * UNIT; c < a.C; c += 32) {
+            T8 wt[NB], xt[MB];
+            auto guarded = [&](const T* p) {  // p: this lane's first chunk of the row
+                T8 v;
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[k] = c + 8 * g + k < a.C ? p[c + k] : (T)0.0f;
+                return v;
+            };
+#pragma unroll
+            for (int n = 0; n < NB; n++) wt[n] = guarded(pw[n]);
+#pragma unroll
+            for (int m = 0; m < MB; m++) xt[m] = guarded(px[m]);
+#pragma unroll
+            for (int n = 0; n < NB; n++)
+#pragma unroll
+                for (int m = 0; m < MB; m++) acc[n][m] = Half<TYPE>::mfma(wt[n], xt[m], acc[n][m]);
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NB; n++)
+#pragma unroll
+        for (int m = 0; m < MB; m++) sums[wave][n * MB + m][lane] = acc[n][m];
+    __syncthreads();
+    // 16 NB values of p a row, next to each other
+    for (int e = threadIdx.x; e < 256 * NB * MB; e += 64 * WAVES) {
+        const int i = e % (16 * NB), q = e / (16 * NB);
+        if (q >= a.nq || p0 + i >= a.np) continue;
+        const int block = (i / 16) * MB + q / 16, from = 16 * (i % 16 / 4) + q % 16, k = i % 4;
+        float v = sums[0][block][from][k];
+#pragma unroll
+        for (int s = 1; s < WAVES; s++) v += sums[s][block][from][k];
+        if (a.splits > 1) a.parts[(split * a.nq + q) * a.ldparts + p0 + i] = v;
+        else finish(a.epi, TYPE, q, p0 + i, v);
+    }
+}
+
+template <int TYPE, int MB, int NB>
+int launch(oz_dev* dev, const Product& a) {
+    const int blocks_p = (int)oz::ceil_div(a.np, 16 * NB);
+    const dim3 grid((unsigned)blocks_p * a.splits), block(64 * WAVES);
+    const bool aligned = !(((uintptr_t)a.P | (uintptr_t)a.Q) & 15) && a.ldp % 8 == 0 && a.ldq % 8 == 0;
+    if (aligned) hipLaunchKernelGGL((few_rows_kernel<TYPE, MB, NB, true>), grid, block, 0, dev->stream, a, blocks_p);
+    else hipLaunchKernelGGL((few_rows_kernel<TYPE, MB, NB, false>), grid, block, 0, dev->stream, a, blocks_p);
+    if (int st = oz::launch_check(dev, "few_rows_kernel")) return st;
+    return a.splits > 1 ? ozl::launch_join(dev, TYPE, a) : OZ_OK;
+}
+
+template <int TYPE>
+int by_rows(oz_dev* dev, const Product& a) {
+    if (a.nq <= 16) return launch<TYPE, 1, 2>(dev, a);
+    return a.nq <= 32 ? launch<TYPE, 2, 2>(dev, a) : launch<TYPE, 4, 2>(dev, a);
+}
+
+}  // namespace
+
+int ozl::launch_few_rows(oz_dev* dev, int type, const Product& a) {
+    return type == OZ_BF16 ? by_rows<OZ_BF16>(dev, a) : by_rows<OZ_F16>(dev, a);
+}
