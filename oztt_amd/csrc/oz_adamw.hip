@@ -16,8 +16,12 @@ namespace {
 
 using namespace ozt;
 
-constexpr int V = 8, THREADS = 256, CHUNK = 4 * V * THREADS;  // values of a lane, lanes, values of a chunk
-static_assert(CHUNK % OZ_ADAMW_BLOCK == 0 && OZ_ADAMW_BLOCK == 8 * V, "a block is 8 lanes' values");
+constexpr int V = 8, THREADS = 256;  // values of a lane, lanes
+static_assert(OZ_ADAMW_BLOCK == 8 * V, "a block is 8 lanes' values");
+
+// Values of a chunk: 8192 of large lists, one round of a workgroup's threads of small ones, whose chunks would leave most of
+// the chip idle (2e5 values: XXX us, 9.6 with 8192).
+int chunk_of(long long values) { return values > 1 << 22 ? 4 * V * THREADS : V * THREADS; }
 
 // The plan's memory: one Entry a tensor, then for each chunk its tensor (uint32), its place in it follows
 // from the tensor's first chunk.
@@ -25,7 +29,7 @@ struct Entry {
     oz_adamw_tensor t;
     long long first_chunk;
     uint32_t first_block;  // blocks of the tensors before, modulo 2^32
-    int aligned;           // every array at 16 bytes (8-bit states: 8)
+    int chunk;             // values of a chunk
 };
 
 struct Step {
@@ -79,7 +83,8 @@ __device__ __forceinline__ uint32_t to_e4m3(float x, int e, float u, bool root) 
 }
 
 __device__ __forceinline__ void from_8bit(const uint8_t* p, uint8_t scale, float* x) {
-    const u32x2 w = *reinterpret_cast<const u32x2*>(p);
+    u32x2 w;
+    __builtin_memcpy(&w, p, 8);
     from_e4m3(w[0], x);
     from_e4m3(w[1], x + 4);
     const float s = power((int)scale - 127);
@@ -87,37 +92,28 @@ __device__ __forceinline__ void from_8bit(const uint8_t* p, uint8_t scale, float
     for (int k = 0; k < V; k++) x[k] *= s;
 }
 
-// 8 values from i on, those from n on zeros.
+// The first `count` of 8 values from i on, the others zeros.
 __device__ __forceinline__ void get(const void* p, int type, long long i, int count, bool whole, float* x) {
-    if (whole) {
-        load8(p, type, i, x);
-        return;
-    }
-#pragma unroll
-    for (int k = 0; k < V; k++) x[k] = k < count ? load(p, type, i + k) : 0.0f;
+    if (whole) load8(p, type, i, x);
+    else load_some(p, type, i, count, x);
 }
 __device__ __forceinline__ void put(void* p, int type, long long i, int count, bool whole, const float* x) {
-    if (whole) {
-        store8(p, type, i, x);
-        return;
-    }
-#pragma unroll
-    for (int k = 0; k < V; k++)
-        if (k < count) store(p, type, i + k, x[k]);
+    if (whole) store8(p, type, i, x);
+    else store_some(p, type, i, count, x);
 }
 
 template <int BITS>
 __global__ void __launch_bounds__(THREADS) adamw_kernel(const Entry* __restrict__ entries, const uint32_t* __restrict__ owner, Step o) {
     const Entry& E = entries[owner[blockIdx.x]];
     const oz_adamw_tensor& t = E.t;
-    const long long n = t.n, begin = (blockIdx.x - E.first_chunk) * CHUNK;
+    const long long n = t.n, begin = (blockIdx.x - E.first_chunk) * E.chunk;
     const float gs = o.grad_scale ? *o.grad_scale : 1.0f;
     const float keep = 1.0f - o.lr * t.weight_decay;
-    const long long end = begin + CHUNK < n ? begin + CHUNK : n;
+    const long long end = begin + E.chunk < n ? begin + E.chunk : n;
     // whole blocks of lanes go through, so that the exchanges of a block's lanes always find them
     for (long long i = begin + V * (long long)threadIdx.x; i - V * (threadIdx.x & 7) < end; i += V * THREADS) {
         const int count = (int)(end - i < V ? (end - i > 0 ? end - i : 0) : V);
-        const bool whole = E.aligned && count == V;
+        const bool whole = count == V;
         float g[V], p[V], m[V], v[V], r[V];
         get(t.grad, t.grad_type, i, count, whole, g);
         get(t.master ? t.master : t.param, t.master ? OZ_F32 : t.param_type, i, count, whole, p);
@@ -167,8 +163,8 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const Entry* __restrict_
             }
             uint8_t *pm = static_cast<uint8_t*>(t.m) + i, *pv = static_cast<uint8_t*>(t.v) + i;
             if (whole) {
-                *reinterpret_cast<u32x2*>(pm) = u32x2{cm[0], cm[1]};
-                *reinterpret_cast<u32x2*>(pv) = u32x2{cv[0], cv[1]};
+                __builtin_memcpy(pm, cm, 8);
+                __builtin_memcpy(pv, cv, 8);
             } else {
 #pragma unroll
                 for (int k = 0; k < V; k++)
@@ -185,20 +181,26 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const Entry* __restrict_
     }
 }
 
-long long chunks_of(long long n) { return (n + CHUNK - 1) / CHUNK; }
+long long chunks_of(long long n, int chunk) { return (n + chunk - 1) / chunk; }
 
-// Tensors and chunks of a list, or a negative status and what is wrong.
-int check(const oz_adamw_tensor* t, int count, long long* chunks, const char** what) {
+// Chunks of a list and their size, or a negative status and what is wrong.
+int check(const oz_adamw_tensor* t, int count, long long* chunks, int* chunk, const char** what) {
     *chunks = 0;
+    *chunk = 0;
     *what = "no tensors";
     if (count < 0 || (count > 0 && !t)) return OZ_ERR_ARG;
+    long long values = 0;
     for (int k = 0; k < count; k++) {
         *what = "a tensor's size";
-        if (t[k].n < 0 || t[k].n > 1ll << 40) return OZ_ERR_ARG;
-        *chunks += chunks_of(t[k].n);
-        if (*chunks > 1ll << 23) return OZ_ERR_ARG;
+        if (t[k].n < 0 || t[k].n > 1ll << 36) return OZ_ERR_ARG;
+        values += t[k].n;
+        *what = "too many values";
+        if (values > 1ll << 36) return OZ_ERR_ARG;
     }
-    return OZ_OK;
+    *chunk = chunk_of(values);
+    for (int k = 0; k < count; k++) *chunks += chunks_of(t[k].n, *chunk);
+    *what = "too many values";
+    return *chunks > 1ll << 23 ? OZ_ERR_ARG : OZ_OK;
 }
 
 long long bytes_of(int count, long long chunks) { return (long long)count * sizeof(Entry) + chunks * 4 + 16; }
@@ -209,8 +211,9 @@ extern "C" {
 
 long long oz_adamw_plan_bytes(const oz_adamw_tensor* tensors, int count) {
     long long chunks;
+    int chunk;
     const char* what;
-    if (int st = check(tensors, count, &chunks, &what)) return st;
+    if (int st = check(tensors, count, &chunks, &chunk, &what)) return st;
     return bytes_of(count, chunks);
 }
 
@@ -220,8 +223,9 @@ int oz_adamw_make_plan(oz_dev* dev, const oz_adamw_tensor* tensors, int count, i
     *plan = oz_adamw_plan{};
     if (state_bits != 32 && state_bits != 8) return oz::fail(dev, OZ_ERR_ARG, "oz_adamw_make_plan: states of %d bits", state_bits);
     long long chunks;
+    int chunk;
     const char* what;
-    if (int st = check(tensors, count, &chunks, &what)) return oz::fail(dev, st, "oz_adamw_make_plan: %s", what);
+    if (int st = check(tensors, count, &chunks, &chunk, &what)) return oz::fail(dev, st, "oz_adamw_make_plan: %s", what);
     for (int k = 0; k < count; k++) {
         const oz_adamw_tensor& t = tensors[k];
         const auto known = [](int type) { return type == OZ_F32 || is_16bit(type); };
@@ -244,14 +248,12 @@ int oz_adamw_make_plan(oz_dev* dev, const oz_adamw_tensor* tensors, int count, i
         std::vector<unsigned char> image((size_t)need);
         Entry* e = reinterpret_cast<Entry*>(image.data());
         uint32_t* owner = reinterpret_cast<uint32_t*>(image.data() + (size_t)count * sizeof(Entry));
-        long long chunk = 0;
+        long long first = 0;
         uint32_t block = 0;
         for (int k = 0; k < count; k++) {
             const oz_adamw_tensor& t = tensors[k];
-            const uintptr_t wide = (uintptr_t)t.param | (uintptr_t)t.grad | (uintptr_t)t.master |
-                                   (state_bits == 32 ? (uintptr_t)t.m | (uintptr_t)t.v : 2 * ((uintptr_t)t.m | (uintptr_t)t.v));
-            e[k] = Entry{t, chunk, block, (wide & 15) == 0};
-            for (long long c = chunks_of(t.n); c > 0; c--) owner[chunk++] = (uint32_t)k;
+            e[k] = Entry{t, first, block, chunk};
+            for (long long c = chunks_of(t.n, chunk); c > 0; c--) owner[first++] = (uint32_t)k;
             block += (uint32_t)((t.n + OZ_ADAMW_BLOCK - 1) / OZ_ADAMW_BLOCK);
         }
         if (int st = oz_memcpy_h2d(dev, memory, image.data(), image.size())) return st;

@@ -26,39 +26,84 @@ __device__ __forceinline__ long long token(const void* ids, int wide, long long 
     return wide ? static_cast<const long long*>(ids)[t] : static_cast<const int*>(ids)[t];
 }
 
-// Rows by tokens: a wave takes one row's 512 columns at a time. VEC: rows of whole 16-byte pieces (8
-// values, of FP32 two pieces), otherwise value by value.
-template <bool VEC>
+// Eight columns of a lane among a wave's 512: two pieces of four, c0 + 4 lane + k and c0 + 256 + 4 lane + k, those below D, so that
+// FP32 rows too move in runs of 16 bytes a lane.
+struct Columns {
+    int c, left;  // the first piece's column; columns from it on
+    __device__ Columns(int c0, int lane, int D) : c(c0 + 4 * lane), left(D - (c0 + 4 * lane)) {}
+    __device__ void get(const void* p, int type, long long row, float* x) const {
+        load4(p, type, row + c, left, x);
+        load4(p, type, row + c + 256, left - 256, x + 4);
+    }
+    __device__ void put(void* p, int type, long long row, const float* x) const {
+        store4(p, type, row + c, left, x);
+        store4(p, type, row + c + 256, left - 256, x + 4);
+    }
+    // the table's row v from its sum
+    __device__ void finish(void* table, const Shape& s, long long v, float* x) const {
+        float old[8] = {};
+        if (s.accumulate) get(table, s.grad_type, v * s.ldt, old);
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[k] = s.accumulate ? old[k] + x[k] * s.scale : x[k] * s.scale;
+        put(table, s.grad_type, v * s.ldt, x);
+    }
+};
+
+// Rows by tokens: a wave takes 512 columns of a row.
 __global__ void __launch_bounds__(256) embedding_kernel(const void* __restrict__ table, const void* __restrict__ ids,
                                                         void* __restrict__ out, uint32_t* __restrict__ flags, Shape s, unsigned slices) {
     const unsigned lane = threadIdx.x & 63;
     const long long item = 4ll * blockIdx.x + (threadIdx.x >> 6), t = item / slices;
     if (t >= s.T) return;
-    const int c0 = (int)(item % slices) * 512;
+    const int c0 = (int)(item - t * slices) * 512;
     const long long v = token(ids, s.wide, t);
     const bool known = v >= 0 && v < s.vocab;
     if (!known && flags && c0 == 0 && lane == 0) atomicOr(flags, 1u);
-    if constexpr (VEC) {
-        const int c = c0 + 8 * lane;
-        if (c >= s.D) return;
-        float x[8] = {};
-        if (known) load8(table, s.type, v * s.ldt + c, x);
+    const Columns cols(c0, lane, s.D);
+    float x[8] = {};
+    if (known) cols.get(table, s.type, v * s.ldt, x);
 #pragma unroll
-        for (int k = 0; k < 8; k++) x[k] *= s.scale;
-        if (!known)
-#pragma unroll
-            for (int k = 0; k < 8; k++) x[k] = 0.0f;
-        store8(out, s.type, t * s.ldo + c, x);
-    } else {
-        for (int c = c0 + lane; c < s.D && c < c0 + 512; c += 64)
-            store(out, s.type, t * s.ldo + c, known ? load(table, s.type, v * s.ldt + c) * s.scale : 0.0f);
-    }
+    for (int k = 0; k < 8; k++) x[k] = known ? x[k] * s.scale : 0.0f;
+    cols.put(out, s.type, t * s.ldo, x);
 }
 
+// Zeros for part `part` of `parts` of the table's rows, by workgroups `first` to gridDim.x - 1 of a launch, which stride over
+// it in 16-byte pieces.
+struct Zeros {
+    void* table;
+    int part, parts;
+    unsigned first;
+};
+__device__ __forceinline__ void zero_rows(const Zeros& z, const Shape& s) {
+    const int size = size_of(s.grad_type);
+    const long long row_bytes = (long long)s.D * size, first_row = s.vocab * z.part / z.parts, rows = s.vocab * (z.part + 1) / z.parts - first_row;
+    char* base = static_cast<char*>(z.table) + first_row * s.ldt * size;
+    const long long me = (long long)(blockIdx.x - z.first) * blockDim.x + threadIdx.x, stride = (long long)(gridDim.x - z.first) * blockDim.x;
+    const u32x4 none = {0, 0, 0, 0};
+    if (s.ldt == s.D) {
+        const long long bytes = rows * row_bytes;
+        for (long long i = me; i < bytes / 16; i += stride) put16(base + 16 * i, none);
+        for (long long i = bytes / 16 * 16 + 2 * me; i < bytes; i += 2 * stride) *reinterpret_cast<uint16_t*>(base + i) = 0;
+    } else {
+        const long long across = (row_bytes + 15) / 16;
+        for (long long i = me; i < rows * across; i += stride) {
+            const long long row = i / across, at = 16 * (i - row * across);
+            char* to = base + row * s.ldt * size + at;
+            if (at + 16 <= row_bytes) put16(to, none);
+            else
+                for (long long k = at; k < row_bytes; k += 2) *reinterpret_cast<uint16_t*>(to + k - at) = 0;
+        }
+    }
+}
+__global__ void __launch_bounds__(256) zero_rows_kernel(Zeros z, Shape s) { zero_rows(z, s); }
+
 // ---- sort ---------------------------------------------------------------------------------------------
-// Least digit first, DIGITS values a digit; keys are the tokens, those without a gradient as `vocab`, behind all
-// others. A tile is TILE consecutive entries, a quarter for each of 4 waves.
-constexpr int TILE = 4096, MAX_BITS = 9, DIGITS = 1 << MAX_BITS;
+// Least digit first, DIGITS values a digit; keys are the tokens, those without a gradient as `vocab`, behind all others. A tile
+// is 1024 ITEMS consecutive entries, a sixteenth for each of 16 waves. Per digit a launch counts the tiles' digits and one moves
+// the entries; where a tile's entries of a digit begin each workgroup sums up by itself from the counts of all tiles, up to
+// SUMMED tiles, and a third launch does for more. The launches also write the table's zeros, by workgroups of their own:
+// what the sort takes is hidden behind them where the table is large.
+constexpr int MAX_BITS = 9, DIGITS = 1 << MAX_BITS, SORT_THREADS = 1024, SORT_WAVES = 16, SUMMED = 256;
 
 __device__ __forceinline__ uint32_t key_of(const void* ids, const Shape& s, long long t, uint32_t* flags) {
     const long long v = token(ids, s.wide, t);
@@ -79,188 +124,206 @@ __device__ __forceinline__ uint64_t same_digit(uint32_t d, int bits, uint64_t am
     return among;
 }
 
-// counts[digit][tile]
-template <bool FIRST>
-__global__ void __launch_bounds__(256) count_kernel(const void* __restrict__ ids, const uint32_t* __restrict__ keys, Shape s, int shift,
-                                                    int bits, uint32_t* __restrict__ counts, unsigned tiles, uint32_t* __restrict__ flags) {
+// counts[tile][digit]
+template <bool FIRST, int ITEMS>
+__global__ void __launch_bounds__(SORT_THREADS) count_kernel(const void* __restrict__ ids, const uint32_t* __restrict__ keys, Shape s, int shift,
+                                                             int bits, uint32_t* __restrict__ counts, uint32_t* __restrict__ flags, Zeros z) {
+    if (blockIdx.x >= z.first) {
+        zero_rows(z, s);
+        return;
+    }
     __shared__ uint32_t n[DIGITS];
-    for (int d = threadIdx.x; d < DIGITS; d += 256) n[d] = 0;
+    if (threadIdx.x < DIGITS) n[threadIdx.x] = 0;
     __syncthreads();
-    for (int e = threadIdx.x; e < TILE; e += 256) {
-        const long long t = (long long)blockIdx.x * TILE + e;
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++) {
+        const long long t = ((long long)blockIdx.x * ITEMS + i) * SORT_THREADS + threadIdx.x;
         if (t < s.T) atomicAdd(&n[((FIRST ? key_of(ids, s, t, flags) : keys[t]) >> shift) & ((1 << bits) - 1)], 1u);
     }
     __syncthreads();
-    for (int d = threadIdx.x; d < 1 << bits; d += 256) counts[(size_t)d * tiles + blockIdx.x] = n[d];
+    if (threadIdx.x < 1 << bits) counts[((size_t)blockIdx.x << bits) + threadIdx.x] = n[threadIdx.x];
 }
 
-// Exclusive prefix sums of n counts in place, by one workgroup: 8 a thread and round.
-__global__ void __launch_bounds__(1024) scan_kernel(uint32_t* __restrict__ counts, long long n) {
-    __shared__ uint32_t waves[17];
-    uint32_t before = 0;
-    for (long long b = 0; b < n; b += 8192) {
-        const long long i = b + 8 * threadIdx.x;
-        uint32_t x[8], sum = 0;
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-            x[k] = i + k < n ? counts[i + k] : 0;
-            sum += x[k];
-        }
-        uint32_t upto = sum;
-        for (int d = 1; d < 64; d *= 2) {
-            const uint32_t y = __shfl_up(upto, d);
-            if ((threadIdx.x & 63) >= d) upto += y;
-        }
-        if ((threadIdx.x & 63) == 63) waves[threadIdx.x >> 6] = upto;
-        __syncthreads();
-        uint32_t at = before + upto - sum, total = 0;
-        for (int w = 0; w < 16; w++) {
-            if (w < (int)(threadIdx.x >> 6)) at += waves[w];
-            total += waves[w];
-        }
-#pragma unroll
-        for (int k = 0; k < 8; k++) {
-            if (i + k < n) counts[i + k] = at;
-            at += x[k];
-        }
-        before += total;
-        __syncthreads();
+// The counts of many tiles to where each tile's entries of a digit begin, by one workgroup, a digit a thread.
+__global__ void __launch_bounds__(DIGITS) scan_kernel(uint32_t* __restrict__ counts, int bits, long long tiles) {
+    __shared__ uint32_t total[DIGITS];
+    const int d = threadIdx.x;
+    uint32_t sum = 0;
+    if (d < 1 << bits) {
+#pragma unroll 8
+        for (long long t = 0; t < tiles; t++) sum += counts[(t << bits) + d];
     }
-}
-
-// Every entry of a tile to its place: first the waves' counts of each digit, from them where each
-// wave's entries of a digit begin, then 64 entries at a time in order.
-template <bool FIRST>
-__global__ void __launch_bounds__(256) scatter_kernel(const void* __restrict__ ids, const uint32_t* __restrict__ keys,
-                                                      const uint32_t* __restrict__ order, Shape s, int shift, int bits,
-                                                      const uint32_t* __restrict__ starts, unsigned tiles,
-                                                      uint32_t* __restrict__ keys_out, uint32_t* __restrict__ order_out) {
-    __shared__ volatile uint32_t at[4][DIGITS];  // written by one lane of the owning wave, read by its others
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int d = threadIdx.x; d < 4 * DIGITS; d += 256) at[d / DIGITS][d % DIGITS] = 0;
+    total[d] = d < 1 << bits ? sum : 0;
     __syncthreads();
-    const long long t0 = (long long)blockIdx.x * TILE + wave * (TILE / 4);
-    const uint64_t below = (1ull << lane) - 1;
-    for (int round = 0; round < 2; round++) {
-        for (int e = 0; e < TILE / 4; e += 64) {
-            const long long t = t0 + e + lane;
-            const bool in = t < s.T;
-            const uint32_t key = in ? (FIRST ? key_of(ids, s, t, nullptr) : keys[t]) : 0;
-            const uint32_t d = (key >> shift) & ((1 << bits) - 1);
-            const uint64_t same = same_digit(d, bits, __ballot(in));
-            if (in) {
-                const uint32_t first = at[wave][d];
-                __builtin_amdgcn_wave_barrier();
-                if (!(same & below)) at[wave][d] = first + __popcll(same);
-                if (round) {
-                    const uint32_t place = first + __popcll(same & below);
-                    keys_out[place] = key;
-                    order_out[place] = FIRST ? (uint32_t)t : order[t];
-                }
+    if (d >= 1 << bits) return;
+    uint32_t at = 0;
+    for (int k = 0; k < d; k++) at += total[k];
+    for (long long t = 0; t < tiles; t += 8) {
+        uint32_t n[8];
+#pragma unroll
+        for (int k = 0; k < 8; k++) n[k] = t + k < tiles ? counts[((t + k) << bits) + d] : 0;
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (t + k < tiles) {
+                counts[((t + k) << bits) + d] = at;
+                at += n[k];
             }
-        }
-        __syncthreads();
-        if (!round) {
-            for (int d = threadIdx.x; d < 1 << bits; d += 256) {
-                uint32_t a = starts[(size_t)d * tiles + blockIdx.x];
-                for (int w = 0; w < 4; w++) {
-                    const uint32_t n = at[w][d];
-                    at[w][d] = a;
-                    a += n;
-                }
+    }
+}
+
+// Every entry of a tile to its place: its rank among its wave's entries of its digit, 64 entries at a time in order; behind the
+// entries of smaller digits, of earlier tiles and of earlier waves. SCANNED: `counts` are scan_kernel's.
+template <bool FIRST, int ITEMS, bool SCANNED>
+__global__ void __launch_bounds__(SORT_THREADS) scatter_kernel(const void* __restrict__ ids, const uint32_t* __restrict__ keys,
+                                                               const uint32_t* __restrict__ order, Shape s, int shift, int bits,
+                                                               const uint32_t* __restrict__ counts, unsigned tiles,
+                                                               uint32_t* __restrict__ keys_out, uint32_t* __restrict__ order_out, Zeros z) {
+    if (blockIdx.x >= z.first) {
+        zero_rows(z, s);
+        return;
+    }
+    __shared__ volatile uint16_t seen[SORT_WAVES][DIGITS];  // written by one lane of the owning wave, read by its others
+    __shared__ uint32_t start[SORT_WAVES][DIGITS], totals[SORT_WAVES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, digits = 1 << bits;
+    for (int d = threadIdx.x; d < SORT_WAVES * DIGITS; d += SORT_THREADS) seen[d / DIGITS][d % DIGITS] = 0;
+    const long long first = ((long long)blockIdx.x * SORT_WAVES + wave) * ITEMS * 64 + lane;
+    uint32_t key[ITEMS], who[ITEMS], rank[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++) {
+        const long long t = first + 64 * i;
+        key[i] = t < s.T ? (FIRST ? key_of(ids, s, t, nullptr) : keys[t]) : 0;
+        who[i] = t < s.T ? (FIRST ? (uint32_t)t : order[t]) : 0;
+    }
+    // this tile's part of the counts, while those loads are on their way
+    uint32_t before = 0, all = 0;
+    if (threadIdx.x < digits) {
+        if (SCANNED) {
+            before = counts[(size_t)blockIdx.x * digits + threadIdx.x];
+        } else {
+#pragma unroll 8
+            for (unsigned t = 0; t < tiles; t++) {
+                const uint32_t n = counts[(size_t)t * digits + threadIdx.x];
+                before += t < blockIdx.x ? n : 0;
+                all += n;
             }
-            __syncthreads();
         }
     }
+    __syncthreads();
+    const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++) {
+        const bool in = first + 64 * i < s.T;
+        const uint32_t d = (key[i] >> shift) & (digits - 1);
+        const uint64_t same = same_digit(d, bits, __ballot(in));
+        rank[i] = 0;
+        if (in) {
+            const uint32_t n = seen[wave][d];
+            __builtin_amdgcn_wave_barrier();
+            if (!(same & below)) seen[wave][d] = (uint16_t)(n + __popcll(same));
+            rank[i] = n + __popcll(same & below);
+        }
+    }
+    if (!SCANNED) {
+        uint32_t upto = all;
+        for (int k = 1; k < 64; k *= 2) {
+            const uint32_t y = __shfl_up(upto, k);
+            if (lane >= k) upto += y;
+        }
+        if (lane == 63) totals[wave] = upto;
+        __syncthreads();
+        before += upto - all;
+        for (int w = 0; w < wave; w++) before += totals[w];
+    } else {
+        __syncthreads();
+    }
+    if (threadIdx.x < digits)
+        for (int w = 0; w < SORT_WAVES; w++) {
+            start[w][threadIdx.x] = before;
+            before += seen[w][threadIdx.x];
+        }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < ITEMS; i++)
+        if (first + 64 * i < s.T) {
+            const uint32_t place = start[wave][(key[i] >> shift) & (digits - 1)] + rank[i];
+            keys_out[place] = key[i];
+            order_out[place] = who[i];
+        }
 }
 
 // ---- sums ---------------------------------------------------------------------------------------------
-
-__global__ void __launch_bounds__(256) zero_rows_kernel(void* __restrict__ table, Shape s) {
-    const long long n = s.vocab * s.D, stride = 256ll * gridDim.x;
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += stride) store(table, s.grad_type, i / s.D * s.ldt + i % s.D, 0.0f);
-}
-
-// Eight columns of a lane: c0 + 8 lane + k (VEC), or c0 + lane + 64 k.
-template <bool VEC>
-struct Columns {
-    int c, D;
-    __device__ Columns(int c0, int lane, int D) : c(VEC ? c0 + 8 * lane : c0 + lane), D(D) {}
-    __device__ void get(const void* p, int type, long long row, float* x) const {
-        if constexpr (VEC) {
-            if (c < D) load8(p, type, row + c, x);
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; k++) x[k] = c + 64 * k < D ? load(p, type, row + c + 64 * k) : 0.0f;
-        }
-    }
-    __device__ void put(void* p, int type, long long row, const float* x) const {
-        if constexpr (VEC) {
-            if (c < D) store8(p, type, row + c, x);
-        } else {
-#pragma unroll
-            for (int k = 0; k < 8; k++)
-                if (c + 64 * k < D) store(p, type, row + c + 64 * k, x[k]);
-        }
-    }
-    // the table's row v from its sum
-    __device__ void finish(void* table, const Shape& s, long long v, float* x) const {
-        float old[8] = {};
-        if (s.accumulate) get(table, s.grad_type, v * s.ldt, old);
-#pragma unroll
-        for (int k = 0; k < 8; k++) x[k] = s.accumulate ? old[k] + x[k] * s.scale : x[k] * s.scale;
-        put(table, s.grad_type, v * s.ldt, x);
-    }
-};
-
-// A wave sums run r of R sorted entries, 512 columns. Sums of tokens that the run's beginning cuts go to
-// parts[2 r], of those that its end cuts to parts[2 r + 1] (a token that fills the run: parts[2 r]).
-template <bool VEC>
+// A wave sums run r of R <= 64 sorted entries, 512 columns, 8 rows asked for at a time. Sums of tokens that the run's beginning
+// cuts go to parts[2 r], of those that its end cuts to parts[2 r + 1] (a token that fills the run: parts[2 r]).
 __global__ void __launch_bounds__(256) sums_kernel(const void* __restrict__ dOut, const uint32_t* __restrict__ keys,
                                                    const uint32_t* __restrict__ order, void* __restrict__ table,
                                                    float* __restrict__ parts, Shape s, int R, unsigned slices) {
+    const int lane = threadIdx.x & 63;
     const long long item = 4ll * blockIdx.x + (threadIdx.x >> 6), r = item / slices;
     const long long begin = r * R, end = begin + R < s.T ? begin + R : s.T;
     if (begin >= s.T) return;
-    const Columns<VEC> cols((int)(item % slices) * 512, threadIdx.x & 63, s.D);
-    uint32_t key = keys[begin];
+    const Columns cols((int)(item - r * slices) * 512, lane, s.D);
+    const int n = (int)(end - begin);
     const uint32_t none = (uint32_t)s.vocab;
-    bool cut = begin > 0 && keys[begin - 1] == key;
+    // entry `lane` of the run, its successor's key, and whether the run's first token began before
+    const uint32_t mine = lane < n ? keys[begin + lane] : none, place = lane < n ? order[begin + lane] : 0;
+    const uint32_t after = end < s.T ? keys[end] : none, before = begin > 0 ? keys[begin - 1] : none;
+    bool cut = before == (uint32_t)__builtin_amdgcn_readfirstlane(mine);
     float sum[8] = {};
-    for (long long i = begin; i < end && key != none; i++) {
-        float x[8] = {};
-        cols.get(dOut, s.type, order[i] * s.ldo, x);
+    for (int i0 = 0; i0 < n; i0 += 8) {
+        float x[8][8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) sum[k] += x[k];
-        const uint32_t next = i + 1 < s.T ? keys[i + 1] : none;
-        if (next == key && i + 1 < end) continue;
-        if (cut) cols.put(parts, OZ_F32, 2 * r * s.D, sum);
-        else if (next == key) cols.put(parts, OZ_F32, (2 * r + 1) * s.D, sum);
-        else cols.finish(table, s, key, sum);
-        cut = false;
-        key = next;
+        for (int j = 0; j < 8; j++) {
+            const int i = i0 + j < n ? i0 + j : n - 1;
+            cols.get(dOut, s.type, (long long)(uint32_t)__builtin_amdgcn_readlane(place, i) * s.ldo, x[j]);
+        }
 #pragma unroll
-        for (int k = 0; k < 8; k++) sum[k] = 0.0f;
+        for (int j = 0; j < 8; j++) {
+            const int i = i0 + j;
+            if (i >= n) break;
+            const uint32_t key = __builtin_amdgcn_readlane(mine, i);
+            if (key == none) return;  // they are the last
+#pragma unroll
+            for (int k = 0; k < 8; k++) sum[k] += x[j][k];
+            const uint32_t next = i + 1 < n ? (uint32_t)__builtin_amdgcn_readlane(mine, i + 1) : after;
+            if (next == key && i + 1 < n) continue;
+            if (cut) cols.put(parts, OZ_F32, 2 * r * s.D, sum);
+            else if (next == key) cols.put(parts, OZ_F32, (2 * r + 1) * s.D, sum);
+            else cols.finish(table, s, key, sum);
+            cut = false;
+#pragma unroll
+            for (int k = 0; k < 8; k++) sum[k] = 0.0f;
+        }
     }
 }
 
-// Joins the sums of a token that run r's end cuts and that begins in run r.
-template <bool VEC>
+// Joins the sums of a token that run r's end cuts and that begins in run r, in the runs' order, 8 asked for at a time.
 __global__ void __launch_bounds__(256) join_kernel(const uint32_t* __restrict__ keys, void* __restrict__ table,
                                                    const float* __restrict__ parts, Shape s, int R, unsigned slices) {
+    const int lane = threadIdx.x & 63;
     const long long item = 4ll * blockIdx.x + (threadIdx.x >> 6), r = item / slices;
     const long long begin = r * R, end = begin + R;
     if (end >= s.T) return;
     const uint32_t key = keys[end - 1];
-    if (key == (uint32_t)s.vocab || keys[end] != key || (begin > 0 && keys[begin - 1] == key)) return;
-    const Columns<VEC> cols((int)(item % slices) * 512, threadIdx.x & 63, s.D);
-    float sum[8] = {}, x[8] = {};
+    if (key == (uint32_t)s.vocab || keys[end] != key || (begin > 0 && keys[begin] == key && keys[begin - 1] == key)) return;
+    const Columns cols((int)(item - r * slices) * 512, lane, s.D);
+    float sum[8] = {};
     cols.get(parts, OZ_F32, (2 * r + 1) * s.D, sum);
-    for (long long q = r + 1;; q++) {
-        cols.get(parts, OZ_F32, 2 * q * s.D, x);
+    for (long long q = r + 1;; q += 64) {
+        // how many of the next 64 runs begin with the token
+        const bool on = (q + lane) * R < s.T && keys[(q + lane) * R] == key;
+        const uint64_t off = ~__ballot(on);
+        const int m = off ? __ffsll((unsigned long long)off) - 1 : 64;
+        for (int i0 = 0; i0 < m; i0 += 8) {
+            float x[8][8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) sum[k] += x[k];
-        if ((q + 1) * R >= s.T || keys[(q + 1) * R] != key) break;
+            for (int j = 0; j < 8; j++) cols.get(parts, OZ_F32, 2 * (q + (i0 + j < m ? i0 + j : m - 1)) * s.D, x[j]);
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (i0 + j < m)
+#pragma unroll
+                    for (int k = 0; k < 8; k++) sum[k] += x[j][k];
+        }
+        if (m < 64) break;
     }
     cols.finish(table, s, key, sum);
 }
@@ -285,28 +348,50 @@ Shape shape_of(const oz_embedding_desc* d) {
 
 bool misaligned(const void* p, int bytes) { return ((uintptr_t)p & (bytes - 1)) != 0; }
 
-// Whether rows are whole 16-byte pieces from 16-byte boundaries on.
-bool wide_rows(const Shape& s, const void* a, const void* b) {
-    return s.D % 8 == 0 && s.ldt % 8 == 0 && s.ldo % 8 == 0 && !(((uintptr_t)a | (uintptr_t)b) & 15);
-}
-
 // Sizes of the gradient's workspace: two lists of keys and places, the digits' counts, the cut sums.
 struct Work {
+    int items, R;
     long long tiles, runs;
-    int R;
     size_t list, counts, parts, bytes;
 };
 Work work_of(const oz_embedding_desc* d) {
     Work w;
     const auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
-    w.tiles = (d->T + TILE - 1) / TILE;
-    w.R = 32;
+    w.items = d->T <= 64 * SORT_THREADS ? 1 : 4;  // 64 tiles' counts cost a workgroup 2 us
+    w.tiles = (d->T + w.items * SORT_THREADS - 1) / (w.items * SORT_THREADS);
+    // runs of 32, of 8 where those are too few to fill the chip
+    w.R = d->T * ((d->D + 511) / 512) <= 1 << 15 ? 8 : 32;
     w.runs = (d->T + w.R - 1) / w.R;
     w.list = up(4 * d->T);
     w.counts = up(4 * DIGITS * w.tiles);
     w.parts = up(8 * (size_t)d->D * w.runs);
     w.bytes = 4 * w.list + w.counts + w.parts;
     return w;
+}
+
+// The sorted lists of keys and places (0, 1: which of the two), in 2 launches a digit, 3 of more than SUMMED tiles; `zeros`
+// workgroups of each write the table's zeros.
+template <int ITEMS>
+int sort(oz_dev* dev, const void* ids, void* table, const Shape& s, const Work& w, uint32_t* const* keys, uint32_t* const* order,
+         uint32_t* counts, uint32_t* flags, unsigned zeros) {
+    int total = 1;  // bits of the keys 0..vocab
+    while (s.vocab >> total) total++;
+    const int passes = (total + MAX_BITS - 1) / MAX_BITS, bits = (total + passes - 1) / passes;
+    const unsigned tiles = (unsigned)w.tiles;
+    const dim3 grid(tiles + zeros), block(SORT_THREADS);
+    constexpr bool MANY = ITEMS > 1;
+    const bool scan = MANY && w.tiles > SUMMED;
+    for (int k = 0; k < passes; k++) {
+        uint32_t *ki = keys[(k + 1) & 1], *oi = order[(k + 1) & 1], *ko = keys[k & 1], *oo = order[k & 1];
+        const Zeros z0{table, 2 * k, 2 * passes, tiles}, z1{table, 2 * k + 1, 2 * passes, tiles};
+        const auto count = k ? count_kernel<false, ITEMS> : count_kernel<true, ITEMS>;
+        hipLaunchKernelGGL(count, grid, block, 0, dev->stream, ids, ki, s, k * bits, bits, counts, k ? nullptr : flags, z0);
+        if (scan) hipLaunchKernelGGL(scan_kernel, dim3(1), dim3(DIGITS), 0, dev->stream, counts, bits, w.tiles);
+        const auto scatter = k ? (scan ? scatter_kernel<false, ITEMS, MANY> : scatter_kernel<false, ITEMS, false>)
+                               : (scan ? scatter_kernel<true, ITEMS, MANY> : scatter_kernel<true, ITEMS, false>);
+        hipLaunchKernelGGL(scatter, grid, block, 0, dev->stream, ids, ki, oi, s, k * bits, bits, counts, tiles, ko, oo, z1);
+    }
+    return (passes - 1) & 1;
 }
 
 }  // namespace
@@ -324,10 +409,7 @@ int oz_embedding(oz_dev* dev, const oz_embedding_desc* d, const void* table, con
     if (groups > kMaxGroups) return oz::fail(dev, OZ_ERR_ARG, "oz_embedding: %lld tokens of %d values are too many", s.T, s.D);
     if (int st = oz::use(dev)) return st;
     if (!s.T) return OZ_OK;
-    if (wide_rows(s, table, out))
-        hipLaunchKernelGGL(embedding_kernel<true>, dim3((unsigned)groups), dim3(256), 0, dev->stream, table, ids, out, flags, s, slices);
-    else
-        hipLaunchKernelGGL(embedding_kernel<false>, dim3((unsigned)groups), dim3(256), 0, dev->stream, table, ids, out, flags, s, slices);
+    hipLaunchKernelGGL(embedding_kernel, dim3((unsigned)groups), dim3(256), 0, dev->stream, table, ids, out, flags, s, slices);
     return oz::launch_check(dev, "embedding_kernel");
 }
 
@@ -351,38 +433,24 @@ int oz_embedding_grad(oz_dev* dev, const oz_embedding_desc* d, const void* dOut,
     if (groups > kMaxGroups) return oz::fail(dev, OZ_ERR_ARG, "oz_embedding_grad: %lld tokens of %d values are too many", s.T, s.D);
     if (int st = oz::use(dev)) return st;
     hipStream_t q = dev->stream;
-    if (!s.accumulate) {
-        const unsigned blocks = (unsigned)std::min<long long>((s.vocab * s.D + 255) / 256, 8192);
-        hipLaunchKernelGGL(zero_rows_kernel, dim3(blocks), dim3(256), 0, q, dTable, s);
+    // workgroups that write zeros, in each launch: at most 8 a CU, 16 pieces of 16 bytes a thread or more
+    const long long pieces = s.vocab * ((long long)s.D * size_of(s.grad_type) / 16 + 1);
+    const unsigned zeros = s.accumulate ? 0 : (unsigned)std::max(1ll, std::min<long long>(pieces / (16 * SORT_THREADS), 8 * dev->cus));
+    if (!s.T) {
+        if (zeros) hipLaunchKernelGGL(zero_rows_kernel, dim3(4 * zeros), dim3(256), 0, q, Zeros{dTable, 0, 1, 0}, s);
+        return oz::launch_check(dev, "zero_rows_kernel");
     }
-    if (s.T) {
-        char* p = static_cast<char*>(work);
-        uint32_t* keys[2] = {(uint32_t*)p, (uint32_t*)(p + w.list)};
-        uint32_t* order[2] = {(uint32_t*)(p + 2 * w.list), (uint32_t*)(p + 3 * w.list)};
-        uint32_t* counts = (uint32_t*)(p + 4 * w.list);
-        float* parts = (float*)(p + 4 * w.list + w.counts);
-        int total = 1;  // bits of the keys 0..vocab
-        while (s.vocab >> total) total++;
-        const int passes = (total + MAX_BITS - 1) / MAX_BITS, bits = (total + passes - 1) / passes;
-        const dim3 tiles((unsigned)w.tiles), block(256);
-        for (int k = 0; k < passes; k++) {
-            uint32_t *ki = keys[(k + 1) & 1], *oi = order[(k + 1) & 1], *ko = keys[k & 1], *oo = order[k & 1];
-            if (!k) hipLaunchKernelGGL(count_kernel<true>, tiles, block, 0, q, ids, ki, s, 0, bits, counts, tiles.x, flags);
-            else hipLaunchKernelGGL(count_kernel<false>, tiles, block, 0, q, ids, ki, s, k * bits, bits, counts, tiles.x, flags);
-            hipLaunchKernelGGL(scan_kernel, dim3(1), dim3(1024), 0, q, counts, w.tiles << bits);
-            if (!k) hipLaunchKernelGGL(scatter_kernel<true>, tiles, block, 0, q, ids, ki, oi, s, 0, bits, counts, tiles.x, ko, oo);
-            else hipLaunchKernelGGL(scatter_kernel<false>, tiles, block, 0, q, ids, ki, oi, s, k * bits, bits, counts, tiles.x, ko, oo);
-        }
-        const uint32_t *sk = keys[(passes - 1) & 1], *so = order[(passes - 1) & 1];
-        const dim3 grid((unsigned)groups);
-        if (wide_rows(s, dOut, dTable)) {
-            hipLaunchKernelGGL(sums_kernel<true>, grid, block, 0, q, dOut, sk, so, dTable, parts, s, w.R, slices);
-            hipLaunchKernelGGL(join_kernel<true>, grid, block, 0, q, sk, dTable, parts, s, w.R, slices);
-        } else {
-            hipLaunchKernelGGL(sums_kernel<false>, grid, block, 0, q, dOut, sk, so, dTable, parts, s, w.R, slices);
-            hipLaunchKernelGGL(join_kernel<false>, grid, block, 0, q, sk, dTable, parts, s, w.R, slices);
-        }
-    }
+    char* p = static_cast<char*>(work);
+    uint32_t* keys[2] = {(uint32_t*)p, (uint32_t*)(p + w.list)};
+    uint32_t* order[2] = {(uint32_t*)(p + 2 * w.list), (uint32_t*)(p + 3 * w.list)};
+    uint32_t* counts = (uint32_t*)(p + 4 * w.list);
+    float* parts = (float*)(p + 4 * w.list + w.counts);
+    const int sorted = w.items == 1 ? sort<1>(dev, ids, dTable, s, w, keys, order, counts, flags, zeros)
+                                    : sort<4>(dev, ids, dTable, s, w, keys, order, counts, flags, zeros);
+    if (int st = oz::launch_check(dev, "sort")) return st;
+    const dim3 block(256);
+    hipLaunchKernelGGL(sums_kernel, dim3((unsigned)groups), block, 0, q, dOut, keys[sorted], order[sorted], dTable, parts, s, w.R, slices);
+    hipLaunchKernelGGL(join_kernel, dim3((unsigned)groups), block, 0, q, keys[sorted], dTable, parts, s, w.R, slices);
     return oz::launch_check(dev, "embedding gradient");
 }
 

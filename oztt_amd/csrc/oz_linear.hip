@@ -8,6 +8,9 @@
 #include "oz_internal.hpp"
 #include "oz_linear.hpp"
 
+#include <algorithm>
+#include <type_traits>
+
 namespace {
 
 using namespace ozt;
@@ -64,52 +67,62 @@ __global__ void __launch_bounds__(256) product_any_kernel(const ozl::Product a) 
         }
 }
 
-// dZ = dY act'(Z), rounded for the products (left out where dz is null), and the sums of its columns over `rows` rows each
-// (left out where parts is null): 8 columns a lane, 256 by 8 rows at a time by a workgroup. One pass over dY and Z.
-// VEC: rows of whole 16-byte pieces.
-template <bool VEC>
+// dZ = dY act'(Z), rounded for the products (left out where dz is null), and the sums of its columns over `rows` rows each,
+// to dbias if one range holds all rows, else to parts (left out where both are null): 8 columns a lane, 8 LANES columns by
+// 256 / LANES rows at a time by a workgroup. One pass over dY and Z, which are not read again and pass the caches by.
+template <int LANES>
 __global__ void __launch_bounds__(256) act_grad_kernel(const void* __restrict__ dY, const void* __restrict__ Z,
-                                                       void* __restrict__ dz, float* __restrict__ parts, int type, int act,
-                                                       long long M, int N, long long lddy, long long ldz, long long lddz,
-                                                       int rows, int strips) {
-    const int strip = blockIdx.x % strips, chunk = blockIdx.x / strips;
-    const int col = strip * 256 + 8 * (threadIdx.x & 31), r = threadIdx.x >> 5;
+                                                       void* __restrict__ dz, float* __restrict__ parts, void* __restrict__ dbias,
+                                                       int type, int dw_type, int act, int accumulate, long long M, int N,
+                                                       long long lddy, long long ldz, long long lddz, int rows, int strips) {
+    constexpr int COLS = 8 * LANES, R = 256 / LANES;
+    const int strip = blockIdx.x % strips, chunk = blockIdx.x / strips, l = threadIdx.x % LANES, r = threadIdx.x / LANES;
+    const int col = strip * COLS + 8 * l;
     const long long end = (long long)(chunk + 1) * rows < M ? (long long)(chunk + 1) * rows : M;
     float sum[8] = {};
     if (col < N) {
-        auto get = [&](const void* p, long long at, float* x) {
-            if (VEC) {
-                load8(p, type, at, x);
-            } else {
+        auto rows_of = [&](auto WHOLE) {
+            constexpr bool whole = decltype(WHOLE)::value;
+            auto get = [&](const void* p, long long at, float* x) {
+                if constexpr (whole) load8(p, type, at, x);
+                else load_some(p, type, at, N - col, x);
+            };
+#pragma unroll 4
+            for (long long m = (long long)chunk * rows + r; m < end; m += R) {
+                float x[8], y[8];
+                get(dY, m * lddy + col, x);
+                if (act != OZ_ACT_NONE) {
+                    get(Z, m * ldz + col, y);
 #pragma unroll
-                for (int k = 0; k < 8; k++) x[k] = col + k < N ? load(p, type, at + k) : 0.0f;
+                    for (int k = 0; k < 8; k++) x[k] *= act_grad(y[k], act);
+                }
+                if (dz) store8(dz, type, m * lddz + col, x);
+#pragma unroll
+                for (int k = 0; k < 8; k++) sum[k] += x[k];
             }
         };
-#pragma unroll 4
-        for (long long m = (long long)chunk * rows + r; m < end; m += 8) {
-            float d[8], z[8];
-            get(dY, m * lddy + col, d);
-            if (act != OZ_ACT_NONE) {
-                get(Z, m * ldz + col, z);
-#pragma unroll
-                for (int k = 0; k < 8; k++) d[k] *= act_grad(z[k], act);
-            }
-            if (dz) store8(dz, type, m * lddz + col, d);
-#pragma unroll
-            for (int k = 0; k < 8; k++) sum[k] += d[k];
-        }
+        if (col + 8 <= N) rows_of(std::true_type{});
+        else rows_of(std::false_type{});
     }
-    if (!parts) return;
-    __shared__ float part[8][256];
+    if (!parts && !dbias) return;
+    __shared__ float part[R][COLS];
 #pragma unroll
-    for (int k = 0; k < 8; k++) part[r][8 * (threadIdx.x & 31) + k] = sum[k];
+    for (int k = 0; k < 8; k++) part[r][8 * l + k] = sum[k];
     __syncthreads();
-    const int c = strip * 256 + threadIdx.x;
-    if (c < N) {
-        float s = 0.0f;
-#pragma unroll
-        for (int k = 0; k < 8; k++) s += part[k][threadIdx.x];
-        parts[(long long)chunk * N + c] = s;
+    // R rows of sums to one, halving
+    for (int h = R / 2; h > 0; h /= 2) {
+        for (int e = threadIdx.x; e < h * COLS; e += 256) part[e / COLS][e % COLS] += part[e / COLS + h][e % COLS];
+        __syncthreads();
+    }
+    const int c = strip * COLS + threadIdx.x;
+    if (threadIdx.x < COLS && c < N) {
+        float s = part[0][threadIdx.x];
+        if (dbias) {
+            if (accumulate) s += load(dbias, dw_type, c);
+            store(dbias, dw_type, c, s);
+        } else {
+            parts[(long long)chunk * N + c] = s;
+        }
     }
 }
 
@@ -131,7 +144,7 @@ __global__ void __launch_bounds__(256) bias_grad_kernel(const float* __restrict_
     }
 }
 
-// Operands whose rows are not whole 16-byte pieces, laid out so: rows x cols values at src to rows of `ldd` values, zeros
+// Operands whose rows begin at odd addresses, laid out anew: rows x cols values at src to rows of `ldd` values, zeros
 // behind the last one. Two operands by one launch, 8 values a thread.
 struct Layout {
     const uint16_t* src;
@@ -151,7 +164,7 @@ __global__ void __launch_bounds__(256) lay_out_kernel(Layout a, Layout b, long l
         u32x4 w;
     } x;
     if (col + 8 <= l.cols) {
-        __builtin_memcpy(&x, from, 16);
+        x.w = get16<u32x4>(from);
     } else {
 #pragma unroll
         for (int k = 0; k < 8; k++) x.v[k] = col + k < l.cols ? from[k] : 0;
@@ -161,13 +174,8 @@ __global__ void __launch_bounds__(256) lay_out_kernel(Layout a, Layout b, long l
 
 constexpr long long kMaxTiles = 1ll << 23;  // workgroups of 256 threads in one launch
 
-// Whether rows are whole 16-byte pieces.
-bool whole_rows(const void* p, long long ld) { return !((uintptr_t)p & 15) && ld % 8 == 0; }
-
-bool vec(const Epilogue& e) {
-    return (!e.Y || whole_rows(e.Y, e.ldy)) && (!e.Z || whole_rows(e.Z, e.ldz)) && whole_rows(e.bias, 0) &&
-           (!e.residual || whole_rows(e.residual, e.ldr));
-}
+// Whether rows begin at multiples of 4 bytes, as the tiles' copies need them.
+bool even_rows(const void* p, long long ld) { return !((uintptr_t)p & 3) && ld % 2 == 0; }
 
 size_t up(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 
@@ -193,8 +201,8 @@ float estimate(const Shape& t, int cus, long long nq, long long np, long long C,
     return us;
 }
 
-// Few rows: their own kernel, c in ranges where the rows of W are too few to keep all CUs reading (2 workgroups a CU,
-// each range long enough for its 8 waves). 1 row, N = K = 2048: 6.4 us in one range, 7.7 in four; K = 8192: 18.4 and 10.3.
+// Few rows: their own kernel, c in ranges where the rows of W are too few to keep the CUs reading (at least 2048 values
+// a range). 1 row, 2048 of W, K = 8192: 11.5 us in one range, 10.5 in four; 512 of W, K = 8192: XXX.
 // More: the tile and ranges with the least estimate. 1000 x 704 x 1504: 9.4 us by 64 x 64, 17 by 128 x 128; 2048 x 4096 x
 // 4096: 66 by 128 x 128, 74 by 256 x 256 in two ranges, 101 by 64 x 64; 256 x 1024 x 8192: 15.5 by 64 x 64 in 4 ranges, 38 in one.
 Route route_of(int cus, long long nq, long long np, long long C, bool contiguous, bool aligned) {
@@ -202,8 +210,8 @@ Route route_of(int cus, long long nq, long long np, long long C, bool contiguous
     r.splits = 1;
     if (contiguous && (nq <= kFewRows || (!aligned && nq <= 64))) {
         r.few = true;
-        const long long groups = (np + 31) / 32;
-        while (r.splits < 8 && groups * r.splits * 2 <= 2 * cus && C / (r.splits * 2) >= 2048) r.splits *= 2;
+        const long long groups = (np + few_rows_block(nq) - 1) / few_rows_block(nq);
+        while (r.splits < 8 && groups * r.splits * 4 <= cus && C / (r.splits * 2) >= 2048) r.splits *= 2;
     } else {
         float best = 0.0f;
         for (int t = 0; t < TILES; t++)
@@ -237,14 +245,13 @@ size_t product_bytes(int cus, long long nq, long long np, long long C, bool q_ma
     return r.parts + (copy_q ? copy_bytes(nq, C, q_major) : 0) + (copy_p ? copy_bytes(np, C, p_major) : 0);
 }
 
-// Runs a product in `bytes` bytes of workspace. Operands whose rows are not whole are laid out in it; where that has no room (the
-// sizes are asked for by leading dimensions, operands may be at odd addresses besides) the element by element kernel runs.
+// Runs a product in `bytes` bytes of workspace. Operands whose rows begin at odd addresses are laid out in it; where that has no room
+// (the size is asked for by leading dimensions, an operand may lie at an odd address besides) the element by element kernel runs.
 int launch_product(oz_dev* dev, int type, Product a, void* work, size_t bytes) {
     if (!a.nq || !a.np) return OZ_OK;
-    a.epi.vec = vec(a.epi);
     a.splits = 1;
     if (!a.C) return launch_any(dev, type, a);
-    const bool copy_q = !whole_rows(a.Q, a.ldq), copy_p = !whole_rows(a.P, a.ldp);
+    const bool copy_q = !even_rows(a.Q, a.ldq), copy_p = !even_rows(a.P, a.ldp);
     const Route r = route_of(dev->cus, a.nq, a.np, a.C, !a.q_major && !a.p_major, !copy_q && !copy_p);
     const size_t need = product_bytes(dev->cus, a.nq, a.np, a.C, a.q_major, a.p_major, copy_q, copy_p);
     if (need > bytes) return launch_any(dev, type, a);
@@ -312,27 +319,28 @@ const char* refuse(const oz_linear_grad_desc* d) {
 bool misaligned16(const void* p) { return ((uintptr_t)p & 15) != 0; }
 bool misaligned(const void* p, int type) { return ((uintptr_t)p & (size_of(type) - 1)) != 0; }
 
-// Workspace of the gradients: dZ where it is not dY (or dY's rows are not whole), the columns' sums, and the larger of the
+// Workspace of the gradients: dZ where it is not dY (or dY's rows are not even), the columns' sums, and the larger of the
 // products' own.
 struct GradWork {
     bool make_dz;
     long long lddz;
+    int lanes;         // act_grad_kernel's
     int rows, chunks;  // of M for the columns' sums
     size_t dz, sums, product, bytes;
 };
-GradWork grad_work(int cus, const oz_linear_grad_desc* d, bool whole_dy) {
+GradWork grad_work(int cus, const oz_linear_grad_desc* d, bool even_dy) {
     GradWork w{};
-    w.make_dz = d->act != OZ_ACT_NONE || !whole_dy;
+    w.make_dz = d->act != OZ_ACT_NONE || !even_dy;
     w.lddz = (d->N + 7) / 8 * 8;
     w.dz = w.make_dz ? up(2 * (size_t)d->M * w.lddz) : 0;
-    // enough workgroups of 256 columns to fill the chip twice, 16 to 256 rows each
-    const long long strips = (d->N + 255) / 256;
-    long long rows = (long long)d->M * strips / (4 * cus);
-    w.rows = (int)std::min(256ll, std::max(16ll, (rows + 7) / 8 * 8));
+    // Strips of 256 columns, 64 of few values, and of the rows so many that the chip is filled four times, 16 to 256 at a time.
+    w.lanes = (long long)d->M * d->N <= 1 << 22 ? 8 : 32;
+    const long long strips = (d->N + 8 * w.lanes - 1) / (8 * w.lanes), rows = (long long)d->M * strips / (4 * cus), least = 512 / w.lanes;
+    w.rows = (int)std::min(256ll, std::max(least, (rows + least - 1) / least * least));
     w.chunks = (int)std::max(1ll, ((long long)d->M + w.rows - 1) / w.rows);
     w.sums = up(4 * (size_t)w.chunks * d->N);
-    w.product = std::max(product_bytes(cus, d->M, d->K, d->N, false, true, false, or_row(d->ldw, d->K) % 8 != 0),
-                         product_bytes(cus, d->N, d->K, d->M, true, true, false, or_row(d->ldx, d->K) % 8 != 0));
+    w.product = std::max(product_bytes(cus, d->M, d->K, d->N, false, true, false, or_row(d->ldw, d->K) % 2 != 0),
+                         product_bytes(cus, d->N, d->K, d->M, true, true, false, or_row(d->ldx, d->K) % 2 != 0));
     w.bytes = w.dz + w.sums + w.product;
     return w;
 }
@@ -345,7 +353,7 @@ extern "C" {
 
 long long oz_linear_workspace(oz_dev* dev, const oz_linear_desc* d) {
     if (const char* e = refuse(d)) return oz::fail(dev, OZ_ERR_ARG, "oz_linear: %s", e);
-    return (long long)product_bytes(cus_of(dev), d->M, d->N, d->K, false, false, or_row(d->ldx, d->K) % 8 != 0, or_row(d->ldw, d->K) % 8 != 0);
+    return (long long)product_bytes(cus_of(dev), d->M, d->N, d->K, false, false, or_row(d->ldx, d->K) % 2 != 0, or_row(d->ldw, d->K) % 2 != 0);
 }
 
 int oz_linear(oz_dev* dev, const oz_linear_desc* d, const void* X, const void* W, const void* bias,
@@ -370,7 +378,7 @@ int oz_linear(oz_dev* dev, const oz_linear_desc* d, const void* X, const void* W
 
 long long oz_linear_grad_workspace(oz_dev* dev, const oz_linear_grad_desc* d) {
     if (const char* e = refuse(d)) return oz::fail(dev, OZ_ERR_ARG, "oz_linear_grad: %s", e);
-    return (long long)grad_work(cus_of(dev), d, or_row(d->lddy, d->N) % 8 == 0).bytes;
+    return (long long)grad_work(cus_of(dev), d, or_row(d->lddy, d->N) % 2 == 0).bytes;
 }
 
 int oz_linear_grad(oz_dev* dev, const oz_linear_grad_desc* d, const void* dY, const void* X, const void* W,
@@ -382,12 +390,12 @@ int oz_linear_grad(oz_dev* dev, const oz_linear_grad_desc* d, const void* dY, co
     if (misaligned(dY, d->type) || misaligned(X, d->type) || misaligned(W, d->type) || misaligned(Z, d->type) ||
         misaligned(dX, d->type) || misaligned(dW, d->dw_type) || misaligned(dbias, d->dw_type))
         return oz::fail(dev, OZ_ERR_ARG, "oz_linear_grad: operands at addresses that their types do not allow");
-    const size_t least = grad_work(cus_of(dev), d, or_row(d->lddy, d->N) % 8 == 0).bytes;
+    const size_t least = grad_work(cus_of(dev), d, or_row(d->lddy, d->N) % 2 == 0).bytes;
     if (!work || bytes < least || misaligned16(work))
         return oz::fail(dev, OZ_ERR_ARG, "oz_linear_grad: workspace of %zu bytes, %zu needed (16-byte aligned)", bytes, least);
     if (int st = oz::use(dev)) return st;
     const long long lddy = or_row(d->lddy, d->N), ldz = or_row(d->ldz, d->N);
-    GradWork w = grad_work(cus_of(dev), d, whole_rows(dY, lddy));
+    GradWork w = grad_work(cus_of(dev), d, even_rows(dY, lddy));
     if (w.bytes > bytes) w.make_dz = false, w.dz = 0;  // dY at an odd address without room for a copy
     char* at = static_cast<char*>(work);
     const void* dz = dY;
@@ -397,20 +405,17 @@ int oz_linear_grad(oz_dev* dev, const oz_linear_grad_desc* d, const void* dY, co
         void* make = w.make_dz && products ? at : nullptr;
         if (make) dz = make, lddz = w.lddz;
         float* sums = dbias ? reinterpret_cast<float*>(at + w.dz) : nullptr;
-        const int strips = (int)oz::ceil_div(d->N, 256), chunks = d->M ? w.chunks : 0;
-        const bool wide = d->N % 8 == 0 && whole_rows(dY, lddy) && (!curved || whole_rows(Z, ldz));
+        const int strips = (int)oz::ceil_div(d->N, 8 * w.lanes), chunks = d->M ? w.chunks : 0;
         if ((long long)strips * w.chunks > kMaxTiles) return oz::fail(dev, OZ_ERR_ARG, "oz_linear_grad: %d x %d outputs are too many", d->M, d->N);
+        const bool one = chunks == 1;
         if (chunks) {
             const dim3 grid((unsigned)(strips * chunks));
-            if (wide)
-                hipLaunchKernelGGL(act_grad_kernel<true>, grid, dim3(256), 0, dev->stream, dY, Z, make, sums, d->type, d->act,
-                                   (long long)d->M, d->N, lddy, ldz, w.lddz, w.rows, strips);
-            else
-                hipLaunchKernelGGL(act_grad_kernel<false>, grid, dim3(256), 0, dev->stream, dY, Z, make, sums, d->type, d->act,
-                                   (long long)d->M, d->N, lddy, ldz, w.lddz, w.rows, strips);
+            const auto kernel = w.lanes == 8 ? act_grad_kernel<8> : act_grad_kernel<32>;
+            hipLaunchKernelGGL(kernel, grid, dim3(256), 0, dev->stream, dY, Z, make, one ? nullptr : sums, one ? dbias : nullptr,
+                               d->type, d->dw_type, d->act, d->accumulate, (long long)d->M, d->N, lddy, ldz, w.lddz, w.rows, strips);
             if (int st = oz::launch_check(dev, "act_grad_kernel")) return st;
         }
-        if (dbias) {
+        if (dbias && !one) {
             hipLaunchKernelGGL(bias_grad_kernel, dim3(oz::ceil_div(d->N, 16)), dim3(256), 0, dev->stream, sums, dbias, d->dw_type,
                                d->accumulate, chunks, d->N);
             if (int st = oz::launch_check(dev, "bias_grad_kernel")) return st;

@@ -17,7 +17,6 @@ struct Epilogue {
     const void* residual;
     long long ldr;
     int act;
-    int vec;  // every array at 16 bytes, rows of a multiple of 8 values
 };
 
 // C(q, p) = sum over c < C of Q(q, c) P(p, c), q < nq, p < np. Q(q, c) is at q ldq + c, or at c ldq + q where
@@ -41,34 +40,35 @@ __device__ __forceinline__ void finish(const Epilogue& e, int type, long long q,
     ozt::store(e.Y, e.y_type, q * e.ldy + p, v);
 }
 
-// Eight values in a row from p on, p a multiple of 8.
+// Eight values in a row from p on, of them those below np. Everything is read before anything is written: with one
+// wave on a SIMD every wait for memory counts.
 template <int TYPE>
 __device__ __forceinline__ void finish8(const Epilogue& e, long long np, long long q, long long p, float* v) {
-    if (e.vec && p + 8 <= np) {
-        float x[8];
-        if (e.bias) {
-            ozt::load8(e.bias, TYPE, p, x);
-#pragma unroll
-            for (int k = 0; k < 8; k++) v[k] += x[k];
-        }
-        if (e.Z) ozt::store8(e.Z, TYPE, q * e.ldz + p, v);
-        if (e.act != OZ_ACT_NONE)
-#pragma unroll
-            for (int k = 0; k < 8; k++) v[k] = ozt::act(v[k], e.act);
-        if (e.residual) {
-            ozt::load8(e.residual, e.y_type, q * e.ldr + p, x);
-#pragma unroll
-            for (int k = 0; k < 8; k++) v[k] += x[k];
-        }
-        ozt::store8(e.Y, e.y_type, q * e.ldy + p, v);
+    const int count = p + 8 <= np ? 8 : (int)(np - p);
+    float b[8] = {}, r[8] = {};
+    if (count == 8) {
+        if (e.bias) ozt::load8(e.bias, TYPE, p, b);
+        if (e.residual) ozt::load8(e.residual, e.y_type, q * e.ldr + p, r);
     } else {
-#pragma unroll
-        for (int k = 0; k < 8; k++)
-            if (p + k < np) finish(e, TYPE, q, p + k, v[k]);
+        if (e.bias) ozt::load_some(e.bias, TYPE, p, count, b);
+        if (e.residual) ozt::load_some(e.residual, e.y_type, q * e.ldr + p, count, r);
     }
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] += b[k];
+    if (e.Z) {
+        if (count == 8) ozt::store8(e.Z, TYPE, q * e.ldz + p, v);
+        else ozt::store_some(e.Z, TYPE, q * e.ldz + p, count, v);
+    }
+    if (e.act != OZ_ACT_NONE)
+#pragma unroll
+        for (int k = 0; k < 8; k++) v[k] = ozt::act(v[k], e.act);
+#pragma unroll
+    for (int k = 0; k < 8; k++) v[k] += r[k];
+    if (count == 8) ozt::store8(e.Y, e.y_type, q * e.ldy + p, v);
+    else ozt::store_some(e.Y, e.y_type, q * e.ldy + p, count, v);
 }
 
-// Tiles of an aligned product, rows x columns of outputs.
+// Tiles of a product whose operands' rows begin at multiples of 4 bytes; rows x columns of outputs.
 enum Tile { T256, T128, T64, T64X32, T32, TILES };
 struct Shape {
     int q, p;            // outputs
@@ -84,7 +84,8 @@ inline const Shape& shape_of(Tile t) {
     return shapes[t];
 }
 int launch_tile(oz_dev* dev, int type, Tile tile, const Product& a);
-// At most 64 rows of Q, operands along c at any address; splits as in Product.
+// At most 64 rows of Q, operands along c at any address; splits as in Product. A workgroup has few_rows_block rows of P.
+inline int few_rows_block(long long nq) { return nq <= 16 ? 16 : 32; }
 int launch_few_rows(oz_dev* dev, int type, const Product& a);
 // Joins the ranges of c in order.
 int launch_join(oz_dev* dev, int type, const Product& a);

@@ -16,17 +16,8 @@ using namespace ozt;
 
 constexpr int WAVES = 8;
 
-// Eight values from p on. !ALIGNED: at any even address (the hardware's loads allow it).
-template <class T8, bool ALIGNED>
-__device__ __forceinline__ T8 load_chunk(const void* p) {
-    T8 v;
-    if constexpr (ALIGNED) v = *static_cast<const T8*>(p);
-    else __builtin_memcpy(&v, p, 16);
-    return v;
-}
-
-template <int TYPE, int MB, int NB, bool ALIGNED>
-__global__ void __launch_bounds__(64 * WAVES, 4) few_rows_kernel(const Product a, int blocks_p) {
+template <int TYPE, int MB, int NB>
+__global__ void __launch_bounds__(64 * WAVES, MB == 4 ? 2 : 4) few_rows_kernel(const Product a, int blocks_p) {
     typedef typename Half<TYPE>::t T;
     typedef typename Half<TYPE>::x8 T8;
     constexpr int F = MB == 1 ? 4 : 2, UNIT = 32 * F;  // values of c that a wave takes at a time
@@ -50,11 +41,11 @@ __global__ void __launch_bounds__(64 * WAVES, 4) few_rows_kernel(const Product a
 #pragma unroll
             for (int n = 0; n < NB; n++)
 #pragma unroll
-                for (int f = 0; f < F; f++) w[b][n][f] = load_chunk<T8, ALIGNED>(pw[n] + (long long)u * UNIT + 32 * f);
+                for (int f = 0; f < F; f++) w[b][n][f] = get16<T8>(pw[n] + (long long)u * UNIT + 32 * f);
 #pragma unroll
             for (int m = 0; m < MB; m++)
 #pragma unroll
-                for (int f = 0; f < F; f++) x[b][m][f] = load_chunk<T8, ALIGNED>(px[m] + (long long)u * UNIT + 32 * f);
+                for (int f = 0; f < F; f++) x[b][m][f] = get16<T8>(px[m] + (long long)u * UNIT + 32 * f);
         }
     };
     auto multiply = [&](int b) {
@@ -112,18 +103,17 @@ __global__ void __launch_bounds__(64 * WAVES, 4) few_rows_kernel(const Product a
 
 template <int TYPE, int MB, int NB>
 int launch(oz_dev* dev, const Product& a) {
-    const int blocks_p = (int)oz::ceil_div(a.np, 16 * NB);
+    const int blocks_p = (int)oz::ceil_div(a.np, ozl::few_rows_block(a.nq));
+    static_assert(NB == (MB == 1 ? 1 : 2), "few_rows_block");
     const dim3 grid((unsigned)blocks_p * a.splits), block(64 * WAVES);
-    const bool aligned = !(((uintptr_t)a.P | (uintptr_t)a.Q) & 15) && a.ldp % 8 == 0 && a.ldq % 8 == 0;
-    if (aligned) hipLaunchKernelGGL((few_rows_kernel<TYPE, MB, NB, true>), grid, block, 0, dev->stream, a, blocks_p);
-    else hipLaunchKernelGGL((few_rows_kernel<TYPE, MB, NB, false>), grid, block, 0, dev->stream, a, blocks_p);
+    hipLaunchKernelGGL((few_rows_kernel<TYPE, MB, NB>), grid, block, 0, dev->stream, a, blocks_p);
     if (int st = oz::launch_check(dev, "few_rows_kernel")) return st;
     return a.splits > 1 ? ozl::launch_join(dev, TYPE, a) : OZ_OK;
 }
 
 template <int TYPE>
 int by_rows(oz_dev* dev, const Product& a) {
-    if (a.nq <= 16) return launch<TYPE, 1, 2>(dev, a);
+    if (a.nq <= 16) return launch<TYPE, 1, 1>(dev, a);
     return a.nq <= 32 ? launch<TYPE, 2, 2>(dev, a) : launch<TYPE, 4, 2>(dev, a);
 }
 

@@ -10,13 +10,15 @@
 // i's 4 values; the columns' 32-byte pieces are swizzled by the row, so that the rows that a read takes at once fall on
 // different banks. Both give a lane the same 8 values of c.
 //
-// The copies are buffer loads: what lies outside an operand is outside its buffer's range and reads as zero, so
-// no load is guarded and nothing beyond an operand is touched.
+// The copies are buffer loads, whose range is checked by the 4-byte word: what lies outside an operand is outside its
+// buffer's range and reads as zero, so no load is guarded and nothing beyond the word with an operand's last value is
+// touched. Rows may begin at any multiple of 4 bytes.
 #pragma once
 #include "oz_gemm_common.hpp"
 #include "oz_linear.hpp"
 
 #include <type_traits>
+#include <utility>
 
 namespace ozl {
 
@@ -49,7 +51,7 @@ struct Operand {
     static constexpr int RB = 2 * ROWS;       // MAJOR: bytes of a row of c
     static constexpr int PIECES = RB / 32;    // 32-byte pieces of it
     v4i rs;              // buffer of the stage to load next
-    long long left;      // MAJOR: bytes from its address to the operand's end
+    long long left;      // bytes from its address to the operand's end
     unsigned step;       // bytes of a stage's advance
     unsigned off[N];     // of this lane's copies
     unsigned dead, last; // !MAJOR: OUTSIDE for a lane whose chunk is beyond C, in the stage to load and in the last one
@@ -65,7 +67,7 @@ struct Operand {
         unsigned long long base;
         if constexpr (MAJOR) {
             base = (unsigned long long)p + c0 * ldb + 2 * row0;
-            left = (C - 1 - c0) * ldb + ((2 * (n - row0) + 15) & ~15ll);  // chunks that hold a value are read whole
+            left = (C - 1 - c0) * ldb + ((2 * (n - row0) + 3) & ~3ll);
             step = (unsigned)(BC * ldb);
 #pragma unroll
             for (int j = 0; j < N; j++) {
@@ -75,6 +77,7 @@ struct Operand {
             }
         } else {
             base = (unsigned long long)p + row0 * ldb + 2 * c0;
+            left = (n - 1 - row0) * ldb + ((2 * (C - c0) + 3) & ~3ll);
             step = 2 * BC;
             const int r = lane >> 3, chunk = (lane & 7) ^ r;
 #pragma unroll
@@ -86,14 +89,13 @@ struct Operand {
         }
         rs[0] = __builtin_amdgcn_readfirstlane((int)base);
         rs[1] = __builtin_amdgcn_readfirstlane((int)(base >> 32) & 0xFFFF);
-        rs[2] = (int)RANGE;
         rs[3] = 0x00020000;
         range();
     }
     // What of the stage to load next lies in the operand and the range of c.
     __device__ __forceinline__ void range() {
-        if constexpr (MAJOR) rs[2] = __builtin_amdgcn_readfirstlane((int)(left < 0 || steps <= 0 ? 0 : left < RANGE ? left : RANGE));
-        else dead = steps > 1 ? 0u : steps == 1 ? last : OUTSIDE;
+        rs[2] = __builtin_amdgcn_readfirstlane((int)(left < 0 || steps <= 0 ? 0 : left < RANGE ? left : RANGE));
+        if constexpr (!MAJOR) dead = steps == 1 ? last : 0u;
     }
     __device__ __forceinline__ void copy(uint8_t* stage, int j, int wave) const {
         lds_copy(rs, stage + 1024 * (W * j + wave), MAJOR ? off[j] : off[j] | dead);
@@ -103,7 +105,7 @@ struct Operand {
         const unsigned long long base = ((unsigned long long)(unsigned)rs[1] << 32 | (unsigned)rs[0]) + step;
         rs[0] = (int)base;
         rs[1] = (int)(base >> 32);
-        if constexpr (MAJOR) left -= step;
+        left -= step;
         range();
     }
 
@@ -153,6 +155,16 @@ __device__ __forceinline__ void place_of(const Product& a, int tiles_q, int tile
     tp = __builtin_amdgcn_readfirstlane(tp);
 }
 
+// f(0), ..., f(N - 1), the numbers as types: what indexes registers is a constant whatever the compiler unrolls.
+template <class F, int... I>
+__device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, class F>
+__device__ __forceinline__ void each(F&& f) {
+    each_of(f, std::make_integer_sequence<int, N>{});
+}
+
 // The sums of a wave to the outputs. Register k of lane l holds p = 4 (l / 16) + k, q = l % 16. They go through LDS (`tile`,
 // ROOM floats of the wave's own), RI bands of 16 rows at a time, in rows of 16 TJ values whose 16-byte pieces are swizzled
 // by the row; then a lane takes 8 values in a row, the same columns each time, so that outputs, residual
@@ -170,14 +182,13 @@ __device__ __forceinline__ void put_sums(const Product& a, const f32x4 (&acc)[TI
     const Epilogue& e = a.epi;
     const int r = lane & 15, g = lane >> 4, piece = 2 * (lane % (2 * TJ)), rr = lane / (2 * TJ);
     const long long p = p0 + 4 * piece;
-    const bool fast = a.splits == 1 && e.vec && (a.np % 8 == 0 || p0 + 16 * TJ <= a.np);
-    auto write = [&](int h) {
+    auto write = [&](auto H) {
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int i = 0; i < RI; i++)
 #pragma unroll
             for (int j = 0; j < TJ; j++)
-                *reinterpret_cast<f32x4*>(tile + (16 * i + r) * ROW + 4 * ((4 * j + g) ^ (r & XM))) = acc[h * RI + i][j];
+                *reinterpret_cast<f32x4*>(tile + (16 * i + r) * ROW + 4 * ((4 * j + g) ^ (r & XM))) = acc[decltype(H)::value * RI + i][j];
         __builtin_amdgcn_wave_barrier();
     };
     auto read = [&](int row, float* v) {
@@ -188,67 +199,10 @@ __device__ __forceinline__ void put_sums(const Product& a, const f32x4 (&acc)[TI
             for (int m = 0; m < 4; m++) v[4 * k + m] = x[m];
         }
     };
-    if (fast) {
-        const bool in = p < a.np;
-        float bias[8] = {};
-        if (e.bias && in) load8(e.bias, TYPE, p, bias);
-        const int wide = e.y_type == OZ_F32;
-        const char* pr = static_cast<const char*>(e.residual) + ((q0 + rr) * e.ldr + p) * (wide ? 4 : 2);
-        char* py = static_cast<char*>(e.Y) + ((q0 + rr) * e.ldy + p) * (wide ? 4 : 2);
-        char* pz = static_cast<char*>(e.Z) + ((q0 + rr) * e.ldz + p) * 2;
-        const long long dr = RT * e.ldr * (wide ? 4 : 2), dy = RT * e.ldy * (wide ? 4 : 2), dz = RT * e.ldz * 2;
-        u32x4 res[2][BATCH][2] = {};
-        auto ask = [&](int b) {  // batch b of all TI / RI * BATCHES
-            if (!e.residual) return;
-#pragma unroll
-            for (int t = 0; t < BATCH; t++) {
-                if (!in || q0 + (b * BATCH + t) * RT + rr >= a.nq) continue;
-                const u32x4* at = reinterpret_cast<const u32x4*>(pr + (b * BATCH + t) * dr);
-                res[b & 1][t][0] = at[0];
-                if (wide) res[b & 1][t][1] = at[1];
-            }
-        };
-        ask(0);
-#pragma unroll
-        for (int h = 0; h < TI / RI; h++) {
-            write(h);
-#pragma unroll
-            for (int c = 0; c < BATCHES; c++) {
-                const int b = h * BATCHES + c;
-                if (b + 1 < TI / RI * BATCHES) ask(b + 1);
-#pragma unroll
-                for (int t = 0; t < BATCH; t++) {
-                    const int turn = c * BATCH + t;
-                    if (!in || q0 + (h * NT + turn) * RT + rr >= a.nq) continue;
-                    float v[8];
-                    read(RT * turn + rr, v);
-#pragma unroll
-                    for (int k = 0; k < 8; k++) v[k] += bias[k];
-                    if (e.Z) store8(pz + (h * NT + turn) * dz, TYPE, 0, v);
-                    if (e.act != OZ_ACT_NONE)
-#pragma unroll
-                        for (int k = 0; k < 8; k++) v[k] = act(v[k], e.act);
-                    if (e.residual) {
-                        float x[8];
-                        if (wide) {
-#pragma unroll
-                            for (int k = 0; k < 8; k++) x[k] = __uint_as_float(res[b & 1][t][k >> 2][k & 3]);
-                        } else {
-                            load8(&res[b & 1][t][0], TYPE, 0, x);
-                        }
-#pragma unroll
-                        for (int k = 0; k < 8; k++) v[k] += x[k];
-                    }
-                    store8(py + (h * NT + turn) * dy, e.y_type, 0, v);
-                }
-            }
-        }
-        return;
-    }
-#pragma unroll
-    for (int h = 0; h < TI / RI; h++) {
-        write(h);
-        if (a.splits > 1) {
+    if (a.splits > 1) {
+        each<TI / RI>([&](auto H) {
+            constexpr int h = decltype(H)::value;
+            write(H);
 #pragma unroll 4
             for (int turn = 0; turn < NT; turn++) {
                 const long long q = q0 + 16 * h * RI + RT * turn + rr;
@@ -256,40 +210,72 @@ __device__ __forceinline__ void put_sums(const Product& a, const f32x4 (&acc)[TI
                 read(RT * turn + rr, v);
                 if (q < a.nq && p < a.np) store8(a.parts, OZ_F32, (split * a.nq + q) * a.ldparts + p, v);
             }
-            continue;
+        });
+        return;
+    }
+    const bool in = p + 8 <= a.np;  // all 8 values
+    float bias[8] = {};
+    if (e.bias && in) load8(e.bias, TYPE, p, bias);
+    const int wide = e.y_type == OZ_F32;
+    const char* pr = static_cast<const char*>(e.residual) + ((q0 + rr) * e.ldr + p) * (wide ? 4 : 2);
+    char* py = static_cast<char*>(e.Y) + ((q0 + rr) * e.ldy + p) * (wide ? 4 : 2);
+    char* pz = static_cast<char*>(e.Z) + ((q0 + rr) * e.ldz + p) * 2;
+    const long long dr = RT * e.ldr * (wide ? 4 : 2), dy = RT * e.ldy * (wide ? 4 : 2), dz = RT * e.ldz * 2;
+    u32x4 res[2][BATCH][2] = {};
+    auto ask = [&](auto B) {  // batch B of all TI / RI * BATCHES
+        constexpr int b = decltype(B)::value;
+        if (!e.residual) return;
+#pragma unroll
+        for (int t = 0; t < BATCH; t++) {
+            if (!in || q0 + (b * BATCH + t) * RT + rr >= a.nq) continue;
+            const char* from = pr + (b * BATCH + t) * dr;
+            res[b & 1][t][0] = get16<u32x4>(from);
+            if (wide) res[b & 1][t][1] = get16<u32x4>(from + 16);
         }
-        // Where rows are not whole 16-byte pieces: value by value, a row's next to each other, eight residuals asked for at
-        // a time.
-        constexpr int CW = ROW < 64 ? ROW : 64, RW = 64 / CW;  // columns and rows of a turn
-        const int c1 = lane % CW, r1 = lane / CW;
+    };
+    ask(std::integral_constant<int, 0>{});
+    each<TI / RI>([&](auto H) {
+        constexpr int h = decltype(H)::value;
+        write(H);
+        each<BATCHES>([&](auto C) {
+            constexpr int c = decltype(C)::value, b = h * BATCHES + c;
+            if constexpr (b + 1 < TI / RI * BATCHES) ask(std::integral_constant<int, b + 1>{});
+#pragma unroll
+            for (int t = 0; t < BATCH; t++) {
+                const int turn = c * BATCH + t;
+                if (!in || q0 + (h * NT + turn) * RT + rr >= a.nq) continue;
+                float v[8];
+                read(RT * turn + rr, v);
+#pragma unroll
+                for (int k = 0; k < 8; k++) v[k] += bias[k];
+                if (e.Z) store8(pz + (h * NT + turn) * dz, TYPE, 0, v);
+                if (e.act != OZ_ACT_NONE)
+#pragma unroll
+                    for (int k = 0; k < 8; k++) v[k] = act(v[k], e.act);
+                if (e.residual) {
+                    float x[8];
+                    if (wide) {
+#pragma unroll
+                        for (int k = 0; k < 8; k++) x[k] = __uint_as_float(res[b & 1][t][k >> 2][k & 3]);
+                    } else {
+                        widen8(res[b & 1][t][0], TYPE, x);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; k++) v[k] += x[k];
+                }
+                store8(py + (h * NT + turn) * dy, e.y_type, 0, v);
+            }
+        });
+        if (!in && p < a.np) {  // the row's last, fewer than 8 values
 #pragma unroll 1
-        for (int n = 0; n < 16 * RI / RW; n += 8) {
-#pragma unroll
-            for (int c = 0; c < ROW; c += CW) {
-                const long long pp = p0 + c + c1;
-                float res[8] = {};
-                if (e.residual && pp < a.np) {
-#pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        const long long q = q0 + 16 * h * RI + RW * (n + k) + r1;
-                        if (q < a.nq) res[k] = load(e.residual, e.y_type, q * e.ldr + pp);
-                    }
-                }
-                if (pp < a.np) {
-                    const float bias = e.bias ? load(e.bias, TYPE, pp) : 0.0f;
-#pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        const int row = RW * (n + k) + r1, col = c + c1;
-                        const long long q = q0 + 16 * h * RI + row;
-                        if (q >= a.nq) continue;
-                        float v = tile[row * ROW + 4 * ((col >> 2) ^ (row & XM)) + (col & 3)] + bias;
-                        if (e.Z) store(e.Z, TYPE, q * e.ldz + pp, v);
-                        store(e.Y, e.y_type, q * e.ldy + pp, act(v, e.act) + res[k]);
-                    }
-                }
+            for (int turn = 0; turn < NT; turn++) {
+                const long long q = q0 + (h * NT + turn) * RT + rr;
+                float v[8];
+                read(RT * turn + rr, v);
+                if (q < a.nq) finish8<TYPE>(e, a.np, q, p, v);
             }
         }
-    }
+    });
 }
 
 // The values of c in the last stage where they do not fill its chunks, else 0 (of the last range only).

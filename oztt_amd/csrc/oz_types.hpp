@@ -46,38 +46,117 @@ __device__ __forceinline__ void store(void* p, int type, long long i, float x) {
     else static_cast<_Float16*>(p)[i] = (_Float16)x;
 }
 
-// Eight values from i on, 16-byte aligned (type uniform over the wave: one branch).
+// Sixteen bytes at any address that a value's type allows: the hardware's vector accesses of global memory take them.
+template <class T>
+__device__ __forceinline__ T get16(const void* p) {
+    T x;
+    __builtin_memcpy(&x, __builtin_assume_aligned(p, 2), 16);
+    return x;
+}
+template <class T>
+__device__ __forceinline__ void put16(void* p, T x) {
+    __builtin_memcpy(__builtin_assume_aligned(p, 2), &x, 16);
+}
+
+// Eight values of a register's 16 bytes, of a 16-bit type.
+__device__ __forceinline__ void widen8(u32x4 w, int type, float* x) {
+    union {
+        u32x4 w;
+        bf16x8 b;
+        f16x8 h;
+    } u;
+    u.w = w;
+    if (type == OZ_BF16) {
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[k] = (float)u.b[k];
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; k++) x[k] = (float)u.h[k];
+    }
+}
+
+// Eight values from i on (type uniform over the wave: one branch).
 __device__ __forceinline__ void load8(const void* p, int type, long long i, float* x) {
     if (type == OZ_F32) {
-        const f32x4* q = reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + i);
-        const f32x4 a = q[0], b = q[1];
+        const float* q = static_cast<const float*>(p) + i;
+        const f32x4 a = get16<f32x4>(q), b = get16<f32x4>(q + 4);
 #pragma unroll
         for (int k = 0; k < 4; k++) x[k] = a[k], x[4 + k] = b[k];
-    } else if (type == OZ_BF16) {
-        const bf16x8 a = *reinterpret_cast<const bf16x8*>(static_cast<const __bf16*>(p) + i);
-#pragma unroll
-        for (int k = 0; k < 8; k++) x[k] = (float)a[k];
     } else {
-        const f16x8 a = *reinterpret_cast<const f16x8*>(static_cast<const _Float16*>(p) + i);
-#pragma unroll
-        for (int k = 0; k < 8; k++) x[k] = (float)a[k];
+        widen8(get16<u32x4>(static_cast<const uint16_t*>(p) + i), type, x);
     }
 }
 __device__ __forceinline__ void store8(void* p, int type, long long i, const float* x) {
     if (type == OZ_F32) {
-        f32x4* q = reinterpret_cast<f32x4*>(static_cast<float*>(p) + i);
-        q[0] = f32x4{x[0], x[1], x[2], x[3]};
-        q[1] = f32x4{x[4], x[5], x[6], x[7]};
+        float* q = static_cast<float*>(p) + i;
+        put16(q, f32x4{x[0], x[1], x[2], x[3]});
+        put16(q + 4, f32x4{x[4], x[5], x[6], x[7]});
     } else if (type == OZ_BF16) {
         bf16x8 a;
 #pragma unroll
         for (int k = 0; k < 8; k++) a[k] = (__bf16)x[k];
-        *reinterpret_cast<bf16x8*>(static_cast<__bf16*>(p) + i) = a;
+        put16(static_cast<__bf16*>(p) + i, a);
     } else {
         f16x8 a;
 #pragma unroll
         for (int k = 0; k < 8; k++) a[k] = (_Float16)x[k];
-        *reinterpret_cast<f16x8*>(static_cast<_Float16*>(p) + i) = a;
+        put16(static_cast<_Float16*>(p) + i, a);
+    }
+}
+// The first `count` of eight values.
+__device__ __forceinline__ void load_some(const void* p, int type, long long i, int count, float* x) {
+#pragma unroll
+    for (int k = 0; k < 8; k++) x[k] = k < count ? load(p, type, i + k) : 0.0f;
+}
+__device__ __forceinline__ void store_some(void* p, int type, long long i, int count, const float* x) {
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+        if (k < count) store(p, type, i + k, x[k]);
+}
+
+// Four values from i on, those of them that `left` allows (8 or 16 bytes at once where all do).
+__device__ __forceinline__ void load4(const void* p, int type, long long i, int left, float* x) {
+    if (left >= 4) {
+        if (type == OZ_F32) {
+            const f32x4 a = get16<f32x4>(static_cast<const float*>(p) + i);
+#pragma unroll
+            for (int k = 0; k < 4; k++) x[k] = a[k];
+        } else {
+            union {
+                u32x2 w;
+                __bf16 b[4];
+                _Float16 h[4];
+            } u;
+            __builtin_memcpy(&u, __builtin_assume_aligned(static_cast<const uint16_t*>(p) + i, 2), 8);
+#pragma unroll
+            for (int k = 0; k < 4; k++) x[k] = type == OZ_BF16 ? (float)u.b[k] : (float)u.h[k];
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++) x[k] = k < left ? load(p, type, i + k) : 0.0f;
+    }
+}
+__device__ __forceinline__ void store4(void* p, int type, long long i, int left, const float* x) {
+    if (left >= 4) {
+        if (type == OZ_F32) {
+            put16(static_cast<float*>(p) + i, f32x4{x[0], x[1], x[2], x[3]});
+        } else {
+            union {
+                u32x2 w;
+                __bf16 b[4];
+                _Float16 h[4];
+            } u;
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if (type == OZ_BF16) u.b[k] = (__bf16)x[k];
+                else u.h[k] = (_Float16)x[k];
+            }
+            __builtin_memcpy(__builtin_assume_aligned(static_cast<uint16_t*>(p) + i, 2), &u, 8);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (k < left) store(p, type, i + k, x[k]);
     }
 }
 

@@ -83,10 +83,11 @@ def gradient(dev, kind, T, vocab, D, t="bf16", dw="f32", bits=32, scale=0.3, acc
     torch.cuda.synchronize()
     dev.embedding_grad(d, Ptr(dout), Ptr(ids), Ptr(table), Ptr(flags), Ptr(work), n)
     dev.sync()
-    keep = ids.long() != padding
-    idx, x = ids.long()[keep], dout.double()[keep]
-    count = torch.zeros((vocab, 1), dtype=torch.float64, device="cuda:0").index_add_(0, idx, torch.ones((len(idx), 1), dtype=torch.float64, device="cuda:0"))
-    add = lambda v: torch.zeros((vocab, D), dtype=torch.float64, device="cuda:0").index_add_(0, idx, v)  # noqa: E731
+    # the sums on the host: added up on the GPU, a million values of one row wait for each other
+    keep = (ids.long() != padding).cpu()
+    idx, x = ids.long().cpu()[keep], dout.double().cpu()[keep]
+    count = torch.bincount(idx, minlength=vocab).double()[:, None].cuda()
+    add = lambda v: torch.zeros((vocab, D), dtype=torch.float64).index_add_(0, idx, v).cuda()  # noqa: E731
     s = float(torch.tensor(scale))
     want, size = s * add(x), s * add(x.abs())
     bound = (count + 2) * U32 * size
@@ -104,7 +105,8 @@ def gradient(dev, kind, T, vocab, D, t="bf16", dw="f32", bits=32, scale=0.3, acc
 # from no token to lists longer than a tile, and vocabularies of one to three digits
 @pytest.mark.parametrize("kind", ["random", "same", "frequent", "sorted"])
 @pytest.mark.parametrize("T,vocab,D", [(0, 6, 8), (1, 1, 1), (2, 70, 520), (31, 9, 64), (32, 40, 7), (33, 400, 8), (65, 600, 1032),
-                                       (700, 70, 500), (4095, 511, 64), (4097, 513, 72), (9000, 3000, 136), (40000, 300000, 8)])
+                                       (700, 70, 500), (4095, 511, 64), (4097, 513, 72), (9000, 3000, 136), (40000, 300000, 8),
+                                       (70000, 1 << 17, 16), (1100000, 70000, 8)])
 def test_gradient(dev, kind, T, vocab, D):
     print("embedding_grad", kind, T, vocab, D, flush=True)
     gradient(dev, kind, T, vocab, D)
