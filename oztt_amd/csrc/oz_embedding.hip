@@ -26,18 +26,17 @@ __device__ __forceinline__ long long token(const void* ids, int wide, long long 
     return wide ? static_cast<const long long*>(ids)[t] : static_cast<const int*>(ids)[t];
 }
 
-// Eight columns of a lane among a wave's 512: two pieces of four, c0 + 4 lane + k and c0 + 256 + 4 lane + k, those below D, so that
-// FP32 rows too move in runs of 16 bytes a lane.
+// Eight columns of a lane, c + k, those below D.
 struct Columns {
-    int c, left;  // the first piece's column; columns from it on
-    __device__ Columns(int c0, int lane, int D) : c(c0 + 4 * lane), left(D - (c0 + 4 * lane)) {}
+    int c, count;
+    __device__ Columns(int c0, int lane, int D) : c(c0 + 8 * lane), count(D - (c0 + 8 * lane)) {}
     __device__ void get(const void* p, int type, long long row, float* x) const {
-        load4(p, type, row + c, left, x);
-        load4(p, type, row + c + 256, left - 256, x + 4);
+        if (count >= 8) load8(p, type, row + c, x);
+        else if (count > 0) load_some(p, type, row + c, count, x);
     }
     __device__ void put(void* p, int type, long long row, const float* x) const {
-        store4(p, type, row + c, left, x);
-        store4(p, type, row + c + 256, left - 256, x + 4);
+        if (count >= 8) store8(p, type, row + c, x);
+        else if (count > 0) store_some(p, type, row + c, count, x);
     }
     // the table's row v from its sum
     __device__ void finish(void* table, const Shape& s, long long v, float* x) const {
@@ -46,6 +45,57 @@ struct Columns {
 #pragma unroll
         for (int k = 0; k < 8; k++) x[k] = s.accumulate ? old[k] + x[k] * s.scale : x[k] * s.scale;
         put(table, s.grad_type, v * s.ldt, x);
+    }
+};
+
+// The same columns of rows that are asked for ahead: the bytes stay as they came until they are used, and no lane's request
+// depends on a branch, so that several rows are on their way at once (with branches the compiler waits for each row where they
+// meet, and 2.2 TB/s are read). A lane with fewer than 8 columns left asks for the row's last 8 and
+// takes its own from them. SMALL: rows of fewer than 8 values, one by one.
+template <int TYPE, bool SMALL>
+struct Ahead {
+    static constexpr int WORDS = TYPE == OZ_F32 ? 8 : 4;
+    typedef u32x4 Raw[WORDS / 4];
+    int c, shift, D;
+    __device__ Ahead(const Columns& cols, int D) : D(D) {
+        c = SMALL || cols.count >= 8 ? cols.c : D - 8;
+        shift = cols.count > 0 ? cols.c - c : 0;
+    }
+    __device__ void ask(const void* p, long long row, Raw& w) const {
+        if constexpr (SMALL) {
+            float x[8] = {};
+            if (c == 0) load_some(p, TYPE, row, D, x);
+            if constexpr (WORDS == 8) __builtin_memcpy(&w, x, 32);
+            else narrow8(x, w[0]);
+        } else {
+            const char* from = static_cast<const char*>(p) + (row + c) * (WORDS / 2);
+#pragma unroll
+            for (int k = 0; k < WORDS / 4; k++) w[k] = get16<u32x4>(from + 16 * k);
+        }
+    }
+    __device__ void take(const Raw& w, float* x) const {
+        if constexpr (WORDS == 8) {
+#pragma unroll
+            for (int k = 0; k < 8; k++) x[k] = __uint_as_float(w[k / 4][k & 3]);
+        } else {
+            widen8(w[0], TYPE, x);
+        }
+        for (int n = 0; n < shift; n++)
+#pragma unroll
+            for (int k = 0; k < 7; k++) x[k] = x[k + 1];
+    }
+    __device__ static void narrow8(const float* x, u32x4& w) {
+        union {
+            u32x4 w;
+            __bf16 b[8];
+            _Float16 h[8];
+        } u;
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            if (TYPE == OZ_BF16) u.b[k] = (__bf16)x[k];
+            else u.h[k] = (_Float16)x[k];
+        }
+        w = u.w;
     }
 };
 
@@ -82,7 +132,12 @@ __device__ __forceinline__ void zero_rows(const Zeros& z, const Shape& s) {
     const u32x4 none = {0, 0, 0, 0};
     if (s.ldt == s.D) {
         const long long bytes = rows * row_bytes;
-        for (long long i = me; i < bytes / 16; i += stride) put16(base + 16 * i, none);
+        // past the caches, which the sums' rows need (32768 x 2048 into 65536 rows: 179 us against 167)
+        const bool even = !((uintptr_t)base & 15);
+        for (long long i = me; i < bytes / 16; i += stride) {
+            if (even) __builtin_nontemporal_store(none, reinterpret_cast<u32x4*>(base + 16 * i));
+            else put16(base + 16 * i, none);
+        }
         for (long long i = bytes / 16 * 16 + 2 * me; i < bytes; i += 2 * stride) *reinterpret_cast<uint16_t*>(base + i) = 0;
     } else {
         const long long across = (row_bytes + 15) / 16;
@@ -252,8 +307,9 @@ __global__ void __launch_bounds__(SORT_THREADS) scatter_kernel(const void* __res
 }
 
 // ---- sums ---------------------------------------------------------------------------------------------
-// A wave sums run r of R <= 64 sorted entries, 512 columns, 8 rows asked for at a time. Sums of tokens that the run's beginning
+// A wave sums run r of R <= 64 sorted entries, 512 columns, the next 8 rows on their way while 8 are added. Sums of tokens that the run's beginning
 // cuts go to parts[2 r], of those that its end cuts to parts[2 r + 1] (a token that fills the run: parts[2 r]).
+template <int TYPE, bool SMALL>
 __global__ void __launch_bounds__(256) sums_kernel(const void* __restrict__ dOut, const uint32_t* __restrict__ keys,
                                                    const uint32_t* __restrict__ order, void* __restrict__ table,
                                                    float* __restrict__ parts, Shape s, int R, unsigned slices) {
@@ -269,21 +325,28 @@ __global__ void __launch_bounds__(256) sums_kernel(const void* __restrict__ dOut
     const uint32_t after = end < s.T ? keys[end] : none, before = begin > 0 ? keys[begin - 1] : none;
     bool cut = before == (uint32_t)__builtin_amdgcn_readfirstlane(mine);
     float sum[8] = {};
-    for (int i0 = 0; i0 < n; i0 += 8) {
-        float x[8][8];
+    typedef Ahead<TYPE, SMALL> A;
+    const A rows(cols, s.D);
+    typename A::Raw w[2][8];
+    auto ask = [&](int i0, typename A::Raw (&to)[8]) {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int i = i0 + j < n ? i0 + j : n - 1;
-            cols.get(dOut, s.type, (long long)(uint32_t)__builtin_amdgcn_readlane(place, i) * s.ldo, x[j]);
+            rows.ask(dOut, (long long)(uint32_t)__builtin_amdgcn_readlane(place, i) * s.ldo, to[j]);
         }
+    };
+    // false: the tokens without a gradient are reached, the last ones
+    auto add = [&](int i0, const typename A::Raw (&from)[8]) -> bool {
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int i = i0 + j;
             if (i >= n) break;
             const uint32_t key = __builtin_amdgcn_readlane(mine, i);
-            if (key == none) return;  // they are the last
+            if (key == none) return false;
+            float x[8];
+            rows.take(from[j], x);
 #pragma unroll
-            for (int k = 0; k < 8; k++) sum[k] += x[j][k];
+            for (int k = 0; k < 8; k++) sum[k] += x[k];
             const uint32_t next = i + 1 < n ? (uint32_t)__builtin_amdgcn_readlane(mine, i + 1) : after;
             if (next == key && i + 1 < n) continue;
             if (cut) cols.put(parts, OZ_F32, 2 * r * s.D, sum);
@@ -293,10 +356,20 @@ __global__ void __launch_bounds__(256) sums_kernel(const void* __restrict__ dOut
 #pragma unroll
             for (int k = 0; k < 8; k++) sum[k] = 0.0f;
         }
+        return true;
+    };
+    ask(0, w[0]);
+    for (int i0 = 0; i0 < n; i0 += 16) {
+        if (i0 + 8 < n) ask(i0 + 8, w[1]);
+        if (!add(i0, w[0])) return;
+        if (i0 + 8 >= n) return;
+        if (i0 + 16 < n) ask(i0 + 16, w[0]);
+        if (!add(i0 + 8, w[1])) return;
     }
 }
 
 // Joins the sums of a token that run r's end cuts and that begins in run r, in the runs' order, 8 asked for at a time.
+template <bool SMALL>
 __global__ void __launch_bounds__(256) join_kernel(const uint32_t* __restrict__ keys, void* __restrict__ table,
                                                    const float* __restrict__ parts, Shape s, int R, unsigned slices) {
     const int lane = threadIdx.x & 63;
@@ -308,20 +381,25 @@ __global__ void __launch_bounds__(256) join_kernel(const uint32_t* __restrict__ 
     const Columns cols((int)(item - r * slices) * 512, lane, s.D);
     float sum[8] = {};
     cols.get(parts, OZ_F32, (2 * r + 1) * s.D, sum);
+    typedef Ahead<OZ_F32, SMALL> A;
+    const A rows(cols, s.D);
     for (long long q = r + 1;; q += 64) {
         // how many of the next 64 runs begin with the token
         const bool on = (q + lane) * R < s.T && keys[(q + lane) * R] == key;
         const uint64_t off = ~__ballot(on);
         const int m = off ? __ffsll((unsigned long long)off) - 1 : 64;
         for (int i0 = 0; i0 < m; i0 += 8) {
-            float x[8][8];
+            typename A::Raw w[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) cols.get(parts, OZ_F32, 2 * (q + (i0 + j < m ? i0 + j : m - 1)) * s.D, x[j]);
+            for (int j = 0; j < 8; j++) rows.ask(parts, 2 * (q + (i0 + j < m ? i0 + j : m - 1)) * s.D, w[j]);
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                if (i0 + j < m)
+                if (i0 + j < m) {
+                    float x[8];
+                    rows.take(w[j], x);
 #pragma unroll
-                    for (int k = 0; k < 8; k++) sum[k] += x[j][k];
+                    for (int k = 0; k < 8; k++) sum[k] += x[k];
+                }
         }
         if (m < 64) break;
     }
@@ -359,8 +437,10 @@ Work work_of(const oz_embedding_desc* d) {
     const auto up = [](size_t n) { return (n + 255) & ~(size_t)255; };
     w.items = d->T <= 64 * SORT_THREADS ? 1 : 4;  // 64 tiles' counts cost a workgroup 2 us
     w.tiles = (d->T + w.items * SORT_THREADS - 1) / (w.items * SORT_THREADS);
-    // runs of 32, of 8 where those are too few to fill the chip
-    w.R = d->T * ((d->D + 511) / 512) <= 1 << 15 ? 8 : 32;
+    // runs of 32 entries, shorter where those would leave most of the chip idle: 512 tokens of 500 values 28 us by 8, 47 by 32;
+    // 8192 of 1024 68 by 16, 73 by 32; 18651 of 134 50 by 32, 108 by 8 (more cut sums to join)
+    const long long waves = d->T * ((d->D + 511) / 512);
+    w.R = waves <= 1 << 11 ? 8 : waves <= 1 << 14 ? 16 : 32;
     w.runs = (d->T + w.R - 1) / w.R;
     w.list = up(4 * d->T);
     w.counts = up(4 * DIGITS * w.tiles);
@@ -449,8 +529,12 @@ int oz_embedding_grad(oz_dev* dev, const oz_embedding_desc* d, const void* dOut,
                                     : sort<4>(dev, ids, dTable, s, w, keys, order, counts, flags, zeros);
     if (int st = oz::launch_check(dev, "sort")) return st;
     const dim3 block(256);
-    hipLaunchKernelGGL(sums_kernel, dim3((unsigned)groups), block, 0, q, dOut, keys[sorted], order[sorted], dTable, parts, s, w.R, slices);
-    hipLaunchKernelGGL(join_kernel, dim3((unsigned)groups), block, 0, q, keys[sorted], dTable, parts, s, w.R, slices);
+    const bool small = s.D < 8;
+    const auto sums = s.type == OZ_F32 ? (small ? sums_kernel<OZ_F32, true> : sums_kernel<OZ_F32, false>)
+                      : s.type == OZ_F16 ? (small ? sums_kernel<OZ_F16, true> : sums_kernel<OZ_F16, false>)
+                                         : (small ? sums_kernel<OZ_BF16, true> : sums_kernel<OZ_BF16, false>);
+    hipLaunchKernelGGL(sums, dim3((unsigned)groups), block, 0, q, dOut, keys[sorted], order[sorted], dTable, parts, s, w.R, slices);
+    hipLaunchKernelGGL(small ? join_kernel<true> : join_kernel<false>, dim3((unsigned)groups), block, 0, q, keys[sorted], dTable, parts, s, w.R, slices);
     return oz::launch_check(dev, "embedding gradient");
 }
 

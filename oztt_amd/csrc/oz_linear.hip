@@ -77,15 +77,16 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const void* __restrict__ 
                                                        long long lddy, long long ldz, long long lddz, int rows, int strips) {
     constexpr int COLS = 8 * LANES, R = 256 / LANES;
     const int strip = blockIdx.x % strips, chunk = blockIdx.x / strips, l = threadIdx.x % LANES, r = threadIdx.x / LANES;
-    const int col = strip * COLS + 8 * l;
+    // a row's last, fewer than 8 values: its last 8, of which the lane beside has the first `twice` too and writes the same
+    const int at = strip * COLS + 8 * l, col = at + 8 <= N || N < 8 ? at : N - 8, twice = at - col;
     const long long end = (long long)(chunk + 1) * rows < M ? (long long)(chunk + 1) * rows : M;
     float sum[8] = {};
-    if (col < N) {
+    if (at < N) {
         auto rows_of = [&](auto WHOLE) {
             constexpr bool whole = decltype(WHOLE)::value;
-            auto get = [&](const void* p, long long at, float* x) {
-                if constexpr (whole) load8(p, type, at, x);
-                else load_some(p, type, at, N - col, x);
+            auto get = [&](const void* p, long long i, float* x) {
+                if constexpr (whole) load8(p, type, i, x);
+                else load_some(p, type, i, N, x);
             };
 #pragma unroll 4
             for (long long m = (long long)chunk * rows + r; m < end; m += R) {
@@ -101,13 +102,14 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const void* __restrict__ 
                 for (int k = 0; k < 8; k++) sum[k] += x[k];
             }
         };
-        if (col + 8 <= N) rows_of(std::true_type{});
+        if (N >= 8) rows_of(std::true_type{});
         else rows_of(std::false_type{});
     }
     if (!parts && !dbias) return;
     __shared__ float part[R][COLS];
 #pragma unroll
-    for (int k = 0; k < 8; k++) part[r][8 * l + k] = sum[k];
+    for (int k = 0; k < 8; k++)
+        if (k >= twice) part[r][8 * l + k - twice] = sum[k];
     __syncthreads();
     // R rows of sums to one, halving
     for (int h = R / 2; h > 0; h /= 2) {

@@ -33,7 +33,6 @@ typedef __attribute__((address_space(3))) uint8_t lds_u8;
 
 constexpr int BC = 64;                       // c of a stage, two steps of 32
 constexpr unsigned OUTSIDE = 0x80000000u;    // an offset beyond every range
-constexpr long long RANGE = 0x7FFFFFF0ll;    // the largest range
 
 // Copies 16 bytes a lane from buffer rs at offset voff to LDS byte lbase + 16 lane. M0 carries the LDS base;
 // the wait state between its write and the copy is the s_nop.
@@ -50,12 +49,12 @@ struct Operand {
     static_assert(N * W == BLOCKS, "whole blocks per wave");
     static constexpr int RB = 2 * ROWS;       // MAJOR: bytes of a row of c
     static constexpr int PIECES = RB / 32;    // 32-byte pieces of it
-    v4i rs;              // buffer of the stage to load next
-    long long left;      // bytes from its address to the operand's end
-    unsigned step;       // bytes of a stage's advance
-    unsigned off[N];     // of this lane's copies
-    unsigned dead, last; // !MAJOR: OUTSIDE for a lane whose chunk is beyond C, in the stage to load and in the last one
-    int steps;           // stages left to load
+    v4i rs;          // buffer of the stage to load next: its address, and what of the operand lies from there on (of this stage)
+    unsigned range;  // !MAJOR: from its address to the end of the tile's last row; MAJOR: of a whole stage
+    unsigned last;   // MAJOR: of the last stage
+    unsigned step;   // bytes of a stage's advance
+    unsigned off[N]; // of this lane's copies
+    int steps;       // stages left to load
 
     // a row's swizzle in 32-byte pieces: rows 8 g + j and 8 g + 4 + j (j < 4) of g and g + 1 differ
     __device__ static int piece_swizzle(int row) { return ((row & 3) | ((row >> 3) & 1) << 2) & (PIECES - 1); }
@@ -67,8 +66,10 @@ struct Operand {
         unsigned long long base;
         if constexpr (MAJOR) {
             base = (unsigned long long)p + c0 * ldb + 2 * row0;
-            left = (C - 1 - c0) * ldb + ((2 * (n - row0) + 3) & ~3ll);
             step = (unsigned)(BC * ldb);
+            const long long end = C - c0 - (long long)BC * (stages - 1);  // rows of the last stage
+            range = (unsigned)(BC * ldb);
+            last = (unsigned)((end < BC ? end - 1 : BC - 1) * ldb + ((2 * (n - row0) + 3) & ~3ll));
 #pragma unroll
             for (int j = 0; j < N; j++) {
                 const int byte = 1024 * (W * j + wave) + 16 * lane, row = byte / RB;
@@ -77,44 +78,50 @@ struct Operand {
             }
         } else {
             base = (unsigned long long)p + row0 * ldb + 2 * c0;
-            left = (n - 1 - row0) * ldb + ((2 * (C - c0) + 3) & ~3ll);
             step = 2 * BC;
+            range = (unsigned)(((n - row0 < ROWS ? n - row0 : ROWS) - 1) * ldb + ((2 * (C - c0) + 3) & ~3ll));
+            last = 0;
             const int r = lane >> 3, chunk = (lane & 7) ^ r;
 #pragma unroll
             for (int j = 0; j < N; j++) {
                 const int row = 8 * (W * j + wave) + r;
                 off[j] = row0 + row < n ? (unsigned)(row * ldb + 16 * chunk) : OUTSIDE;
             }
-            last = c0 + (long long)BC * (stages - 1) + 8 * chunk >= C ? OUTSIDE : 0u;
         }
         rs[0] = __builtin_amdgcn_readfirstlane((int)base);
         rs[1] = __builtin_amdgcn_readfirstlane((int)(base >> 32) & 0xFFFF);
         rs[3] = 0x00020000;
-        range();
+        range = __builtin_amdgcn_readfirstlane(range);
+        last = __builtin_amdgcn_readfirstlane(last);
+        step = __builtin_amdgcn_readfirstlane(step);
+        limit();
     }
-    // What of the stage to load next lies in the operand and the range of c.
-    __device__ __forceinline__ void range() {
-        rs[2] = __builtin_amdgcn_readfirstlane((int)(left < 0 || steps <= 0 ? 0 : left < RANGE ? left : RANGE));
-        if constexpr (!MAJOR) dead = steps == 1 ? last : 0u;
+    // A few scalar instructions a stage: whatever more there was showed (85 cycles a stage, 2% of 8192^3, 15% of small
+    // products, for 64-bit ranges and a mask of the last chunks).
+    __device__ __forceinline__ void limit() {
+        if constexpr (MAJOR) rs[2] = steps > 1 ? range : steps == 1 ? last : 0u;
+        else rs[2] = steps > 0 ? range : 0u;
     }
-    __device__ __forceinline__ void copy(uint8_t* stage, int j, int wave) const {
-        lds_copy(rs, stage + 1024 * (W * j + wave), MAJOR ? off[j] : off[j] | dead);
-    }
+    __device__ __forceinline__ void copy(uint8_t* stage, int j, int wave) const { lds_copy(rs, stage + 1024 * (W * j + wave), off[j]); }
     __device__ __forceinline__ void next() {
         steps--;
         const unsigned long long base = ((unsigned long long)(unsigned)rs[1] << 32 | (unsigned)rs[0]) + step;
         rs[0] = (int)base;
         rs[1] = (int)(base >> 32);
-        left -= step;
-        range();
+        if constexpr (!MAJOR) range -= step;
+        limit();
     }
 
-    // Zeros for what lies behind the `valid` last values of c in a stage's 16-byte chunks (rows of c are left out whole).
+    // Zeros for what lies behind the `valid` last values of c in a stage: there stand a window's other columns or the next
+    // row (rows of c beyond the last are zeros).
     __device__ static void zero_tail(uint8_t* stage, int valid, int thread) {
         if constexpr (!MAJOR) {
+            const v4i none = {0, 0, 0, 0};
             for (int row = thread; row < ROWS; row += 64 * W) {
-                uint16_t* chunk = reinterpret_cast<uint16_t*>(stage + 128 * row + 16 * ((valid >> 3) ^ (row & 7)));
-                for (int e = valid & 7; e < 8; e++) chunk[e] = 0;
+                uint8_t* at = stage + 128 * row;
+                uint16_t* cut = reinterpret_cast<uint16_t*>(at + 16 * ((valid >> 3) ^ (row & 7)));
+                for (int e = valid & 7; e < 8; e++) cut[e] = 0;
+                for (int c = (valid >> 3) + 1; c < 8; c++) *reinterpret_cast<v4i*>(at + 16 * (c ^ (row & 7))) = none;
             }
         }
     }
@@ -213,13 +220,16 @@ __device__ __forceinline__ void put_sums(const Product& a, const f32x4 (&acc)[TI
         });
         return;
     }
-    const bool in = p + 8 <= a.np;  // all 8 values
+    // A row's last, fewer than 8 values: the lane takes the row's last 8 instead, of which its neighbour has the first ones too
+    // and writes the same. (Only where fewer than 8 are left for the wave are they written one by one.)
+    const long long pl = p + 8 <= a.np || a.np - 8 < p0 ? p : a.np - 8;
+    const bool in = p < a.np && pl + 8 <= a.np;
     float bias[8] = {};
-    if (e.bias && in) load8(e.bias, TYPE, p, bias);
+    if (e.bias && in) load8(e.bias, TYPE, pl, bias);
     const int wide = e.y_type == OZ_F32;
-    const char* pr = static_cast<const char*>(e.residual) + ((q0 + rr) * e.ldr + p) * (wide ? 4 : 2);
-    char* py = static_cast<char*>(e.Y) + ((q0 + rr) * e.ldy + p) * (wide ? 4 : 2);
-    char* pz = static_cast<char*>(e.Z) + ((q0 + rr) * e.ldz + p) * 2;
+    const char* pr = static_cast<const char*>(e.residual) + ((q0 + rr) * e.ldr + pl) * (wide ? 4 : 2);
+    char* py = static_cast<char*>(e.Y) + ((q0 + rr) * e.ldy + pl) * (wide ? 4 : 2);
+    char* pz = static_cast<char*>(e.Z) + ((q0 + rr) * e.ldz + pl) * 2;
     const long long dr = RT * e.ldr * (wide ? 4 : 2), dy = RT * e.ldy * (wide ? 4 : 2), dz = RT * e.ldz * 2;
     u32x4 res[2][BATCH][2] = {};
     auto ask = [&](auto B) {  // batch B of all TI / RI * BATCHES
@@ -245,7 +255,13 @@ __device__ __forceinline__ void put_sums(const Product& a, const f32x4 (&acc)[TI
                 const int turn = c * BATCH + t;
                 if (!in || q0 + (h * NT + turn) * RT + rr >= a.nq) continue;
                 float v[8];
-                read(RT * turn + rr, v);
+                if (pl == p) {
+                    read(RT * turn + rr, v);
+                } else {
+                    const int row = RT * turn + rr, col = (int)(pl - p0);
+#pragma unroll
+                    for (int k = 0; k < 8; k++) v[k] = tile[row * ROW + 4 * (((col + k) >> 2) ^ (row & XM)) + ((col + k) & 3)];
+                }
 #pragma unroll
                 for (int k = 0; k < 8; k++) v[k] += bias[k];
                 if (e.Z) store8(pz + (h * NT + turn) * dz, TYPE, 0, v);
@@ -266,7 +282,7 @@ __device__ __forceinline__ void put_sums(const Product& a, const f32x4 (&acc)[TI
                 store8(py + (h * NT + turn) * dy, e.y_type, 0, v);
             }
         });
-        if (!in && p < a.np) {  // the row's last, fewer than 8 values
+        if (!in && p < a.np) {
 #pragma unroll 1
             for (int turn = 0; turn < NT; turn++) {
                 const long long q = q0 + (h * NT + turn) * RT + rr;
@@ -278,9 +294,9 @@ __device__ __forceinline__ void put_sums(const Product& a, const f32x4 (&acc)[TI
     });
 }
 
-// The values of c in the last stage where they do not fill its chunks, else 0 (of the last range only).
+// The values of c in the last stage where they do not fill it, else 0 (of the last range only).
 __device__ __forceinline__ int ragged_tail(const Product& a, int split) {
-    return split == a.splits - 1 && a.C % 8 ? (int)(a.C % BC) : 0;
+    return split == a.splits - 1 ? (int)(a.C % BC) : 0;
 }
 
 // WQ x WP waves of 16 TI x 16 TJ outputs each; a ring of NSTG stages, one barrier a stage. The fragments of the next
@@ -326,7 +342,7 @@ __global__ void __launch_bounds__(64 * WQ * WP, NSTG * 16 * BC * 2 * (TI * WQ + 
     auto landed = [&](auto LEFT, int k, uint8_t* at) {
         wait_vmcnt_lgkm0<LD * decltype(LEFT)::value>();
         stage_barrier();
-        if (tail && k == nst - 1) {
+        if (!(QM && PM) && tail && k == nst - 1) {
             OQ::zero_tail(at, tail, threadIdx.x);
             OP::zero_tail(at + STG_Q, tail, threadIdx.x);
             wait_vmcnt_lgkm0<LD * decltype(LEFT)::value>();
@@ -416,7 +432,7 @@ __global__ void __launch_bounds__(256) product_big_kernel(const Product a, int t
     auto landed = [&](auto LEFT, int k, int uq, int up) {  // stage k, whose units are at uq and up
         wait_vmcnt_lgkm0<decltype(LEFT)::value>();
         stage_barrier();
-        if (tail && k == nst - 1) {
+        if (!(QM && PM) && tail && k == nst - 1) {
             OQ::zero_tail(lds + uq, tail, threadIdx.x);
             OP::zero_tail(lds + up, tail, threadIdx.x);
             wait_vmcnt_lgkm0<decltype(LEFT)::value>();

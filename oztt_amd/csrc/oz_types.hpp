@@ -114,52 +114,6 @@ __device__ __forceinline__ void store_some(void* p, int type, long long i, int c
         if (k < count) store(p, type, i + k, x[k]);
 }
 
-// Four values from i on, those of them that `left` allows (8 or 16 bytes at once where all do).
-__device__ __forceinline__ void load4(const void* p, int type, long long i, int left, float* x) {
-    if (left >= 4) {
-        if (type == OZ_F32) {
-            const f32x4 a = get16<f32x4>(static_cast<const float*>(p) + i);
-#pragma unroll
-            for (int k = 0; k < 4; k++) x[k] = a[k];
-        } else {
-            union {
-                u32x2 w;
-                __bf16 b[4];
-                _Float16 h[4];
-            } u;
-            __builtin_memcpy(&u, __builtin_assume_aligned(static_cast<const uint16_t*>(p) + i, 2), 8);
-#pragma unroll
-            for (int k = 0; k < 4; k++) x[k] = type == OZ_BF16 ? (float)u.b[k] : (float)u.h[k];
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; k++) x[k] = k < left ? load(p, type, i + k) : 0.0f;
-    }
-}
-__device__ __forceinline__ void store4(void* p, int type, long long i, int left, const float* x) {
-    if (left >= 4) {
-        if (type == OZ_F32) {
-            put16(static_cast<float*>(p) + i, f32x4{x[0], x[1], x[2], x[3]});
-        } else {
-            union {
-                u32x2 w;
-                __bf16 b[4];
-                _Float16 h[4];
-            } u;
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                if (type == OZ_BF16) u.b[k] = (__bf16)x[k];
-                else u.h[k] = (_Float16)x[k];
-            }
-            __builtin_memcpy(__builtin_assume_aligned(static_cast<uint16_t*>(p) + i, 2), &u, 8);
-        }
-    } else {
-#pragma unroll
-        for (int k = 0; k < 4; k++)
-            if (k < left) store(p, type, i + k, x[k]);
-    }
-}
-
 // Activations. GELU in its tanh form is z / (1 + exp(-2u)), u = sqrt(2/pi) (z + 0.044715 z^3), since
 // (1 + tanh u)/2 = 1/(1 + exp(-2u)); an overflow of z^3 or of the exponential gives the limits z and -0.
 // The exponential and the reciprocal are the hardware's (a few units in the last place of FP32).
