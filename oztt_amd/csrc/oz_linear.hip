@@ -213,7 +213,7 @@ Route route_of(int cus, long long nq, long long np, long long C, bool contiguous
     if (contiguous && (nq <= kFewRows || (!aligned && nq <= 64))) {
         r.few = true;
         const long long groups = (np + few_rows_block(nq) - 1) / few_rows_block(nq);
-        while (r.splits < 8 && groups * r.splits * 4 <= cus && C / (r.splits * 2) >= 2048) r.splits *= 2;
+        while (nq > kStreamRows && r.splits < 8 && groups * r.splits * 4 <= cus && C / (r.splits * 2) >= 2048) r.splits *= 2;
     } else {
         float best = 0.0f;
         for (int t = 0; t < TILES; t++)
