@@ -70,10 +70,10 @@ __global__ void __launch_bounds__(256) product_any_kernel(const ozl::Product a) 
 // dZ = dY act'(Z), rounded for the products (left out where dz is null), and the sums of its columns over `rows` rows each,
 // to dbias if one range holds all rows, else to parts (left out where both are null): 8 columns a lane, 8 LANES columns by
 // 256 / LANES rows at a time by a workgroup. One pass over dY and Z, which are not read again and pass the caches by.
-template <int LANES>
+template <int LANES, int ACT>
 __global__ void __launch_bounds__(256) act_grad_kernel(const void* __restrict__ dY, const void* __restrict__ Z,
                                                        void* __restrict__ dz, float* __restrict__ parts, void* __restrict__ dbias,
-                                                       int type, int dw_type, int act, int accumulate, long long M, int N,
+                                                       int type, int dw_type, int accumulate, long long M, int N,
                                                        long long lddy, long long ldz, long long lddz, int rows, int strips) {
     constexpr int COLS = 8 * LANES, R = 256 / LANES;
     const int strip = blockIdx.x % strips, chunk = blockIdx.x / strips, l = threadIdx.x % LANES, r = threadIdx.x / LANES;
@@ -92,10 +92,10 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const void* __restrict__ 
             for (long long m = (long long)chunk * rows + r; m < end; m += R) {
                 float x[8], y[8];
                 get(dY, m * lddy + col, x);
-                if (act != OZ_ACT_NONE) {
+                if constexpr (ACT != OZ_ACT_NONE) {
                     get(Z, m * ldz + col, y);
 #pragma unroll
-                    for (int k = 0; k < 8; k++) x[k] *= act_grad(y[k], act);
+                    for (int k = 0; k < 8; k++) x[k] *= act_grad(y[k], ACT);
                 }
                 if (dz) store8(dz, type, m * lddz + col, x);
 #pragma unroll
@@ -126,6 +126,14 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const void* __restrict__ 
             parts[(long long)chunk * N + c] = s;
         }
     }
+}
+
+template <int LANES>
+auto act_grad_of(int act) {
+    return act == OZ_ACT_GELU   ? act_grad_kernel<LANES, OZ_ACT_GELU>
+           : act == OZ_ACT_SILU ? act_grad_kernel<LANES, OZ_ACT_SILU>
+           : act == OZ_ACT_RELU ? act_grad_kernel<LANES, OZ_ACT_RELU>
+                                : act_grad_kernel<LANES, OZ_ACT_NONE>;
 }
 
 // dbias from the chunks' sums, 16 chunks at a time by 16 lanes: lane k of a column sums chunks k, k + 16, ..., then the lanes.
@@ -412,9 +420,9 @@ int oz_linear_grad(oz_dev* dev, const oz_linear_grad_desc* d, const void* dY, co
         const bool one = chunks == 1;
         if (chunks) {
             const dim3 grid((unsigned)(strips * chunks));
-            const auto kernel = w.lanes == 8 ? act_grad_kernel<8> : act_grad_kernel<32>;
+            const auto kernel = w.lanes == 8 ? act_grad_of<8>(d->act) : act_grad_of<32>(d->act);
             hipLaunchKernelGGL(kernel, grid, dim3(256), 0, dev->stream, dY, Z, make, one ? nullptr : sums, one ? dbias : nullptr,
-                               d->type, d->dw_type, d->act, d->accumulate, (long long)d->M, d->N, lddy, ldz, w.lddz, w.rows, strips);
+                               d->type, d->dw_type, d->accumulate, (long long)d->M, d->N, lddy, ldz, w.lddz, w.rows, strips);
             if (int st = oz::launch_check(dev, "act_grad_kernel")) return st;
         }
         if (dbias && !one) {

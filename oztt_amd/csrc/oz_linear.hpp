@@ -59,9 +59,7 @@ __device__ __forceinline__ void finish8(const Epilogue& e, long long np, long lo
         if (count == 8) ozt::store8(e.Z, TYPE, q * e.ldz + p, v);
         else ozt::store_some(e.Z, TYPE, q * e.ldz + p, count, v);
     }
-    if (e.act != OZ_ACT_NONE)
-#pragma unroll
-        for (int k = 0; k < 8; k++) v[k] = ozt::act(v[k], e.act);
+    ozt::act8(v, e.act);
 #pragma unroll
     for (int k = 0; k < 8; k++) v[k] += r[k];
     if (count == 8) ozt::store8(e.Y, e.y_type, q * e.ldy + p, v);

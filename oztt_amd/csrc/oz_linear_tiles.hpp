@@ -265,9 +265,7 @@ __device__ __forceinline__ void put_sums(const Product& a, const f32x4 (&acc)[TI
 #pragma unroll
                 for (int k = 0; k < 8; k++) v[k] += bias[k];
                 if (e.Z) store8(pz + (h * NT + turn) * dz, TYPE, 0, v);
-                if (e.act != OZ_ACT_NONE)
-#pragma unroll
-                    for (int k = 0; k < 8; k++) v[k] = act(v[k], e.act);
+                act8(v, e.act);
                 if (e.residual) {
                     float x[8];
                     if (wide) {
