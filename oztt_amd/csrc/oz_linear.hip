@@ -199,22 +199,26 @@ struct Route {
     size_t parts;   // bytes of the ranges' sums
 };
 
-// Estimated us of a tile's launch with its c cut into `splits` ranges: whole rounds of workgroups over the CUs and the
-// last, partly filled one, and the join's launch and traffic (8 bytes an output and range at 4 TB/s).
+// Estimated us of a tile's launch with its c cut into `splits` ranges: whole rounds of workgroups over the CUs and the last,
+// partly filled one, not less than the operands take from memory (4.6 TB/s), and the join's launch and traffic (8 bytes an
+// output and range at 4 TB/s).
 float estimate(const Shape& t, int cus, long long nq, long long np, long long C, int splits) {
     const long long tiles = (nq + t.q - 1) / t.q * ((np + t.p - 1) / t.p) * splits, slots = (long long)cus * t.per_cu;
     const float stages = (float)(((C + 63) / 64 + splits - 1) / splits);
     const long long rest = tiles % slots;
     float us = (float)(tiles / slots) * (t.fixed + stages * t.full);
     if (rest) us += t.fixed + stages * (rest <= cus ? t.alone : t.full);
+    us = std::max(us, t.fixed + 2.0f * ((float)nq + (float)np) * (float)C / 4.6e6f);
     if (splits > 1) us += 3.0f + (float)splits * (float)nq * (float)np * 8.0f / 4e6f;
     return us;
 }
 
-// Few rows: their own kernel, c in ranges where the rows of W are too few to keep the CUs reading (at least 2048 values
-// a range). 1 row, 2048 of W, K = 8192: 11.5 us in one range, 10.5 in four; 512 of W, K = 8192: XXX.
-// More: the tile and ranges with the least estimate. 1000 x 704 x 1504: 9.4 us by 64 x 64, 17 by 128 x 128; 2048 x 4096 x
-// 4096: 66 by 128 x 128, 74 by 256 x 256 in two ranges, 101 by 64 x 64; 256 x 1024 x 8192: 15.5 by 64 x 64 in 4 ranges, 38 in one.
+// Few rows: their own kernels, c in ranges where 16 rows of W each are too few to keep the CUs reading (3 to 16 rows of X, at least
+// 2048 values a range). 5 rows, 512 of W, K = 8192: 8.0 us in four ranges, 9.1 in one.
+// More: the tile and ranges with the least estimate; measured against the other tiles and numbers of ranges, the choice is the
+// fastest or within 10% of it: 1000 x 704 x 1504 10.1 us by 64 x 64 (17 by 128 x 128), 2048 x 4096 x 4096 62 by 128 x 128 (70 by 256 x
+// 256 in two ranges, 98 by 64 x 64), 256 x 1024 x 8192 15.5 by 64 x 64 in 4 ranges (38 in one), 3500^3 88 by 256 x 256 (120 by 128 x
+// 128), 8192^2 of K = 512 101 by 128 x 128 (124 by 256 x 256). 256 x 8192^2 takes 70 by 64 x 64 where 256 x 256 in 8 ranges takes 61.
 Route route_of(int cus, long long nq, long long np, long long C, bool contiguous, bool aligned) {
     Route r{};
     r.splits = 1;
@@ -449,3 +453,10 @@ int oz_linear_grad(oz_dev* dev, const oz_linear_grad_desc* d, const void* dY, co
 }
 
 }  // extern "C"
+
+// The route of a product of nq x np outputs over C, for tests: -1 for the kernels of few rows, else the tile; *splits its ranges of c.
+extern "C" int oz_rule_linear_route(int cus, long long nq, long long np, long long C, int contiguous, int even, int* splits) {
+    const Route r = route_of(cus, nq, np, C, contiguous != 0, even != 0);
+    if (splits) *splits = r.splits;
+    return r.few ? -1 : (int)r.tile;
+}

@@ -74,11 +74,13 @@ struct Shape {
     float alone, full;   // us for a stage of 64 values of c: one workgroup on a CU, per_cu of them
     float fixed;         // us from the first copy to the first product, and from the last to the outputs
 };
-// Measured on 256 CUs, BF16: alone from 256 tiles of K = 512, 1024 and 2048, full from 512.
+// Fitted to times on 256 CUs in BF16: 4096^2 of K = 256 and 1024 and 8192^2 of 512 by 256 x 256 tiles (25.8, 42.8 and 124 us) and
+// by 128 x 128 (18.4, 38.5 and 101), 2048^2 of K = 512 and 2048 by 128 x 128 (10.2, 24.1; one workgroup a CU) and by 64 x 64 (13.2,
+// 28.7), 1024^3 by 64 x 64 (7.5), 64 rows of 2048^2 by 32 x 32.
 inline const Shape& shape_of(Tile t) {
     static const Shape shapes[TILES] = {
-        {256, 256, 1, 1.5f, 1.5f, 10.0f}, {128, 128, 2, 0.58f, 0.93f, 5.6f}, {64, 64, 2, 0.22f, 0.35f, 3.7f},
-        {64, 32, 2, 0.21f, 0.29f, 3.7f},  {32, 32, 2, 0.18f, 0.22f, 3.4f}};
+        {256, 256, 1, 1.42f, 1.42f, 20.0f}, {128, 128, 2, 0.58f, 0.85f, 5.8f}, {64, 64, 2, 0.21f, 0.32f, 4.0f},
+        {64, 32, 2, 0.20f, 0.28f, 3.9f},    {32, 32, 2, 0.18f, 0.22f, 3.4f}};
     return shapes[t];
 }
 int launch_tile(oz_dev* dev, int type, Tile tile, const Product& a);

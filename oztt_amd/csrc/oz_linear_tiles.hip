@@ -14,6 +14,7 @@ __global__ void __launch_bounds__(256) join_kernel(const Product a) {
     if (q >= a.nq) return;
     float v[8], x[8];
     load8(a.parts, OZ_F32, q * a.ldparts + p, v);
+#pragma unroll 8
     for (int s = 1; s < a.splits; s++) {
         load8(a.parts, OZ_F32, (s * a.nq + q) * a.ldparts + p, x);
 #pragma unroll
