@@ -189,7 +189,7 @@ bool even_rows(const void* p, long long ld) { return !((uintptr_t)p & 3) && ld %
 
 size_t up(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 
-constexpr int kFewRows = 16;
+constexpr int kFewRows = 16, kFewOddRows = 32;  // rows that begin at odd addresses: laid out for the tiles from 33 on
 
 // How a product runs, from its sizes alone.
 struct Route {
@@ -213,19 +213,19 @@ float estimate(const Shape& t, int cus, long long nq, long long np, long long C,
     return us;
 }
 
-// Few rows: their own kernels, c in ranges where 16 rows of W each are too few to keep the CUs reading (3 to 16 rows of X, at least
-// 2048 values a range). 5 rows, 512 of W, K = 8192: 8.0 us in four ranges, 9.1 in one.
+// Few rows: their own kernels, c in ranges where 16 rows of W each are too few to keep the CUs reading (at least 512 values a
+// range). 5 rows, 512 of W, K = 8192: 8.0 us in four ranges, 9.1 in one.
 // More: the tile and ranges with the least estimate; measured against the other tiles and numbers of ranges, the choice is the
 // fastest or within 10% of it: 1000 x 704 x 1504 10.1 us by 64 x 64 (17 by 128 x 128), 2048 x 4096 x 4096 62 by 128 x 128 (70 by 256 x
 // 256 in two ranges, 98 by 64 x 64), 256 x 1024 x 8192 15.5 by 64 x 64 in 4 ranges (38 in one), 3500^3 88 by 256 x 256 (120 by 128 x
 // 128), 8192^2 of K = 512 101 by 128 x 128 (124 by 256 x 256). 256 x 8192^2 takes 70 by 64 x 64 where 256 x 256 in 8 ranges takes 61.
-Route route_of(int cus, long long nq, long long np, long long C, bool contiguous, bool aligned) {
+Route route_of(int cus, long long nq, long long np, long long C, bool contiguous, bool even) {
     Route r{};
     r.splits = 1;
-    if (contiguous && (nq <= kFewRows || (!aligned && nq <= 64))) {
+    if (contiguous && (nq <= kFewRows || (!even && nq <= kFewOddRows))) {
         r.few = true;
         const long long groups = (np + few_rows_block(nq) - 1) / few_rows_block(nq);
-        while (nq > kStreamRows && r.splits < 8 && groups * r.splits * 4 <= cus && C / (r.splits * 2) >= 2048) r.splits *= 2;
+        while (nq > kStreamRows && r.splits < 16 && groups * r.splits * 4 <= cus && C / (r.splits * 2) >= 512) r.splits *= 2;
     } else {
         float best = 0.0f;
         for (int t = 0; t < TILES; t++)

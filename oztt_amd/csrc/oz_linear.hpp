@@ -84,7 +84,7 @@ inline const Shape& shape_of(Tile t) {
     return shapes[t];
 }
 int launch_tile(oz_dev* dev, int type, Tile tile, const Product& a);
-// At most 64 rows of Q, operands along c at any address; splits as in Product (1 for at most kStreamRows). A workgroup has
+// At most 32 rows of Q, operands along c at any address; splits as in Product (1 for at most kStreamRows). A workgroup has
 // few_rows_block rows of P.
 constexpr int kStreamRows = 2;
 inline int few_rows_block(long long nq) { return nq <= 16 ? 16 : 32; }

@@ -1,4 +1,4 @@
-// Products of few rows (an answering program's tokens): Y = act(X W^T + bias) + residual with M <= 64.
+// Products of few rows (an answering program's tokens): Y = act(X W^T + bias) + residual with M <= 32.
 //
 // The weights are read once and used M times, so the time is theirs: the waves stream them straight into registers, with
 // no LDS and no barrier on the way, as one operand of the matrix instructions (16 rows of W x 32 values of c; M = 1 wastes
@@ -17,7 +17,7 @@ using namespace ozt;
 constexpr int WAVES = 8;
 
 template <int TYPE, int MB, int NB>
-__global__ void __launch_bounds__(64 * WAVES, MB == 4 ? 2 : 4) few_rows_kernel(const Product a, int blocks_p) {
+__global__ void __launch_bounds__(64 * WAVES, 4) few_rows_kernel(const Product a, int blocks_p) {
     typedef typename Half<TYPE>::t T;
     typedef typename Half<TYPE>::x8 T8;
     constexpr int F = MB == 1 ? 4 : 2, UNIT = 32 * F;  // values of c that a wave takes at a time
@@ -214,7 +214,7 @@ template <int TYPE>
 int by_rows(oz_dev* dev, const Product& a) {
     if (a.nq <= kStreamRows) return a.nq == 1 ? launch_stream<TYPE, 1>(dev, a) : launch_stream<TYPE, 2>(dev, a);
     if (a.nq <= 16) return launch<TYPE, 1, 1>(dev, a);
-    return a.nq <= 32 ? launch<TYPE, 2, 2>(dev, a) : launch<TYPE, 4, 2>(dev, a);
+    return launch<TYPE, 2, 2>(dev, a);
 }
 
 }  // namespace

@@ -69,6 +69,24 @@ def test_forward_sizes(dev, size, t):
     forward(dev, *size, t=t, a="gelu")
 
 
+# the large tiles, in one range of c and in several, at sizes that fit none of them
+LARGE = [(3498, 3506, 3502), (2050, 2043, 32766), (2052, 2310, 1000), (40, 6000, 4096), (5000, 516, 520)]
+
+
+@pytest.mark.parametrize("size", LARGE, ids=str)
+def test_forward_large(dev, size):
+    print("linear", size, flush=True)
+    forward(dev, *size, t="f16", a="silu")
+    forward(dev, *size, t="bf16", a="none", y="f32", bias=False, keep=False, pad=6)
+
+
+@pytest.mark.parametrize("size", [(3498, 3506, 3502), (4100, 520, 516), (5000, 1030, 2052), (130, 2052, 4100)], ids=str)
+def test_gradient_large(dev, size):
+    print("linear_grad", size, flush=True)
+    gradients(dev, *size, t="bf16", a="gelu")
+    gradients(dev, *size, t="f16", a="none", dw="f32", pad=2, accumulate=True)
+
+
 @pytest.mark.parametrize("pad,shift", [(8, 0), (5, 0), (0, 1), (16, 8), (3, 2)])
 @pytest.mark.parametrize("size", [(1, 300, 512), (20, 304, 1000), (300, 264, 520), (520, 1030, 257)], ids=str)
 def test_forward_windows(dev, size, pad, shift):

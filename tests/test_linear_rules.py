@@ -29,9 +29,9 @@ def test_forward(size, want):
 
 
 def test_odd_rows():
-    """Operands whose rows begin at odd addresses: up to 64 rows by the kernel that reads them in place, more laid out first."""
-    assert route(17, 1000, 999, even=0)[0] == FEW and route(64, 1000, 999, even=0)[0] == FEW
-    assert route(65, 1000, 999, even=0)[0] != FEW
+    """Operands whose rows begin at odd addresses: up to 32 rows by the kernel that reads them in place, more laid out first."""
+    assert route(17, 1000, 999, even=0)[0] == FEW and route(32, 1000, 999, even=0)[0] == FEW
+    assert route(33, 1000, 999, even=0)[0] != FEW
     # gradients' operands run along their own index: always tiles
     assert route(1, 1000, 999, contiguous=0)[0] != FEW
 
