@@ -362,9 +362,9 @@ enum oz_act { OZ_ACT_NONE = 0, OZ_ACT_RELU = 1, OZ_ACT_GELU = 2, OZ_ACT_SILU = 3
  * products on the BF16 or FP16 matrix cores, sums in FP32, each output rounded once. Z, when not null,
  * receives X W^T + bias (what oz_linear_grad takes). bias (N values) and residual (M x N) may be null.
  * M may be 0 (nothing is done), and 1 (one token) to 2^31 - 1; N and K from 1. Any leading dimension
- * from the row length up to 2^22 (0: the row length) and any alignment to the type's own size is taken; operands at 16-byte
- * boundaries with rows of a multiple of 8 values are read in place, other ones of larger products are
- * laid out in the workspace first. residual may be Y itself (the same leading dimension). */
+ * from the row length up to 2^22 (0: the row length) and any alignment to the type's own size is taken; operands whose rows
+ * begin at multiples of 4 bytes are read in place, other ones of more than 32 rows are laid out in the workspace
+ * first. residual may be Y itself (the same leading dimension). */
 typedef struct oz_linear_desc {
     int M, N, K;
     int type;   /* oz_type of X, W, bias and Z: OZ_BF16 or OZ_F16 */
