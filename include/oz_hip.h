@@ -349,7 +349,8 @@ int oz1_recon_block_f64(oz_dev* dev, const int32_t* P, int M, int N, int ldp, lo
  * What a program that trains a network, or answers with one, runs beside its products: a product with
  * its epilogue and its gradients, embeddings and their gradient, and the optimizer's step. Operands
  * stay in device memory; every call is stream-ordered on the handle, allocates nothing, and gives the
- * same bits for the same inputs. A workspace (16-byte aligned, its size asked for first; 0 means none is
+ * same bits for the same inputs. The handle's stream waits for no other one: what other streams write to inputs, or still
+ * do with the memory of outputs and workspaces, has to be complete before a call. A workspace (16-byte aligned, its size asked for first; 0 means none is
  * needed) holds intermediates of the call only. Leading dimensions count elements. Sums, activations and
  * states are computed in FP32. Outputs must not overlap inputs unless said so.
  */
@@ -448,7 +449,8 @@ typedef struct oz_adamw_tensor {
 } oz_adamw_tensor;
 /* The plan of a list of tensors (host array): the list and the division of its values over the
  * workgroups, copied into device memory of oz_adamw_plan_bytes bytes (16-byte aligned), which the caller
- * keeps unchanged as long as it steps with the plan. Returns when the copy is done. state_bits: 32 or 8. */
+ * keeps unchanged as long as it steps with the plan. Waits for all work of the device (the memory may have been another
+ * stream's) and returns when the copy is done. state_bits: 32 or 8. */
 typedef struct oz_adamw_plan {
     const void* memory;
     long long chunks; /* workgroups of a step */

@@ -256,6 +256,10 @@ int oz_adamw_make_plan(oz_dev* dev, const oz_adamw_tensor* tensors, int count, i
             for (long long c = chunks_of(t.n, chunk); c > 0; c--) owner[first++] = (uint32_t)k;
             block += (uint32_t)((t.n + OZ_ADAMW_BLOCK - 1) / OZ_ADAMW_BLOCK);
         }
+        // The memory may come from an allocator that hands out again what kernels of its own stream still write: the kernel
+        // takes its addresses from here, so the copy waits for the device.
+        if (int st = oz::use(dev)) return st;
+        if (int st = oz::hip_check(dev, hipDeviceSynchronize(), "hipDeviceSynchronize")) return st;
         if (int st = oz_memcpy_h2d(dev, memory, image.data(), image.size())) return st;
     } catch (const std::bad_alloc&) {
         return oz::fail(dev, OZ_ERR_NOMEM, "oz_adamw_make_plan: host memory");

@@ -263,3 +263,19 @@ def test_refusals_name_what_is_wrong(dev):
             dev.adamw_step(plan, **o)
     dev.sync()
     assert not x.any()
+
+
+def test_plan_in_memory_that_another_stream_still_writes(dev):
+    """Memory as another library's allocator hands it out: kernels queued before may still write to it. The plan, which holds
+    the addresses that a step uses, is copied behind them (the first entry begins with its tensor's size)."""
+    t = [torch.zeros(256, device="cuda:0") for _ in range(4)]
+    tensors = [ozd.adamw_tensor(256, *(x.data_ptr() for x in t))]
+    n = dev.adamw_plan_bytes(tensors)
+    memory = torch.zeros(n, dtype=torch.uint8, device="cuda:0")
+    a = torch.ones((4096, 4096), device="cuda:0")
+    for _ in range(20):
+        a = a @ a * 2.0**-12
+    memory.fill_(0x55)
+    dev.adamw_plan(tensors, 32, Ptr(memory))
+    torch.cuda.synchronize()
+    assert int(memory[:8].cpu().numpy().view(np.int64)[0]) == 256
