@@ -302,8 +302,11 @@ __global__ void __launch_bounds__(SORT_THREADS) scatter_kernel(const void* __res
     for (int i = 0; i < ITEMS; i++)
         if (first + 64 * i < s.T) {
             const uint32_t place = start[wave][(key[i] >> shift) & (digits - 1)] + rank[i];
-            keys_out[place] = key[i];
-            order_out[place] = who[i];
+            // ids that another stream still writes give other digits here than when they were counted
+            if (place < (uint32_t)s.T) {
+                keys_out[place] = key[i];
+                order_out[place] = who[i];
+            }
         }
 }
 
@@ -382,7 +385,8 @@ __global__ void __launch_bounds__(256) sums_kernel(const void* __restrict__ dOut
     const int n = (int)(end - begin);
     const uint32_t none = (uint32_t)s.vocab;
     // entry `lane` of the run, its successor's key, and whether the run's first token began before
-    const uint32_t mine = lane < n ? keys[begin + lane] : none, place = lane < n ? order[begin + lane] : 0;
+    const uint32_t mine = lane < n ? keys[begin + lane] : none;
+    const uint32_t place = lane < n ? min(order[begin + lane], (uint32_t)s.T - 1) : 0;  // as the sort's places are checked
     const uint32_t after = end < s.T ? keys[end] : none, before = begin > 0 ? keys[begin - 1] : none;
     bool cut = before == (uint32_t)__builtin_amdgcn_readfirstlane(mine);
     float sum[8] = {};
@@ -403,7 +407,7 @@ __global__ void __launch_bounds__(256) sums_kernel(const void* __restrict__ dOut
             const int i = i0 + j;
             if (i >= n) break;
             const uint32_t key = __builtin_amdgcn_readlane(mine, i);
-            if (key == none) return false;
+            if (key >= none) return false;
             float x[8];
             rows.take(from[j], x);
 #pragma unroll
@@ -438,7 +442,7 @@ __global__ void __launch_bounds__(256) join_kernel(const uint32_t* __restrict__ 
     const long long begin = r * R, end = begin + R;
     if (end >= s.T) return;
     const uint32_t key = keys[end - 1];
-    if (key == (uint32_t)s.vocab || keys[end] != key || (begin > 0 && keys[begin] == key && keys[begin - 1] == key)) return;
+    if (key >= (uint32_t)s.vocab || keys[end] != key || (begin > 0 && keys[begin] == key && keys[begin - 1] == key)) return;
     const Columns cols((int)(item - r * slices) * 512, lane, s.D);
     float sum[8] = {};
     cols.get(parts, OZ_F32, (2 * r + 1) * s.D, sum);
