@@ -7,6 +7,7 @@
 // block and its maximum is three exchanges away. The file is compiled without contraction: the order of
 // operations is the header's, each rounded once.
 #include <cmath>
+#include <type_traits>
 #include <vector>
 
 #include "oz_internal.hpp"
@@ -92,19 +93,16 @@ __device__ __forceinline__ void from_8bit(const uint8_t* p, uint8_t scale, float
     for (int k = 0; k < V; k++) x[k] *= s;
 }
 
-// The first `count` of 8 values from i on, the others zeros.
-__device__ __forceinline__ void get(const void* p, int type, long long i, int count, bool whole, float* x) {
-    if (whole) load8(p, type, i, x);
-    else load_some(p, type, i, count, x);
-}
+// The first `count` of 8 values from i on.
 __device__ __forceinline__ void put(void* p, int type, long long i, int count, bool whole, const float* x) {
     if (whole) store8(p, type, i, x);
     else store_some(p, type, i, count, x);
 }
 
-template <int BITS>
-__global__ void __launch_bounds__(THREADS) adamw_kernel(const Entry* __restrict__ entries, const uint32_t* __restrict__ owner, Step o) {
-    const Entry& E = entries[owner[blockIdx.x]];
+// One chunk of a tensor whose types are known here: with a branch on them at every access the loads of a round would each be
+// waited for where the branches meet.
+template <int BITS, int PARAM, int GRAD, bool MASTER>
+__device__ __forceinline__ void step_chunk(const Entry& E, const Step& o) {
     const oz_adamw_tensor& t = E.t;
     const long long n = t.n, begin = (blockIdx.x - E.first_chunk) * E.chunk;
     const float gs = o.grad_scale ? *o.grad_scale : 1.0f;
@@ -115,18 +113,27 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const Entry* __restrict_
         const int count = (int)(end - i < V ? (end - i > 0 ? end - i : 0) : V);
         const bool whole = count == V;
         float g[V], p[V], m[V], v[V], r[V];
-        get(t.grad, t.grad_type, i, count, whole, g);
-        get(t.master ? t.master : t.param, t.master ? OZ_F32 : t.param_type, i, count, whole, p);
-        if constexpr (BITS == 32) {
-            get(t.m, OZ_F32, i, count, whole, m);
-            get(t.v, OZ_F32, i, count, whole, v);
-        } else {
-            const uint8_t *pm = static_cast<uint8_t*>(t.m) + i, *pv = static_cast<uint8_t*>(t.v) + i;
-            const int ms = count ? t.m_scale[i / OZ_ADAMW_BLOCK] : 0, vs = count ? t.v_scale[i / OZ_ADAMW_BLOCK] : 0;
-            if (whole) {
-                from_8bit(pm, ms, m);
-                from_8bit(pv, vs, r);
+        const void* from = MASTER ? t.master : t.param;
+        constexpr int FROM = MASTER ? OZ_F32 : PARAM;
+        if (whole) {
+            load8(t.grad, GRAD, i, g);
+            load8(from, FROM, i, p);
+            if constexpr (BITS == 32) {
+                load8(t.m, OZ_F32, i, m);
+                load8(t.v, OZ_F32, i, v);
             } else {
+                from_8bit(static_cast<uint8_t*>(t.m) + i, t.m_scale[i / OZ_ADAMW_BLOCK], m);
+                from_8bit(static_cast<uint8_t*>(t.v) + i, t.v_scale[i / OZ_ADAMW_BLOCK], r);
+            }
+        } else {
+            load_some(t.grad, GRAD, i, count, g);
+            load_some(from, FROM, i, count, p);
+            if constexpr (BITS == 32) {
+                load_some(t.m, OZ_F32, i, count, m);
+                load_some(t.v, OZ_F32, i, count, v);
+            } else {
+                const uint8_t *pm = static_cast<uint8_t*>(t.m) + i, *pv = static_cast<uint8_t*>(t.v) + i;
+                const int ms = count ? t.m_scale[i / OZ_ADAMW_BLOCK] : 0, vs = count ? t.v_scale[i / OZ_ADAMW_BLOCK] : 0;
 #pragma unroll
                 for (int k = 0; k < V; k++) {
                     float x[4];
@@ -135,6 +142,8 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const Entry* __restrict_
                     r[k] = x[1] * power(vs - 127);
                 }
             }
+        }
+        if constexpr (BITS == 8) {
 #pragma unroll
             for (int k = 0; k < V; k++) v[k] = r[k] * r[k];
         }
@@ -146,8 +155,8 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const Entry* __restrict_
             r[k] = sqrtf(v[k]);
             p[k] = p[k] * keep - (m[k] / (r[k] * o.root + o.eps)) * o.rate;
         }
-        put(t.param, t.param_type, i, count, whole, p);
-        if (t.master) put(t.master, OZ_F32, i, count, whole, p);
+        put(t.param, PARAM, i, count, whole, p);
+        if constexpr (MASTER) put(t.master, OZ_F32, i, count, whole, p);
         if constexpr (BITS == 32) {
             put(t.m, OZ_F32, i, count, whole, m);
             put(t.v, OZ_F32, i, count, whole, v);
@@ -179,6 +188,25 @@ __global__ void __launch_bounds__(THREADS) adamw_kernel(const Entry* __restrict_
             }
         }
     }
+}
+
+template <int BITS>
+__global__ void __launch_bounds__(THREADS) adamw_kernel(const Entry* __restrict__ entries, const uint32_t* __restrict__ owner, Step o) {
+    const Entry& E = entries[owner[blockIdx.x]];
+    const auto by_grad = [&](auto P, auto M) {
+        constexpr int p = decltype(P)::value;
+        constexpr bool m = decltype(M)::value;
+        if (E.t.grad_type == OZ_F32) step_chunk<BITS, p, OZ_F32, m>(E, o);
+        else if (E.t.grad_type == OZ_BF16) step_chunk<BITS, p, OZ_BF16, m>(E, o);
+        else step_chunk<BITS, p, OZ_F16, m>(E, o);
+    };
+    const auto by_param = [&](auto M) {
+        if (E.t.param_type == OZ_BF16) by_grad(std::integral_constant<int, OZ_BF16>{}, M);
+        else by_grad(std::integral_constant<int, OZ_F16>{}, M);
+    };
+    if (E.t.param_type == OZ_F32) by_grad(std::integral_constant<int, OZ_F32>{}, std::false_type{});
+    else if (E.t.master) by_param(std::true_type{});
+    else by_param(std::false_type{});
 }
 
 long long chunks_of(long long n, int chunk) { return (n + chunk - 1) / chunk; }
