@@ -20,9 +20,10 @@ using namespace ozt;
 constexpr int V = 8, THREADS = 256;  // values of a lane, lanes
 static_assert(OZ_ADAMW_BLOCK == 8 * V, "a block is 8 lanes' values");
 
-// Values of a chunk: 8192 of large lists, one round of a workgroup's threads of small ones, whose chunks would leave most of
-// the chip idle (2e5 values: 5.6 us, 9.6 with 8192).
-int chunk_of(long long values) { return values > 1 << 22 ? 4 * V * THREADS : V * THREADS; }
+// Values of a chunk: one round of a workgroup's threads, 8 of lists of which those would be too many workgroups. Rounds in turn
+// by one workgroup are slower, as the next one's loads wait for this one's stores: 1e8 values with 32-bit states take 523 us in
+// chunks of one round, 537 of two, 549 of four, 590 of sixteen. Loads and stores past the caches gain nothing (521 us; loads 577).
+int chunk_of(long long values) { return values >> 33 ? 8 * V * THREADS : V * THREADS; }
 
 // The plan's memory: one Entry a tensor, then for each chunk its tensor (uint32), its place in it follows
 // from the tensor's first chunk.
