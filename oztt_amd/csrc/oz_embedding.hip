@@ -100,22 +100,39 @@ struct Ahead {
 };
 
 // Rows by tokens: a wave takes 512 columns of a row, or of narrow rows 2^rows_log rows, 64 >> rows_log lanes each (19056 rows of
-// 22 values: 9.6 us by a row a wave).
+// 22 values: 9.6 us by a row a wave); of wide rows the token is the whole wave's. The loads are one for every lane, whatever its columns (8192 rows of 4093 values 19 us, 25
+// with a branch on the columns left); two, four or eight pieces a wave are slower (8192 rows of 4096: 17.7 us by one, 18.8 by four).
+template <int TYPE, bool SMALL, bool NARROW>
 __global__ void __launch_bounds__(256) embedding_kernel(const void* __restrict__ table, const void* __restrict__ ids,
                                                         void* __restrict__ out, uint32_t* __restrict__ flags, Shape s, unsigned slices, int rows_log) {
-    const unsigned wide = 64u >> rows_log, lane = threadIdx.x & (wide - 1);
-    const long long item = ((4ll * blockIdx.x + (threadIdx.x >> 6)) << rows_log) + (threadIdx.x & 63) / wide, t = item / slices;
+    const long long wave = 4ll * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & ((64u >> (NARROW ? rows_log : 0)) - 1);
+    long long t;
+    int c0 = 0;
+    if constexpr (NARROW) {
+        t = (wave << rows_log) + ((threadIdx.x & 63) >> (6 - rows_log));
+    } else {
+        t = wave / slices;
+        c0 = (int)(wave - t * slices) * 512;
+    }
     if (t >= s.T) return;
-    const int c0 = (int)(item - t * slices) * 512;
     const long long v = token(ids, s.wide, t);
     const bool known = v >= 0 && v < s.vocab;
     if (!known && flags && c0 == 0 && lane == 0) atomicOr(flags, 1u);
     const Columns cols(c0, lane, s.D);
-    float x[8] = {};
-    if (known) cols.get(table, s.type, v * s.ldt, x);
+    const Ahead<TYPE, SMALL> rows(cols, s.D);
+    typename Ahead<TYPE, SMALL>::Raw w;
+    float x[8];
+    rows.ask(table, known ? v * s.ldt : 0, w);
+    rows.take(w, x);
 #pragma unroll
     for (int k = 0; k < 8; k++) x[k] = known ? x[k] * s.scale : 0.0f;
-    cols.put(out, s.type, t * s.ldo, x);
+    cols.put(out, TYPE, t * s.ldo, x);
+}
+
+template <int TYPE>
+auto lookup_of(int D, int rows_log) {
+    return D < 8 ? embedding_kernel<TYPE, true, true> : rows_log ? embedding_kernel<TYPE, false, true> : embedding_kernel<TYPE, false, false>;
 }
 
 // Zeros for part `part` of `parts` of the table's rows, by workgroups `first` to gridDim.x - 1 of a launch, which stride over
@@ -560,7 +577,10 @@ int oz_embedding(oz_dev* dev, const oz_embedding_desc* d, const void* table, con
     if (groups > kMaxGroups) return oz::fail(dev, OZ_ERR_ARG, "oz_embedding: %lld tokens of %d values are too many", s.T, s.D);
     if (int st = oz::use(dev)) return st;
     if (!s.T) return OZ_OK;
-    hipLaunchKernelGGL(embedding_kernel, dim3((unsigned)groups), dim3(256), 0, dev->stream, table, ids, out, flags, s, slices, rows_log);
+    const auto kernel = s.type == OZ_F32   ? lookup_of<OZ_F32>(s.D, rows_log)
+                        : s.type == OZ_F16 ? lookup_of<OZ_F16>(s.D, rows_log)
+                                           : lookup_of<OZ_BF16>(s.D, rows_log);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), 0, dev->stream, table, ids, out, flags, s, slices, rows_log);
     return oz::launch_check(dev, "embedding_kernel");
 }
 
