@@ -395,7 +395,7 @@ __global__ void __launch_bounds__(256) sums_kernel(const void* __restrict__ dOut
                                                    const uint32_t* __restrict__ order, void* __restrict__ table,
                                                    float* __restrict__ parts, Shape s, int R, unsigned slices) {
     const int lane = threadIdx.x & 63;
-    const long long item = 4ll * blockIdx.x + (threadIdx.x >> 6), r = item / slices;
+    const long long item = 4ll * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = item / slices;
     const long long begin = r * R, end = begin + R < s.T ? begin + R : s.T;
     if (begin >= s.T) return;
     const Columns cols((int)(item - r * slices) * 512, lane, s.D);
@@ -455,7 +455,7 @@ template <bool SMALL>
 __global__ void __launch_bounds__(256) join_kernel(const uint32_t* __restrict__ keys, void* __restrict__ table,
                                                    const float* __restrict__ parts, Shape s, int R, unsigned slices) {
     const int lane = threadIdx.x & 63;
-    const long long item = 4ll * blockIdx.x + (threadIdx.x >> 6), r = item / slices;
+    const long long item = 4ll * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = item / slices;
     const long long begin = r * R, end = begin + R;
     if (end >= s.T) return;
     const uint32_t key = keys[end - 1];
