@@ -43,6 +43,24 @@ def test_lookup(dev, T, vocab, D, t, bits):
         assert bool((around == 5.0).all()) and not int(flags)
 
 
+@pytest.mark.parametrize("D", [9, 16, 22, 33, 64, 100, 129, 200, 256, 257, 511, 513])
+def test_lookup_widths(dev, D):
+    """Several rows a wave, one, and a second wave for a few values; tokens outside the vocabulary among them."""
+    T, vocab = 301, 70
+    for t in ("bf16", "f32"):
+        print("embedding", D, t, flush=True)
+        table = torch.randn((vocab, D), device="cuda:0", generator=generator(1)).to(DTYPE[t])
+        ids = tokens("random", T, vocab, 32, 3)
+        ids[::7] = vocab
+        out, flags = torch.full((T, D), 7.0, device="cuda:0", dtype=DTYPE[t]), torch.zeros(1, dtype=torch.int32, device="cuda:0")
+        torch.cuda.synchronize()
+        dev.embedding(ozd.embedding_desc(T, vocab, D, t, 32, scale=0.3), Ptr(table), Ptr(ids), Ptr(out), Ptr(flags))
+        dev.sync()
+        want = (table[ids.long().clamp(max=vocab - 1)].float() * torch.tensor(0.3)).to(DTYPE[t])
+        want[::7] = 0
+        assert torch.equal(out, want) and int(flags) == 1
+
+
 @pytest.mark.parametrize("bits", [32, 64])
 def test_tokens_outside_the_vocabulary(dev, bits):
     """They give rows of zeros and no gradient, set the flag, and leave the others alone; infinities of the table do
