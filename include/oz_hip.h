@@ -381,8 +381,9 @@ int oz_linear(oz_dev* dev, const oz_linear_desc* d, const void* X, const void* W
 /* Gradients of oz_linear from dY (M x N, `type`): with dZ = dY act'(Z),
  *   dX (M x K, `type`) = dZ W,  dW (N x K, dw_type) = dZ^T X,  dbias (N, dw_type) = sum over the rows of dZ.
  * dX, dW and dbias may each be null; the gradient of the residual is dY. Z may be null for OZ_ACT_NONE
- * (it is not read then); X may be null without dW, W without dX. The products take dZ rounded to
- * `type`, what the matrix cores read; dbias sums it unrounded. accumulate: dW and dbias are added to what
+ * (it is not read then); X may be null without dW, W without dX. The matrix cores read 16 bits: the products take
+ * dZ rounded to `type`, and a dW in FP32 behind GELU or SILU also what that leaves, rounded to `type` in turn (dZ to 16
+ * bits in BF16, 22 in FP16 or 2^-25; an infinity in X may give NaN there); dbias sums it unrounded. accumulate: dW and dbias are added to what
  * is there (gradients of several batches). M = 0: dW and dbias are sums of nothing. */
 typedef struct oz_linear_grad_desc {
     int M, N, K;

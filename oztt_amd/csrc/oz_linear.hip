@@ -70,10 +70,14 @@ __global__ void __launch_bounds__(256) product_any_kernel(const ozl::Product a) 
 // dZ = dY act'(Z), rounded for the products (left out where dz is null), and the sums of its columns over `rows` rows each,
 // to dbias if one range holds all rows, else to parts (left out where both are null): 8 columns a lane, 8 LANES columns by
 // 256 / LANES rows at a time by a workgroup. One pass over dY and Z, which are not read again and pass the caches by.
-template <int LANES, int ACT>
+// The matrix cores read 16 bits. For gradients in 16 bits one rounding of dZ is as large as the outputs' own (8192 x 8192 x 2048
+// in BF16: 2.3e-3 of their norm against 1.7e-3 for the outputs' rounding alone) and two products would take twice the time; a dW
+// in FP32 would show it, so its products also get what the rounding leaves, rounded in turn, in `rest` (TWO): together 16 bits
+// of a BF16 dZ, 22 of an FP16 one, in 720 us for 492. What rounds to an infinity leaves nothing.
+template <int LANES, int ACT, bool TWO>
 __global__ void __launch_bounds__(256) act_grad_kernel(const void* __restrict__ dY, const void* __restrict__ Z,
-                                                       void* __restrict__ dz, float* __restrict__ parts, void* __restrict__ dbias,
-                                                       int type, int dw_type, int accumulate, long long M, int N,
+                                                       void* __restrict__ dz, void* __restrict__ rest, float* __restrict__ parts,
+                                                       void* __restrict__ dbias, int type, int dw_type, int accumulate, long long M, int N,
                                                        long long lddy, long long ldz, long long lddz, int rows, int strips) {
     constexpr int COLS = 8 * LANES, R = 256 / LANES;
     const int strip = blockIdx.x % strips, chunk = blockIdx.x / strips, l = threadIdx.x % LANES, r = threadIdx.x / LANES;
@@ -98,6 +102,14 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const void* __restrict__ 
                     for (int k = 0; k < 8; k++) x[k] *= act_grad(y[k], ACT);
                 }
                 if (dz) store8(dz, type, m * lddz + col, x);
+                if constexpr (TWO) {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        const float h = type == OZ_BF16 ? (float)(__bf16)x[k] : (float)(_Float16)x[k];
+                        y[k] = fabsf(h) < INFINITY ? x[k] - h : 0.0f;
+                    }
+                    store8(rest, type, m * lddz + col, y);
+                }
 #pragma unroll
                 for (int k = 0; k < 8; k++) sum[k] += x[k];
             }
@@ -129,11 +141,11 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const void* __restrict__ 
 }
 
 template <int LANES>
-auto act_grad_of(int act) {
-    return act == OZ_ACT_GELU   ? act_grad_kernel<LANES, OZ_ACT_GELU>
-           : act == OZ_ACT_SILU ? act_grad_kernel<LANES, OZ_ACT_SILU>
-           : act == OZ_ACT_RELU ? act_grad_kernel<LANES, OZ_ACT_RELU>
-                                : act_grad_kernel<LANES, OZ_ACT_NONE>;
+auto act_grad_of(int act, bool two) {
+    return act == OZ_ACT_GELU   ? (two ? act_grad_kernel<LANES, OZ_ACT_GELU, true> : act_grad_kernel<LANES, OZ_ACT_GELU, false>)
+           : act == OZ_ACT_SILU ? (two ? act_grad_kernel<LANES, OZ_ACT_SILU, true> : act_grad_kernel<LANES, OZ_ACT_SILU, false>)
+           : act == OZ_ACT_RELU ? act_grad_kernel<LANES, OZ_ACT_RELU, false>
+                                : act_grad_kernel<LANES, OZ_ACT_NONE, false>;
 }
 
 // dbias from the chunks' sums, 16 chunks at a time by 16 lanes: lane k of a column sums chunks k, k + 16, ..., then the lanes.
@@ -333,20 +345,23 @@ const char* refuse(const oz_linear_grad_desc* d) {
 bool misaligned16(const void* p) { return ((uintptr_t)p & 15) != 0; }
 bool misaligned(const void* p, int type) { return ((uintptr_t)p & (size_of(type) - 1)) != 0; }
 
-// Workspace of the gradients: dZ where it is not dY (or dY's rows are not even), the columns' sums, and the larger of the
-// products' own.
+// Workspace of the gradients: dZ where it is not dY (or dY's rows are not even), what its rounding leaves where dW takes that too,
+// the columns' sums, and the larger of the products' own.
 struct GradWork {
     bool make_dz;
+    bool two;          // dZ in two parts of `part` bytes: ReLU's is dY or 0, exact in one
     long long lddz;
     int lanes;         // act_grad_kernel's
     int rows, chunks;  // of M for the columns' sums
-    size_t dz, sums, product, bytes;
+    size_t part, dz, sums, product, bytes;
 };
 GradWork grad_work(int cus, const oz_linear_grad_desc* d, bool even_dy) {
     GradWork w{};
     w.make_dz = d->act != OZ_ACT_NONE || !even_dy;
     w.lddz = (d->N + 7) / 8 * 8;
-    w.dz = w.make_dz ? up(2 * (size_t)d->M * w.lddz) : 0;
+    w.two = d->dw_type == OZ_F32 && (d->act == OZ_ACT_GELU || d->act == OZ_ACT_SILU);
+    w.part = up(2 * (size_t)d->M * w.lddz);
+    w.dz = w.make_dz ? (1 + w.two) * w.part : 0;
     // Strips of 256 columns, 64 of few values, and of the rows so many that the chip is filled four times, 16 to 256 at a time.
     w.lanes = (long long)d->M * d->N <= 1 << 22 ? 8 : 32;
     const long long strips = (d->N + 8 * w.lanes - 1) / (8 * w.lanes), rows = (long long)d->M * strips / (4 * cus), least = 512 / w.lanes;
@@ -418,15 +433,16 @@ int oz_linear_grad(oz_dev* dev, const oz_linear_grad_desc* d, const void* dY, co
     if ((w.make_dz && products) || dbias) {
         void* make = w.make_dz && products ? at : nullptr;
         if (make) dz = make, lddz = w.lddz;
+        void* rest = make && w.two && dW ? at + w.part : nullptr;
         float* sums = dbias ? reinterpret_cast<float*>(at + w.dz) : nullptr;
         const int strips = (int)oz::ceil_div(d->N, 8 * w.lanes), chunks = d->M ? w.chunks : 0;
         if ((long long)strips * w.chunks > kMaxTiles) return oz::fail(dev, OZ_ERR_ARG, "oz_linear_grad: %d x %d outputs are too many", d->M, d->N);
         const bool one = chunks == 1;
         if (chunks) {
             const dim3 grid((unsigned)(strips * chunks));
-            const auto kernel = w.lanes == 8 ? act_grad_of<8>(d->act) : act_grad_of<32>(d->act);
-            hipLaunchKernelGGL(kernel, grid, dim3(256), 0, dev->stream, dY, Z, make, one ? nullptr : sums, one ? dbias : nullptr,
-                               d->type, d->dw_type, d->accumulate, (long long)d->M, d->N, lddy, ldz, w.lddz, w.rows, strips);
+            const auto kernel = w.lanes == 8 ? act_grad_of<8>(d->act, rest) : act_grad_of<32>(d->act, rest);
+            hipLaunchKernelGGL(kernel, grid, dim3(256), 0, dev->stream, dY, Z, make, rest, one ? nullptr : sums,
+                               one ? dbias : nullptr, d->type, d->dw_type, d->accumulate, (long long)d->M, d->N, lddy, ldz, w.lddz, w.rows, strips);
             if (int st = oz::launch_check(dev, "act_grad_kernel")) return st;
         }
         if (dbias && !one) {
@@ -447,6 +463,12 @@ int oz_linear_grad(oz_dev* dev, const oz_linear_grad_desc* d, const void* dY, co
         ozl::Product p{};
         p.Q = dz, p.P = X, p.nq = d->N, p.np = d->K, p.C = d->M, p.ldq = lddz, p.ldp = or_row(d->ldx, d->K), p.q_major = p.p_major = 1;
         p.epi = {dW, or_row(d->lddw, d->K), d->dw_type, nullptr, 0, nullptr, d->accumulate ? dW : nullptr, or_row(d->lddw, d->K), OZ_ACT_NONE};
+        if (w.two && d->M > 0) {  // the smaller part's product first, the other's added to it
+            ozl::Product r = p;
+            r.Q = at + w.part;
+            if (int st = launch_product(dev, d->type, r, room, left)) return st;
+            p.epi.residual = dW;
+        }
         if (int st = launch_product(dev, d->type, p, room, left)) return st;
     }
     return OZ_OK;
