@@ -355,7 +355,8 @@ int oz1_recon_block_f64(oz_dev* dev, const int32_t* P, int M, int N, int ldp, lo
  * states are computed in FP32. Outputs must not overlap inputs unless said so.
  */
 enum oz_type { OZ_BF16 = 0, OZ_F16 = 1, OZ_F32 = 2 };
-/* GELU is its tanh form, z/2 (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))); SILU is z / (1 + exp(-z)). */
+/* RELU is max(z, 0), its slope 1 where z > 0 and 0 elsewhere; there it leaves out infinities of dY too.
+ * GELU is its tanh form, z/2 (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))); SILU is z / (1 + exp(-z)). */
 enum oz_act { OZ_ACT_NONE = 0, OZ_ACT_RELU = 1, OZ_ACT_GELU = 2, OZ_ACT_SILU = 3 };
 
 /* ---- product with bias, activation and residual ------------------------------------------------

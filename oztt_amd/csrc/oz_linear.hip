@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const void* __restrict__ 
                 if constexpr (ACT != OZ_ACT_NONE) {
                     get(Z, m * ldz + col, y);
 #pragma unroll
-                    for (int k = 0; k < 8; k++) x[k] *= act_grad(y[k], ACT);
+                    for (int k = 0; k < 8; k++) x[k] = act_grad(x[k], y[k], ACT);
                 }
                 if (dz) store8(dz, type, m * lddz + col, x);
                 if constexpr (TWO) {

@@ -144,18 +144,20 @@ __device__ __forceinline__ void act8(float* z, int a) {
     else if (a == OZ_ACT_SILU) all(std::integral_constant<int, OZ_ACT_SILU>{});
     else if (a == OZ_ACT_RELU) all(std::integral_constant<int, OZ_ACT_RELU>{});
 }
-__device__ __forceinline__ float act_grad(float z, int a) {
+// dY act'(z). ReLU selects, so that what it masks goes no further whatever it is; a z that is not a number, which the activation
+// hands on, is handed on here too.
+__device__ __forceinline__ float act_grad(float dy, float z, int a) {
     switch (a) {
-        case OZ_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
+        case OZ_ACT_RELU: return z > 0.0f ? dy : z != z ? z : 0.0f;
         case OZ_ACT_GELU: {
             const float zz = fminf(z * z, 1e4f), s = gelu_s(z, zz);
-            return __builtin_fmaf(z * __builtin_fmaf(-s, s, s), __builtin_fmaf(zz, 6.0f * kGelu0 * kGelu1, 2.0f * kGelu0), s);
+            return dy * __builtin_fmaf(z * __builtin_fmaf(-s, s, s), __builtin_fmaf(zz, 6.0f * kGelu0 * kGelu1, 2.0f * kGelu0), s);
         }
         case OZ_ACT_SILU: {
             const float s = logistic2(-kLog2e * z);
-            return __builtin_fmaf(z, __builtin_fmaf(-s, s, s), s);
+            return dy * __builtin_fmaf(z, __builtin_fmaf(-s, s, s), s);
         }
-        default: return 1.0f;
+        default: return dy;
     }
 }
 
