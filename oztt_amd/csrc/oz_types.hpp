@@ -145,17 +145,19 @@ __device__ __forceinline__ void act8(float* z, int a) {
     else if (a == OZ_ACT_RELU) all(std::integral_constant<int, OZ_ACT_RELU>{});
 }
 // dY act'(z). ReLU selects, so that what it masks goes no further whatever it is; a z that is not a number, which the activation
-// hands on, is handed on here too.
+// hands on, is handed on here too. GELU's and SILU's slopes at infinity (an FP16 Z beyond its range) are their limits: the z that
+// multiplies s - s^2 is held within 100, beyond which that difference is 0.
+__device__ __forceinline__ float held(float z) { return __builtin_amdgcn_fmed3f(z, -100.0f, 100.0f); }
 __device__ __forceinline__ float act_grad(float dy, float z, int a) {
     switch (a) {
         case OZ_ACT_RELU: return z > 0.0f ? dy : z != z ? z : 0.0f;
         case OZ_ACT_GELU: {
-            const float zz = fminf(z * z, 1e4f), s = gelu_s(z, zz);
-            return dy * __builtin_fmaf(z * __builtin_fmaf(-s, s, s), __builtin_fmaf(zz, 6.0f * kGelu0 * kGelu1, 2.0f * kGelu0), s);
+            const float y = held(z), zz = y * y, s = gelu_s(z, zz);
+            return dy * __builtin_fmaf(y * __builtin_fmaf(-s, s, s), __builtin_fmaf(zz, 6.0f * kGelu0 * kGelu1, 2.0f * kGelu0), s);
         }
         case OZ_ACT_SILU: {
             const float s = logistic2(-kLog2e * z);
-            return dy * __builtin_fmaf(z, __builtin_fmaf(-s, s, s), s);
+            return dy * __builtin_fmaf(held(z), __builtin_fmaf(-s, s, s), s);
         }
         default: return dy;
     }

@@ -58,3 +58,18 @@ def test_relu_leaves_out_what_it_masks(dev, size, t):
     assert same(gradients(dev, dY, Z, X, W, t, "relu"), want)
     Z[2, 4] = float("nan")
     only_there(gradients(dev, masked, Z, X, W, t, "relu"), want, 2, 4)
+
+
+@pytest.mark.parametrize("size", SIZES, ids=str)
+@pytest.mark.parametrize("a", ["gelu", "silu"])
+@pytest.mark.parametrize("t,dw", [("bf16", "bf16"), ("f16", "f32")])
+def test_slopes_at_infinities(dev, size, a, t, dw):
+    """A Z that left FP16's range is kept as infinite; its slope is the limit, 1 or 0, as of any large z."""
+    print("linear_grad", a, size, t, flush=True)
+    dY, Z, X, W = inputs(*size, t)
+    Z[1, 2], Z[2, 3], Z[0, 1] = 300.0, -300.0, 300.0
+    want = gradients(dev, dY, Z, X, W, t, a, dw)
+    Z[1, 2], Z[2, 3], Z[0, 1] = float("inf"), -float("inf"), float("inf")
+    assert same(gradients(dev, dY, Z, X, W, t, a, dw), want)
+    Z[2, 4] = float("nan")
+    only_there(gradients(dev, dY, Z, X, W, t, a, dw), want, 2, 4)
