@@ -387,14 +387,17 @@ class Device:
         arr = (AdamwTensor * max(len(tensors), 1))(*tensors)
         return self._bytes(hip().oz_adamw_plan_bytes(arr, len(tensors)), "oz_adamw_plan_bytes")
 
-    def adamw_plan(self, tensors, state_bits: int, memory: Buffer = None) -> AdamwPlan:
+    def adamw_plan(self, tensors, state_bits: int, memory: Buffer = None, memory_bytes: int = None) -> AdamwPlan:
         """The plan of a list of adamw_tensor()s, in `memory` (adamw_plan_bytes; allocated here if none is
-        given), which lives as long as the plan."""
+        given), which lives as long as the plan. Memory of fewer bytes than the list needs is refused: a Buffer has its
+        own size, of an object with an address alone it is memory_bytes (None: there is room)."""
         arr = (AdamwTensor * max(len(tensors), 1))(*tensors)
-        nbytes = self.adamw_plan_bytes(tensors)
-        memory = memory if memory is not None else self.alloc(nbytes)
+        need = self.adamw_plan_bytes(tensors)
+        memory = memory if memory is not None else self.alloc(need)
+        if memory_bytes is None:
+            memory_bytes = getattr(memory, "nbytes", need)
         plan = AdamwPlan()
-        self._check(hip().oz_adamw_make_plan(self.h, arr, len(tensors), state_bits, memory.ptr, ctypes.c_size_t(nbytes),
+        self._check(hip().oz_adamw_make_plan(self.h, arr, len(tensors), state_bits, memory.ptr, ctypes.c_size_t(memory_bytes),
                                              ctypes.byref(plan)), "oz_adamw_make_plan")
         plan.buffer = memory
         return plan
