@@ -366,13 +366,18 @@ enum oz_act { OZ_ACT_NONE = 0, OZ_ACT_RELU = 1, OZ_ACT_GELU = 2, OZ_ACT_SILU = 3
  * M may be 0 (nothing is done), and 1 (one token) to 2^31 - 1; N and K from 1. Any leading dimension
  * from the row length up to 2^22 (0: the row length) and any alignment to the type's own size is taken; operands whose rows
  * begin at multiples of 4 bytes are read in place, other ones of more than 32 rows are laid out in the workspace
- * first. residual may be Y itself (the same leading dimension). */
+ * first. Odd leading dimensions the descriptor shows; of an operand at an address that is no multiple of 4 bytes
+ * (a window that begins at an odd column) it has to be told, by `odd`, so that the workspace has room for its copy. Where it is
+ * not, the operand is read in place, value by value, which takes 7 to 15 times as long (40 x 1024 x 1024 86 us for 9.8, 4096^3
+ * 1588 for 140). residual may be Y itself (the same leading dimension). */
+enum oz_odd { OZ_ODD_X = 1, OZ_ODD_W = 2, OZ_ODD_DY = 4 };
 typedef struct oz_linear_desc {
     int M, N, K;
     int type;   /* oz_type of X, W, bias and Z: OZ_BF16 or OZ_F16 */
     int y_type; /* oz_type of Y and residual: type or OZ_F32 */
     int act;    /* oz_act */
     long long ldx, ldw, ldy, ldr, ldz;
+    int odd; /* OZ_ODD_X, OZ_ODD_W: operands at such addresses, or 0 */
 } oz_linear_desc;
 /* Bytes of workspace, or a negative oz_status where the descriptor is refused. */
 long long oz_linear_workspace(oz_dev* dev, const oz_linear_desc* d);
@@ -393,6 +398,7 @@ typedef struct oz_linear_grad_desc {
     int act;        /* oz_act */
     int accumulate; /* 0 or 1 */
     long long lddy, ldx, ldw, ldz, lddx, lddw;
+    int odd;        /* as above, and OZ_ODD_DY */
 } oz_linear_grad_desc;
 long long oz_linear_grad_workspace(oz_dev* dev, const oz_linear_grad_desc* d);
 int oz_linear_grad(oz_dev* dev, const oz_linear_grad_desc* d, const void* dY, const void* X, const void* W,

@@ -271,16 +271,26 @@ size_t product_bytes(int cus, long long nq, long long np, long long C, bool q_ma
     return r.parts + (copy_q ? copy_bytes(nq, C, q_major) : 0) + (copy_p ? copy_bytes(np, C, p_major) : 0);
 }
 
+// The same where operands may need copies (their addresses are said to be odd), enough whether they turn out to or not.
+size_t reserve(int cus, long long nq, long long np, long long C, bool q_major, bool p_major, bool copy_q, bool copy_p, bool may_q, bool may_p) {
+    return std::max(product_bytes(cus, nq, np, C, q_major, p_major, copy_q, copy_p),
+                    product_bytes(cus, nq, np, C, q_major, p_major, copy_q || may_q, copy_p || may_p));
+}
+
 // Runs a product in `bytes` bytes of workspace. Operands whose rows begin at odd addresses are laid out in it; where that has no room
-// (the size is asked for by leading dimensions, an operand may lie at an odd address besides) the element by element kernel runs.
+// (an operand at an odd address of which the descriptor does not say so) few rows take one range, and of more the element by
+// element kernel runs.
 int launch_product(oz_dev* dev, int type, Product a, void* work, size_t bytes) {
     if (!a.nq || !a.np) return OZ_OK;
     a.splits = 1;
     if (!a.C) return launch_any(dev, type, a);
     const bool copy_q = !even_rows(a.Q, a.ldq), copy_p = !even_rows(a.P, a.ldp);
-    const Route r = route_of(dev->cus, a.nq, a.np, a.C, !a.q_major && !a.p_major, !copy_q && !copy_p);
+    Route r = route_of(dev->cus, a.nq, a.np, a.C, !a.q_major && !a.p_major, !copy_q && !copy_p);
     const size_t need = product_bytes(dev->cus, a.nq, a.np, a.C, a.q_major, a.p_major, copy_q, copy_p);
-    if (need > bytes) return launch_any(dev, type, a);
+    if (need > bytes) {
+        if (!r.few) return launch_any(dev, type, a);
+        r.splits = 1, r.parts = 0;
+    }
     char* at = static_cast<char*>(work);
     a.splits = r.splits;
     a.parts = reinterpret_cast<float*>(at);
@@ -325,6 +335,7 @@ const char* refuse(const oz_linear_desc* d) {
     if (d->act < OZ_ACT_NONE || d->act > OZ_ACT_SILU) return "the activation";
     if (bad_ld(d->ldx, d->K) || bad_ld(d->ldw, d->K) || bad_ld(d->ldy, d->N) || bad_ld(d->ldr, d->N) || bad_ld(d->ldz, d->N))
         return "a leading dimension";
+    if (d->odd & ~(OZ_ODD_X | OZ_ODD_W)) return "odd operands";
     return nullptr;
 }
 
@@ -339,6 +350,7 @@ const char* refuse(const oz_linear_grad_desc* d) {
     if (bad_ld(d->lddy, d->N) || bad_ld(d->ldx, d->K) || bad_ld(d->ldw, d->K) || bad_ld(d->ldz, d->N) ||
         bad_ld(d->lddx, d->K) || bad_ld(d->lddw, d->K))
         return "a leading dimension";
+    if (d->odd & ~(OZ_ODD_X | OZ_ODD_W | OZ_ODD_DY)) return "odd operands";
     return nullptr;
 }
 
@@ -368,11 +380,14 @@ GradWork grad_work(int cus, const oz_linear_grad_desc* d, bool even_dy) {
     w.rows = (int)std::min(256ll, std::max(least, (rows + least - 1) / least * least));
     w.chunks = (int)std::max(1ll, ((long long)d->M + w.rows - 1) / w.rows);
     w.sums = up(4 * (size_t)w.chunks * d->N);
-    w.product = std::max(product_bytes(cus, d->M, d->K, d->N, false, true, false, or_row(d->ldw, d->K) % 2 != 0),
-                         product_bytes(cus, d->N, d->K, d->M, true, true, false, or_row(d->ldx, d->K) % 2 != 0));
+    w.product = std::max(reserve(cus, d->M, d->K, d->N, false, true, false, or_row(d->ldw, d->K) % 2 != 0, false, d->odd & OZ_ODD_W),
+                         reserve(cus, d->N, d->K, d->M, true, true, false, or_row(d->ldx, d->K) % 2 != 0, false, d->odd & OZ_ODD_X));
     w.bytes = w.dz + w.sums + w.product;
     return w;
 }
+
+// Whether dY's rows begin at even addresses, as the descriptor says it.
+bool even_dy(const oz_linear_grad_desc* d) { return or_row(d->lddy, d->N) % 2 == 0 && !(d->odd & OZ_ODD_DY); }
 
 int cus_of(const oz_dev* dev) { return dev && dev->cus > 0 ? dev->cus : 256; }
 
@@ -382,7 +397,8 @@ extern "C" {
 
 long long oz_linear_workspace(oz_dev* dev, const oz_linear_desc* d) {
     if (const char* e = refuse(d)) return oz::fail(dev, OZ_ERR_ARG, "oz_linear: %s", e);
-    return (long long)product_bytes(cus_of(dev), d->M, d->N, d->K, false, false, or_row(d->ldx, d->K) % 2 != 0, or_row(d->ldw, d->K) % 2 != 0);
+    return (long long)reserve(cus_of(dev), d->M, d->N, d->K, false, false, or_row(d->ldx, d->K) % 2 != 0, or_row(d->ldw, d->K) % 2 != 0,
+                              d->odd & OZ_ODD_X, d->odd & OZ_ODD_W);
 }
 
 int oz_linear(oz_dev* dev, const oz_linear_desc* d, const void* X, const void* W, const void* bias,
@@ -407,7 +423,7 @@ int oz_linear(oz_dev* dev, const oz_linear_desc* d, const void* X, const void* W
 
 long long oz_linear_grad_workspace(oz_dev* dev, const oz_linear_grad_desc* d) {
     if (const char* e = refuse(d)) return oz::fail(dev, OZ_ERR_ARG, "oz_linear_grad: %s", e);
-    return (long long)grad_work(cus_of(dev), d, or_row(d->lddy, d->N) % 2 == 0).bytes;
+    return (long long)grad_work(cus_of(dev), d, even_dy(d)).bytes;
 }
 
 int oz_linear_grad(oz_dev* dev, const oz_linear_grad_desc* d, const void* dY, const void* X, const void* W,
@@ -419,7 +435,7 @@ int oz_linear_grad(oz_dev* dev, const oz_linear_grad_desc* d, const void* dY, co
     if (misaligned(dY, d->type) || misaligned(X, d->type) || misaligned(W, d->type) || misaligned(Z, d->type) ||
         misaligned(dX, d->type) || misaligned(dW, d->dw_type) || misaligned(dbias, d->dw_type))
         return oz::fail(dev, OZ_ERR_ARG, "oz_linear_grad: operands at addresses that their types do not allow");
-    const size_t least = grad_work(cus_of(dev), d, or_row(d->lddy, d->N) % 2 == 0).bytes;
+    const size_t least = grad_work(cus_of(dev), d, even_dy(d)).bytes;
     if (!work || bytes < least || misaligned16(work))
         return oz::fail(dev, OZ_ERR_ARG, "oz_linear_grad: workspace of %zu bytes, %zu needed (16-byte aligned)", bytes, least);
     if (int st = oz::use(dev)) return st;

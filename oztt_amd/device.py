@@ -96,6 +96,7 @@ def crt_desc(moduli, b: int, nd: int) -> CrtDesc:
 
 TYPES = {"bf16": 0, "f16": 1, "f32": 2}
 ACTS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+ODD = {"X": 1, "W": 2, "dY": 4}
 ADAMW_BLOCK = 64
 
 
@@ -107,12 +108,12 @@ def _number(names: dict, name) -> int:
 
 class LinearDesc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int) for n in ("M", "N", "K", "type", "y_type", "act")] + \
-               [(n, ctypes.c_longlong) for n in ("ldx", "ldw", "ldy", "ldr", "ldz")]
+               [(n, ctypes.c_longlong) for n in ("ldx", "ldw", "ldy", "ldr", "ldz")] + [("odd", ctypes.c_int)]
 
 
 class LinearGradDesc(ctypes.Structure):
     _fields_ = [(n, ctypes.c_int) for n in ("M", "N", "K", "type", "dw_type", "act", "accumulate")] + \
-               [(n, ctypes.c_longlong) for n in ("lddy", "ldx", "ldw", "ldz", "lddx", "lddw")]
+               [(n, ctypes.c_longlong) for n in ("lddy", "ldx", "ldw", "ldz", "lddx", "lddw")] + [("odd", ctypes.c_int)]
 
 
 class EmbeddingDesc(ctypes.Structure):
@@ -136,17 +137,20 @@ class AdamwOptions(ctypes.Structure):
                [("step", ctypes.c_longlong), ("seed", ctypes.c_uint32), ("grad_scale", ctypes.c_void_p)]
 
 
-def linear_desc(M, N, K, type="bf16", act="none", y_type=None, ldx=0, ldw=0, ldy=0, ldr=0, ldz=0) -> LinearDesc:
-    """Sizes and types of Device.linear; y_type None: `type`, a leading dimension of 0: the row length."""
+def linear_desc(M, N, K, type="bf16", act="none", y_type=None, ldx=0, ldw=0, ldy=0, ldr=0, ldz=0, odd=()) -> LinearDesc:
+    """Sizes and types of Device.linear; y_type None: `type`, a leading dimension of 0: the row length. odd: those of "X" and "W"
+    whose address is no multiple of 4 bytes; the workspace then has room for their copies."""
     t = _number(TYPES, type)
-    return LinearDesc(M, N, K, t, t if y_type is None else _number(TYPES, y_type), _number(ACTS, act), ldx, ldw, ldy, ldr, ldz)
+    return LinearDesc(M, N, K, t, t if y_type is None else _number(TYPES, y_type), _number(ACTS, act), ldx, ldw, ldy, ldr, ldz,
+                      sum(_number(ODD, o) for o in set(odd)))
 
 
 def linear_grad_desc(M, N, K, type="bf16", act="none", dw_type=None, accumulate=False, lddy=0, ldx=0, ldw=0, ldz=0,
-                     lddx=0, lddw=0) -> LinearGradDesc:
+                     lddx=0, lddw=0, odd=()) -> LinearGradDesc:
+    """Those of Device.linear_grad; odd: as above, of "X", "W" and "dY"."""
     t = _number(TYPES, type)
     return LinearGradDesc(M, N, K, t, t if dw_type is None else _number(TYPES, dw_type), _number(ACTS, act),
-                          int(accumulate), lddy, ldx, ldw, ldz, lddx, lddw)
+                          int(accumulate), lddy, ldx, ldw, ldz, lddx, lddw, sum(_number(ODD, o) for o in set(odd)))
 
 
 def embedding_desc(T, vocab, D, type="bf16", id_bits=64, scale=1.0, grad_type=None, accumulate=False, padding=-1, ldt=0,
