@@ -25,8 +25,9 @@ __global__ void __launch_bounds__(256) product_any_kernel(const ozl::Product a) 
     constexpr int LD = 40;  // 16-byte rows, on other banks each
     __shared__ __attribute__((aligned(16))) T lq[64 * LD], lp[64 * LD];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const unsigned across = (unsigned)((a.np + 63) / 64);
-    const long long q0 = 64ll * (blockIdx.x / across), p0 = 64ll * (blockIdx.x % across);
+    const long long across = (a.np + 63) / 64, tile = blockIdx.x + (long long)gridDim.x * blockIdx.y;
+    const long long q0 = 64 * (tile / across), p0 = 64 * (tile % across);
+    if (q0 >= a.nq) return;
     const T* Q = static_cast<const T*>(a.Q);
     const T* P = static_cast<const T*>(a.P);
     const int wq = 32 * (wave >> 1), wp = 32 * (wave & 1), r = lane & 15, g = lane >> 4;
@@ -174,7 +175,7 @@ struct Layout {
     long long rows, cols, ld, ldd;
 };
 __global__ void __launch_bounds__(256) lay_out_kernel(Layout a, Layout b, long long pieces_a, long long pieces_b) {
-    long long i = 256ll * blockIdx.x + threadIdx.x;
+    long long i = 256 * (blockIdx.x + (long long)gridDim.x * blockIdx.y) + threadIdx.x;
     const bool first = i < pieces_a;
     if (!first) i -= pieces_a;
     if (!first && i >= pieces_b) return;
@@ -194,7 +195,13 @@ __global__ void __launch_bounds__(256) lay_out_kernel(Layout a, Layout b, long l
     *reinterpret_cast<u32x4*>(l.dst + row * l.ldd + col) = x.w;
 }
 
-constexpr long long kMaxTiles = 1ll << 23;  // workgroups of 256 threads in one launch
+// A grid of at least `groups` workgroups of 256 threads: along x 2^31 threads, the rest along y. The kernels go by
+// blockIdx.x + gridDim.x blockIdx.y and leave what is too much.
+dim3 grid_of(long long groups) {
+    const long long x = std::min(groups, 1ll << 23);
+    return dim3((unsigned)x, (unsigned)((groups + x - 1) / x));
+}
+constexpr long long kMaxGroups = (1ll << 24) - 1;  // workgroups of 256 threads along x
 
 // Whether rows begin at multiples of 4 bytes, as the tiles' copies need them.
 bool even_rows(const void* p, long long ld) { return !((uintptr_t)p & 3) && ld % 2 == 0; }
@@ -215,7 +222,7 @@ struct Route {
 // partly filled one, not less than the operands take from memory (4.6 TB/s), and the join's launch and traffic (8 bytes an
 // output and range at 4 TB/s).
 float estimate(const Shape& t, int cus, long long nq, long long np, long long C, int splits) {
-    const long long tiles = (nq + t.q - 1) / t.q * ((np + t.p - 1) / t.p) * splits, slots = (long long)cus * t.per_cu;
+    const long long tiles = tiles_of(t, nq, np, splits), slots = (long long)cus * t.per_cu;
     const float stages = (float)(((C + 63) / 64 + splits - 1) / splits);
     const long long rest = tiles % slots;
     float us = (float)(tiles / slots) * (t.fixed + stages * t.full);
@@ -242,7 +249,7 @@ Route route_of(int cus, long long nq, long long np, long long C, bool contiguous
         float best = 0.0f;
         for (int t = 0; t < TILES; t++)
             for (int s = 1; s <= 16; s *= 2) {
-                if (s > 1 && (C + 63) / 64 / s < 4) break;
+                if ((s > 1 && (C + 63) / 64 / s < 4) || !fits(shape_of((Tile)t), nq, np, s)) break;
                 const float us = estimate(shape_of((Tile)t), cus, nq, np, C, s);
                 if (best == 0.0f || us < best) best = us, r.tile = (Tile)t, r.splits = s;
             }
@@ -252,9 +259,7 @@ Route route_of(int cus, long long nq, long long np, long long C, bool contiguous
 }
 
 int launch_any(oz_dev* dev, int type, const Product& a) {
-    const long long tiles = (long long)oz::ceil_div(a.np, 64) * oz::ceil_div(a.nq, 64);
-    if (tiles > kMaxTiles) return oz::fail(dev, OZ_ERR_ARG, "a product of %lld x %lld outputs is too large", a.nq, a.np);
-    const dim3 grid((unsigned)tiles);
+    const dim3 grid = grid_of((long long)oz::ceil_div(a.np, 64) * oz::ceil_div(a.nq, 64));
     if (type == OZ_BF16) hipLaunchKernelGGL(product_any_kernel<OZ_BF16>, grid, dim3(256), 0, dev->stream, a);
     else hipLaunchKernelGGL(product_any_kernel<OZ_F16>, grid, dim3(256), 0, dev->stream, a);
     return oz::launch_check(dev, "product_any_kernel");
@@ -297,8 +302,7 @@ int launch_product(oz_dev* dev, int type, Product a, void* work, size_t bytes) {
     a.ldparts = (a.np + 7) / 8 * 8;
     at += r.parts;
     if (r.few) return launch_few_rows(dev, type, a);
-    const long long tiles = (long long)oz::ceil_div(a.np, shape_of(r.tile).p) * oz::ceil_div(a.nq, shape_of(r.tile).q) * r.splits;
-    if (tiles > kMaxTiles) return oz::fail(dev, OZ_ERR_ARG, "a product of %lld x %lld outputs is too large", a.nq, a.np);
+    if (!fits(shape_of(r.tile), a.nq, a.np, r.splits)) return oz::fail(dev, OZ_ERR_ARG, "a product of %lld x %lld outputs is too large", a.nq, a.np);
     if (copy_q || copy_p) {
         Layout l[2] = {};
         long long pieces[2] = {};
@@ -312,9 +316,7 @@ int launch_product(oz_dev* dev, int type, Product a, void* work, size_t bytes) {
         };
         if (copy_q) lay(a.Q, a.ldq, a.nq, a.q_major, 0);
         if (copy_p) lay(a.P, a.ldp, a.np, a.p_major, 1);
-        const long long groups = (pieces[0] + pieces[1] + 255) / 256;
-        if (groups > kMaxTiles) return oz::fail(dev, OZ_ERR_ARG, "operands of %lld and %lld rows are too large to lay out", l[0].rows, l[1].rows);
-        hipLaunchKernelGGL(lay_out_kernel, dim3((unsigned)groups), dim3(256), 0, dev->stream, l[0], l[1], pieces[0], pieces[1]);
+        hipLaunchKernelGGL(lay_out_kernel, grid_of((pieces[0] + pieces[1] + 255) / 256), dim3(256), 0, dev->stream, l[0], l[1], pieces[0], pieces[1]);
         if (int st = oz::launch_check(dev, "lay_out_kernel")) return st;
     }
     return launch_tile(dev, type, r.tile, a);
@@ -452,7 +454,7 @@ int oz_linear_grad(oz_dev* dev, const oz_linear_grad_desc* d, const void* dY, co
         void* rest = make && w.two && dW ? at + w.part : nullptr;
         float* sums = dbias ? reinterpret_cast<float*>(at + w.dz) : nullptr;
         const int strips = (int)oz::ceil_div(d->N, 8 * w.lanes), chunks = d->M ? w.chunks : 0;
-        if ((long long)strips * w.chunks > kMaxTiles) return oz::fail(dev, OZ_ERR_ARG, "oz_linear_grad: %d x %d outputs are too many", d->M, d->N);
+        if ((long long)strips * w.chunks > kMaxGroups) return oz::fail(dev, OZ_ERR_ARG, "oz_linear_grad: %d x %d outputs are too many", d->M, d->N);
         const bool one = chunks == 1;
         if (chunks) {
             const dim3 grid((unsigned)(strips * chunks));

@@ -70,6 +70,7 @@ __device__ __forceinline__ void finish8(const Epilogue& e, long long np, long lo
 enum Tile { T256, T128, T64, T64X32, T32, TILES };
 struct Shape {
     int q, p;            // outputs
+    int threads;         // of a workgroup
     int per_cu;          // workgroups that a CU holds (LDS)
     float alone, full;   // us for a stage of 64 values of c: one workgroup on a CU, per_cu of them
     float fixed;         // us from the first copy to the first product, and from the last to the outputs
@@ -79,10 +80,14 @@ struct Shape {
 // 28.7), 1024^3 by 64 x 64 (7.5), 64 rows of 2048^2 by 32 x 32.
 inline const Shape& shape_of(Tile t) {
     static const Shape shapes[TILES] = {
-        {256, 256, 1, 1.42f, 1.42f, 20.0f}, {128, 128, 2, 0.58f, 0.85f, 5.8f}, {64, 64, 2, 0.21f, 0.32f, 4.0f},
-        {64, 32, 2, 0.20f, 0.28f, 3.9f},    {32, 32, 2, 0.18f, 0.22f, 3.4f}};
+        {256, 256, 256, 1, 1.42f, 1.42f, 20.0f}, {128, 128, 512, 2, 0.58f, 0.85f, 5.8f}, {64, 64, 256, 2, 0.21f, 0.32f, 4.0f},
+        {64, 32, 128, 2, 0.20f, 0.28f, 3.9f},    {32, 32, 128, 2, 0.18f, 0.22f, 3.4f}};
     return shapes[t];
 }
+// A launch takes fewer than 2^32 threads along a dimension of its grid. The products of 2^31 - 1 rows that memory holds fit it with
+// the largest tile.
+inline long long tiles_of(const Shape& t, long long nq, long long np, int splits) { return (nq + t.q - 1) / t.q * ((np + t.p - 1) / t.p) * splits; }
+inline bool fits(const Shape& t, long long nq, long long np, int splits) { return tiles_of(t, nq, np, splits) * t.threads < 1ll << 32; }
 int launch_tile(oz_dev* dev, int type, Tile tile, const Product& a);
 // At most 32 rows of Q, operands along c at any address; splits as in Product (1 for at most kStreamRows). A workgroup has
 // few_rows_block rows of P.
