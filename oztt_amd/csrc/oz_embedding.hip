@@ -9,12 +9,24 @@
 #include "oz_internal.hpp"
 #include "oz_types.hpp"
 
+#include <algorithm>
+
 namespace {
 
 using namespace ozt;
 
 constexpr long long kMaxD = 1ll << 22;
-constexpr long long kMaxGroups = 1ll << 23;  // workgroups of 256 threads in one launch
+
+// Workgroups of 256 threads: 2^23 along x (a launch takes fewer than 2^32 threads along a dimension), the rest along y. What is too
+// much of the last row finds no work.
+constexpr int ROW_LOG = 23;
+dim3 grid_of(long long groups) {
+    const long long x = std::max(1ll, std::min(groups, 1ll << ROW_LOG));
+    return dim3((unsigned)x, (unsigned)((groups + x - 1) / x));
+}
+__device__ __forceinline__ long long wave_number() {
+    return 4 * (((long long)blockIdx.y << ROW_LOG) + blockIdx.x) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+}
 
 struct Shape {
     long long T, vocab, ldt, ldo, padding;
@@ -106,7 +118,7 @@ struct Ahead {
 template <int TYPE, bool SMALL, bool NARROW>
 __global__ void __launch_bounds__(256) embedding_kernel(const void* __restrict__ table, const void* __restrict__ ids,
                                                         void* __restrict__ out, uint32_t* __restrict__ flags, Shape s, unsigned slices, int rows_log) {
-    const long long wave = 4ll * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long long wave = wave_number();
     const int lane = threadIdx.x & ((64u >> (NARROW ? rows_log : 0)) - 1);
     long long t;
     int c0 = 0;
@@ -396,7 +408,7 @@ __global__ void __launch_bounds__(256) sums_kernel(const void* __restrict__ dOut
                                                    const uint32_t* __restrict__ order, void* __restrict__ table,
                                                    float* __restrict__ parts, Shape s, int R, unsigned slices) {
     const int lane = threadIdx.x & 63;
-    const long long item = 4ll * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = item / slices;
+    const long long item = wave_number(), r = item / slices;
     const long long begin = r * R, end = begin + R < s.T ? begin + R : s.T;
     if (begin >= s.T) return;
     const Columns cols((int)(item - r * slices) * 512, lane, s.D);
@@ -456,7 +468,7 @@ template <bool SMALL>
 __global__ void __launch_bounds__(256) join_kernel(const uint32_t* __restrict__ keys, void* __restrict__ table,
                                                    const float* __restrict__ parts, Shape s, int R, unsigned slices) {
     const int lane = threadIdx.x & 63;
-    const long long item = 4ll * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = item / slices;
+    const long long item = wave_number(), r = item / slices;
     const long long begin = r * R, end = begin + R;
     if (end >= s.T) return;
     const uint32_t key = keys[end - 1];
@@ -575,13 +587,12 @@ int oz_embedding(oz_dev* dev, const oz_embedding_desc* d, const void* table, con
     int rows_log = 0;
     while (rows_log < 6 && s.D <= 256 >> rows_log) rows_log++;
     const long long per = 4ll << rows_log, groups = (s.T * slices + per - 1) / per;
-    if (groups > kMaxGroups) return oz::fail(dev, OZ_ERR_ARG, "oz_embedding: %lld tokens of %d values are too many", s.T, s.D);
     if (int st = oz::use(dev)) return st;
     if (!s.T) return OZ_OK;
     const auto kernel = s.type == OZ_F32   ? lookup_of<OZ_F32>(s.D, rows_log)
                         : s.type == OZ_F16 ? lookup_of<OZ_F16>(s.D, rows_log)
                                            : lookup_of<OZ_BF16>(s.D, rows_log);
-    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), 0, dev->stream, table, ids, out, flags, s, slices, rows_log);
+    hipLaunchKernelGGL(kernel, grid_of(groups), dim3(256), 0, dev->stream, table, ids, out, flags, s, slices, rows_log);
     return oz::launch_check(dev, "embedding_kernel");
 }
 
@@ -602,7 +613,6 @@ int oz_embedding_grad(oz_dev* dev, const oz_embedding_desc* d, const void* dOut,
         return oz::fail(dev, OZ_ERR_ARG, "oz_embedding_grad: workspace of %zu bytes, %zu needed (16-byte aligned)", bytes, w.bytes);
     const unsigned slices = oz::ceil_div(s.D, 512);
     const long long groups = (w.runs * slices + 3) / 4;
-    if (groups > kMaxGroups) return oz::fail(dev, OZ_ERR_ARG, "oz_embedding_grad: %lld tokens of %d values are too many", s.T, s.D);
     if (int st = oz::use(dev)) return st;
     hipStream_t q = dev->stream;
     // workgroups that write zeros, in each launch: at most 8 a CU, 16 pieces of 16 bytes a thread or more
@@ -625,9 +635,9 @@ int oz_embedding_grad(oz_dev* dev, const oz_embedding_desc* d, const void* dOut,
     const auto sums = s.type == OZ_F32 ? (small ? sums_kernel<OZ_F32, true> : sums_kernel<OZ_F32, false>)
                       : s.type == OZ_F16 ? (small ? sums_kernel<OZ_F16, true> : sums_kernel<OZ_F16, false>)
                                          : (small ? sums_kernel<OZ_BF16, true> : sums_kernel<OZ_BF16, false>);
-    hipLaunchKernelGGL(sums, dim3((unsigned)groups), block, 0, q, dOut, keys[sorted], order[sorted], dTable, parts, s, w.R, slices);
+    hipLaunchKernelGGL(sums, grid_of(groups), block, 0, q, dOut, keys[sorted], order[sorted], dTable, parts, s, w.R, slices);
     if (w.runs > 1)  // otherwise nothing is cut
-        hipLaunchKernelGGL(small ? join_kernel<true> : join_kernel<false>, dim3((unsigned)groups), block, 0, q, keys[sorted], dTable, parts, s, w.R, slices);
+        hipLaunchKernelGGL(small ? join_kernel<true> : join_kernel<false>, grid_of(groups), block, 0, q, keys[sorted], dTable, parts, s, w.R, slices);
     return oz::launch_check(dev, "embedding gradient");
 }
 
