@@ -30,6 +30,13 @@ def test_the_rule_takes_tiles_that_a_launch_holds(M, N, K):
         assert -(-nq // q) * -(-np // p) * s.value * threads < 2**32, (t, s.value)
 
 
+@pytest.fixture
+def memory():
+    """Up to 70 GB a test are given back."""
+    yield
+    torch.cuda.empty_cache()
+
+
 def check(dev, M, K, X, W, Y, **kw):
     d = ozd.linear_desc(M, 1, K, **kw)
     n = dev.linear_workspace(d)
@@ -41,7 +48,7 @@ def check(dev, M, K, X, W, Y, **kw):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("M,shift", [(TOP, 0), (2**29 + 100, 1)])
-def test_as_many_rows_as_there_may_be(dev, M, shift):
+def test_as_many_rows_as_there_may_be(dev, memory, M, shift):
     """All rows that an int counts; and more than 2^29 at an odd address, which the kernel that reads value by value takes."""
     print("linear", M, shift, flush=True)
     base = torch.empty(M + shift, dtype=torch.bfloat16, device="cuda:0")
@@ -55,7 +62,7 @@ def test_as_many_rows_as_there_may_be(dev, M, shift):
 
 
 @pytest.mark.gpu
-def test_an_operand_of_more_pieces_than_a_row_of_a_grid(dev):
+def test_an_operand_of_more_pieces_than_a_row_of_a_grid(dev, memory):
     """2^22 rows of 4097 values, which are laid out first: 2^23 workgroups and more."""
     M, K = 2**22, 4097
     print("linear", M, K, flush=True)
