@@ -107,7 +107,7 @@ class Network:
         loss = float(-np.log(p[rows, targets]).mean())
         p[rows, targets] -= 1
         self.gradients(ids, p / len(ids))
-        self.dev.adamw_step(self.plan, lr, 0.9, 0.95, 1e-8, number, number)
+        self.dev.adamw_step(self.plan, lr, 0.9, 0.95, 1e-8, number)
         return loss
 
 

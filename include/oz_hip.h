@@ -470,7 +470,9 @@ int oz_adamw_make_plan(oz_dev* dev, const oz_adamw_tensor* tensors, int count, i
 typedef struct oz_adamw_options {
     double lr, beta1, beta2, eps;
     long long step;          /* from 1 */
-    uint32_t seed;           /* of the random bits; another one for each step */
+    uint32_t seed;           /* of the random bits: another one for each step, spread over 32 bits, such as mix(step). With
+                              * small numbers, the step itself among them, an aligned group of places draws the same set
+                              * of bits every time, dealt out anew, and its mean rounding error adds up. */
     const float* grad_scale; /* one device value that every gradient is multiplied by, or null */
 } oz_adamw_options;
 int oz_adamw_step(oz_dev* dev, const oz_adamw_plan* plan, const oz_adamw_options* o);

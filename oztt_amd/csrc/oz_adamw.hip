@@ -50,6 +50,8 @@ __device__ __forceinline__ void from_e4m3(uint32_t w, float* x) {
 __device__ __forceinline__ float power(int e) { return __uint_as_float(e < -126 ? 0x00400000u : (uint32_t)(e + 127) << 23); }
 __device__ __forceinline__ int exponent(float x) { return (int)(__float_as_uint(x) >> 23) - 127; }  // x >= 0
 
+// The header's hash: two rounds of shift, xor and odd product, a bijection of 32 bits, its shifts and factors those that C. Wellons'
+// search for such hashes of low bias published in 2018.
 __device__ __forceinline__ uint32_t mix(uint32_t x) {
     x ^= x >> 16;
     x *= 0x7FEB352Du;

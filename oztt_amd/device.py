@@ -167,6 +167,16 @@ def adamw_tensor(n, param, grad, m, v, master=0, m_scale=0, v_scale=0, param_typ
                        _number(TYPES, grad_type), weight_decay)
 
 
+def adamw_seed(step: int) -> int:
+    """The seed of a step's random bits: the hash that gives the bits, of the step's 32 lower bits and the hash of those above."""
+    def mix(x: int) -> int:
+        x = ((x ^ (x >> 16)) * 0x7FEB352D) & 0xFFFFFFFF
+        x = ((x ^ (x >> 15)) * 0x846CA68B) & 0xFFFFFFFF
+        return x ^ (x >> 16)
+
+    return mix((step & 0xFFFFFFFF) ^ mix((step >> 32) & 0xFFFFFFFF))
+
+
 def _at(buf) -> ctypes.c_void_p:
     return buf.ptr if buf is not None else ctypes.c_void_p()
 
@@ -406,8 +416,10 @@ class Device:
         plan.buffer = memory
         return plan
 
-    def adamw_step(self, plan: AdamwPlan, lr, beta1=0.9, beta2=0.999, eps=1e-8, step=1, seed=0, grad_scale=None):
-        o = AdamwOptions(lr, beta1, beta2, eps, step, seed, _at(grad_scale))
+    def adamw_step(self, plan: AdamwPlan, lr, beta1=0.9, beta2=0.999, eps=1e-8, step=1, seed=None, grad_scale=None):
+        """One step (from 1) of the plan's tensors. seed: 32 bits for the rounding of 8-bit states, spread and another for
+        each step; None: adamw_seed(step)."""
+        o = AdamwOptions(lr, beta1, beta2, eps, step, adamw_seed(step) if seed is None else seed, _at(grad_scale))
         self._check(hip().oz_adamw_step(self.h, ctypes.byref(plan), ctypes.byref(o)), "oz_adamw_step")
 
     def crt(self, C: Buffer, M, N, ldc, sC, desc: CrtDesc, dA: Buffer, dB: Buffer, out: Buffer, ldo):
