@@ -2,7 +2,8 @@
 //
 // Every value is independent but for the scale that the 64 values of a block share in 8-bit states, so the
 // step is one pass over memory: 28 bytes a value with 32-bit states (BF16 param and gradient, FP32 master),
-// 16 with 8-bit ones; 1e8 values take 522 us (5.4 TB/s) and 320 us (5.0 TB/s). A workgroup takes one chunk of one tensor, found in the plan's list; a lane takes 8 values
+// 16 with 8-bit ones; 1e8 values take 522 us (5.4 TB/s) and 320 us (5.0 TB/s; the VALU counts too: 360 to 410 us in long rows of passes, whose clock
+// falls to 1.8 GHz). A workgroup takes one chunk of one tensor, found in the plan's list; a lane takes 8 values
 // in a row (one or two 16-byte accesses of every array, 8 bytes of 8-bit states), so 8 neighbouring lanes hold a
 // block and its maximum is three exchanges away. The file is compiled without contraction: the order of
 // operations is the header's, each rounded once.

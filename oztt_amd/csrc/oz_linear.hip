@@ -234,10 +234,13 @@ float estimate(const Shape& t, int cus, long long nq, long long np, long long C,
 
 // Few rows: their own kernels, c in ranges where 16 rows of W each are too few to keep the CUs reading (at least 512 values a
 // range). 5 rows, 512 of W, K = 8192: 8.0 us in four ranges, 9.1 in one.
-// More: the tile and ranges with the least estimate; measured against the other tiles and numbers of ranges, the choice is the
-// fastest or within 10% of it: 1000 x 704 x 1504 10.1 us by 64 x 64 (17 by 128 x 128), 2048 x 4096 x 4096 62 by 128 x 128 (70 by 256 x
-// 256 in two ranges, 98 by 64 x 64), 256 x 1024 x 8192 15.5 by 64 x 64 in 4 ranges (38 in one), 3500^3 88 by 256 x 256 (120 by 128 x
-// 128), 8192^2 of K = 512 101 by 128 x 128 (124 by 256 x 256). 256 x 8192^2 takes 70 by 64 x 64 where 256 x 256 in 8 ranges takes 61.
+// More: the tile and ranges with the least estimate; 1000 x 704 x 1504 10.1 us by 64 x 64 (17 by 128 x 128), 2048 x 4096 x 4096 62
+// by 128 x 128 (70 by 256 x 256 in two ranges, 98 by 64 x 64), 256 x 1024 x 8192 15.5 by 64 x 64 in 4 ranges (38 in one), 3500^3 88 by
+// 256 x 256 (120 by 128 x 128), 8192^2 of K = 512 101 by 128 x 128 (124 by 256 x 256). Measured against all other tiles and numbers
+// of ranges at 52 sizes, the choice is the fastest or up to 9% slower at 50 of them with operands in the caches and at 46 without.
+// It is further off where c is long and tiles are few, as the estimate takes their stages for shorter than they are: without caches
+// 512 x 8192^2 96 us for 81 by 256 x 256 in 4 ranges, 256 x 8192^2 73 (estimate: 45) for 64 by 128 x 128 in 4, and of few rows 16 x
+// 8192^2 36 for 30 by 32 x 32.
 Route route_of(int cus, long long nq, long long np, long long C, bool contiguous, bool even) {
     Route r{};
     r.splits = 1;

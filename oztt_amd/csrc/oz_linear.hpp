@@ -75,7 +75,7 @@ struct Shape {
     float alone, full;   // us for a stage of 64 values of c: one workgroup on a CU, per_cu of them
     float fixed;         // us from the first copy to the first product, and from the last to the outputs
 };
-// Fitted to times on 256 CUs in BF16: 4096^2 of K = 256 and 1024 and 8192^2 of 512 by 256 x 256 tiles (25.8, 42.8 and 124 us) and
+// Fitted to times of passes over the same operands on 256 CUs in BF16: 4096^2 of K = 256 and 1024 and 8192^2 of 512 by 256 x 256 tiles (25.8, 42.8 and 124 us) and
 // by 128 x 128 (18.4, 38.5 and 101), 2048^2 of K = 512 and 2048 by 128 x 128 (10.2, 24.1; one workgroup a CU) and by 64 x 64 (13.2,
 // 28.7), 1024^3 by 64 x 64 (7.5), 64 rows of 2048^2 by 32 x 32.
 inline const Shape& shape_of(Tile t) {
