@@ -477,6 +477,102 @@ typedef struct oz_adamw_options {
 } oz_adamw_options;
 int oz_adamw_step(oz_dev* dev, const oz_adamw_plan* plan, const oz_adamw_options* o);
 
+/* ---- 8-bit integers with a scale for each row --------------------------------------------------------
+ * Row m of X (M x K) as integers of -127 to 127 and a scale, X = Q scale: with a the largest of the row's |x|, and at
+ * least 127 2^-126,
+ *   scale = a / 127,  Q = x (127 / a) rounded to the nearest integer, ties to even,
+ * quotients and products in FP32. A row with a value that is not finite gives a NaN as scale, and zeros. Activations are quantized
+ * by token, weights (N x K, a row for each output) by channel. Rows of Q are ldq bytes apart, what lies between them is left as it
+ * is. M may be 0. */
+typedef struct oz_quantize_desc {
+    long long M;        /* up to 2^31 - 1 */
+    int K, type;        /* K from 1 to 2^22; oz_type of X: any */
+    long long ldx, ldq; /* 0: K */
+} oz_quantize_desc;
+int oz_quantize_rows(oz_dev* dev, const oz_quantize_desc* d, const void* X, int8_t* Q, float* scale);
+
+/* ---- product of 8-bit integers with bias, activation and residual --------------------------------------
+ * Y = act(w_scale_n x_scale_m sum_k Xq_mk Wq_nk + bias_n) + residual: oz_linear for answering, with weights of half the bytes and the
+ * INT8 matrix cores. W: N x K bytes with N scales, as oz_quantize_rows gives them. X is M x K bytes with M scales (x_int8), or M x K
+ * values of `type`, which the call quantizes in the same way. The sums are exact in int32, whatever the bytes, for K up to 131071;
+ * they are rounded to FP32 and multiplied by w_scale and x_scale in turn. bias (N values of `type`) and residual (M x N) may
+ * be null. Rows of 8-bit operands begin at multiples of 4 bytes (addresses and leading dimensions that are none are refused),
+ * what lies behind a row's K values may be anything. M may be 0. residual may be Y itself (the same leading dimension). */
+typedef struct oz_linear_i8_desc {
+    int M, N, K;
+    int type;   /* oz_type of X and bias: OZ_BF16 or OZ_F16 */
+    int y_type; /* oz_type of Y and residual: type or OZ_F32 */
+    int act;    /* oz_act */
+    int x_int8; /* 1: X is 8-bit integers */
+    long long ldx, ldw, ldy, ldr; /* in values of their operand (0: the row length) */
+} oz_linear_i8_desc;
+/* Bytes of workspace, or a negative oz_status where the descriptor is refused. */
+long long oz_linear_i8_workspace(oz_dev* dev, const oz_linear_i8_desc* d);
+int oz_linear_i8(oz_dev* dev, const oz_linear_i8_desc* d, const void* X, const float* x_scale, const int8_t* W,
+                 const float* w_scale, const void* bias, const void* residual, void* Y, void* work, size_t bytes);
+
+/* ---- orthogonalized matrices -----------------------------------------------------------------------
+ * O = the Newton-Schulz iteration's result on each of `count` matrices G (rows x cols, row-major): with X = G / (|G|_F + eps),
+ * steps times X <- a X + (b A + c A^2) X, A = X X^T (from the right, with A = X^T X, where rows > cols), which moves
+ * singular values s by a s + b s^3 + c s^5: with a, b, c = 3.4445, -4.7750, 2.0315 and 5 steps near 1, but for those that are
+ * zero or nearly so. The norm is summed in FP64, the iteration's products in FP32; X is kept in 22 bits. A BF16
+ * result of more than 512 rows and columns takes products of 11 bits and is off by up to 2e-3 of its norm before it is rounded, all
+ * others products of 22 bits: 1e-5 of its norm. (To both comes what rounding X leaves in directions of singular values near zero, which
+ * a step makes a times larger: a^steps 2^-22 sqrt(steps) of the sum of squares' root, 1.3e-4.) X's values must stay below 16 (with the factors above they
+ * stay below 1.3). A matrix of zeros gives zeros, one with a value that is not finite NaN. O may be G itself (the same type
+ * and strides); matrices do not overlap each other. count may be 0. */
+typedef struct oz_orthogonalize_desc {
+    int rows, cols, count; /* rows and cols from 1 to 2^20 */
+    int type;              /* oz_type of G and O: any */
+    int steps;             /* 1 to 100 */
+    double a, b, c, eps;
+    long long ldg, ldo, stride_g, stride_o; /* rows and matrices apart (0: one behind the other) */
+} oz_orthogonalize_desc;
+/* Bytes of workspace, or a negative oz_status where the descriptor is refused. */
+long long oz_orthogonalize_workspace(oz_dev* dev, const oz_orthogonalize_desc* d);
+int oz_orthogonalize(oz_dev* dev, const oz_orthogonalize_desc* d, const void* G, void* O, void* work, size_t bytes);
+
+/* ---- Muon over many matrices ------------------------------------------------------------------------
+ * One step of every matrix p with gradient g, in FP32 but for the iteration's products (as above: those of 11 bits are taken where
+ * both sides are over 512):
+ *   m' = momentum m + (1 - momentum) g grad_scale
+ *   u  = momentum m' + (1 - momentum) g grad_scale (nesterov), or m'
+ *   p' = p (1 - lr weight_decay) - lr lr_scale orthogonalized(u)
+ * With a master, p is the FP32 master and param receives p' rounded; without, p is param itself. Matrices are row-major and without
+ * gaps. A gradient that is not finite makes its whole matrix NaN. */
+#define OZ_MUON_SHAPES 16
+typedef struct oz_muon_tensor {
+    int rows, cols; /* up to 2^20; either may be 0 */
+    void* param;
+    const void* grad;
+    float* master;             /* or null; must be null where param_type is OZ_F32 */
+    float* m;                  /* the momentum; zeros at a first step */
+    int param_type, grad_type; /* oz_type */
+    float weight_decay, lr_scale;
+} oz_muon_tensor;
+/* The plan of a list of matrices (host array) of at most OZ_MUON_SHAPES different sizes: the list by size, copied into device
+ * memory of oz_muon_plan_bytes bytes (16-byte aligned), which the caller keeps unchanged as long as it steps with the plan.
+ * Waits for all work of the device (the memory may have been another stream's) and returns when the copy is done. */
+typedef struct oz_muon_shape {
+    int rows, cols, count, first;
+} oz_muon_shape;
+typedef struct oz_muon_plan {
+    const void* memory;
+    int count, shapes;
+    oz_muon_shape shape[OZ_MUON_SHAPES];
+} oz_muon_plan;
+long long oz_muon_plan_bytes(const oz_muon_tensor* tensors, int count);
+int oz_muon_make_plan(oz_dev* dev, const oz_muon_tensor* tensors, int count, void* memory, size_t bytes, oz_muon_plan* plan);
+/* Bytes of workspace of a step: about 6 for each value of the matrices (10 with products of 22 bits) and 4 (8) of their shorter sides' squares. */
+long long oz_muon_workspace(oz_dev* dev, const oz_muon_plan* plan);
+typedef struct oz_muon_options {
+    double lr, momentum;
+    int nesterov, steps; /* steps as above */
+    double a, b, c, eps;
+    const float* grad_scale; /* one device value that every gradient is multiplied by, or null */
+} oz_muon_options;
+int oz_muon_step(oz_dev* dev, const oz_muon_plan* plan, const oz_muon_options* o, void* work, size_t bytes);
+
 #ifdef __cplusplus
 }
 #endif

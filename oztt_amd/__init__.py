@@ -140,7 +140,8 @@ def hip() -> ctypes.CDLL:
     if _hip is None:
         _hip = _load("liboz_hip.so")
         _hip.oz_last_error.restype = ctypes.c_char_p
-        for name in ("oz_linear_workspace", "oz_linear_grad_workspace", "oz_embedding_grad_workspace", "oz_adamw_plan_bytes"):
+        for name in ("oz_linear_workspace", "oz_linear_grad_workspace", "oz_embedding_grad_workspace", "oz_adamw_plan_bytes", "oz_linear_i8_workspace",
+                     "oz_orthogonalize_workspace", "oz_muon_plan_bytes", "oz_muon_workspace"):
             getattr(_hip, name).restype = ctypes.c_longlong
     return _hip
 

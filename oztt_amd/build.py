@@ -54,6 +54,10 @@ HIP_SOURCES = {
     "oz_linear_tiles.hip": [],
     "oz_embedding.hip": [],
     "oz_adamw.hip": [],
+    "oz_quantize.hip": [],
+    "oz_linear_i8.hip": [],
+    "oz_muon.hip": [],
+    "oz_newton_schulz.hip": [],
 }
 HOST_FLAGS = ["-std=c++20", "-O2", "-fPIC", "-ffp-contract=off", "-fno-fast-math", "-fopenmp",
               "-Wall", "-Wextra", f"-I{INCLUDE}", f"-I{CSRC / 'host'}"]

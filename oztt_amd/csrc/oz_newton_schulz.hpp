@@ -1,0 +1,85 @@
+// The Newton-Schulz iteration over matrices of several sizes at once: what its kernels take (oz_muon.hip, oz_newton_schulz.hip).
+//
+//   X0 = U / (|U|_F + eps);  A = X X^T,  B = b A + c A^2,  X <- a X + B X, `steps` times
+//
+// and from the right (A = X^T X, X <- a X + X B) where a matrix has more rows than columns, so that A has the shorter side.
+// Every singular value s of X0 goes through s <- a s + b s^3 + c s^5; with the usual factors all but the smallest end within 0.7
+// to 1.2.
+//
+// X is held as two FP16 parts, X = h + l, times kScale: together 22 bits. The products read h alone, the term a X both. A gradient has
+// a few strong directions and many weak ones that each step makes a times larger, so what rounding does to X there
+// grows with them: with X in BF16 the result is off by 1e-2 of its norm for a Gaussian matrix and by 0.2 to 0.6 for one of
+// low rank, in FP16 by 1e-3 and 2e-2 to 7e-2. The products do not have that weakness, as B is nearly zero in the directions of small
+// singular values: with both parts in a X the result is off by 1e-4 to 2e-3 whatever the spectrum (64 to 1024 rows, against 64 bits).
+// Where a side is short (the rounding errors of A and B then average over few values: up to 1e-2 at one to four rows) or the result
+// is kept in more than BF16's 8 bits, the products take both parts of both operands, h h + h l + l h: off by 1e-6.
+#pragma once
+#include "oz_types.hpp"
+
+struct oz_dev;
+
+namespace ozn {
+
+constexpr float kScale = 4096.0f;  // X's values are at most about 1: 16 times as large ones still are FP16 numbers
+constexpr int kPad = 64;           // sides in the workspace are multiples of it, the rest zeros, which the iteration keeps
+constexpr int kShapes = OZ_MUON_SHAPES;
+constexpr int kThreeSide = 512;    // up to this shorter side the products take both parts
+
+// `count` matrices of one size. Buffers hold them one after the other, each as one plane of R x C (h) or two (h, l).
+struct Shape {
+    int rows, cols;  // of a matrix
+    int R, C;        // in the workspace
+    int count, first;
+    int three;       // products of both parts
+    int chunks;      // of a matrix, for the sum of its squares
+    _Float16 *x[2], *l, *a, *b;
+    double* sums;
+};
+struct Shapes {
+    int n;
+    Shape s[kShapes];
+};
+// A launch's workgroups: per[s] for each matrix of shape s, the first of shape s is first[s].
+struct Places {
+    int first[kShapes + 1], per[kShapes];
+};
+
+struct Place {
+    int shape, matrix, index;
+};
+__device__ __forceinline__ Place place_of(const Places& p, int n, int w) {
+    int s = 0;
+    while (s + 1 < n && w >= p.first[s + 1]) s++;
+    const int i = w - p.first[s];
+    return {s, i / p.per[s], i % p.per[s]};
+}
+
+__host__ __device__ inline int side_of(const Shape& s) { return s.R < s.C ? s.R : s.C; }
+__host__ __device__ inline bool is_tall(const Shape& s) { return s.rows > s.cols; }
+__device__ __forceinline__ _Float16* h_of(const Shape& s, int b, int i) { return s.x[b] + (long long)(1 + s.three) * i * s.R * s.C; }
+__device__ __forceinline__ _Float16* l_of(const Shape& s, int b, int i) {
+    const long long n = (long long)s.R * s.C;
+    return s.three ? s.x[b] + (2 * i + 1) * n : s.l + i * n;
+}
+// A or B of a matrix
+__device__ __forceinline__ _Float16* square_of(const Shape& s, _Float16* p, int i) { return p + (long long)(1 + s.three) * i * side_of(s) * side_of(s); }
+
+// Where the matrices come from and the results go: one array each (orthogonalize), or a list of tensors (Muon).
+struct Ends {
+    const void* G;
+    void* O;
+    int type;
+    long long ldg, ldo, stride_g, stride_o;
+    const oz_muon_tensor* tensors;
+    float momentum, fresh, lr;  // fresh = 1 - momentum
+    int nesterov;
+    const float* grad_scale;
+};
+struct Factors {
+    float a, b, c;
+};
+
+// The iteration on X0 in the shapes' x[0] (and l), the last step's results to the ends.
+int iterate(oz_dev* dev, const Shapes& m, const Ends& ends, const Factors& f, int steps);
+
+}  // namespace ozn

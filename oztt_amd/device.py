@@ -137,6 +137,42 @@ class AdamwOptions(ctypes.Structure):
                [("step", ctypes.c_longlong), ("seed", ctypes.c_uint32), ("grad_scale", ctypes.c_void_p)]
 
 
+class QuantizeDesc(ctypes.Structure):
+    _fields_ = [("M", ctypes.c_longlong), ("K", ctypes.c_int), ("type", ctypes.c_int), ("ldx", ctypes.c_longlong), ("ldq", ctypes.c_longlong)]
+
+
+class LinearI8Desc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("M", "N", "K", "type", "y_type", "act", "x_int8")] + \
+               [(n, ctypes.c_longlong) for n in ("ldx", "ldw", "ldy", "ldr")]
+
+
+class OrthogonalizeDesc(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("rows", "cols", "count", "type", "steps")] + [(n, ctypes.c_double) for n in ("a", "b", "c", "eps")] + \
+               [(n, ctypes.c_longlong) for n in ("ldg", "ldo", "stride_g", "stride_o")]
+
+
+MUON_SHAPES = 16
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)  # factors that bring all but the smallest singular values near 1 in five steps
+
+
+class MuonTensor(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("rows", "cols")] + [(n, ctypes.c_void_p) for n in ("param", "grad", "master", "m")] + \
+               [("param_type", ctypes.c_int), ("grad_type", ctypes.c_int), ("weight_decay", ctypes.c_float), ("lr_scale", ctypes.c_float)]
+
+
+class MuonShape(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int) for n in ("rows", "cols", "count", "first")]
+
+
+class MuonPlan(ctypes.Structure):
+    _fields_ = [("memory", ctypes.c_void_p), ("count", ctypes.c_int), ("shapes", ctypes.c_int), ("shape", MuonShape * MUON_SHAPES)]
+
+
+class MuonOptions(ctypes.Structure):
+    _fields_ = [("lr", ctypes.c_double), ("momentum", ctypes.c_double), ("nesterov", ctypes.c_int), ("steps", ctypes.c_int)] + \
+               [(n, ctypes.c_double) for n in ("a", "b", "c", "eps")] + [("grad_scale", ctypes.c_void_p)]
+
+
 def linear_desc(M, N, K, type="bf16", act="none", y_type=None, ldx=0, ldw=0, ldy=0, ldr=0, ldz=0, odd=()) -> LinearDesc:
     """Sizes and types of Device.linear; y_type None: `type`, a leading dimension of 0: the row length. odd: those of "X" and "W"
     whose address is no multiple of 4 bytes; the workspace then has room for their copies."""
@@ -158,6 +194,25 @@ def embedding_desc(T, vocab, D, type="bf16", id_bits=64, scale=1.0, grad_type=No
     t = _number(TYPES, type)
     return EmbeddingDesc(T, vocab, D, t, t if grad_type is None else _number(TYPES, grad_type), id_bits, int(accumulate),
                          padding, ldt, ldo, scale)
+
+
+def quantize_desc(M, K, type="bf16", ldx=0, ldq=0) -> QuantizeDesc:
+    return QuantizeDesc(M, K, _number(TYPES, type), ldx, ldq)
+
+
+def linear_i8_desc(M, N, K, type="bf16", act="none", y_type=None, x_int8=False, ldx=0, ldw=0, ldy=0, ldr=0) -> LinearI8Desc:
+    return LinearI8Desc(M, N, K, _number(TYPES, type), _number(TYPES, y_type or type), _number(ACTS, act), int(x_int8), ldx, ldw, ldy, ldr)
+
+
+def orthogonalize_desc(rows, cols, count=1, type="bf16", steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, ldg=0, ldo=0, stride_g=0, stride_o=0) -> OrthogonalizeDesc:
+    return OrthogonalizeDesc(rows, cols, count, _number(TYPES, type), steps, *coefficients, eps, ldg, ldo, stride_g, stride_o)
+
+
+def muon_tensor(rows, cols, param, grad, m, master=0, param_type="f32", grad_type="f32", weight_decay=0.0, lr_scale=None) -> MuonTensor:
+    """A matrix of a Muon step; the arrays by their addresses. lr_scale: None makes the update's values about as large as AdamW's,
+    0.2 sqrt(max(rows, cols))."""
+    lr_scale = 0.2 * max(rows, cols) ** 0.5 if lr_scale is None else lr_scale
+    return MuonTensor(rows, cols, param, grad, master or None, m, _number(TYPES, param_type), _number(TYPES, grad_type), weight_decay, lr_scale)
 
 
 def adamw_tensor(n, param, grad, m, v, master=0, m_scale=0, v_scale=0, param_type="f32", grad_type="f32",
@@ -421,6 +476,50 @@ class Device:
         each step; None: adamw_seed(step)."""
         o = AdamwOptions(lr, beta1, beta2, eps, step, adamw_seed(step) if seed is None else seed, _at(grad_scale))
         self._check(hip().oz_adamw_step(self.h, ctypes.byref(plan), ctypes.byref(o)), "oz_adamw_step")
+
+    def quantize_rows(self, desc: QuantizeDesc, X: Buffer, Q: Buffer, scale: Buffer):
+        """Q and scale: the rows of X as 8-bit integers, X = Q scale."""
+        self._check(hip().oz_quantize_rows(self.h, ctypes.byref(desc), X.ptr, Q.ptr, scale.ptr), "oz_quantize_rows")
+
+    def linear_i8_workspace(self, desc: LinearI8Desc) -> int:
+        return self._bytes(hip().oz_linear_i8_workspace(self.h, ctypes.byref(desc)), "oz_linear_i8_workspace")
+
+    def linear_i8(self, desc: LinearI8Desc, X: Buffer, W: Buffer, w_scale: Buffer, Y: Buffer, x_scale=None, bias=None, residual=None, work=None, work_bytes=0):
+        """Y = act(w_scale x_scale (X W^T) + bias) + residual with 8-bit integers; X is quantized by the call, or has its scales."""
+        self._check(hip().oz_linear_i8(self.h, ctypes.byref(desc), X.ptr, _at(x_scale), W.ptr, w_scale.ptr, _at(bias), _at(residual), Y.ptr,
+                                       _at(work), ctypes.c_size_t(work_bytes)), "oz_linear_i8")
+
+    def orthogonalize_workspace(self, desc: OrthogonalizeDesc) -> int:
+        return self._bytes(hip().oz_orthogonalize_workspace(self.h, ctypes.byref(desc)), "oz_orthogonalize_workspace")
+
+    def orthogonalize(self, desc: OrthogonalizeDesc, G: Buffer, O: Buffer, work=None, work_bytes=0):
+        """O = the Newton-Schulz iteration on each matrix of G; O may be G."""
+        self._check(hip().oz_orthogonalize(self.h, ctypes.byref(desc), G.ptr, O.ptr, _at(work), ctypes.c_size_t(work_bytes)), "oz_orthogonalize")
+
+    def muon_plan_bytes(self, tensors) -> int:
+        arr = (MuonTensor * max(len(tensors), 1))(*tensors)
+        return self._bytes(hip().oz_muon_plan_bytes(arr, len(tensors)), "oz_muon_plan_bytes")
+
+    def muon_plan(self, tensors, memory: Buffer = None, memory_bytes: int = None) -> MuonPlan:
+        """The plan of a list of muon_tensor()s, in `memory` (muon_plan_bytes; allocated here if none is given), which lives as long as
+        the plan; memory_bytes as in adamw_plan."""
+        arr = (MuonTensor * max(len(tensors), 1))(*tensors)
+        need = self.muon_plan_bytes(tensors)
+        memory = memory if memory is not None else self.alloc(need)
+        if memory_bytes is None:
+            memory_bytes = getattr(memory, "nbytes", need)
+        plan = MuonPlan()
+        self._check(hip().oz_muon_make_plan(self.h, arr, len(tensors), memory.ptr, ctypes.c_size_t(memory_bytes), ctypes.byref(plan)), "oz_muon_make_plan")
+        plan.buffer = memory
+        return plan
+
+    def muon_workspace(self, plan: MuonPlan) -> int:
+        return self._bytes(hip().oz_muon_workspace(self.h, ctypes.byref(plan)), "oz_muon_workspace")
+
+    def muon_step(self, plan: MuonPlan, lr, momentum=0.95, nesterov=True, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, grad_scale=None, work=None, work_bytes=0):
+        """One step of the plan's matrices."""
+        o = MuonOptions(lr, momentum, int(nesterov), steps, *coefficients, eps, _at(grad_scale))
+        self._check(hip().oz_muon_step(self.h, ctypes.byref(plan), ctypes.byref(o), _at(work), ctypes.c_size_t(work_bytes)), "oz_muon_step")
 
     def crt(self, C: Buffer, M, N, ldc, sC, desc: CrtDesc, dA: Buffer, dB: Buffer, out: Buffer, ldo):
         self._check(hip().oz2_crt_f64(self.h, C.ptr, M, N, ldc, ctypes.c_longlong(sC), ctypes.byref(desc), dA.ptr,
