@@ -480,8 +480,8 @@ int oz_adamw_step(oz_dev* dev, const oz_adamw_plan* plan, const oz_adamw_options
 /* ---- 8-bit integers with a scale for each row --------------------------------------------------------
  * Row m of X (M x K) as integers of -127 to 127 and a scale, X = Q scale: with a the largest of the row's |x|, and at
  * least 127 2^-126,
- *   scale = a / 127,  Q = x (127 / a) rounded to the nearest integer, ties to even,
- * quotients and products in FP32. A row with a value that is not finite gives a NaN as scale, and zeros. Activations are quantized
+ *   scale = a (1 / 127),  Q = x (127 (1 / a)) rounded to the nearest integer, ties to even,
+ * each quotient and product rounded to FP32. A row with a value that is not finite gives a NaN as scale, and zeros. Activations are quantized
  * by token, weights (N x K, a row for each output) by channel. Rows of Q are ldq bytes apart, what lies between them is left as it
  * is. M may be 0. */
 typedef struct oz_quantize_desc {

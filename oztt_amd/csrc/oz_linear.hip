@@ -210,14 +210,6 @@ size_t up(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 
 constexpr int kFewRows = 16, kFewOddRows = 32;  // rows that begin at odd addresses: laid out for the tiles from 33 on
 
-// How a product runs, from its sizes alone.
-struct Route {
-    bool few;       // oz_linear_rows.hip
-    Tile tile;
-    int splits;
-    size_t parts;   // bytes of the ranges' sums
-};
-
 // Estimated us of a tile's launch with its c cut into `splits` ranges: whole rounds of workgroups over the CUs and the last,
 // partly filled one, not less than the operands take from memory (4.6 TB/s), and the join's launch and traffic (8 bytes an
 // output and range at 4 TB/s).
@@ -232,6 +224,8 @@ float estimate(const Shape& t, int cus, long long nq, long long np, long long C,
     return us;
 }
 
+}  // namespace
+
 // Few rows: their own kernels, c in ranges where 16 rows of W each are too few to keep the CUs reading (at least 512 values a
 // range). 5 rows, 512 of W, K = 8192: 8.0 us in four ranges, 9.1 in one.
 // More: the tile and ranges with the least estimate; 1000 x 704 x 1504 10.1 us by 64 x 64 (17 by 128 x 128), 2048 x 4096 x 4096 62
@@ -241,7 +235,7 @@ float estimate(const Shape& t, int cus, long long nq, long long np, long long C,
 // It is further off where c is long and tiles are few, as the estimate takes their stages for shorter than they are: without caches
 // 512 x 8192^2 96 us for 81 by 256 x 256 in 4 ranges, 256 x 8192^2 73 (estimate: 45) for 64 by 128 x 128 in 4, and of few rows 16 x
 // 8192^2 36 for 30 by 32 x 32.
-Route route_of(int cus, long long nq, long long np, long long C, bool contiguous, bool even) {
+ozl::Route ozl::route_of(int cus, long long nq, long long np, long long C, bool contiguous, bool even) {
     Route r{};
     r.splits = 1;
     if (contiguous && (nq <= kFewRows || (!even && nq <= kFewOddRows))) {
@@ -260,6 +254,8 @@ Route route_of(int cus, long long nq, long long np, long long C, bool contiguous
     if (r.splits > 1) r.parts = up(4 * (size_t)r.splits * nq * ((np + 7) / 8 * 8));
     return r;
 }
+
+namespace {
 
 int launch_any(oz_dev* dev, int type, const Product& a) {
     const dim3 grid = grid_of((long long)oz::ceil_div(a.np, 64) * oz::ceil_div(a.nq, 64));

@@ -31,6 +31,23 @@ struct Product {
     int splits;
 };
 
+// The same of 8-bit integers, sums in int32 (parts too): what goes to the epilogue is sum p_scale[p] q_scale[q]. Sizes along c
+// count pairs of integers; Z is not taken.
+struct ScaledProduct : Product {
+    const float *q_scale, *p_scale;
+    int K;         // integers along c
+    int type;      // oz_type of the bias
+    bool q_zeros;  // zeros behind the K integers of Q's rows, to the end of a stage
+};
+
+// Eight sums in a row from p on to values, of those below np.
+__device__ __forceinline__ void scale8(const ScaledProduct& a, long long q, long long p, float* v) {
+    const float s = a.q_scale[q];
+#pragma unroll
+    for (int k = 0; k < 8; k++)
+        if (p + k < a.np) v[k] = (float)__float_as_int(v[k]) * a.p_scale[p + k] * s;
+}
+
 // One value. bias, Z in the operands' type, residual and Y in y_type.
 __device__ __forceinline__ void finish(const Epilogue& e, int type, long long q, long long p, float v) {
     if (e.bias) v += ozt::load(e.bias, type, p);
@@ -88,6 +105,14 @@ inline const Shape& shape_of(Tile t) {
 // the largest tile.
 inline long long tiles_of(const Shape& t, long long nq, long long np, int splits) { return (nq + t.q - 1) / t.q * ((np + t.p - 1) / t.p) * splits; }
 inline bool fits(const Shape& t, long long nq, long long np, int splits) { return tiles_of(t, nq, np, splits) * t.threads < 1ll << 32; }
+// How a product runs, from its sizes alone: `contiguous` operands along c, whose rows all begin at `even` addresses.
+struct Route {
+    bool few;       // the kernels of few rows
+    Tile tile;
+    int splits;
+    size_t parts;   // bytes of the ranges' sums
+};
+Route route_of(int cus, long long nq, long long np, long long C, bool contiguous, bool even);
 int launch_tile(oz_dev* dev, int type, Tile tile, const Product& a);
 // At most 32 rows of Q, operands along c at any address; splits as in Product (1 for at most kStreamRows). A workgroup has
 // few_rows_block rows of P.

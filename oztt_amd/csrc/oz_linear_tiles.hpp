@@ -41,8 +41,11 @@ __device__ __forceinline__ void lds_copy(v4i rs, void* lbase, unsigned voff) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(l), "v"(voff), "s"(rs) : "memory");
 }
 
-// One operand of a tile of ROWS rows: its copies (wave `wave` of W brings blocks wave, wave + W, ...) and fragments.
-template <bool MAJOR, int ROWS, int W>
+// One operand of a tile of ROWS rows: its copies (wave `wave` of W brings blocks wave, wave + W, ...) and fragments. Sizes count
+// 16-bit values; 8-bit integers are taken two at a time. PARTS: the operand is three stretches of `stages` / 3 stages each, the
+// second and third ones jump[0] and jump[1] bytes behind the end of the one before (whole stages, so that their ranges are the
+// first one's).
+template <bool MAJOR, int ROWS, int W, bool PARTS = false>
 struct Operand {
     static constexpr int BLOCKS = ROWS / 8;   // 1 KB blocks of a stage
     static constexpr int N = BLOCKS / W;      // copies of a wave
@@ -55,6 +58,9 @@ struct Operand {
     unsigned step;   // bytes of a stage's advance
     unsigned off[N]; // of this lane's copies
     int steps;       // stages left to load
+    int part;        // PARTS: stages of a stretch
+    unsigned whole;  // and its first range
+    long long jump[2];
 
     // a row's swizzle in 32-byte pieces: rows 8 g + j and 8 g + 4 + j (j < 4) of g and g + 1 differ
     __device__ static int piece_swizzle(int row) { return ((row & 3) | ((row >> 3) & 1) << 2) & (PIECES - 1); }
@@ -96,32 +102,47 @@ struct Operand {
         step = __builtin_amdgcn_readfirstlane(step);
         limit();
     }
+    __device__ __forceinline__ void parts(int stages, long long first, long long second) {
+        steps = 3 * stages;
+        part = stages;
+        whole = range;
+        jump[0] = first, jump[1] = second;
+        limit();
+    }
     // A few scalar instructions a stage: whatever more there was showed (85 cycles a stage, 2% of 8192^3, 15% of small
     // products, for 64-bit ranges and a mask of the last chunks).
     __device__ __forceinline__ void limit() {
-        if constexpr (MAJOR) rs[2] = steps > 1 ? range : steps == 1 ? last : 0u;
+        if constexpr (MAJOR && !PARTS) rs[2] = steps > 1 ? range : steps == 1 ? last : 0u;
         else rs[2] = steps > 0 ? range : 0u;
     }
     __device__ __forceinline__ void copy(uint8_t* stage, int j, int wave) const { lds_copy(rs, stage + 1024 * (W * j + wave), off[j]); }
     __device__ __forceinline__ void next() {
         steps--;
-        const unsigned long long base = ((unsigned long long)(unsigned)rs[1] << 32 | (unsigned)rs[0]) + step;
+        unsigned long long base = ((unsigned long long)(unsigned)rs[1] << 32 | (unsigned)rs[0]) + step;
+        if constexpr (!MAJOR) range -= step;
+        if constexpr (PARTS) {
+            if (steps == 2 * part || steps == part) {
+                base += steps == part ? jump[1] : jump[0];
+                range = whole;
+            }
+        }
         rs[0] = (int)base;
         rs[1] = (int)(base >> 32);
-        if constexpr (!MAJOR) range -= step;
         limit();
     }
 
-    // Zeros for what lies behind the `valid` last values of c in a stage: there stand a window's other columns or the next
-    // row (rows of c beyond the last are zeros).
+    // Zeros for what lies behind the `valid` last values (of type T) of c in a stage: there stand a window's other columns or the
+    // next row (rows of c beyond the last are zeros).
+    template <class T>
     __device__ static void zero_tail(uint8_t* stage, int valid, int thread) {
         if constexpr (!MAJOR) {
+            constexpr int E = 16 / sizeof(T);
             const v4i none = {0, 0, 0, 0};
             for (int row = thread; row < ROWS; row += 64 * W) {
                 uint8_t* at = stage + 128 * row;
-                uint16_t* cut = reinterpret_cast<uint16_t*>(at + 16 * ((valid >> 3) ^ (row & 7)));
-                for (int e = valid & 7; e < 8; e++) cut[e] = 0;
-                for (int c = (valid >> 3) + 1; c < 8; c++) *reinterpret_cast<v4i*>(at + 16 * (c ^ (row & 7))) = none;
+                T* cut = reinterpret_cast<T*>(at + 16 * ((valid / E) ^ (row & 7)));
+                for (int e = valid % E; e < E; e++) cut[e] = 0;
+                for (int c = valid / E + 1; c < 8; c++) *reinterpret_cast<v4i*>(at + 16 * (c ^ (row & 7))) = none;
             }
         }
     }
@@ -178,8 +199,10 @@ __device__ __forceinline__ void each(F&& f) {
 // and Z move in whole 16-byte pieces and whole rows. The residual's pieces are asked for a batch ahead: with one wave
 // on a SIMD nothing else would hide their latency (8192^3 with everything in the epilogue: 1003 us with a
 // wait for each piece).
-template <int TYPE, int TI, int TJ, int ROOM>
-__device__ __forceinline__ void put_sums(const Product& a, const f32x4 (&acc)[TI][TJ], float* tile, int lane, int split, long long q0, long long p0) {
+// Sums of integers (P is ScaledProduct) go the same way as they are, and become values where they are taken.
+template <int TYPE, int TI, int TJ, int ROOM, class P, class Sums>
+__device__ __forceinline__ void put_sums(const P& a, const Sums (&acc)[TI][TJ], float* tile, int lane, int split, long long q0, long long p0) {
+    constexpr bool SCALED = std::is_same_v<P, ScaledProduct>;
     constexpr int ROW = 16 * TJ;
     constexpr int RI = TI * 16 * ROW <= ROOM ? TI : TI * 8 * ROW <= ROOM ? TI / 2 : TI / 4;
     static_assert(RI >= 1 && RI * 16 * ROW <= ROOM && TI % RI == 0, "staging room");
@@ -195,7 +218,7 @@ __device__ __forceinline__ void put_sums(const Product& a, const f32x4 (&acc)[TI
         for (int i = 0; i < RI; i++)
 #pragma unroll
             for (int j = 0; j < TJ; j++)
-                *reinterpret_cast<f32x4*>(tile + (16 * i + r) * ROW + 4 * ((4 * j + g) ^ (r & XM))) = acc[decltype(H)::value * RI + i][j];
+                *reinterpret_cast<Sums*>(tile + (16 * i + r) * ROW + 4 * ((4 * j + g) ^ (r & XM))) = acc[decltype(H)::value * RI + i][j];
         __builtin_amdgcn_wave_barrier();
     };
     auto read = [&](int row, float* v) {
@@ -224,16 +247,26 @@ __device__ __forceinline__ void put_sums(const Product& a, const f32x4 (&acc)[TI
     // and writes the same. (Only where fewer than 8 are left for the wave are they written one by one.)
     const long long pl = p + 8 <= a.np || a.np - 8 < p0 ? p : a.np - 8;
     const bool in = p < a.np && pl + 8 <= a.np;
-    float bias[8] = {};
+    float bias[8] = {}, scale[8] = {};
     if (e.bias && in) load8(e.bias, TYPE, pl, bias);
+    if constexpr (SCALED)
+        if (in) load8(a.p_scale, OZ_F32, pl, scale);
     const int wide = e.y_type == OZ_F32;
     const char* pr = static_cast<const char*>(e.residual) + ((q0 + rr) * e.ldr + pl) * (wide ? 4 : 2);
     char* py = static_cast<char*>(e.Y) + ((q0 + rr) * e.ldy + pl) * (wide ? 4 : 2);
     char* pz = static_cast<char*>(e.Z) + ((q0 + rr) * e.ldz + pl) * 2;
     const long long dr = RT * e.ldr * (wide ? 4 : 2), dy = RT * e.ldy * (wide ? 4 : 2), dz = RT * e.ldz * 2;
     u32x4 res[2][BATCH][2] = {};
+    float of_row[2][BATCH] = {};  // SCALED: the rows' scales
     auto ask = [&](auto B) {  // batch B of all TI / RI * BATCHES
         constexpr int b = decltype(B)::value;
+        if constexpr (SCALED) {
+#pragma unroll
+            for (int t = 0; t < BATCH; t++) {
+                const long long q = q0 + (b * BATCH + t) * RT + rr;
+                of_row[b & 1][t] = q < a.nq ? a.q_scale[q] : 0.0f;
+            }
+        }
         if (!e.residual) return;
 #pragma unroll
         for (int t = 0; t < BATCH; t++) {
@@ -262,6 +295,10 @@ __device__ __forceinline__ void put_sums(const Product& a, const f32x4 (&acc)[TI
 #pragma unroll
                     for (int k = 0; k < 8; k++) v[k] = tile[row * ROW + 4 * (((col + k) >> 2) ^ (row & XM)) + ((col + k) & 3)];
                 }
+                if constexpr (SCALED) {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) v[k] = (float)__float_as_int(v[k]) * scale[k] * of_row[b & 1][t];
+                }
 #pragma unroll
                 for (int k = 0; k < 8; k++) v[k] += bias[k];
                 if (e.Z) store8(pz + (h * NT + turn) * dz, TYPE, 0, v);
@@ -286,7 +323,9 @@ __device__ __forceinline__ void put_sums(const Product& a, const f32x4 (&acc)[TI
                 const long long q = q0 + (h * NT + turn) * RT + rr;
                 float v[8];
                 read(RT * turn + rr, v);
-                if (q < a.nq) finish8<TYPE>(e, a.np, q, p, v);
+                if (q >= a.nq) continue;
+                if constexpr (SCALED) scale8(a, q, p, v);
+                finish8<TYPE>(e, a.np, q, p, v);
             }
         }
     });
@@ -297,202 +336,231 @@ __device__ __forceinline__ int ragged_tail(const Product& a, int split) {
     return split == a.splits - 1 ? (int)(a.C % BC) : 0;
 }
 
-// WQ x WP waves of 16 TI x 16 TJ outputs each; a ring of NSTG stages, one barrier a stage. The fragments of the next
-// step are read while this one's multiply.
-template <int TYPE, bool QM, bool PM, int TI, int TJ, int WQ, int WP, int NSTG>
-__global__ void __launch_bounds__(64 * WQ * WP, NSTG * 16 * BC * 2 * (TI * WQ + TJ * WP) <= 81920 ? 2 : 1)
-    product_tile_kernel(const Product a, int tiles_q, int tiles_p) {
-    typedef typename Half<TYPE>::x8 T8;
-    constexpr int W = WQ * WP, QR = 16 * TI * WQ, PR = 16 * TJ * WP;
-    typedef Operand<QM, QR, W> OQ;
-    typedef Operand<PM, PR, W> OP;
-    constexpr int STG_Q = 2 * BC * QR, STG = STG_Q + 2 * BC * PR, LD = OQ::N + OP::N;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[NSTG * STG];
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int split, tq, tp;
-    place_of(a, tiles_q, tiles_p, split, tq, tp);
-    const long long q0 = (long long)tq * QR, p0 = (long long)tp * PR;
-    const long long all = (a.C + BC - 1) / BC, s0 = all * split / a.splits;
-    const int nst = (int)(all * (split + 1) / a.splits - s0);
-    OQ oq;
-    OP op;
-    oq.init(a.Q, a.ldq, a.nq, a.C, q0, s0 * BC, nst, lane, wave);
-    op.init(a.P, a.ldp, a.np, a.C, p0, s0 * BC, nst, lane, wave);
-    auto issue = [&](uint8_t* to) {
+// The sums of a tile by WQ x WP waves of 16 TI x 16 TJ outputs each, `nst` stages of the operands oq and op through a ring of NSTG
+// stages in LDS, one barrier a stage. The fragments of the next step are read while this one's multiply. `tail`: values of type
+// TAIL in the last stage, where they do not fill it. When it returns, LDS is free.
+template <class M, bool QM, bool PM, int TI, int TJ, int WQ, int WP, int NSTG, bool PARTS = false>
+struct TileLoop {
+    typedef typename M::x8 T8;
+    typedef typename M::sums Sums;
+    static constexpr int W = WQ * WP, QR = 16 * TI * WQ, PR = 16 * TJ * WP;
+    typedef Operand<QM, QR, W, PARTS> OQ;
+    typedef Operand<PM, PR, W, PARTS> OP;
+    static constexpr int STG_Q = 2 * BC * QR, STG = STG_Q + 2 * BC * PR, LD = OQ::N + OP::N, LDS = NSTG * STG, ROOM = LDS / W / 4;
+
+    template <class TAIL>
+    __device__ static __forceinline__ void run(uint8_t* lds, OQ& oq, OP& op, int nst, int tail, int lane, int wave, Sums (&acc)[TI][TJ]) {
+        auto issue = [&](uint8_t* to) {
 #pragma unroll
-        for (int j = 0; j < OQ::N; j++) oq.copy(to, j, wave);
+            for (int j = 0; j < OQ::N; j++) oq.copy(to, j, wave);
 #pragma unroll
-        for (int j = 0; j < OP::N; j++) op.copy(to + STG_Q, j, wave);
-        oq.next();
-        op.next();
-    };
-    const int wq = wave / WP, wp = wave % WP;
-    const int lq = OQ::lane_offset(lane), lp = OP::lane_offset(lane);
-    f32x4 acc[TI][TJ];
-#pragma unroll
-    for (int i = 0; i < TI; i++)
-#pragma unroll
-        for (int j = 0; j < TJ; j++) acc[i][j] = f32x4{0, 0, 0, 0};
-    const int tail = ragged_tail(a, split);
-    // Stage k, at `at`, has landed for every wave: all but the copies of the NSTG - 2 stages behind it are complete (in the
-    // beginning, of NSTG - 1); this wave's reads before are too.
-    auto landed = [&](auto LEFT, int k, uint8_t* at) {
-        wait_vmcnt_lgkm0<LD * decltype(LEFT)::value>();
-        stage_barrier();
-        if (!(QM && PM) && tail && k == nst - 1) {
-            OQ::zero_tail(at, tail, threadIdx.x);
-            OP::zero_tail(at + STG_Q, tail, threadIdx.x);
-            wait_vmcnt_lgkm0<LD * decltype(LEFT)::value>();
-            stage_barrier();
-        }
-    };
-    T8 fq[2][TI], fp[2][TJ];
-    auto read = [&](const uint8_t* at, int h) {
-#pragma unroll
-        for (int i = 0; i < TI; i++) fq[h][i] = OQ::template fragment<T8>(at, h, wq * TI + i, lq);
-#pragma unroll
-        for (int j = 0; j < TJ; j++) fp[h][j] = OP::template fragment<T8>(at + STG_Q, h, wp * TJ + j, lp);
-    };
-    auto multiply = [&](int h) {
+            for (int j = 0; j < OP::N; j++) op.copy(to + STG_Q, j, wave);
+            oq.next();
+            op.next();
+        };
+        const int wq = wave / WP, wp = wave % WP;
+        const int lq = OQ::lane_offset(lane), lp = OP::lane_offset(lane);
 #pragma unroll
         for (int i = 0; i < TI; i++)
 #pragma unroll
-            for (int j = 0; j < TJ; j++) acc[i][j] = Half<TYPE>::mfma(fp[h][j], fq[h][i], acc[i][j]);
-    };
+            for (int j = 0; j < TJ; j++) acc[i][j] = Sums{0, 0, 0, 0};
+        // Stage k, at `at`, has landed for every wave: all but the copies of the NSTG - 2 stages behind it are complete (in the
+        // beginning, of NSTG - 1); this wave's reads before are too.
+        auto landed = [&](auto LEFT, int k, uint8_t* at) {
+            wait_vmcnt_lgkm0<LD * decltype(LEFT)::value>();
+            stage_barrier();
+            if (!(QM && PM) && tail && k == nst - 1) {
+                OQ::template zero_tail<TAIL>(at, tail, threadIdx.x);
+                OP::template zero_tail<TAIL>(at + STG_Q, tail, threadIdx.x);
+                wait_vmcnt_lgkm0<LD * decltype(LEFT)::value>();
+                stage_barrier();
+            }
+        };
+        T8 fq[2][TI], fp[2][TJ];
+        auto read = [&](const uint8_t* at, int h) {
 #pragma unroll
-    for (int s = 0; s < NSTG; s++) issue(lds + s * STG);
-    landed(std::integral_constant<int, NSTG - 1>{}, 0, lds);
-    read(lds, 0);
-    // The two steps of stage k. Before the second one multiplies stage k + 1 has landed, and behind that barrier nobody reads
-    // stage k's buffer any more, which stage k + NSTG takes.
-    uint8_t* at = lds;
-    for (int k = 0; k < nst; k++) {
-        uint8_t* next = at + STG == lds + NSTG * STG ? lds : at + STG;
-        read(at, 1);
-        multiply(0);
-        landed(std::integral_constant<int, NSTG - 2>{}, k + 1, next);
-        issue(at);
-        read(next, 0);
-        multiply(1);
-        at = next;
+            for (int i = 0; i < TI; i++) fq[h][i] = OQ::template fragment<T8>(at, h, wq * TI + i, lq);
+#pragma unroll
+            for (int j = 0; j < TJ; j++) fp[h][j] = OP::template fragment<T8>(at + STG_Q, h, wp * TJ + j, lp);
+        };
+        auto multiply = [&](int h) {
+#pragma unroll
+            for (int i = 0; i < TI; i++)
+#pragma unroll
+                for (int j = 0; j < TJ; j++) acc[i][j] = M::mfma(fp[h][j], fq[h][i], acc[i][j]);
+        };
+#pragma unroll
+        for (int s = 0; s < NSTG; s++) issue(lds + s * STG);
+        landed(std::integral_constant<int, NSTG - 1>{}, 0, lds);
+        read(lds, 0);
+        // The two steps of stage k. Before the second one multiplies stage k + 1 has landed, and behind that barrier nobody reads
+        // stage k's buffer any more, which stage k + NSTG takes.
+        uint8_t* at = lds;
+        for (int k = 0; k < nst; k++) {
+            uint8_t* next = at + STG == lds + NSTG * STG ? lds : at + STG;
+            read(at, 1);
+            multiply(0);
+            landed(std::integral_constant<int, NSTG - 2>{}, k + 1, next);
+            issue(at);
+            read(next, 0);
+            multiply(1);
+            at = next;
+        }
+        wait_vmcnt<0>();
+        __syncthreads();
     }
-    wait_vmcnt<0>();
-    __syncthreads();
-    constexpr int ROOM = NSTG * STG / W / 4;
-    put_sums<TYPE, TI, TJ, ROOM>(a, acc, reinterpret_cast<float*>(lds) + wave * ROOM, lane, split, q0 + 16 * wq * TI, p0 + 16 * wp * TJ);
+};
+
+// A tile's place and its operands' stages.
+struct Work {
+    int split, nst;
+    long long q0, p0, c0;
+};
+__device__ __forceinline__ Work work_of(const Product& a, int tiles_q, int tiles_p, int rows_q, int rows_p) {
+    Work w;
+    int tq, tp;
+    place_of(a, tiles_q, tiles_p, w.split, tq, tp);
+    w.q0 = (long long)tq * rows_q, w.p0 = (long long)tp * rows_p;
+    const long long all = (a.C + BC - 1) / BC, s0 = all * w.split / a.splits;
+    w.nst = (int)(all * (w.split + 1) / a.splits - s0);
+    w.c0 = s0 * BC;
+    return w;
+}
+
+template <int TYPE, bool QM, bool PM, int TI, int TJ, int WQ, int WP, int NSTG>
+__global__ void __launch_bounds__(64 * WQ * WP, NSTG * 16 * BC * 2 * (TI * WQ + TJ * WP) <= 81920 ? 2 : 1)
+    product_tile_kernel(const Product a, int tiles_q, int tiles_p) {
+    typedef TileLoop<Half<TYPE>, QM, PM, TI, TJ, WQ, WP, NSTG> Loop;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[Loop::LDS];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Work w = work_of(a, tiles_q, tiles_p, Loop::QR, Loop::PR);
+    typename Loop::OQ oq;
+    typename Loop::OP op;
+    oq.init(a.Q, a.ldq, a.nq, a.C, w.q0, w.c0, w.nst, lane, wave);
+    op.init(a.P, a.ldp, a.np, a.C, w.p0, w.c0, w.nst, lane, wave);
+    f32x4 acc[TI][TJ];
+    Loop::template run<uint16_t>(lds, oq, op, w.nst, ragged_tail(a, w.split), lane, wave, acc);
+    put_sums<TYPE, TI, TJ, Loop::ROOM>(a, acc, reinterpret_cast<float*>(lds) + wave * Loop::ROOM, lane, w.split, w.q0 + 16 * (wave / WP) * TI,
+                                       w.p0 + 16 * (wave % WP) * TJ);
 }
 
 // c += a b with c in accumulation registers. Left to itself the compiler moves sums between the two halves of the
 // register file inside the loop (up to 184 moves for its 128 matrix instructions); written so, c stays. Nothing else
 // touches the registers while the loop runs, the same c comes up every 64 instructions, and settle_sums() stands
 // between the loop and the first use of the sums, so that no result is read early.
-template <int TYPE>
-__device__ __forceinline__ void mfma_acc(f32x4& c, typename Half<TYPE>::x8 a, typename Half<TYPE>::x8 b) {
-    if constexpr (TYPE == OZ_BF16) asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
-    else asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+template <class M>
+__device__ __forceinline__ void mfma_acc(typename M::sums& c, typename M::x8 a, typename M::x8 b) {
+    if constexpr (std::is_same_v<M, Half<OZ_BF16>>) asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    else if constexpr (std::is_same_v<M, Half<OZ_F16>>) asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
+    else asm("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
 __device__ __forceinline__ void settle_sums() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
-// 256 x 256 outputs by 4 waves of 128 x 128, one a SIMD, each with 256 sums' registers. The fragments of the next
+// The sums of 256 x 256 outputs by 4 waves of 128 x 128, one a SIMD, each with 256 sums' registers. The fragments of the next
 // step are read while this one's multiply, one or two reads per four matrix instructions. LDS holds five operands'
 // stages, two of each and a spare: the copies of stage k + 2 of Q go out in stage k's first step and those of P in its second,
 // where Q's stage k is free, and have one and a half or two and a half steps to land. (With two whole stages all copies go out
 // in the second step and have one and a half: 852 against 763 us at 8192^3.)
-template <int TYPE, bool QM, bool PM>
-__global__ void __launch_bounds__(256) product_big_kernel(const Product a, int tiles_q, int tiles_p) {
-    typedef typename Half<TYPE>::x8 T8;
-    typedef Operand<QM, 256, 4> OQ;
-    typedef Operand<PM, 256, 4> OP;
-    constexpr int UNIT = 2 * BC * 256, RING = 5 * UNIT, LD = OQ::N;
+template <class M, bool QM, bool PM, bool PARTS = false>
+struct BigLoop {
+    typedef typename M::x8 T8;
+    typedef typename M::sums Sums;
+    typedef Operand<QM, 256, 4, PARTS> OQ;
+    typedef Operand<PM, 256, 4, PARTS> OP;
+    static constexpr int UNIT = 2 * BC * 256, RING = 5 * UNIT, LD = OQ::N, LDS = RING, ROOM = RING / 4 / 4;
     static_assert(OQ::N == OP::N, "copies of a unit");
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[RING];
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int split, tq, tp;
-    place_of(a, tiles_q, tiles_p, split, tq, tp);
-    const long long q0 = 256ll * tq, p0 = 256ll * tp;
-    const long long all = (a.C + BC - 1) / BC, s0 = all * split / a.splits;
-    const int nst = (int)(all * (split + 1) / a.splits - s0);
-    OQ oq;
-    OP op;
-    oq.init(a.Q, a.ldq, a.nq, a.C, q0, s0 * BC, nst, lane, wave);
-    op.init(a.P, a.ldp, a.np, a.C, p0, s0 * BC, nst, lane, wave);
-    const int wq = wave >> 1, wp = wave & 1;
-    const int lq = OQ::lane_offset(lane), lp = OP::lane_offset(lane);
-    f32x4 acc[8][8];
+
+    template <class TAIL>
+    __device__ static __forceinline__ void run(uint8_t* lds, OQ& oq, OP& op, int nst, int tail, int lane, int wave, Sums (&acc)[8][8]) {
+        const int wq = wave >> 1, wp = wave & 1;
+        const int lq = OQ::lane_offset(lane), lp = OP::lane_offset(lane);
 #pragma unroll
-    for (int i = 0; i < 8; i++)
+        for (int i = 0; i < 8; i++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) acc[i][j] = f32x4{0, 0, 0, 0};
-    const int tail = ragged_tail(a, split);
-    // Unit 2 k is Q's stage k, unit 2 k + 1 P's; unit u is at u UNIT modulo RING.
-    auto landed = [&](auto LEFT, int k, int uq, int up) {  // stage k, whose units are at uq and up
-        wait_vmcnt_lgkm0<decltype(LEFT)::value>();
-        stage_barrier();
-        if (!(QM && PM) && tail && k == nst - 1) {
-            OQ::zero_tail(lds + uq, tail, threadIdx.x);
-            OP::zero_tail(lds + up, tail, threadIdx.x);
+            for (int j = 0; j < 8; j++) acc[i][j] = Sums{0, 0, 0, 0};
+        // Unit 2 k is Q's stage k, unit 2 k + 1 P's; unit u is at u UNIT modulo RING.
+        auto landed = [&](auto LEFT, int k, int uq, int up) {  // stage k, whose units are at uq and up
             wait_vmcnt_lgkm0<decltype(LEFT)::value>();
             stage_barrier();
-        }
-    };
-#pragma unroll
-    for (int s = 0; s < 2; s++) {
-#pragma unroll
-        for (int j = 0; j < LD; j++) oq.copy(lds + 2 * s * UNIT, j, wave);
-#pragma unroll
-        for (int j = 0; j < LD; j++) op.copy(lds + (2 * s + 1) * UNIT, j, wave);
-        oq.next();
-        op.next();
-    }
-    T8 fq[8], fp[8], gq[8], gp[8];
-    landed(std::integral_constant<int, 2 * LD>{}, 0, 0, UNIT);
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        fq[i] = OQ::template fragment<T8>(lds, 0, wq * 8 + i, lq);
-        fp[i] = OP::template fragment<T8>(lds + UNIT, 0, wp * 8 + i, lp);
-    }
-    // One step: 64 matrix instructions on (xq, xp); the 16 fragments (yq, yp) of step H of the units at uq and up, in the order
-    // their instructions want them; the copies of a unit of Q (in a stage's first step) or P to `to`.
-    auto step = [&](auto H, T8* xq, T8* xp, T8* yq, T8* yp, int uq, int up, int to) {
-        constexpr int h = decltype(H)::value;
-        const uint8_t *rq = lds + uq, *rp = lds + up;
-#pragma unroll
-        for (int n = 0; n < 64; n++) {
-            const int i = n >> 3, j = n & 7;
-            mfma_acc<TYPE>(acc[i][j], xp[j], xq[i]);
-            if (n % 4 == 0) {
-                const int t = n / 4;
-                if (t == 0) yq[0] = OQ::template fragment<T8>(rq, h, wq * 8, lq);
-                else if (t <= 8) yp[t - 1] = OP::template fragment<T8>(rp, h, wp * 8 + t - 1, lp);
-                else yq[t - 8] = OQ::template fragment<T8>(rq, h, wq * 8 + t - 8, lq);
+            if (!(QM && PM) && tail && k == nst - 1) {
+                OQ::template zero_tail<TAIL>(lds + uq, tail, threadIdx.x);
+                OP::template zero_tail<TAIL>(lds + up, tail, threadIdx.x);
+                wait_vmcnt_lgkm0<decltype(LEFT)::value>();
+                stage_barrier();
             }
-            if (n % 4 == 2 && n / 4 < LD) {
-                if constexpr (h == 1) oq.copy(lds + to, n / 4, wave);
-                else op.copy(lds + to, n / 4, wave);
-            }
-            __builtin_amdgcn_sched_barrier(0);
+        };
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+#pragma unroll
+            for (int j = 0; j < LD; j++) oq.copy(lds + 2 * s * UNIT, j, wave);
+#pragma unroll
+            for (int j = 0; j < LD; j++) op.copy(lds + (2 * s + 1) * UNIT, j, wave);
+            oq.next();
+            op.next();
         }
-    };
-    // The two steps of stage k. Before the second one stage k + 1 has landed and every wave has read all of stage k. What
-    // is read behind the last stage is not used.
-    int at = 0;
-    auto wrap = [](int b) { return b >= RING ? b - RING : b; };
-    for (int k = 0; k < nst; k++) {
-        const int u1 = wrap(at + UNIT), u2 = wrap(at + 2 * UNIT), u3 = wrap(at + 3 * UNIT), u4 = wrap(at + 4 * UNIT);
-        step(std::integral_constant<int, 1>{}, fq, fp, gq, gp, at, u1, u4);
-        oq.next();
-        landed(std::integral_constant<int, LD>{}, k + 1, u2, u3);
-        step(std::integral_constant<int, 0>{}, gq, gp, fq, fp, u2, u3, at);
-        op.next();
-        at = u2;
+        T8 fq[8], fp[8], gq[8], gp[8];
+        landed(std::integral_constant<int, 2 * LD>{}, 0, 0, UNIT);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            fq[i] = OQ::template fragment<T8>(lds, 0, wq * 8 + i, lq);
+            fp[i] = OP::template fragment<T8>(lds + UNIT, 0, wp * 8 + i, lp);
+        }
+        // One step: 64 matrix instructions on (xq, xp); the 16 fragments (yq, yp) of step H of the units at uq and up, in the order
+        // their instructions want them; the copies of a unit of Q (in a stage's first step) or P to `to`.
+        auto step = [&](auto H, T8* xq, T8* xp, T8* yq, T8* yp, int uq, int up, int to) {
+            constexpr int h = decltype(H)::value;
+            const uint8_t *rq = lds + uq, *rp = lds + up;
+#pragma unroll
+            for (int n = 0; n < 64; n++) {
+                const int i = n >> 3, j = n & 7;
+                mfma_acc<M>(acc[i][j], xp[j], xq[i]);
+                if (n % 4 == 0) {
+                    const int t = n / 4;
+                    if (t == 0) yq[0] = OQ::template fragment<T8>(rq, h, wq * 8, lq);
+                    else if (t <= 8) yp[t - 1] = OP::template fragment<T8>(rp, h, wp * 8 + t - 1, lp);
+                    else yq[t - 8] = OQ::template fragment<T8>(rq, h, wq * 8 + t - 8, lq);
+                }
+                if (n % 4 == 2 && n / 4 < LD) {
+                    if constexpr (h == 1) oq.copy(lds + to, n / 4, wave);
+                    else op.copy(lds + to, n / 4, wave);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        // The two steps of stage k. Before the second one stage k + 1 has landed and every wave has read all of stage k. What
+        // is read behind the last stage is not used.
+        int at = 0;
+        auto wrap = [](int b) { return b >= RING ? b - RING : b; };
+        for (int k = 0; k < nst; k++) {
+            const int u1 = wrap(at + UNIT), u2 = wrap(at + 2 * UNIT), u3 = wrap(at + 3 * UNIT), u4 = wrap(at + 4 * UNIT);
+            step(std::integral_constant<int, 1>{}, fq, fp, gq, gp, at, u1, u4);
+            oq.next();
+            landed(std::integral_constant<int, LD>{}, k + 1, u2, u3);
+            step(std::integral_constant<int, 0>{}, gq, gp, fq, fp, u2, u3, at);
+            op.next();
+            at = u2;
+        }
+        settle_sums();
+        wait_vmcnt<0>();
+        __syncthreads();
     }
-    settle_sums();
-    wait_vmcnt<0>();
-    __syncthreads();
-    constexpr int ROOM = RING / 4 / 4;
-    put_sums<TYPE, 8, 8, ROOM>(a, acc, reinterpret_cast<float*>(lds) + wave * ROOM, lane, split, q0 + 128 * wq, p0 + 128 * wp);
+};
+
+template <int TYPE, bool QM, bool PM>
+__global__ void __launch_bounds__(256) product_big_kernel(const Product a, int tiles_q, int tiles_p) {
+    typedef BigLoop<Half<TYPE>, QM, PM> Loop;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[Loop::LDS];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const Work w = work_of(a, tiles_q, tiles_p, 256, 256);
+    typename Loop::OQ oq;
+    typename Loop::OP op;
+    oq.init(a.Q, a.ldq, a.nq, a.C, w.q0, w.c0, w.nst, lane, wave);
+    op.init(a.P, a.ldp, a.np, a.C, w.p0, w.c0, w.nst, lane, wave);
+    f32x4 acc[8][8];
+    Loop::template run<uint16_t>(lds, oq, op, w.nst, ragged_tail(a, w.split), lane, wave, acc);
+    put_sums<TYPE, 8, 8, Loop::ROOM>(a, acc, reinterpret_cast<float*>(lds) + wave * Loop::ROOM, lane, w.split, w.q0 + 128 * (wave >> 1), w.p0 + 128 * (wave & 1));
 }
 
 }  // namespace ozl

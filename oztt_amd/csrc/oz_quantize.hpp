@@ -14,7 +14,7 @@ struct Scale {
 __device__ __forceinline__ Scale scale_of(unsigned top) {
     if (top >= 0x7F800000u) return {__uint_as_float(0x7FC00000u), 0.0f};
     const float a = fmaxf(__uint_as_float(top), 127.0f * 0x1p-126f);
-    return {a / 127.0f, 127.0f / a};
+    return {a * (1.0f / 127.0f), 127.0f * (1.0f / a)};
 }
 __device__ __forceinline__ unsigned bits_of(float x) { return __float_as_uint(x) & 0x7FFFFFFFu; }
 // Four values as bytes; zeros in a row without a scale (inverse 0), whose x may be anything.

@@ -11,6 +11,7 @@
 namespace ozt {
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -26,13 +27,22 @@ template <>
 struct Half<OZ_BF16> {
     typedef __bf16 t;
     typedef bf16x8 x8;
+    typedef f32x4 sums;
     __device__ static f32x4 mfma(x8 a, x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 };
 template <>
 struct Half<OZ_F16> {
     typedef _Float16 t;
     typedef f16x8 x8;
+    typedef f32x4 sums;
     __device__ static f32x4 mfma(x8 a, x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+
+// 8-bit integers: 16 of them where the others have 8 values, the sums exact.
+struct Int8 {
+    typedef i32x4 x8;
+    typedef i32x4 sums;
+    __device__ static i32x4 mfma(x8 a, x8 b, i32x4 c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
 };
 
 // Value i of an array of the given type, as FP32, and back (rounded to nearest even).

@@ -14,8 +14,8 @@ def definition(x: np.ndarray):
     a = np.max(np.abs(x), axis=1)
     bad = ~np.isfinite(a)
     a = np.maximum(np.where(bad, np.float32(1), a), np.float32(127 * 2.0**-126))
-    q = np.rint(np.where(bad[:, None], np.float32(0), x) * (np.float32(127) / a)[:, None])
-    scale = np.where(bad, np.float32(np.nan), a / np.float32(127))
+    q = np.rint(np.where(bad[:, None], np.float32(0), x) * (np.float32(127) * (np.float32(1) / a))[:, None])
+    scale = np.where(bad, np.float32(np.nan), a * (np.float32(1) / np.float32(127)))
     return q.astype(np.int8), scale.astype(np.float32)
 
 
