@@ -58,6 +58,7 @@ HIP_SOURCES = {
     "oz_linear_i8.hip": [],
     "oz_muon.hip": [],
     "oz_newton_schulz.hip": [],
+    "oz_newton_schulz_three.hip": [],
 }
 HOST_FLAGS = ["-std=c++20", "-O2", "-fPIC", "-ffp-contract=off", "-fno-fast-math", "-fopenmp",
               "-Wall", "-Wextra", f"-I{INCLUDE}", f"-I{CSRC / 'host'}"]

@@ -14,6 +14,8 @@
 // Where a side is short (the rounding errors of A and B then average over few values: up to 1e-2 at one to four rows) or the result
 // is kept in more than BF16's 8 bits, the products take both parts of both operands, h h + h l + l h: off by 1e-6.
 #pragma once
+#include <hip/hip_runtime.h>
+
 #include "oz_types.hpp"
 
 struct oz_dev;
@@ -43,14 +45,16 @@ struct Shapes {
 struct Places {
     int first[kShapes + 1], per[kShapes];
 };
-
 struct Place {
     int shape, matrix, index;
 };
-__device__ __forceinline__ Place place_of(const Places& p, int n, int w) {
+__device__ __forceinline__ int shape_of(const Places& p, int n, int w) {
     int s = 0;
     while (s + 1 < n && w >= p.first[s + 1]) s++;
-    const int i = w - p.first[s];
+    return s;
+}
+__device__ __forceinline__ Place place_of(const Places& p, int n, int w) {
+    const int s = shape_of(p, n, w), i = w - p.first[s];
     return {s, i / p.per[s], i % p.per[s]};
 }
 
@@ -78,6 +82,18 @@ struct Ends {
 struct Factors {
     float a, b, c;
 };
+
+// The products of a step. X' goes to the ends in the last one.
+enum Phase { GRAM, SQUARE, UPDATE };
+struct Pass {
+    Places places;
+    Factors f;
+    int from;  // X's buffer, its values go to the other one
+    int last;
+};
+// Tiles of `tile` x `tile` outputs (64, 128, 256) of a phase's products, for shapes that are alike in `three`.
+template <bool THREE>
+void launch_products(hipStream_t stream, Phase phase, int tile, const Shapes& m, const Ends& ends, const Pass& pass);
 
 // The iteration on X0 in the shapes' x[0] (and l), the last step's results to the ends.
 int iterate(oz_dev* dev, const Shapes& m, const Ends& ends, const Factors& f, int steps);

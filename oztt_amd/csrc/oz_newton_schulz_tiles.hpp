@@ -1,0 +1,346 @@
+// Tiled products of the Newton-Schulz iteration (oz_newton_schulz.hpp), on the linear layers' loops over a tile
+// (oz_linear_tiles.hpp).
+//
+// A and A^2 are symmetric: only tiles on and above the diagonal are computed and written twice, as they are and transposed. X's
+// product with the symmetric B takes X as it lies, B X with X read transposed out of LDS, X B for a tall matrix. All sides in the
+// workspace are multiples of 64 with zeros behind the matrices, so no stage is ragged and every access of 8 values is whole.
+// Products of both parts are one loop over three stretches of c, h h, h l and l h.
+#pragma once
+#include "oz_linear_tiles.hpp"
+#include "oz_newton_schulz.hpp"
+
+namespace ozn {
+
+using namespace ozt;
+using ozl::Operand;
+
+// Tile `u` of the T (T + 1) / 2 with row <= column: groups of 4 rows column by column, as the tiles of a whole product.
+__device__ __forceinline__ void triangle(int u, int T, int& row, int& col) {
+    int first = 0;
+    for (;; first += 4) {
+        const int g = min(T - first, 4), here = g * (T - first) - g * (g - 1) / 2;
+        if (u < here) {
+            const int head = g * (g + 1) / 2;  // columns first .. first + g - 1 have 1, 2, ... rows
+            if (u < head) {
+                int c = 0;
+                while (u > c) u -= ++c;
+                row = first + u, col = first + c;
+            } else {
+                row = first + (u - head) % g, col = first + g + (u - head) / g;
+            }
+            return;
+        }
+        u -= here;
+    }
+}
+
+// Workgroup `first` + i of the P that a shape has -> its place in the shape's sequence of tiles: XCD x runs workgroups x, x + 8, ..., and gets a
+// run of their number, the XCDs' runs one behind the other. A bijection for any first and P.
+__device__ __forceinline__ int xcd_run(int first, int i, int P) {
+    constexpr int N = ozg::XCDS;
+    const int x = (first + i) % N, s = first % N;   // its XCD, and that of the shape's first
+    const int k = (x - s) & (N - 1);                // the XCD's first workgroup of the shape
+    const int q = P / N, r = P % N, wrap = max(s + r - N, 0);  // XCDs s .. s + r - 1 (modulo N) have q + 1
+    return x * q + min(x, wrap) + min(max(x - s, 0), r - wrap) + (i - k) / N;
+}
+
+// Workgroup -> shape, matrix and tile. Shapes come one after the other (the long ones first, as they differ in length), within a shape
+// each XCD takes one contiguous run of the tiles, so that what it runs at a time shares rows and columns in its L2.
+template <Phase PHASE>
+__device__ __forceinline__ void tile_place(const Shapes& m, const Places& p, int T, int w, int& shape, int& matrix, int& tq, int& tp) {
+    shape = __builtin_amdgcn_readfirstlane(shape_of(p, m.n, w));
+    const Shape& s = m.s[shape];
+    const int i = xcd_run(p.first[shape], w - p.first[shape], p.per[shape] * s.count);
+    matrix = __builtin_amdgcn_readfirstlane(i / p.per[shape]);
+    const int u = __builtin_amdgcn_readfirstlane(i - matrix * p.per[shape]);
+    if constexpr (PHASE == UPDATE) {
+        const int rows = (s.R + T - 1) / T, cols = (s.C + T - 1) / T;
+        const int group = u / (4 * cols), first = 4 * group, g = min(rows - first, 4), v = u - group * 4 * cols;
+        tq = first + v % g, tp = v / g;
+    } else {
+        triangle(u, (side_of(s) + T - 1) / T, tq, tp);
+    }
+    tq = __builtin_amdgcn_readfirstlane(tq);
+    tp = __builtin_amdgcn_readfirstlane(tp);
+}
+
+// ---- from sums to values ------------------------------------------------------------------------------
+
+union Half8 {
+    u32x4 w;
+    f16x8 v;
+};
+// v in one or two parts to h and l.
+__device__ __forceinline__ void put8(_Float16* h, _Float16* l, long long at, const float* v) {
+    f16x8 x, y;
+#pragma unroll
+    for (int k = 0; k < 8; k++) {
+        x[k] = (_Float16)v[k];
+        y[k] = (_Float16)(v[k] - (float)x[k]);
+    }
+    *reinterpret_cast<f16x8*>(h + at) = x;
+    if (l) *reinterpret_cast<f16x8*>(l + at) = y;
+}
+
+// The sums of a wave, through LDS as in ozl::put_sums, 8 values of a row at a time: ask(P, t, row) loads what the t-th piece of a batch
+// wants, a batch ahead, use(P, t, row, v) finishes it (P: the batch's parity; rows and columns are the wave's own). With TWICE use()'s
+// values go back to LDS, and across(row, col, v) gets 8 values of a column from `row` on.
+template <int TI, int TJ, int ROOM, bool TWICE, class Ask, class Use, class Across>
+__device__ __forceinline__ void put_rows(const f32x4 (&acc)[TI][TJ], float* tile, int lane, bool twice, Ask&& ask, Use&& use, Across&& across) {
+    constexpr int ROW = 16 * TJ;
+    constexpr int RI = TI * 16 * ROW <= ROOM ? TI : TI * 8 * ROW <= ROOM ? TI / 2 : TI / 4;
+    static_assert(RI >= 1 && RI * 16 * ROW <= ROOM && TI % RI == 0, "staging room");
+    constexpr int XM = TJ * 4 >= 8 ? 7 : TJ * 4 - 1;
+    constexpr int RT = 32 / TJ, NT = 16 * RI / RT;  // rows of a turn, turns of RI bands
+    constexpr int BATCH = NT < 4 ? NT : 4, BATCHES = NT / BATCH, ALL = TI / RI * BATCHES;
+    const int r = lane & 15, g = lane >> 4, piece = 2 * (lane % (2 * TJ)), rr = lane / (2 * TJ);
+    auto ask_all = [&](auto B) {
+        constexpr int b = decltype(B)::value;
+        ozl::each<BATCH>([&](auto T) { ask(std::integral_constant<int, b & 1>{}, T, (b * BATCH + decltype(T)::value) * RT + rr); });
+    };
+    ask_all(std::integral_constant<int, 0>{});
+    ozl::each<TI / RI>([&](auto H) {
+        constexpr int h = decltype(H)::value;
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < RI; i++)
+#pragma unroll
+            for (int j = 0; j < TJ; j++) *reinterpret_cast<f32x4*>(tile + (16 * i + r) * ROW + 4 * ((4 * j + g) ^ (r & XM))) = acc[h * RI + i][j];
+        __builtin_amdgcn_wave_barrier();
+        ozl::each<BATCHES>([&](auto C) {
+            constexpr int c = decltype(C)::value, b = h * BATCHES + c;
+            if constexpr (b + 1 < ALL) ask_all(std::integral_constant<int, b + 1>{});
+            ozl::each<BATCH>([&](auto T) {
+                constexpr int t = decltype(T)::value;
+                const int row = (c * BATCH + t) * RT + rr;
+                float v[8];
+                f32x4* at[2];
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    at[k] = reinterpret_cast<f32x4*>(tile + row * ROW + 4 * ((piece + k) ^ (row & XM)));
+                    const f32x4 x = *at[k];
+#pragma unroll
+                    for (int m = 0; m < 4; m++) v[4 * k + m] = x[m];
+                }
+                use(std::integral_constant<int, b & 1>{}, T, 16 * RI * h + row, v);
+                if constexpr (TWICE) {
+#pragma unroll
+                    for (int k = 0; k < 2; k++) *at[k] = f32x4{v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]};
+                }
+            });
+        });
+        if constexpr (TWICE) {
+            if (twice) {
+                constexpr int LANES = ROW < 64 ? ROW : 64, STEP = 8 * 64 / LANES;  // columns at a time, rows of a step
+                __builtin_amdgcn_wave_barrier();
+#pragma unroll
+                for (int c0 = 0; c0 < ROW; c0 += LANES)
+#pragma unroll 2
+                    for (int r0 = 0; r0 < 16 * RI; r0 += STEP) {
+                        const int col = c0 + lane % LANES, row = r0 + 8 * (lane / LANES);
+                        float v[8];
+#pragma unroll
+                        for (int k = 0; k < 8; k++) v[k] = tile[(row + k) * ROW + 4 * ((col >> 2) ^ ((row + k) & XM)) + (col & 3)];
+                        across(16 * RI * h + row, col, v);
+                    }
+                __builtin_amdgcn_wave_barrier();
+            }
+        }
+    });
+}
+
+// What a wave's sums become; q0, p0: its first row and column.
+template <Phase PHASE, bool THREE, int TI, int TJ, int ROOM>
+__device__ __forceinline__ void finish(const Shape& s, const Ends& e, const Pass& pass, int i, bool mirror, const f32x4 (&acc)[TI][TJ], float* tile, int lane,
+                                       int q0, int p0) {
+    const Factors& f = pass.f;
+    const int col = p0 + 8 * (lane % (2 * TJ)), side = side_of(s);
+    u32x4 hs[2][4], ls[2][4];
+    if constexpr (PHASE != UPDATE) {
+        const long long nn = (long long)side * side;
+        const _Float16* a = square_of(s, s.a, i);
+        _Float16* to = PHASE == GRAM ? square_of(s, s.a, i) : square_of(s, s.b, i);
+        _Float16* rest = THREE ? to + nn : nullptr;
+        put_rows<TI, TJ, ROOM, true>(
+            acc, tile, lane, mirror,
+            [&](auto P, auto T, int row) {
+                if constexpr (PHASE == SQUARE) {
+                    constexpr int b = decltype(P)::value, t = decltype(T)::value;
+                    const long long at = (long long)(q0 + row) * side + col;
+                    if (q0 + row < side && col < side) {
+                        hs[b][t] = *reinterpret_cast<const u32x4*>(a + at);
+                        if constexpr (THREE) ls[b][t] = *reinterpret_cast<const u32x4*>(a + nn + at);
+                    }
+                }
+            },
+            [&](auto P, auto T, int row, float* v) {
+                constexpr int b = decltype(P)::value, t = decltype(T)::value;
+                if constexpr (PHASE == GRAM) {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) v[k] *= 1.0f / kScale / kScale;
+                } else {
+                    Half8 h, l;
+                    h.w = hs[b][t];
+                    if constexpr (THREE) l.w = ls[b][t];
+#pragma unroll
+                    for (int k = 0; k < 8; k++) {
+                        float x = (float)h.v[k];
+                        if constexpr (THREE) x += (float)l.v[k];
+                        v[k] = __builtin_fmaf(f.c, v[k], f.b * x);
+                    }
+                }
+                if (q0 + row < side && col < side) put8(to, rest, (long long)(q0 + row) * side + col, v);
+            },
+            [&](int row, int c, const float* v) {
+                if (q0 + row < side && p0 + c < side) put8(to, rest, (long long)(p0 + c) * side + q0 + row, v);
+            });
+    } else {
+        const _Float16 *h = h_of(s, pass.from, i), *l = l_of(s, pass.from, i);
+        _Float16 *to = h_of(s, pass.from ^ 1, i), *rest = l_of(s, pass.from ^ 1, i);
+        auto ask = [&](auto P, auto T, int row) {
+            constexpr int b = decltype(P)::value, t = decltype(T)::value;
+            const long long at = (long long)(q0 + row) * s.C + col;
+            if (q0 + row < s.R && col < s.C) {
+                hs[b][t] = *reinterpret_cast<const u32x4*>(h + at);
+                ls[b][t] = *reinterpret_cast<const u32x4*>(l + at);
+            }
+        };
+        auto value = [&](auto P, auto T, float* v) {
+            Half8 x, y;
+            x.w = hs[decltype(P)::value][decltype(T)::value], y.w = ls[decltype(P)::value][decltype(T)::value];
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = __builtin_fmaf(f.a, (float)x.v[k] + (float)y.v[k], v[k]);
+        };
+        auto none = [](int, int, const float*) {};
+        if (!pass.last) {
+            put_rows<TI, TJ, ROOM, false>(
+                acc, tile, lane, false, ask,
+                [&](auto P, auto T, int row, float* v) {
+                    value(P, T, v);
+                    if (q0 + row < s.R && col < s.C) put8(to, rest, (long long)(q0 + row) * s.C + col, v);
+                },
+                none);
+        } else if (e.tensors) {
+            const oz_muon_tensor t = e.tensors[s.first + i];
+            const float keep = 1.0f - e.lr * t.weight_decay, rate = e.lr * t.lr_scale * (1.0f / kScale);
+            put_rows<TI, TJ, ROOM, false>(
+                acc, tile, lane, false, ask,
+                [&](auto P, auto T, int row, float* v) {
+                    value(P, T, v);
+                    const int q = q0 + row, count = q < s.rows ? min(s.cols - col, 8) : 0;
+                    if (count <= 0) return;
+                    const long long at = (long long)q * s.cols + col;
+                    const void* from = t.master ? t.master : t.param;
+                    const int type = t.master ? OZ_F32 : t.param_type;
+                    float x[8];
+                    if (count == 8) load8(from, type, at, x);
+                    else load_some(from, type, at, count, x);
+#pragma unroll
+                    for (int k = 0; k < 8; k++) x[k] = x[k] * keep - v[k] * rate;
+                    if (count == 8) {
+                        if (t.master) store8(t.master, OZ_F32, at, x);
+                        store8(t.param, t.param_type, at, x);
+                    } else {
+                        if (t.master) store_some(t.master, OZ_F32, at, count, x);
+                        store_some(t.param, t.param_type, at, count, x);
+                    }
+                },
+                none);
+        } else {
+            put_rows<TI, TJ, ROOM, false>(
+                acc, tile, lane, false, ask,
+                [&](auto P, auto T, int row, float* v) {
+                    value(P, T, v);
+                    const int q = q0 + row, count = q < s.rows ? min(s.cols - col, 8) : 0;
+                    if (count <= 0) return;
+                    const long long at = (s.first + i) * e.stride_o + q * e.ldo + col;
+#pragma unroll
+                    for (int k = 0; k < 8; k++) v[k] *= 1.0f / kScale;
+                    if (count == 8) store8(e.O, e.type, at, v);
+                    else store_some(e.O, e.type, at, count, v);
+                },
+                none);
+        }
+    }
+}
+
+// ---- kernels ------------------------------------------------------------------------------------------
+
+struct Tile64 {
+    static constexpr int T = 64, TI = 2, TJ = 2, WP = 2, THREADS = 256, PER_SIMD = 2;
+    template <bool QM, bool PM, bool PARTS>
+    using Loop = ozl::TileLoop<Half<OZ_F16>, QM, PM, 2, 2, 2, 2, 4, PARTS>;
+};
+struct Tile128 {
+    static constexpr int T = 128, TI = 2, TJ = 4, WP = 2, THREADS = 512, PER_SIMD = 2;
+    template <bool QM, bool PM, bool PARTS>
+    using Loop = ozl::TileLoop<Half<OZ_F16>, QM, PM, 2, 4, 4, 2, 2, PARTS>;
+};
+struct Tile256 {
+    static constexpr int T = 256, TI = 8, TJ = 8, WP = 2, THREADS = 256, PER_SIMD = 1;
+    template <bool QM, bool PM, bool PARTS>
+    using Loop = ozl::BigLoop<Half<OZ_F16>, QM, PM, PARTS>;
+};
+
+template <Phase PHASE, class TILE, bool THREE>
+__global__ void __launch_bounds__(TILE::THREADS, TILE::PER_SIMD) newton_schulz_kernel(const Shapes m, const Ends ends, const Pass pass) {
+    constexpr int T = TILE::T;
+    typedef typename TILE::template Loop<false, false, THREE> Any;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[Any::LDS];
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int shape, i, tq, tp;
+    tile_place<PHASE>(m, pass.places, T, blockIdx.x, shape, i, tq, tp);
+    const Shape& s = m.s[shape];
+    const int side = side_of(s), q0 = T * tq, p0 = T * tp;
+    const long long nx = 2ll * s.R * s.C, nn = 2ll * side * side;  // bytes of a plane
+    f32x4 acc[TILE::TI][TILE::TJ];
+    // sum over c < C of Q(q, c) P(p, c)
+    auto run = [&](auto QM, auto PM, const _Float16* Q, int nq, int ldq, long long plane_q, const _Float16* P, int np, int ldp, long long plane_p, int C) {
+        typedef typename TILE::template Loop<decltype(QM)::value, decltype(PM)::value, THREE> Loop;
+        const int stages = C / ozl::BC;
+        typename Loop::OQ oq;
+        typename Loop::OP op;
+        oq.init(Q, ldq, nq, C, q0, 0, stages, lane, wave);
+        op.init(P, ldp, np, C, p0, 0, stages, lane, wave);
+        if constexpr (THREE) {  // h, h, l and h, l, h
+            const long long back_q = (long long)stages * oq.step, back_p = (long long)stages * op.step;
+            oq.parts(stages, -back_q, plane_q - back_q);
+            op.parts(stages, plane_p - back_p, -plane_p - back_p);
+        }
+        Loop::template run<uint16_t>(lds, oq, op, THREE ? 3 * stages : stages, 0, lane, wave, acc);
+    };
+    constexpr std::false_type no{};
+    constexpr std::true_type yes{};
+    const _Float16* x = h_of(s, pass.from, i);
+    if constexpr (PHASE == GRAM) {
+        if (is_tall(s)) run(yes, yes, x, s.C, s.C, nx, x, s.C, s.C, nx, s.R);
+        else run(no, no, x, s.R, s.C, nx, x, s.R, s.C, nx, s.C);
+    } else if constexpr (PHASE == SQUARE) {
+        const _Float16* a = square_of(s, s.a, i);
+        run(no, no, a, side, side, nn, a, side, side, nn, side);
+    } else {
+        const _Float16* b = square_of(s, s.b, i);
+        if (is_tall(s)) run(no, no, x, s.R, s.C, nx, b, side, side, nn, side);
+        else run(no, yes, b, side, side, nn, x, s.C, s.C, nx, side);
+    }
+    finish<PHASE, THREE, TILE::TI, TILE::TJ, Any::ROOM>(s, ends, pass, i, tq != tp, acc, reinterpret_cast<float*>(lds) + wave * Any::ROOM, lane,
+                                                        q0 + 16 * TILE::TI * (wave / TILE::WP), p0 + 16 * TILE::TJ * (wave % TILE::WP));
+}
+
+template <bool THREE>
+void launch_products(hipStream_t stream, Phase phase, int tile, const Shapes& m, const Ends& ends, const Pass& pass) {
+    const dim3 grid((unsigned)pass.places.first[m.n]);
+    auto with = [&](auto TILE) {
+        typedef decltype(TILE) Tile;
+        const dim3 block(Tile::THREADS);
+        if (phase == GRAM) hipLaunchKernelGGL((newton_schulz_kernel<GRAM, Tile, THREE>), grid, block, 0, stream, m, ends, pass);
+        else if (phase == SQUARE) hipLaunchKernelGGL((newton_schulz_kernel<SQUARE, Tile, THREE>), grid, block, 0, stream, m, ends, pass);
+        else hipLaunchKernelGGL((newton_schulz_kernel<UPDATE, Tile, THREE>), grid, block, 0, stream, m, ends, pass);
+    };
+    if (tile == 64) with(Tile64{});
+    else if (tile == 128) with(Tile128{});
+    else with(Tile256{});
+}
+
+}  // namespace ozn
