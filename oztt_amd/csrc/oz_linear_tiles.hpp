@@ -136,13 +136,13 @@ struct Operand {
     template <class T>
     __device__ static void zero_tail(uint8_t* stage, int valid, int thread) {
         if constexpr (!MAJOR) {
-            constexpr int E = 16 / sizeof(T);
+            constexpr int E = 16 / sizeof(T), LOG = sizeof(T) == 2 ? 3 : 4;
             const v4i none = {0, 0, 0, 0};
             for (int row = thread; row < ROWS; row += 64 * W) {
                 uint8_t* at = stage + 128 * row;
-                T* cut = reinterpret_cast<T*>(at + 16 * ((valid / E) ^ (row & 7)));
-                for (int e = valid % E; e < E; e++) cut[e] = 0;
-                for (int c = valid / E + 1; c < 8; c++) *reinterpret_cast<v4i*>(at + 16 * (c ^ (row & 7))) = none;
+                T* cut = reinterpret_cast<T*>(at + 16 * ((valid >> LOG) ^ (row & 7)));
+                for (int e = valid & (E - 1); e < E; e++) cut[e] = 0;
+                for (int c = (valid >> LOG) + 1; c < 8; c++) *reinterpret_cast<v4i*>(at + 16 * (c ^ (row & 7))) = none;
             }
         }
     }
@@ -349,7 +349,9 @@ struct TileLoop {
     static constexpr int STG_Q = 2 * BC * QR, STG = STG_Q + 2 * BC * PR, LD = OQ::N + OP::N, LDS = NSTG * STG, ROOM = LDS / W / 4;
 
     template <class TAIL>
-    __device__ static __forceinline__ void run(uint8_t* lds, OQ& oq, OP& op, int nst, int tail, int lane, int wave, Sums (&acc)[TI][TJ]) {
+    __device__ static __forceinline__ void run(uint8_t* lds, OQ& oq, OP& op, int nst, int tail, int lane, int wave, Sums (&out)[TI][TJ]) {
+        // sums of its own: on the caller's the compiler swaps registers in every stage of the tile of 32 x 32 (24 x 8192 x 2048 9.7 us for 8.9)
+        Sums acc[TI][TJ];
         auto issue = [&](uint8_t* to) {
 #pragma unroll
             for (int j = 0; j < OQ::N; j++) oq.copy(to, j, wave);
@@ -408,6 +410,10 @@ struct TileLoop {
         }
         wait_vmcnt<0>();
         __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TI; i++)
+#pragma unroll
+            for (int j = 0; j < TJ; j++) out[i][j] = acc[i][j];
     }
 };
 
