@@ -468,23 +468,24 @@ __device__ __forceinline__ void settle_sums() { asm volatile("s_nop 15\n\ts_nop 
 // stages, two of each and a spare: the copies of stage k + 2 of Q go out in stage k's first step and those of P in its second,
 // where Q's stage k is free, and have one and a half or two and a half steps to land. (With two whole stages all copies go out
 // in the second step and have one and a half: 852 against 763 us at 8192^3.)
-template <class M, bool QM, bool PM, bool PARTS = false>
+// B: 16 B outputs on a side of a wave, 8 or (128 x 128 outputs, two workgroups a CU) 4.
+template <class M, bool QM, bool PM, bool PARTS = false, int B = 8>
 struct BigLoop {
     typedef typename M::x8 T8;
     typedef typename M::sums Sums;
-    typedef Operand<QM, 256, 4, PARTS> OQ;
-    typedef Operand<PM, 256, 4, PARTS> OP;
-    static constexpr int UNIT = 2 * BC * 256, RING = 5 * UNIT, LD = OQ::N, LDS = RING, ROOM = RING / 4 / 4;
+    typedef Operand<QM, 32 * B, 4, PARTS> OQ;
+    typedef Operand<PM, 32 * B, 4, PARTS> OP;
+    static constexpr int UNIT = 2 * BC * 32 * B, RING = 5 * UNIT, LD = OQ::N, LDS = RING, ROOM = RING / 4 / 4;
     static_assert(OQ::N == OP::N, "copies of a unit");
 
     template <class TAIL>
-    __device__ static __forceinline__ void run(uint8_t* lds, OQ& oq, OP& op, int nst, int tail, int lane, int wave, Sums (&acc)[8][8]) {
+    __device__ static __forceinline__ void run(uint8_t* lds, OQ& oq, OP& op, int nst, int tail, int lane, int wave, Sums (&acc)[B][B]) {
         const int wq = wave >> 1, wp = wave & 1;
         const int lq = OQ::lane_offset(lane), lp = OP::lane_offset(lane);
 #pragma unroll
-        for (int i = 0; i < 8; i++)
+        for (int i = 0; i < B; i++)
 #pragma unroll
-            for (int j = 0; j < 8; j++) acc[i][j] = Sums{0, 0, 0, 0};
+            for (int j = 0; j < B; j++) acc[i][j] = Sums{0, 0, 0, 0};
         // Unit 2 k is Q's stage k, unit 2 k + 1 P's; unit u is at u UNIT modulo RING.
         auto landed = [&](auto LEFT, int k, int uq, int up) {  // stage k, whose units are at uq and up
             wait_vmcnt_lgkm0<decltype(LEFT)::value>();
@@ -505,31 +506,32 @@ struct BigLoop {
             oq.next();
             op.next();
         }
-        T8 fq[8], fp[8], gq[8], gp[8];
+        T8 fq[B], fp[B], gq[B], gp[B];
         landed(std::integral_constant<int, 2 * LD>{}, 0, 0, UNIT);
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-            fq[i] = OQ::template fragment<T8>(lds, 0, wq * 8 + i, lq);
-            fp[i] = OP::template fragment<T8>(lds + UNIT, 0, wp * 8 + i, lp);
+        for (int i = 0; i < B; i++) {
+            fq[i] = OQ::template fragment<T8>(lds, 0, wq * B + i, lq);
+            fp[i] = OP::template fragment<T8>(lds + UNIT, 0, wp * B + i, lp);
         }
-        // One step: 64 matrix instructions on (xq, xp); the 16 fragments (yq, yp) of step H of the units at uq and up, in the order
+        // One step: B B matrix instructions on (xq, xp); the 2 B fragments (yq, yp) of step H of the units at uq and up, in the order
         // their instructions want them; the copies of a unit of Q (in a stage's first step) or P to `to`.
         auto step = [&](auto H, T8* xq, T8* xp, T8* yq, T8* yp, int uq, int up, int to) {
             constexpr int h = decltype(H)::value;
             const uint8_t *rq = lds + uq, *rp = lds + up;
 #pragma unroll
-            for (int n = 0; n < 64; n++) {
-                const int i = n >> 3, j = n & 7;
+            for (int n = 0; n < B * B; n++) {
+                constexpr int R = B / 2;
+                const int i = n / B, j = n % B;
                 mfma_acc<M>(acc[i][j], xp[j], xq[i]);
-                if (n % 4 == 0) {
-                    const int t = n / 4;
-                    if (t == 0) yq[0] = OQ::template fragment<T8>(rq, h, wq * 8, lq);
-                    else if (t <= 8) yp[t - 1] = OP::template fragment<T8>(rp, h, wp * 8 + t - 1, lp);
-                    else yq[t - 8] = OQ::template fragment<T8>(rq, h, wq * 8 + t - 8, lq);
+                if (n % R == 0) {
+                    const int t = n / R;
+                    if (t == 0) yq[0] = OQ::template fragment<T8>(rq, h, wq * B, lq);
+                    else if (t <= B) yp[t - 1] = OP::template fragment<T8>(rp, h, wp * B + t - 1, lp);
+                    else yq[t - B] = OQ::template fragment<T8>(rq, h, wq * B + t - B, lq);
                 }
-                if (n % 4 == 2 && n / 4 < LD) {
-                    if constexpr (h == 1) oq.copy(lds + to, n / 4, wave);
-                    else op.copy(lds + to, n / 4, wave);
+                if (n % R == R / 2 && n / R < LD) {
+                    if constexpr (h == 1) oq.copy(lds + to, n / R, wave);
+                    else op.copy(lds + to, n / R, wave);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }

@@ -85,6 +85,8 @@ __device__ __forceinline__ void put8(_Float16* h, _Float16* l, long long at, con
 // The sums of a wave, through LDS as in ozl::put_sums, 8 values of a row at a time: ask(P, t, row) loads what the t-th piece of a batch
 // wants, a batch ahead, use(P, t, row, v) finishes it (P: the batch's parity; rows and columns are the wave's own). With TWICE use()'s
 // values go back to LDS, and across(row, col, v) gets 8 values of a column from `row` on.
+template <int TI>
+constexpr int kBatch = TI == 8 ? 8 : TI == 4 ? 4 : 2;
 template <int TI, int TJ, int ROOM, bool TWICE, class Ask, class Use, class Across>
 __device__ __forceinline__ void put_rows(const f32x4 (&acc)[TI][TJ], float* tile, int lane, bool twice, Ask&& ask, Use&& use, Across&& across) {
     constexpr int ROW = 16 * TJ;
@@ -92,7 +94,8 @@ __device__ __forceinline__ void put_rows(const f32x4 (&acc)[TI][TJ], float* tile
     static_assert(RI >= 1 && RI * 16 * ROW <= ROOM && TI % RI == 0, "staging room");
     constexpr int XM = TJ * 4 >= 8 ? 7 : TJ * 4 - 1;
     constexpr int RT = 32 / TJ, NT = 16 * RI / RT;  // rows of a turn, turns of RI bands
-    constexpr int BATCH = NT < 4 ? NT : 4, BATCHES = NT / BATCH, ALL = TI / RI * BATCHES;
+    constexpr int BATCH = kBatch<TI>, BATCHES = NT / BATCH, ALL = TI / RI * BATCHES;
+    static_assert(BATCHES * BATCH == NT, "whole batches");
     const int r = lane & 15, g = lane >> 4, piece = 2 * (lane % (2 * TJ)), rr = lane / (2 * TJ);
     auto ask_all = [&](auto B) {
         constexpr int b = decltype(B)::value;
@@ -155,7 +158,7 @@ __device__ __forceinline__ void finish(const Shape& s, const Ends& e, const Pass
                                        int q0, int p0) {
     const Factors& f = pass.f;
     const int col = p0 + 8 * (lane % (2 * TJ)), side = side_of(s);
-    u32x4 hs[2][4], ls[2][4];
+    u32x4 hs[2][kBatch<TI>], ls[2][kBatch<TI>];
     if constexpr (PHASE != UPDATE) {
         const long long nn = (long long)side * side;
         const _Float16* a = square_of(s, s.a, i);
@@ -272,9 +275,9 @@ struct Tile64 {
     using Loop = ozl::TileLoop<Half<OZ_F16>, QM, PM, 2, 2, 2, 2, 4, PARTS>;
 };
 struct Tile128 {
-    static constexpr int T = 128, TI = 2, TJ = 4, WP = 2, THREADS = 512, PER_SIMD = 2;
+    static constexpr int T = 128, TI = 4, TJ = 4, WP = 2, THREADS = 256, PER_SIMD = 2;
     template <bool QM, bool PM, bool PARTS>
-    using Loop = ozl::TileLoop<Half<OZ_F16>, QM, PM, 2, 4, 4, 2, 2, PARTS>;
+    using Loop = ozl::BigLoop<Half<OZ_F16>, QM, PM, PARTS, 4>;
 };
 struct Tile256 {
     static constexpr int T = 256, TI = 8, TJ = 8, WP = 2, THREADS = 256, PER_SIMD = 1;
