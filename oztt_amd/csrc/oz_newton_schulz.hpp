@@ -60,10 +60,10 @@ __device__ __forceinline__ Place place_of(const Places& p, int n, int w) {
 
 __host__ __device__ inline int side_of(const Shape& s) { return s.R < s.C ? s.R : s.C; }
 __host__ __device__ inline bool is_tall(const Shape& s) { return s.rows > s.cols; }
-__device__ __forceinline__ _Float16* h_of(const Shape& s, int b, int i) { return s.x[b] + (long long)(1 + s.three) * i * s.R * s.C; }
+__device__ __forceinline__ _Float16* h_of(const Shape& s, int b, int i) { return (b ? s.x[1] : s.x[0]) + (long long)(1 + s.three) * i * s.R * s.C; }
 __device__ __forceinline__ _Float16* l_of(const Shape& s, int b, int i) {
     const long long n = (long long)s.R * s.C;
-    return s.three ? s.x[b] + (2 * i + 1) * n : s.l + i * n;
+    return s.three ? (b ? s.x[1] : s.x[0]) + (2 * i + 1) * n : s.l + i * n;
 }
 // A or B of a matrix
 __device__ __forceinline__ _Float16* square_of(const Shape& s, _Float16* p, int i) { return p + (long long)(1 + s.three) * i * side_of(s) * side_of(s); }

@@ -46,16 +46,18 @@ __device__ __forceinline__ int xcd_run(int first, int i, int P) {
 
 // Workgroup -> shape, matrix and tile. Shapes come one after the other (the long ones first, as they differ in length), within a shape
 // each XCD takes one contiguous run of the tiles, so that what it runs at a time shares rows and columns in its L2.
-template <Phase PHASE>
-__device__ __forceinline__ void tile_place(const Shapes& m, const Places& p, int T, int w, int& shape, int& matrix, int& tq, int& tp) {
+template <Phase PHASE, int T>
+__device__ __forceinline__ void tile_place(const Shapes& m, const Places& p, int w, int& shape, int& matrix, int& tq, int& tp) {
     shape = __builtin_amdgcn_readfirstlane(shape_of(p, m.n, w));
     const Shape& s = m.s[shape];
     const int i = xcd_run(p.first[shape], w - p.first[shape], p.per[shape] * s.count);
     matrix = __builtin_amdgcn_readfirstlane(i / p.per[shape]);
     const int u = __builtin_amdgcn_readfirstlane(i - matrix * p.per[shape]);
     if constexpr (PHASE == UPDATE) {
+        // groups of rows column by column: what an XCD runs at a time is 8 x 8 tiles of 128 (4 x 16: 782 for 750 us) or 4 x 8 of 256
+        constexpr int G = T == 256 ? 4 : 8;
         const int rows = (s.R + T - 1) / T, cols = (s.C + T - 1) / T;
-        const int group = u / (4 * cols), first = 4 * group, g = min(rows - first, 4), v = u - group * 4 * cols;
+        const int group = u / (G * cols), first = G * group, g = min(rows - first, G), v = u - group * G * cols;
         tq = first + v % g, tp = v / g;
     } else {
         triangle(u, (side_of(s) + T - 1) / T, tq, tp);
@@ -70,7 +72,8 @@ union Half8 {
     u32x4 w;
     f16x8 v;
 };
-// v in one or two parts to h and l.
+// v in one or two parts to h and l. PAST: past the caches, which the products' operands need more.
+template <bool PAST>
 __device__ __forceinline__ void put8(_Float16* h, _Float16* l, long long at, const float* v) {
     f16x8 x, y;
 #pragma unroll
@@ -78,30 +81,46 @@ __device__ __forceinline__ void put8(_Float16* h, _Float16* l, long long at, con
         x[k] = (_Float16)v[k];
         y[k] = (_Float16)(v[k] - (float)x[k]);
     }
-    *reinterpret_cast<f16x8*>(h + at) = x;
-    if (l) *reinterpret_cast<f16x8*>(l + at) = y;
+    if constexpr (PAST) {
+        __builtin_nontemporal_store(x, reinterpret_cast<f16x8*>(h + at));
+        __builtin_nontemporal_store(y, reinterpret_cast<f16x8*>(l + at));
+    } else {
+        *reinterpret_cast<f16x8*>(h + at) = x;
+        if (l) *reinterpret_cast<f16x8*>(l + at) = y;
+    }
 }
 
-// The sums of a wave, through LDS as in ozl::put_sums, 8 values of a row at a time: ask(P, t, row) loads what the t-th piece of a batch
-// wants, a batch ahead, use(P, t, row, v) finishes it (P: the batch's parity; rows and columns are the wave's own). With TWICE use()'s
-// values go back to LDS, and across(row, col, v) gets 8 values of a column from `row` on.
-template <int TI>
-constexpr int kBatch = TI == 8 ? 8 : TI == 4 ? 4 : 2;
+// How a wave's sums go through LDS: RI bands of 16 rows at a time, turns of RT rows, a lane 8 values in a row; pieces of what they
+// are added to are asked for in batches.
+template <int TI, int TJ, int ROOM>
+struct Bands {
+    static constexpr int ROW = 16 * TJ;
+    static constexpr int RI = TI * 16 * ROW <= ROOM ? TI : TI * 8 * ROW <= ROOM ? TI / 2 : TI / 4;
+    static_assert(RI >= 1 && RI * 16 * ROW <= ROOM && TI % RI == 0, "staging room");
+    static constexpr int RT = 32 / TJ, NT = 16 * RI / RT;
+    static constexpr int BATCH = NT < 8 ? NT : 8, ALL = TI / RI * NT / BATCH;  // of a turn's pieces; batches of a tile
+    static_assert(NT % BATCH == 0, "whole batches");
+    // With one batch a tile's pieces are asked for before its products and wait in registers: four large blocks' update in tiles of 128 x
+    // 128 WITHOUT 790 us, with them there WITH. More do not fit: two in turn, a batch ahead.
+    static constexpr bool AHEAD = ALL == 1;
+    static constexpr int BUFFERS = AHEAD ? 1 : 2;
+};
+
+// The sums of a wave, as in ozl::put_sums: ask(P, t, row) loads what the t-th piece of a batch wants, use(P, t, row, v) finishes its 8
+// values (P: the batch's buffer; rows and columns are the wave's own). With TWICE use()'s values go back to LDS, and across(row, col, v)
+// gets 8 values of a column from `row` on.
+template <int TI, int TJ, int ROOM, class Ask, class P>
+__device__ __forceinline__ void ask_batch(int lane, Ask&& ask, int b, P p) {
+    typedef Bands<TI, TJ, ROOM> S;
+    ozl::each<S::BATCH>([&](auto T) { ask(p, T, (b * S::BATCH + decltype(T)::value) * S::RT + lane / (2 * TJ)); });
+}
 template <int TI, int TJ, int ROOM, bool TWICE, class Ask, class Use, class Across>
 __device__ __forceinline__ void put_rows(const f32x4 (&acc)[TI][TJ], float* tile, int lane, bool twice, Ask&& ask, Use&& use, Across&& across) {
-    constexpr int ROW = 16 * TJ;
-    constexpr int RI = TI * 16 * ROW <= ROOM ? TI : TI * 8 * ROW <= ROOM ? TI / 2 : TI / 4;
-    static_assert(RI >= 1 && RI * 16 * ROW <= ROOM && TI % RI == 0, "staging room");
+    typedef Bands<TI, TJ, ROOM> S;
+    constexpr int ROW = S::ROW, RI = S::RI, RT = S::RT, BATCHES = S::NT / S::BATCH;
     constexpr int XM = TJ * 4 >= 8 ? 7 : TJ * 4 - 1;
-    constexpr int RT = 32 / TJ, NT = 16 * RI / RT;  // rows of a turn, turns of RI bands
-    constexpr int BATCH = kBatch<TI>, BATCHES = NT / BATCH, ALL = TI / RI * BATCHES;
-    static_assert(BATCHES * BATCH == NT, "whole batches");
     const int r = lane & 15, g = lane >> 4, piece = 2 * (lane % (2 * TJ)), rr = lane / (2 * TJ);
-    auto ask_all = [&](auto B) {
-        constexpr int b = decltype(B)::value;
-        ozl::each<BATCH>([&](auto T) { ask(std::integral_constant<int, b & 1>{}, T, (b * BATCH + decltype(T)::value) * RT + rr); });
-    };
-    ask_all(std::integral_constant<int, 0>{});
+    if constexpr (!S::AHEAD) ask_batch<TI, TJ, ROOM>(lane, ask, 0, std::integral_constant<int, 0>{});
     ozl::each<TI / RI>([&](auto H) {
         constexpr int h = decltype(H)::value;
         __builtin_amdgcn_wave_barrier();
@@ -112,10 +131,10 @@ __device__ __forceinline__ void put_rows(const f32x4 (&acc)[TI][TJ], float* tile
         __builtin_amdgcn_wave_barrier();
         ozl::each<BATCHES>([&](auto C) {
             constexpr int c = decltype(C)::value, b = h * BATCHES + c;
-            if constexpr (b + 1 < ALL) ask_all(std::integral_constant<int, b + 1>{});
-            ozl::each<BATCH>([&](auto T) {
+            if constexpr (b + 1 < S::ALL) ask_batch<TI, TJ, ROOM>(lane, ask, b + 1, std::integral_constant<int, (b + 1) & 1>{});
+            ozl::each<S::BATCH>([&](auto T) {
                 constexpr int t = decltype(T)::value;
-                const int row = (c * BATCH + t) * RT + rr;
+                const int row = (c * S::BATCH + t) * RT + rr;
                 float v[8];
                 f32x4* at[2];
 #pragma unroll
@@ -125,7 +144,7 @@ __device__ __forceinline__ void put_rows(const f32x4 (&acc)[TI][TJ], float* tile
 #pragma unroll
                     for (int m = 0; m < 4; m++) v[4 * k + m] = x[m];
                 }
-                use(std::integral_constant<int, b & 1>{}, T, 16 * RI * h + row, v);
+                use(std::integral_constant<int, b % S::BUFFERS>{}, T, 16 * RI * h + row, v);
                 if constexpr (TWICE) {
 #pragma unroll
                     for (int k = 0; k < 2; k++) *at[k] = f32x4{v[4 * k], v[4 * k + 1], v[4 * k + 2], v[4 * k + 3]};
@@ -152,120 +171,123 @@ __device__ __forceinline__ void put_rows(const f32x4 (&acc)[TI][TJ], float* tile
     });
 }
 
-// What a wave's sums become; q0, p0: its first row and column.
+// What a wave's sums become: its first row and column q0 and p0, the lane's column. SQUARE adds to A, UPDATE to X.
 template <Phase PHASE, bool THREE, int TI, int TJ, int ROOM>
-__device__ __forceinline__ void finish(const Shape& s, const Ends& e, const Pass& pass, int i, bool mirror, const f32x4 (&acc)[TI][TJ], float* tile, int lane,
-                                       int q0, int p0) {
-    const Factors& f = pass.f;
-    const int col = p0 + 8 * (lane % (2 * TJ)), side = side_of(s);
-    u32x4 hs[2][kBatch<TI>], ls[2][kBatch<TI>];
-    if constexpr (PHASE != UPDATE) {
-        const long long nn = (long long)side * side;
-        const _Float16* a = square_of(s, s.a, i);
-        _Float16* to = PHASE == GRAM ? square_of(s, s.a, i) : square_of(s, s.b, i);
-        _Float16* rest = THREE ? to + nn : nullptr;
-        put_rows<TI, TJ, ROOM, true>(
-            acc, tile, lane, mirror,
-            [&](auto P, auto T, int row) {
-                if constexpr (PHASE == SQUARE) {
-                    constexpr int b = decltype(P)::value, t = decltype(T)::value;
-                    const long long at = (long long)(q0 + row) * side + col;
-                    if (q0 + row < side && col < side) {
-                        hs[b][t] = *reinterpret_cast<const u32x4*>(a + at);
-                        if constexpr (THREE) ls[b][t] = *reinterpret_cast<const u32x4*>(a + nn + at);
-                    }
-                }
-            },
-            [&](auto P, auto T, int row, float* v) {
-                constexpr int b = decltype(P)::value, t = decltype(T)::value;
-                if constexpr (PHASE == GRAM) {
-#pragma unroll
-                    for (int k = 0; k < 8; k++) v[k] *= 1.0f / kScale / kScale;
-                } else {
-                    Half8 h, l;
-                    h.w = hs[b][t];
-                    if constexpr (THREE) l.w = ls[b][t];
-#pragma unroll
-                    for (int k = 0; k < 8; k++) {
-                        float x = (float)h.v[k];
-                        if constexpr (THREE) x += (float)l.v[k];
-                        v[k] = __builtin_fmaf(f.c, v[k], f.b * x);
-                    }
-                }
-                if (q0 + row < side && col < side) put8(to, rest, (long long)(q0 + row) * side + col, v);
-            },
-            [&](int row, int c, const float* v) {
-                if (q0 + row < side && p0 + c < side) put8(to, rest, (long long)(p0 + c) * side + q0 + row, v);
-            });
-    } else {
-        const _Float16 *h = h_of(s, pass.from, i), *l = l_of(s, pass.from, i);
-        _Float16 *to = h_of(s, pass.from ^ 1, i), *rest = l_of(s, pass.from ^ 1, i);
-        auto ask = [&](auto P, auto T, int row) {
-            constexpr int b = decltype(P)::value, t = decltype(T)::value;
-            const long long at = (long long)(q0 + row) * s.C + col;
-            if (q0 + row < s.R && col < s.C) {
-                hs[b][t] = *reinterpret_cast<const u32x4*>(h + at);
-                ls[b][t] = *reinterpret_cast<const u32x4*>(l + at);
-            }
-        };
-        auto value = [&](auto P, auto T, float* v) {
-            Half8 x, y;
-            x.w = hs[decltype(P)::value][decltype(T)::value], y.w = ls[decltype(P)::value][decltype(T)::value];
-#pragma unroll
-            for (int k = 0; k < 8; k++) v[k] = __builtin_fmaf(f.a, (float)x.v[k] + (float)y.v[k], v[k]);
-        };
-        auto none = [](int, int, const float*) {};
-        if (!pass.last) {
-            put_rows<TI, TJ, ROOM, false>(
-                acc, tile, lane, false, ask,
-                [&](auto P, auto T, int row, float* v) {
-                    value(P, T, v);
-                    if (q0 + row < s.R && col < s.C) put8(to, rest, (long long)(q0 + row) * s.C + col, v);
-                },
-                none);
-        } else if (e.tensors) {
-            const oz_muon_tensor t = e.tensors[s.first + i];
-            const float keep = 1.0f - e.lr * t.weight_decay, rate = e.lr * t.lr_scale * (1.0f / kScale);
-            put_rows<TI, TJ, ROOM, false>(
-                acc, tile, lane, false, ask,
-                [&](auto P, auto T, int row, float* v) {
-                    value(P, T, v);
-                    const int q = q0 + row, count = q < s.rows ? min(s.cols - col, 8) : 0;
-                    if (count <= 0) return;
-                    const long long at = (long long)q * s.cols + col;
-                    const void* from = t.master ? t.master : t.param;
-                    const int type = t.master ? OZ_F32 : t.param_type;
-                    float x[8];
-                    if (count == 8) load8(from, type, at, x);
-                    else load_some(from, type, at, count, x);
-#pragma unroll
-                    for (int k = 0; k < 8; k++) x[k] = x[k] * keep - v[k] * rate;
-                    if (count == 8) {
-                        if (t.master) store8(t.master, OZ_F32, at, x);
-                        store8(t.param, t.param_type, at, x);
-                    } else {
-                        if (t.master) store_some(t.master, OZ_F32, at, count, x);
-                        store_some(t.param, t.param_type, at, count, x);
-                    }
-                },
-                none);
-        } else {
-            put_rows<TI, TJ, ROOM, false>(
-                acc, tile, lane, false, ask,
-                [&](auto P, auto T, int row, float* v) {
-                    value(P, T, v);
-                    const int q = q0 + row, count = q < s.rows ? min(s.cols - col, 8) : 0;
-                    if (count <= 0) return;
-                    const long long at = (s.first + i) * e.stride_o + q * e.ldo + col;
-#pragma unroll
-                    for (int k = 0; k < 8; k++) v[k] *= 1.0f / kScale;
-                    if (count == 8) store8(e.O, e.type, at, v);
-                    else store_some(e.O, e.type, at, count, v);
-                },
-                none);
+struct Finish {
+    typedef Bands<TI, TJ, ROOM> S;
+    const Shape s;
+    const Factors f;
+    const int from, last;
+    int i, lane, q0, p0, col, side;
+    u32x4 hs[S::BUFFERS][S::BATCH], ls[S::BUFFERS][S::BATCH];
+
+    __device__ __forceinline__ Finish(const Shape& s, const Pass& pass, int i, int lane, int q0, int p0)
+        : s(s), f(pass.f), from(pass.from), last(pass.last), i(i), lane(lane), q0(q0), p0(p0), col(p0 + 8 * (lane % (2 * TJ))), side(side_of(s)) {}
+
+    template <class P, class T>
+    __device__ __forceinline__ void ask(P, T, int row) {
+        if constexpr (PHASE == GRAM) return;
+        constexpr int b = P::value, t = T::value;
+        const int rows = PHASE == SQUARE ? side : s.R, cols = PHASE == SQUARE ? side : s.C;
+        const _Float16* h = PHASE == SQUARE ? square_of(s, s.a, i) : h_of(s, from, i);
+        const _Float16* l = PHASE == SQUARE ? h + (long long)side * side : l_of(s, from, i);
+        const long long at = (long long)(q0 + row) * cols + col;
+        if (q0 + row < rows && col < cols) {
+            hs[b][t] = *reinterpret_cast<const u32x4*>(h + at);
+            if constexpr (PHASE == UPDATE && !THREE) ls[b][t] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(l + at));
+            else if constexpr (THREE) ls[b][t] = *reinterpret_cast<const u32x4*>(l + at);
         }
     }
-}
+    __device__ __forceinline__ void ahead() {
+        if constexpr (S::AHEAD) ask_batch<TI, TJ, ROOM>(lane, [&](auto P, auto T, int row) { ask(P, T, row); }, 0, std::integral_constant<int, 0>{});
+    }
+    // v = factor times what it is added to, and `of` v
+    template <class P, class T>
+    __device__ __forceinline__ void add(P, T, float factor, float of, float* v) const {
+        Half8 x, y;
+        x.w = hs[P::value][T::value], y.w = ls[P::value][T::value];
+#pragma unroll
+        for (int k = 0; k < 8; k++) {
+            float z = (float)x.v[k];
+            if constexpr (THREE || PHASE == UPDATE) z += (float)y.v[k];
+            v[k] = __builtin_fmaf(of, v[k], factor * z);
+        }
+    }
+
+    __device__ __forceinline__ void put(const Ends& e, bool mirror, const f32x4 (&acc)[TI][TJ], float* tile) {
+        const auto get = [&](auto P, auto T, int row) { ask(P, T, row); };
+        if constexpr (PHASE != UPDATE) {
+            _Float16* to = PHASE == GRAM ? square_of(s, s.a, i) : square_of(s, s.b, i);
+            _Float16* rest = THREE ? to + (long long)side * side : nullptr;
+            put_rows<TI, TJ, ROOM, true>(
+                acc, tile, lane, mirror, get,
+                [&](auto P, auto T, int row, float* v) {
+                    if constexpr (PHASE == GRAM) {
+#pragma unroll
+                        for (int k = 0; k < 8; k++) v[k] *= 1.0f / kScale / kScale;
+                    } else {
+                        add(P, T, f.b, f.c, v);
+                    }
+                    if (q0 + row < side && col < side) put8<false>(to, rest, (long long)(q0 + row) * side + col, v);
+                },
+                [&](int row, int c, const float* v) {
+                    if (q0 + row < side && p0 + c < side) put8<false>(to, rest, (long long)(p0 + c) * side + q0 + row, v);
+                });
+        } else {
+            auto none = [](int, int, const float*) {};
+            if (!last) {
+                _Float16 *to = h_of(s, from ^ 1, i), *rest = l_of(s, from ^ 1, i);
+                put_rows<TI, TJ, ROOM, false>(
+                    acc, tile, lane, false, get,
+                    [&](auto P, auto T, int row, float* v) {
+                        add(P, T, f.a, 1.0f, v);
+                        if (q0 + row < s.R && col < s.C) put8<!THREE>(to, rest, (long long)(q0 + row) * s.C + col, v);
+                    },
+                    none);
+            } else if (e.tensors) {
+                const oz_muon_tensor t = e.tensors[s.first + i];
+                const float keep = 1.0f - e.lr * t.weight_decay, rate = e.lr * t.lr_scale * (1.0f / kScale);
+                put_rows<TI, TJ, ROOM, false>(
+                    acc, tile, lane, false, get,
+                    [&](auto P, auto T, int row, float* v) {
+                        add(P, T, f.a, 1.0f, v);
+                        const int q = q0 + row, count = q < s.rows ? min(s.cols - col, 8) : 0;
+                        if (count <= 0) return;
+                        const long long at = (long long)q * s.cols + col;
+                        const void* from = t.master ? t.master : t.param;
+                        const int type = t.master ? OZ_F32 : t.param_type;
+                        float x[8];
+                        if (count == 8) load8(from, type, at, x);
+                        else load_some(from, type, at, count, x);
+#pragma unroll
+                        for (int k = 0; k < 8; k++) x[k] = x[k] * keep - v[k] * rate;
+                        if (count == 8) {
+                            if (t.master) store8(t.master, OZ_F32, at, x);
+                            store8(t.param, t.param_type, at, x);
+                        } else {
+                            if (t.master) store_some(t.master, OZ_F32, at, count, x);
+                            store_some(t.param, t.param_type, at, count, x);
+                        }
+                    },
+                    none);
+            } else {
+                put_rows<TI, TJ, ROOM, false>(
+                    acc, tile, lane, false, get,
+                    [&](auto P, auto T, int row, float* v) {
+                        add(P, T, f.a, 1.0f, v);
+                        const int q = q0 + row, count = q < s.rows ? min(s.cols - col, 8) : 0;
+                        if (count <= 0) return;
+                        const long long at = (s.first + i) * e.stride_o + q * e.ldo + col;
+#pragma unroll
+                        for (int k = 0; k < 8; k++) v[k] *= 1.0f / kScale;
+                        if (count == 8) store8(e.O, e.type, at, v);
+                        else store_some(e.O, e.type, at, count, v);
+                    },
+                    none);
+            }
+        }
+    }
+};
 
 // ---- kernels ------------------------------------------------------------------------------------------
 
@@ -293,8 +315,8 @@ __global__ void __launch_bounds__(TILE::THREADS, TILE::PER_SIMD) newton_schulz_k
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int shape, i, tq, tp;
-    tile_place<PHASE>(m, pass.places, T, blockIdx.x, shape, i, tq, tp);
-    const Shape& s = m.s[shape];
+    tile_place<PHASE, T>(m, pass.places, blockIdx.x, shape, i, tq, tp);
+    const Shape s = m.s[shape];
     const int side = side_of(s), q0 = T * tq, p0 = T * tp;
     const long long nx = 2ll * s.R * s.C, nn = 2ll * side * side;  // bytes of a plane
     f32x4 acc[TILE::TI][TILE::TJ];
@@ -316,6 +338,10 @@ __global__ void __launch_bounds__(TILE::THREADS, TILE::PER_SIMD) newton_schulz_k
     constexpr std::false_type no{};
     constexpr std::true_type yes{};
     const _Float16* x = h_of(s, pass.from, i);
+    typedef Finish<PHASE, THREE, TILE::TI, TILE::TJ, Any::ROOM> Put;
+    const int q1 = q0 + 16 * TILE::TI * (wave / TILE::WP), p1 = p0 + 16 * TILE::TJ * (wave % TILE::WP);
+    Put put(s, pass, i, lane, q1, p1);
+    put.ahead();
     if constexpr (PHASE == GRAM) {
         if (is_tall(s)) run(yes, yes, x, s.C, s.C, nx, x, s.C, s.C, nx, s.R);
         else run(no, no, x, s.R, s.C, nx, x, s.R, s.C, nx, s.C);
@@ -327,8 +353,9 @@ __global__ void __launch_bounds__(TILE::THREADS, TILE::PER_SIMD) newton_schulz_k
         if (is_tall(s)) run(no, no, x, s.R, s.C, nx, b, side, side, nn, side);
         else run(no, yes, b, side, side, nn, x, s.C, s.C, nx, side);
     }
-    finish<PHASE, THREE, TILE::TI, TILE::TJ, Any::ROOM>(s, ends, pass, i, tq != tp, acc, reinterpret_cast<float*>(lds) + wave * Any::ROOM, lane,
-                                                        q0 + 16 * TILE::TI * (wave / TILE::WP), p0 + 16 * TILE::TJ * (wave % TILE::WP));
+    float* room = reinterpret_cast<float*>(lds) + wave * Any::ROOM;
+    if constexpr (Put::S::AHEAD) put.put(ends, tq != tp, acc, room);
+    else Put(s, pass, i, lane, q1, p1).put(ends, tq != tp, acc, room);
 }
 
 template <bool THREE>
