@@ -18,9 +18,9 @@ using namespace ozt;
 using namespace ozn;
 
 constexpr int THREADS = 256, V = 8;
-constexpr int kChunk = V * THREADS * 4;  // least values of a chunk
+constexpr int kChunk = V * THREADS;      // least values of a chunk
 constexpr int kMaxChunks = 512;          // of a matrix: each workgroup of the second pass adds them all
-constexpr int kRounds = 8;               // pieces of a thread in the second pass
+constexpr int kRounds = 8;               // pieces of a thread in the second pass, where they are many
 
 // Eight values in a row, `count` of them there.
 __device__ __forceinline__ void get(const void* p, int type, long long i, int count, float* x) {
@@ -93,7 +93,7 @@ __global__ void __launch_bounds__(THREADS) squares_kernel(const Shapes shapes, c
 }
 
 // X0 in the shapes' x[0].
-__global__ void __launch_bounds__(THREADS) start_kernel(const Shapes shapes, const Ends e, const Places places, double eps) {
+__global__ void __launch_bounds__(THREADS) start_kernel(const Shapes shapes, const Ends e, const Places places, double eps, int rounds) {
     const Place w = place_of(places, shapes.n, blockIdx.x);
     const Shape& s = shapes.s[w.shape];
     double sum = 0.0;
@@ -106,8 +106,8 @@ __global__ void __launch_bounds__(THREADS) start_kernel(const Shapes shapes, con
     const long long n = (long long)across * s.R;
     _Float16 *h = h_of(s, 0, w.matrix), *l = l_of(s, 0, w.matrix);
     const float gs = e.grad_scale ? *e.grad_scale : 1.0f;
-    for (int round = 0; round < kRounds; round++) {
-        const long long j = THREADS * ((long long)kRounds * w.index + round) + threadIdx.x;
+    for (int round = 0; round < rounds; round++) {
+        const long long j = THREADS * ((long long)rounds * w.index + round) + threadIdx.x;
         if (j >= n) return;
         const unsigned row = (unsigned)j / across, col = V * ((unsigned)j % across);
         const int count = (int)row < s.rows ? min(max((int)(s.cols - col), 0), V) : 0;
@@ -166,10 +166,12 @@ size_t lay_out(Shape* s, int rows, int cols, int count, int first, bool exact, c
 // Both passes and the iteration.
 int orthogonalize(oz_dev* dev, const Shapes& m, const Ends& e, const Factors& f, double eps, int steps) {
     Places squares{}, start{};
-    long long a = 0, b = 0;
+    long long a = 0, b = 0, all = 0;
+    for (int k = 0; k < m.n; k++) all += (long long)m.s[k].R * m.s[k].C * m.s[k].count;
+    const int rounds = all >= (long long)V * THREADS * kRounds * 4 * dev->cus ? kRounds : 1;
     for (int k = 0; k < m.n; k++) {
         const Shape& s = m.s[k];
-        const long long pieces = (long long)s.R * s.C / V, per = (pieces + THREADS * kRounds - 1) / (THREADS * kRounds);
+        const long long pieces = (long long)s.R * s.C / V, per = (pieces + THREADS * rounds - 1) / (THREADS * rounds);
         squares.first[k] = (int)a, squares.per[k] = s.chunks;
         start.first[k] = (int)b, start.per[k] = (int)per;
         a += (long long)s.chunks * s.count;
@@ -179,7 +181,7 @@ int orthogonalize(oz_dev* dev, const Shapes& m, const Ends& e, const Factors& f,
     squares.first[m.n] = (int)a, start.first[m.n] = (int)b;
     hipLaunchKernelGGL(squares_kernel, dim3((unsigned)a), dim3(THREADS), 0, dev->stream, m, e, squares);
     if (int st = oz::launch_check(dev, "squares_kernel")) return st;
-    hipLaunchKernelGGL(start_kernel, dim3((unsigned)b), dim3(THREADS), 0, dev->stream, m, e, start, eps);
+    hipLaunchKernelGGL(start_kernel, dim3((unsigned)b), dim3(THREADS), 0, dev->stream, m, e, start, eps, rounds);
     if (int st = oz::launch_check(dev, "start_kernel")) return st;
     return iterate(dev, m, e, f, steps);
 }

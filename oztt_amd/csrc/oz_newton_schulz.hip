@@ -4,12 +4,31 @@
 
 #include <algorithm>
 
-extern template void ozn::launch_products<true>(hipStream_t, Phase, int, const Shapes&, const Ends&, const Pass&);
-template void ozn::launch_products<false>(hipStream_t, Phase, int, const Shapes&, const Ends&, const Pass&);
+extern template void ozn::launch_products<true>(hipStream_t, Phase, Kind, const Shapes&, const Ends&, const Pass&);
+template void ozn::launch_products<false>(hipStream_t, Phase, Kind, const Shapes&, const Ends&, const Pass&);
 
 namespace {
 
 using namespace ozn;
+
+constexpr Kind kKinds[] = {K256, K128, K64, K64_PARTS};
+
+// Tiles of one size: outputs on a side, workgroups that a CU holds, us for a stage of 64 values of c (three such of products of both parts
+// with `parts`) with one of them there and with all, us besides for A and B and for X. Fitted to launches on 256 CUs: 8192^2's 512 and 1024 tiles of 256 x
+// 256 (423, 409 and 863 us) and 2048 of 128 x 128 (484), 9216 of 32 stages for four large blocks (695) and 216 of 33 (26.8), 3 to 198 tiles of 64 x 64 of 6 to
+// 72 stages (6.0 to 24.4; 5.8 to 18.9 by three groups).
+struct Cost {
+    int tile, per_cu;
+    bool parts;
+    float alone, full, square, update;
+};
+const Cost& cost_of(Kind k) {
+    static const Cost costs[] = {{256, 1, false, 1.42f, 1.42f, 26.0f, 34.0f},
+                                 {128, 2, false, 0.57f, 0.86f, 10.0f, 10.0f},
+                                 {64, 2, false, 0.26f, 0.34f, 4.7f, 5.2f},
+                                 {64, 1, true, 0.565f, 0.565f, 5.3f, 6.2f}};
+    return costs[k];
+}
 
 long long up(int n, int tile) { return (n + tile - 1) / tile; }
 
@@ -18,64 +37,123 @@ long long tiles_of(const Shape& s, Phase phase, int tile) {
     const long long t = up(side_of(s), tile);
     return phase == UPDATE ? up(s.R, tile) * up(s.C, tile) : t * (t + 1) / 2;
 }
-int stages_of(const Shape& s, Phase phase) { return (phase == GRAM ? std::max(s.R, s.C) : side_of(s)) / 64 * (s.three ? 3 : 1); }
+int stages_of(const Shape& s, Phase phase) { return (phase == GRAM ? std::max(s.R, s.C) : side_of(s)) / 64; }
 
-// Estimated us of a phase in tiles of one size: what the workgroups of all shapes take together, dealt out over the CUs, and, as shapes
-// end at different times, half of a workgroup's time more; whole rounds where there is one shape.
-float estimate(const Shapes& m, Phase phase, ozl::Tile tile, int cus) {
-    const ozl::Shape& t = ozl::shape_of(tile);
-    const long long slots = (long long)cus * t.per_cu;
-    float all = 0.0f, longest = 0.0f, rounds = 0.0f;
-    for (int k = 0; k < m.n; k++) {
-        const long long n = tiles_of(m.s[k], phase, t.q) * m.s[k].count;
-        const float us = t.fixed + (float)stages_of(m.s[k], phase) * (n > cus ? t.full : t.alone);
-        all += us * (float)n / (float)slots;
-        longest = std::max(longest, us);
-        const long long rest = n % slots;
-        rounds = (float)(n / slots) * us + (rest ? t.fixed + (float)stages_of(m.s[k], phase) * (rest > cus ? t.full : t.alone) : 0.0f);
+// The tiles of a sequence that a launch has: of shape k, n[k] from begin[k] on.
+struct Stretch {
+    long long begin[kShapes], n[kShapes];
+    long long all(const Shapes& m) const {
+        long long a = 0;
+        for (int k = 0; k < m.n; k++) a += n[k];
+        return a;
     }
-    return m.n == 1 ? rounds : std::max(longest, all + 0.5f * longest);
+};
+
+// Estimated us of a launch: whole rounds of workgroups over the CUs and the last, partly filled one where all tiles are alike; else what they
+// take together, dealt out over the CUs, and, as they end at different times, half of the longest one's more.
+float estimate(const Shapes& m, Phase phase, const Cost& c, int cus, const Stretch& t) {
+    const long long slots = (long long)cus * c.per_cu, tiles = t.all(m);
+    float all = 0.0f, longest = 0.0f, same = -1.0f;
+    bool alike = true;
+    for (int k = 0; k < m.n; k++) {
+        if (!t.n[k]) continue;
+        const float stages = (float)stages_of(m.s[k], phase) * (m.s[k].three && !c.parts ? 3.0f : 1.0f), fixed = phase == UPDATE ? c.update : c.square;
+        const float us = fixed + stages * (tiles > cus ? c.full : c.alone);
+        all += us * (float)t.n[k] / (float)slots;
+        longest = std::max(longest, us);
+        if (same >= 0.0f && same != us) alike = false;
+        same = us;
+    }
+    if (alike) return (float)((tiles + slots - 1) / slots) * longest;
+    return std::max(longest, all + 0.5f * longest);
 }
 
-// Places of a phase, or false where there are too many.
-bool places(const Shapes& m, Phase phase, int tile, Places* p) {
-    long long at = 0;
-    for (int k = 0; k < m.n; k++) {
-        const long long per = tiles_of(m.s[k], phase, tile);
-        if (per >> 22 || (at + per * m.s[k].count) >> 22) return false;
-        p->first[k] = (int)at;
-        p->per[k] = (int)per;
-        at += per * m.s[k].count;
+// A phase in tiles of one kind, and what a last, partly filled round of them would have in smaller ones by a launch of its own: 8192^2's A in
+// 512 tiles of 256 x 256 and the other 16 of 528 as 256 of 64 x 64 takes 455 us for 563. The launch costs 3 us.
+struct Choice {
+    Kind kind, rest_kind;
+    Stretch main, rest;
+};
+Choice choose(const Shapes& m, Phase phase, int cus, bool three) {
+    Choice best{};
+    float least = 0.0f;
+    for (const Kind kind : kKinds) {
+        const Cost& c = cost_of(kind);
+        if (c.parts && !three) continue;
+        Choice all{};
+        all.kind = kind;
+        for (int k = 0; k < m.n; k++) all.main.n[k] = tiles_of(m.s[k], phase, c.tile) * m.s[k].count;
+        float us = estimate(m, phase, c, cus, all.main);
+        if (least == 0.0f || us < least) least = us, best = all;
+        const long long slots = (long long)cus * c.per_cu, over = all.main.all(m) % slots;
+        if (!over || over == all.main.all(m)) continue;
+        Choice cut = all;
+        long long left = over;
+        for (int k = m.n - 1; k >= 0 && left; k--) {
+            const long long n = std::min(left, cut.main.n[k]);
+            cut.main.n[k] -= n;
+            cut.rest.n[k] = n;
+            cut.rest.begin[k] = cut.main.n[k];
+            left -= n;
+        }
+        us = estimate(m, phase, c, cus, cut.main) + 3.0f;
+        for (const Kind small : kKinds) {
+            const Cost& d = cost_of(small);
+            if (d.tile >= c.tile || (d.parts && !three)) continue;
+            Stretch r = cut.rest;
+            for (int k = 0; k < m.n; k++) r.n[k] *= (c.tile / d.tile) * (c.tile / d.tile);
+            const float more = estimate(m, phase, d, cus, r);
+            if (us + more < least) least = us + more, best = cut, best.rest_kind = small;
+        }
     }
-    p->first[m.n] = (int)at;
+    return best;
+}
+
+// A launch's places, or false where there are too many.
+bool places(const Shapes& m, Phase phase, int parent, int tile, const Stretch& t, Pass* p) {
+    long long at = 0;
+    p->parent = parent;
+    for (int k = 0; k < m.n; k++) {
+        const long long per = tiles_of(m.s[k], phase, parent);
+        p->places.first[k] = (int)at;
+        p->places.per[k] = (int)per;
+        p->begin[k] = (int)t.begin[k];
+        at += t.n[k] * (parent / tile) * (parent / tile);
+        if (per >> 22 || at >> 22 || (t.begin[k] + t.n[k]) >> 30) return false;
+    }
+    p->places.first[m.n] = (int)at;
     return true;
 }
 
 int iterate_alike(oz_dev* dev, const Shapes& m, const Ends& ends, const Factors& f, int steps) {
     if (!m.n) return OZ_OK;
-    Pass pass[3] = {};
-    int tile[3];
+    const bool three = m.s[0].three;
+    Pass pass[3][2] = {};
+    Choice choice[3];
     Shapes order[3];
     for (const Phase phase : {GRAM, SQUARE, UPDATE}) {
         order[phase] = m;
         std::stable_sort(order[phase].s, order[phase].s + m.n, [&](const Shape& a, const Shape& b) { return stages_of(a, phase) > stages_of(b, phase); });
-        float best = 0.0f;
-        for (const ozl::Tile t : {ozl::T256, ozl::T128, ozl::T64}) {
-            const float us = estimate(m, phase, t, dev->cus);
-            if (best == 0.0f || us < best) best = us, tile[phase] = ozl::shape_of(t).q;
-        }
-        pass[phase].f = f;
-        if (!places(order[phase], phase, tile[phase], &pass[phase].places)) return oz::fail(dev, OZ_ERR_ARG, "too many values in matrices");
+        Choice& c = choice[phase];
+        c = choose(order[phase], phase, dev->cus, three);
+        const int tile = cost_of(c.kind).tile;
+        if (!places(order[phase], phase, tile, tile, c.main, &pass[phase][0]) ||
+            !places(order[phase], phase, tile, cost_of(c.rest_kind).tile, c.rest, &pass[phase][1]))
+            return oz::fail(dev, OZ_ERR_ARG, "too many values in matrices");
     }
     for (int k = 0; k < steps; k++)
-        for (const Phase phase : {GRAM, SQUARE, UPDATE}) {
-            Pass& p = pass[phase];
-            p.from = k & 1;
-            p.last = k + 1 == steps;
-            if (m.s[0].three) launch_products<true>(dev->stream, phase, tile[phase], order[phase], ends, p);
-            else launch_products<false>(dev->stream, phase, tile[phase], order[phase], ends, p);
-            if (int st = oz::launch_check(dev, "newton_schulz_kernel")) return st;
-        }
+        for (const Phase phase : {GRAM, SQUARE, UPDATE})
+            for (int part = 0; part < 2; part++) {
+                Pass& p = pass[phase][part];
+                if (!p.places.first[m.n]) continue;
+                p.f = f;
+                p.from = k & 1;
+                p.last = k + 1 == steps;
+                const Kind kind = part ? choice[phase].rest_kind : choice[phase].kind;
+                if (three) launch_products<true>(dev->stream, phase, kind, order[phase], ends, p);
+                else launch_products<false>(dev->stream, phase, kind, order[phase], ends, p);
+                if (int st = oz::launch_check(dev, "newton_schulz_kernel")) return st;
+            }
     return OZ_OK;
 }
 

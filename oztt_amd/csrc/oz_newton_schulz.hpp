@@ -86,14 +86,17 @@ struct Factors {
 // The products of a step. X' goes to the ends in the last one.
 enum Phase { GRAM, SQUARE, UPDATE };
 struct Pass {
-    Places places;
+    Places places;       // per: tiles of `parent` x `parent` outputs
+    int parent;
+    int begin[kShapes];  // of a shape's tiles, the first that the launch has
     Factors f;
     int from;  // X's buffer, its values go to the other one
     int last;
 };
-// Tiles of `tile` x `tile` outputs (64, 128, 256) of a phase's products, for shapes that are alike in `three`.
+// Tiles of a phase's products, for shapes that are alike in `three` (K64_PARTS: those where it is set).
+enum Kind { K256, K128, K64, K64_PARTS };
 template <bool THREE>
-void launch_products(hipStream_t stream, Phase phase, int tile, const Shapes& m, const Ends& ends, const Pass& pass);
+void launch_products(hipStream_t stream, Phase phase, Kind kind, const Shapes& m, const Ends& ends, const Pass& pass);
 
 // The iteration on X0 in the shapes' x[0] (and l), the last step's results to the ends.
 int iterate(oz_dev* dev, const Shapes& m, const Ends& ends, const Factors& f, int steps);

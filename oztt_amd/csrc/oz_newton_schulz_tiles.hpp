@@ -44,26 +44,34 @@ __device__ __forceinline__ int xcd_run(int first, int i, int P) {
     return x * q + min(x, wrap) + min(max(x - s, 0), r - wrap) + (i - k) / N;
 }
 
-// Workgroup -> shape, matrix and tile. Shapes come one after the other (the long ones first, as they differ in length), within a shape
-// each XCD takes one contiguous run of the tiles, so that what it runs at a time shares rows and columns in its L2.
+// Workgroup -> shape, matrix and tile; false where there is nothing for it. Shapes come one after the other (the long ones first, as they
+// differ in length), within a shape each XCD takes one contiguous run of the tiles, so that what it runs at a time shares rows and columns
+// in its L2. A launch may have the first or the last tiles of a sequence of larger ones (Pass): `parent` / T by as many tiles in each.
 template <Phase PHASE, int T>
-__device__ __forceinline__ void tile_place(const Shapes& m, const Places& p, int w, int& shape, int& matrix, int& tq, int& tp) {
+__device__ __forceinline__ bool tile_place(const Shapes& m, const Pass& pass, int w, int& shape, int& matrix, int& tq, int& tp) {
+    const Places& p = pass.places;
     shape = __builtin_amdgcn_readfirstlane(shape_of(p, m.n, w));
     const Shape& s = m.s[shape];
-    const int i = xcd_run(p.first[shape], w - p.first[shape], p.per[shape] * s.count);
-    matrix = __builtin_amdgcn_readfirstlane(i / p.per[shape]);
-    const int u = __builtin_amdgcn_readfirstlane(i - matrix * p.per[shape]);
+    const int split = pass.parent / T, sub = split * split, P = pass.parent;
+    int j = xcd_run(p.first[shape], w - p.first[shape], p.first[shape + 1] - p.first[shape]);
+    const int inside = __builtin_amdgcn_readfirstlane(j % sub);
+    j = __builtin_amdgcn_readfirstlane(j / sub + pass.begin[shape]);
+    matrix = __builtin_amdgcn_readfirstlane(j / p.per[shape]);
+    const int u = j - matrix * p.per[shape];
     if constexpr (PHASE == UPDATE) {
         // groups of rows column by column: what an XCD runs at a time is 8 x 8 tiles of 128 (4 x 16: 782 for 750 us) or 4 x 8 of 256
-        constexpr int G = T == 256 ? 4 : 8;
-        const int rows = (s.R + T - 1) / T, cols = (s.C + T - 1) / T;
+        const int G = P == 256 ? 4 : 8;
+        const int rows = (s.R + P - 1) / P, cols = (s.C + P - 1) / P;
         const int group = u / (G * cols), first = G * group, g = min(rows - first, G), v = u - group * G * cols;
         tq = first + v % g, tp = v / g;
     } else {
-        triangle(u, (side_of(s) + T - 1) / T, tq, tp);
+        triangle(u, (side_of(s) + P - 1) / P, tq, tp);
     }
-    tq = __builtin_amdgcn_readfirstlane(tq);
-    tp = __builtin_amdgcn_readfirstlane(tp);
+    tq = __builtin_amdgcn_readfirstlane(tq * split + inside / split);
+    tp = __builtin_amdgcn_readfirstlane(tp * split + inside % split);
+    if (split == 1) return true;
+    if (PHASE != UPDATE) return tq <= tp && T * tp < side_of(s);
+    return T * tq < s.R && T * tp < s.C;
 }
 
 // ---- from sums to values ------------------------------------------------------------------------------
@@ -101,7 +109,7 @@ struct Bands {
     static constexpr int BATCH = NT < 8 ? NT : 8, ALL = TI / RI * NT / BATCH;  // of a turn's pieces; batches of a tile
     static_assert(NT % BATCH == 0, "whole batches");
     // With one batch a tile's pieces are asked for before its products and wait in registers: four large blocks' update in tiles of 128 x
-    // 128 WITHOUT 790 us, with them there WITH. More do not fit: two in turn, a batch ahead.
+    // 128 785 us, with them there 769. More do not fit: two in turn, a batch ahead.
     static constexpr bool AHEAD = ALL == 1;
     static constexpr int BUFFERS = AHEAD ? 1 : 2;
 };
@@ -292,48 +300,59 @@ struct Finish {
 // ---- kernels ------------------------------------------------------------------------------------------
 
 struct Tile64 {
-    static constexpr int T = 64, TI = 2, TJ = 2, WP = 2, THREADS = 256, PER_SIMD = 2;
+    static constexpr int T = 64, TI = 2, TJ = 2, WP = 2, THREADS = 256, PER_SIMD = 2, GROUPS = 1;
     template <bool QM, bool PM, bool PARTS>
     using Loop = ozl::TileLoop<Half<OZ_F16>, QM, PM, 2, 2, 2, 2, 4, PARTS>;
 };
+// Products of both parts where there are few tiles: three groups of waves, one for h h, h l and l h each, joined in LDS.
+struct Tile64Parts {
+    static constexpr int T = 64, TI = 2, TJ = 2, WP = 2, THREADS = 768, PER_SIMD = 3, GROUPS = 3;
+    template <bool QM, bool PM, bool>
+    using Loop = ozl::TileLoop<Half<OZ_F16>, QM, PM, 2, 2, 2, 2, 3>;
+};
 struct Tile128 {
-    static constexpr int T = 128, TI = 4, TJ = 4, WP = 2, THREADS = 256, PER_SIMD = 2;
+    static constexpr int T = 128, TI = 4, TJ = 4, WP = 2, THREADS = 256, PER_SIMD = 2, GROUPS = 1;
     template <bool QM, bool PM, bool PARTS>
     using Loop = ozl::BigLoop<Half<OZ_F16>, QM, PM, PARTS, 4>;
 };
 struct Tile256 {
-    static constexpr int T = 256, TI = 8, TJ = 8, WP = 2, THREADS = 256, PER_SIMD = 1;
+    static constexpr int T = 256, TI = 8, TJ = 8, WP = 2, THREADS = 256, PER_SIMD = 1, GROUPS = 1;
     template <bool QM, bool PM, bool PARTS>
     using Loop = ozl::BigLoop<Half<OZ_F16>, QM, PM, PARTS>;
 };
 
 template <Phase PHASE, class TILE, bool THREE>
 __global__ void __launch_bounds__(TILE::THREADS, TILE::PER_SIMD) newton_schulz_kernel(const Shapes m, const Ends ends, const Pass pass) {
-    constexpr int T = TILE::T;
-    typedef typename TILE::template Loop<false, false, THREE> Any;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[Any::LDS];
+    constexpr int T = TILE::T, GROUPS = TILE::GROUPS, WAVES = TILE::THREADS / 64 / GROUPS;
+    constexpr bool PARTS = THREE && GROUPS == 1;
+    typedef typename TILE::template Loop<false, false, PARTS> Any;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[GROUPS * Any::LDS];
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) % WAVES), group = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) / WAVES);
     int shape, i, tq, tp;
-    tile_place<PHASE, T>(m, pass.places, blockIdx.x, shape, i, tq, tp);
+    if (!tile_place<PHASE, T>(m, pass, blockIdx.x, shape, i, tq, tp)) return;
     const Shape s = m.s[shape];
     const int side = side_of(s), q0 = T * tq, p0 = T * tp;
-    const long long nx = 2ll * s.R * s.C, nn = 2ll * side * side;  // bytes of a plane
+    const long long nx = (long long)s.R * s.C, nn = (long long)side * side;  // values of a plane
     f32x4 acc[TILE::TI][TILE::TJ];
     // sum over c < C of Q(q, c) P(p, c)
     auto run = [&](auto QM, auto PM, const _Float16* Q, int nq, int ldq, long long plane_q, const _Float16* P, int np, int ldp, long long plane_p, int C) {
-        typedef typename TILE::template Loop<decltype(QM)::value, decltype(PM)::value, THREE> Loop;
+        typedef typename TILE::template Loop<decltype(QM)::value, decltype(PM)::value, PARTS> Loop;
         const int stages = C / ozl::BC;
         typename Loop::OQ oq;
         typename Loop::OP op;
+        if constexpr (GROUPS > 1) {
+            Q += group == 2 ? plane_q : 0;
+            P += group == 1 ? plane_p : 0;
+        }
         oq.init(Q, ldq, nq, C, q0, 0, stages, lane, wave);
         op.init(P, ldp, np, C, p0, 0, stages, lane, wave);
-        if constexpr (THREE) {  // h, h, l and h, l, h
+        if constexpr (PARTS) {  // h, h, l and h, l, h
             const long long back_q = (long long)stages * oq.step, back_p = (long long)stages * op.step;
-            oq.parts(stages, -back_q, plane_q - back_q);
-            op.parts(stages, plane_p - back_p, -plane_p - back_p);
+            oq.parts(stages, -back_q, 2 * plane_q - back_q);
+            op.parts(stages, 2 * plane_p - back_p, -2 * plane_p - back_p);
         }
-        Loop::template run<uint16_t>(lds, oq, op, THREE ? 3 * stages : stages, 0, lane, wave, acc);
+        Loop::template run<uint16_t>(lds + group * Any::LDS, oq, op, PARTS ? 3 * stages : stages, 0, lane, wave, acc);
     };
     constexpr std::false_type no{};
     constexpr std::true_type yes{};
@@ -341,7 +360,7 @@ __global__ void __launch_bounds__(TILE::THREADS, TILE::PER_SIMD) newton_schulz_k
     typedef Finish<PHASE, THREE, TILE::TI, TILE::TJ, Any::ROOM> Put;
     const int q1 = q0 + 16 * TILE::TI * (wave / TILE::WP), p1 = p0 + 16 * TILE::TJ * (wave % TILE::WP);
     Put put(s, pass, i, lane, q1, p1);
-    put.ahead();
+    if (group == 0) put.ahead();
     if constexpr (PHASE == GRAM) {
         if (is_tall(s)) run(yes, yes, x, s.C, s.C, nx, x, s.C, s.C, nx, s.R);
         else run(no, no, x, s.R, s.C, nx, x, s.R, s.C, nx, s.C);
@@ -353,13 +372,28 @@ __global__ void __launch_bounds__(TILE::THREADS, TILE::PER_SIMD) newton_schulz_k
         if (is_tall(s)) run(no, no, x, s.R, s.C, nx, b, side, side, nn, side);
         else run(no, yes, b, side, side, nn, x, s.C, s.C, nx, side);
     }
+    if constexpr (GROUPS > 1) {
+        constexpr int PIECES = TILE::TI * TILE::TJ;
+        f32x4* sums = reinterpret_cast<f32x4*>(lds + Any::LDS) + 64 * PIECES * wave + lane;  // behind the first group's
+        constexpr int NEXT = 64 * PIECES * WAVES;
+        if (group > 0)
+#pragma unroll
+            for (int k = 0; k < PIECES; k++) sums[NEXT * (group - 1) + 64 * k] = acc[k / TILE::TJ][k % TILE::TJ];
+        __syncthreads();
+        if (group > 0) return;
+#pragma unroll
+        for (int k = 0; k < PIECES; k++) {
+            acc[k / TILE::TJ][k % TILE::TJ] += sums[64 * k];
+            acc[k / TILE::TJ][k % TILE::TJ] += sums[NEXT + 64 * k];
+        }
+    }
     float* room = reinterpret_cast<float*>(lds) + wave * Any::ROOM;
     if constexpr (Put::S::AHEAD) put.put(ends, tq != tp, acc, room);
     else Put(s, pass, i, lane, q1, p1).put(ends, tq != tp, acc, room);
 }
 
 template <bool THREE>
-void launch_products(hipStream_t stream, Phase phase, int tile, const Shapes& m, const Ends& ends, const Pass& pass) {
+void launch_products(hipStream_t stream, Phase phase, Kind kind, const Shapes& m, const Ends& ends, const Pass& pass) {
     const dim3 grid((unsigned)pass.places.first[m.n]);
     auto with = [&](auto TILE) {
         typedef decltype(TILE) Tile;
@@ -368,9 +402,14 @@ void launch_products(hipStream_t stream, Phase phase, int tile, const Shapes& m,
         else if (phase == SQUARE) hipLaunchKernelGGL((newton_schulz_kernel<SQUARE, Tile, THREE>), grid, block, 0, stream, m, ends, pass);
         else hipLaunchKernelGGL((newton_schulz_kernel<UPDATE, Tile, THREE>), grid, block, 0, stream, m, ends, pass);
     };
-    if (tile == 64) with(Tile64{});
-    else if (tile == 128) with(Tile128{});
-    else with(Tile256{});
+    switch (kind) {
+        case K256: with(Tile256{}); break;
+        case K128: with(Tile128{}); break;
+        case K64: with(Tile64{}); break;
+        case K64_PARTS:
+            if constexpr (THREE) with(Tile64Parts{});
+            break;
+    }
 }
 
 }  // namespace ozn
