@@ -42,10 +42,8 @@ __device__ __forceinline__ void lds_copy(v4i rs, void* lbase, unsigned voff) {
 }
 
 // One operand of a tile of ROWS rows: its copies (wave `wave` of W brings blocks wave, wave + W, ...) and fragments. Sizes count
-// 16-bit values; 8-bit integers are taken two at a time. PARTS: the operand is three stretches of `stages` / 3 stages each, the
-// second and third ones jump[0] and jump[1] bytes behind the end of the one before (whole stages, so that their ranges are the
-// first one's).
-template <bool MAJOR, int ROWS, int W, bool PARTS = false>
+// 16-bit values; 8-bit integers are taken two at a time.
+template <bool MAJOR, int ROWS, int W>
 struct Operand {
     static constexpr int BLOCKS = ROWS / 8;   // 1 KB blocks of a stage
     static constexpr int N = BLOCKS / W;      // copies of a wave
@@ -58,9 +56,6 @@ struct Operand {
     unsigned step;   // bytes of a stage's advance
     unsigned off[N]; // of this lane's copies
     int steps;       // stages left to load
-    int part;        // PARTS: stages of a stretch
-    unsigned whole;  // and its first range
-    long long jump[2];
 
     // a row's swizzle in 32-byte pieces: rows 8 g + j and 8 g + 4 + j (j < 4) of g and g + 1 differ
     __device__ static int piece_swizzle(int row) { return ((row & 3) | ((row >> 3) & 1) << 2) & (PIECES - 1); }
@@ -102,32 +97,19 @@ struct Operand {
         step = __builtin_amdgcn_readfirstlane(step);
         limit();
     }
-    __device__ __forceinline__ void parts(int stages, long long first, long long second) {
-        steps = 3 * stages;
-        part = stages;
-        whole = range;
-        jump[0] = first, jump[1] = second;
-        limit();
-    }
     // A few scalar instructions a stage: whatever more there was showed (85 cycles a stage, 2% of 8192^3, 15% of small
     // products, for 64-bit ranges and a mask of the last chunks).
     __device__ __forceinline__ void limit() {
-        if constexpr (MAJOR && !PARTS) rs[2] = steps > 1 ? range : steps == 1 ? last : 0u;
+        if constexpr (MAJOR) rs[2] = steps > 1 ? range : steps == 1 ? last : 0u;
         else rs[2] = steps > 0 ? range : 0u;
     }
     __device__ __forceinline__ void copy(uint8_t* stage, int j, int wave) const { lds_copy(rs, stage + 1024 * (W * j + wave), off[j]); }
     __device__ __forceinline__ void next() {
         steps--;
-        unsigned long long base = ((unsigned long long)(unsigned)rs[1] << 32 | (unsigned)rs[0]) + step;
-        if constexpr (!MAJOR) range -= step;
-        if constexpr (PARTS) {
-            if (steps == 2 * part || steps == part) {
-                base += steps == part ? jump[1] : jump[0];
-                range = whole;
-            }
-        }
+        const unsigned long long base = ((unsigned long long)(unsigned)rs[1] << 32 | (unsigned)rs[0]) + step;
         rs[0] = (int)base;
         rs[1] = (int)(base >> 32);
+        if constexpr (!MAJOR) range -= step;
         limit();
     }
 
@@ -339,13 +321,13 @@ __device__ __forceinline__ int ragged_tail(const Product& a, int split) {
 // The sums of a tile by WQ x WP waves of 16 TI x 16 TJ outputs each, `nst` stages of the operands oq and op through a ring of NSTG
 // stages in LDS, one barrier a stage. The fragments of the next step are read while this one's multiply. `tail`: values of type
 // TAIL in the last stage, where they do not fill it. When it returns, LDS is free.
-template <class M, bool QM, bool PM, int TI, int TJ, int WQ, int WP, int NSTG, bool PARTS = false>
+template <class M, bool QM, bool PM, int TI, int TJ, int WQ, int WP, int NSTG>
 struct TileLoop {
     typedef typename M::x8 T8;
     typedef typename M::sums Sums;
     static constexpr int W = WQ * WP, QR = 16 * TI * WQ, PR = 16 * TJ * WP;
-    typedef Operand<QM, QR, W, PARTS> OQ;
-    typedef Operand<PM, PR, W, PARTS> OP;
+    typedef Operand<QM, QR, W> OQ;
+    typedef Operand<PM, PR, W> OP;
     static constexpr int STG_Q = 2 * BC * QR, STG = STG_Q + 2 * BC * PR, LD = OQ::N + OP::N, LDS = NSTG * STG, ROOM = LDS / W / 4;
 
     template <class TAIL>
@@ -469,12 +451,12 @@ __device__ __forceinline__ void settle_sums() { asm volatile("s_nop 15\n\ts_nop 
 // where Q's stage k is free, and have one and a half or two and a half steps to land. (With two whole stages all copies go out
 // in the second step and have one and a half: 852 against 763 us at 8192^3.)
 // B: 16 B outputs on a side of a wave, 8 or (128 x 128 outputs, two workgroups a CU) 4.
-template <class M, bool QM, bool PM, bool PARTS = false, int B = 8>
+template <class M, bool QM, bool PM, int B = 8>
 struct BigLoop {
     typedef typename M::x8 T8;
     typedef typename M::sums Sums;
-    typedef Operand<QM, 32 * B, 4, PARTS> OQ;
-    typedef Operand<PM, 32 * B, 4, PARTS> OP;
+    typedef Operand<QM, 32 * B, 4> OQ;
+    typedef Operand<PM, 32 * B, 4> OP;
     static constexpr int UNIT = 2 * BC * 32 * B, RING = 5 * UNIT, LD = OQ::N, LDS = RING, ROOM = RING / 4 / 4;
     static_assert(OQ::N == OP::N, "copies of a unit");
 

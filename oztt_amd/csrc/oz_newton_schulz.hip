@@ -4,31 +4,23 @@
 
 #include <algorithm>
 
-extern template void ozn::launch_products<true>(hipStream_t, Phase, Kind, const Shapes&, const Ends&, const Pass&);
-template void ozn::launch_products<false>(hipStream_t, Phase, Kind, const Shapes&, const Ends&, const Pass&);
+extern template void ozn::launch_products<true>(hipStream_t, Phase, int, const Shapes&, const Ends&, const Pass&);
+template void ozn::launch_products<false>(hipStream_t, Phase, int, const Shapes&, const Ends&, const Pass&);
 
 namespace {
 
 using namespace ozn;
 
-constexpr Kind kKinds[] = {K256, K128, K64, K64_PARTS};
-
-// Tiles of one size: outputs on a side, workgroups that a CU holds, us for a stage of 64 values of c (three such of products of both parts
-// with `parts`) with one of them there and with all, us besides for A and B and for X. Fitted to launches on 256 CUs: 8192^2's 512 and 1024 tiles of 256 x
-// 256 (423, 409 and 863 us) and 2048 of 128 x 128 (484), 9216 of 32 stages for four large blocks (695) and 216 of 33 (26.8), 3 to 198 tiles of 64 x 64 of 6 to
-// 72 stages (6.0 to 24.4; 5.8 to 18.9 by three groups).
+// Tiles of one size: outputs on a side, workgroups that a CU holds, us for a stage of 64 values of c with one of them there and with all,
+// us besides for A and B and for X. Fitted to launches on 256 CUs: 8192^2's 512 and 1024 tiles of 256 x 256 (423, 409 and 863 us) and 2048 of
+// 128 x 128 (484), 9216 of 32 stages for four large blocks (695), 3 to 198 tiles of 64 x 64 of 6 to 72 stages (6.0 to 24.4); of both
+// parts 3 to 198 of 64 x 64 of 2 to 24 stages (5.2 to 16.6) and 540 of 8 and 24 (27.6), 216 of 128 x 128 of 11 (22.2) and 512 of 8 (42).
 struct Cost {
     int tile, per_cu;
-    bool parts;
     float alone, full, square, update;
 };
-const Cost& cost_of(Kind k) {
-    static const Cost costs[] = {{256, 1, false, 1.42f, 1.42f, 26.0f, 34.0f},
-                                 {128, 2, false, 0.57f, 0.86f, 10.0f, 10.0f},
-                                 {64, 2, false, 0.26f, 0.34f, 4.7f, 5.2f},
-                                 {64, 1, true, 0.565f, 0.565f, 5.3f, 6.2f}};
-    return costs[k];
-}
+constexpr Cost kOne[] = {{256, 1, 1.42f, 1.42f, 26.0f, 34.0f}, {128, 2, 0.57f, 0.86f, 10.0f, 10.0f}, {64, 2, 0.26f, 0.34f, 4.7f, 5.2f}};
+constexpr Cost kBoth[] = {{128, 1, 1.0f, 1.0f, 13.5f, 12.0f}, {64, 2, 0.455f, 0.8f, 4.8f, 5.2f}};
 
 long long up(int n, int tile) { return (n + tile - 1) / tile; }
 
@@ -57,8 +49,7 @@ float estimate(const Shapes& m, Phase phase, const Cost& c, int cus, const Stret
     bool alike = true;
     for (int k = 0; k < m.n; k++) {
         if (!t.n[k]) continue;
-        const float stages = (float)stages_of(m.s[k], phase) * (m.s[k].three && !c.parts ? 3.0f : 1.0f), fixed = phase == UPDATE ? c.update : c.square;
-        const float us = fixed + stages * (tiles > cus ? c.full : c.alone);
+        const float us = (phase == UPDATE ? c.update : c.square) + (float)stages_of(m.s[k], phase) * (tiles > cus ? c.full : c.alone);
         all += us * (float)t.n[k] / (float)slots;
         longest = std::max(longest, us);
         if (same >= 0.0f && same != us) alike = false;
@@ -68,20 +59,19 @@ float estimate(const Shapes& m, Phase phase, const Cost& c, int cus, const Stret
     return std::max(longest, all + 0.5f * longest);
 }
 
-// A phase in tiles of one kind, and what a last, partly filled round of them would have in smaller ones by a launch of its own: 8192^2's A in
+// A phase in tiles of one size, and what a last, partly filled round of them would have in smaller ones by a launch of its own: 8192^2's A in
 // 512 tiles of 256 x 256 and the other 16 of 528 as 256 of 64 x 64 takes 455 us for 563. The launch costs 3 us.
 struct Choice {
-    Kind kind, rest_kind;
+    int tile, rest_tile;
     Stretch main, rest;
 };
-Choice choose(const Shapes& m, Phase phase, int cus, bool three) {
+template <int N>
+Choice choose(const Shapes& m, Phase phase, int cus, const Cost (&costs)[N]) {
     Choice best{};
     float least = 0.0f;
-    for (const Kind kind : kKinds) {
-        const Cost& c = cost_of(kind);
-        if (c.parts && !three) continue;
+    for (const Cost& c : costs) {
         Choice all{};
-        all.kind = kind;
+        all.tile = all.rest_tile = c.tile;
         for (int k = 0; k < m.n; k++) all.main.n[k] = tiles_of(m.s[k], phase, c.tile) * m.s[k].count;
         float us = estimate(m, phase, c, cus, all.main);
         if (least == 0.0f || us < least) least = us, best = all;
@@ -97,13 +87,12 @@ Choice choose(const Shapes& m, Phase phase, int cus, bool three) {
             left -= n;
         }
         us = estimate(m, phase, c, cus, cut.main) + 3.0f;
-        for (const Kind small : kKinds) {
-            const Cost& d = cost_of(small);
-            if (d.tile >= c.tile || (d.parts && !three)) continue;
+        for (const Cost& d : costs) {
+            if (d.tile >= c.tile) continue;
             Stretch r = cut.rest;
             for (int k = 0; k < m.n; k++) r.n[k] *= (c.tile / d.tile) * (c.tile / d.tile);
             const float more = estimate(m, phase, d, cus, r);
-            if (us + more < least) least = us + more, best = cut, best.rest_kind = small;
+            if (us + more < least) least = us + more, best = cut, best.rest_tile = d.tile;
         }
     }
     return best;
@@ -135,10 +124,8 @@ int iterate_alike(oz_dev* dev, const Shapes& m, const Ends& ends, const Factors&
         order[phase] = m;
         std::stable_sort(order[phase].s, order[phase].s + m.n, [&](const Shape& a, const Shape& b) { return stages_of(a, phase) > stages_of(b, phase); });
         Choice& c = choice[phase];
-        c = choose(order[phase], phase, dev->cus, three);
-        const int tile = cost_of(c.kind).tile;
-        if (!places(order[phase], phase, tile, tile, c.main, &pass[phase][0]) ||
-            !places(order[phase], phase, tile, cost_of(c.rest_kind).tile, c.rest, &pass[phase][1]))
+        c = three ? choose(order[phase], phase, dev->cus, kBoth) : choose(order[phase], phase, dev->cus, kOne);
+        if (!places(order[phase], phase, c.tile, c.tile, c.main, &pass[phase][0]) || !places(order[phase], phase, c.tile, c.rest_tile, c.rest, &pass[phase][1]))
             return oz::fail(dev, OZ_ERR_ARG, "too many values in matrices");
     }
     for (int k = 0; k < steps; k++)
@@ -149,9 +136,9 @@ int iterate_alike(oz_dev* dev, const Shapes& m, const Ends& ends, const Factors&
                 p.f = f;
                 p.from = k & 1;
                 p.last = k + 1 == steps;
-                const Kind kind = part ? choice[phase].rest_kind : choice[phase].kind;
-                if (three) launch_products<true>(dev->stream, phase, kind, order[phase], ends, p);
-                else launch_products<false>(dev->stream, phase, kind, order[phase], ends, p);
+                const int tile = part ? choice[phase].rest_tile : choice[phase].tile;
+                if (three) launch_products<true>(dev->stream, phase, tile, order[phase], ends, p);
+                else launch_products<false>(dev->stream, phase, tile, order[phase], ends, p);
                 if (int st = oz::launch_check(dev, "newton_schulz_kernel")) return st;
             }
     return OZ_OK;

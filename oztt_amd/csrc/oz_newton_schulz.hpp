@@ -93,10 +93,9 @@ struct Pass {
     int from;  // X's buffer, its values go to the other one
     int last;
 };
-// Tiles of a phase's products, for shapes that are alike in `three` (K64_PARTS: those where it is set).
-enum Kind { K256, K128, K64, K64_PARTS };
+// Tiles of `tile` x `tile` outputs of a phase's products, 64, 128 or (of the first parts) 256, for shapes that are alike in `three`.
 template <bool THREE>
-void launch_products(hipStream_t stream, Phase phase, Kind kind, const Shapes& m, const Ends& ends, const Pass& pass);
+void launch_products(hipStream_t stream, Phase phase, int tile, const Shapes& m, const Ends& ends, const Pass& pass);
 
 // The iteration on X0 in the shapes' x[0] (and l), the last step's results to the ends.
 int iterate(oz_dev* dev, const Shapes& m, const Ends& ends, const Factors& f, int steps);

@@ -4,7 +4,6 @@
 // A and A^2 are symmetric: only tiles on and above the diagonal are computed and written twice, as they are and transposed. X's
 // product with the symmetric B takes X as it lies, B X with X read transposed out of LDS, X B for a tall matrix. All sides in the
 // workspace are multiples of 64 with zeros behind the matrices, so no stage is ragged and every access of 8 values is whole.
-// Products of both parts are one loop over three stretches of c, h h, h l and l h.
 #pragma once
 #include "oz_linear_tiles.hpp"
 #include "oz_newton_schulz.hpp"
@@ -299,68 +298,166 @@ struct Finish {
 
 // ---- kernels ------------------------------------------------------------------------------------------
 
-struct Tile64 {
-    static constexpr int T = 64, TI = 2, TJ = 2, WP = 2, THREADS = 256, PER_SIMD = 2, GROUPS = 1;
-    template <bool QM, bool PM, bool PARTS>
-    using Loop = ozl::TileLoop<Half<OZ_F16>, QM, PM, 2, 2, 2, 2, 4, PARTS>;
+// Products of both parts: h h + h l + l h in one loop, which brings each part of an operand once for the two products that read it
+// (one after the other they would be brought, and read out of LDS, half as often again: three matrices of
+// 700 x 1500 in 306 us for 265). As ozl::BigLoop, with pairs of units: 4 waves
+// of 16 B x 16 B outputs, a ring of five pairs, the copies of stage k + 2 of Q in stage k's first step, those of P in its second.
+template <bool QM, bool PM, int B>
+struct PairLoop {
+    typedef Half<OZ_F16> M;
+    typedef typename M::x8 T8;
+    typedef Operand<QM, 32 * B, 4> OQ;
+    typedef Operand<PM, 32 * B, 4> OP;
+    static constexpr int UNIT = 2 * ozl::BC * 32 * B, PAIR = 2 * UNIT, RING = 5 * PAIR, LD = OQ::N, LDS = RING, ROOM = RING / 4 / 4;
+    static_assert(OQ::N == OP::N, "copies of a unit");
+    struct Parts {
+        T8 h[B], l[B];
+    };
+
+    __device__ static __forceinline__ void run(uint8_t* lds, OQ (&oq)[2], OP (&op)[2], int nst, int lane, int wave, f32x4 (&out)[B][B]) {
+        const int wq = B * (wave >> 1), wp = B * (wave & 1);
+        const int lq = OQ::lane_offset(lane), lp = OP::lane_offset(lane);
+        f32x4 acc[B][B];
+#pragma unroll
+        for (int i = 0; i < B; i++)
+#pragma unroll
+            for (int j = 0; j < B; j++) acc[i][j] = f32x4{0, 0, 0, 0};
+        auto copy_q = [&](int to, int j) { oq[j / LD].copy(lds + to + UNIT * (j / LD), j % LD, wave); };
+        auto copy_p = [&](int to, int j) { op[j / LD].copy(lds + to + UNIT * (j / LD), j % LD, wave); };
+        auto landed = [&](auto LEFT) {
+            ozl::wait_vmcnt_lgkm0<decltype(LEFT)::value>();
+            ozl::stage_barrier();
+        };
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+#pragma unroll
+            for (int j = 0; j < 2 * LD; j++) copy_q(2 * s * PAIR, j);
+#pragma unroll
+            for (int j = 0; j < 2 * LD; j++) copy_p((2 * s + 1) * PAIR, j);
+            oq[0].next(), oq[1].next(), op[0].next(), op[1].next();
+        }
+        // fragment t of a step, in the order its instructions want them
+        auto read = [&](Parts& q, Parts& p, int t, int h, int uq, int up) {
+            if (t == 0) q.h[0] = OQ::template fragment<T8>(lds + uq, h, wq, lq);
+            else if (t <= B) p.h[t - 1] = OP::template fragment<T8>(lds + up, h, wp + t - 1, lp);
+            else if (t < 2 * B) q.h[t - B] = OQ::template fragment<T8>(lds + uq, h, wq + t - B, lq);
+            else if (t < 3 * B) p.l[t - 2 * B] = OP::template fragment<T8>(lds + up + UNIT, h, wp + t - 2 * B, lp);
+            else q.l[t - 3 * B] = OQ::template fragment<T8>(lds + uq + UNIT, h, wq + t - 3 * B, lq);
+        };
+        Parts fq, fp, gq, gp;
+        landed(std::integral_constant<int, 4 * LD>{});
+#pragma unroll
+        for (int t = 0; t < 4 * B; t++) read(fq, fp, t, 0, 0, PAIR);
+        // One step: 3 B B matrix instructions on (xq, xp), the 4 B fragments (yq, yp) of step H of the pairs at uq and up, the copies of a pair
+        // of Q (in a stage's first step) or P to `to`.
+        auto step = [&](auto H, Parts& xq, Parts& xp, Parts& yq, Parts& yp, int uq, int up, int to) {
+            constexpr int h = decltype(H)::value, R = B == 4 ? 3 : 1, C = B == 4 ? 3 : 2;
+#pragma unroll
+            for (int n = 0; n < 3 * B * B; n++) {
+                const int part = n / (B * B), i = n / B % B, j = n % B;
+                const T8 p = part == 1 ? xp.l[j] : xp.h[j], q = part == 2 ? xq.l[i] : xq.h[i];
+                // (written as in the large loop only where a sum comes up again 16 instructions later)
+                if constexpr (B == 4) ozl::mfma_acc<M>(acc[i][j], p, q);
+                else acc[i][j] = M::mfma(p, q, acc[i][j]);
+                if (n % R == 0 && n / R < 4 * B) read(yq, yp, n / R, h, uq, up);
+                if (n % C == C - 1 && n / C < 2 * LD) {
+                    if constexpr (h == 1) copy_q(to, n / C);
+                    else copy_p(to, n / C);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        int at = 0;
+        auto wrap = [](int b) { return b >= RING ? b - RING : b; };
+        for (int k = 0; k < nst; k++) {
+            const int u1 = wrap(at + PAIR), u2 = wrap(at + 2 * PAIR), u3 = wrap(at + 3 * PAIR), u4 = wrap(at + 4 * PAIR);
+            step(std::integral_constant<int, 1>{}, fq, fp, gq, gp, at, u1, u4);
+            oq[0].next(), oq[1].next();
+            landed(std::integral_constant<int, 2 * LD>{});
+            step(std::integral_constant<int, 0>{}, gq, gp, fq, fp, u2, u3, at);
+            op[0].next(), op[1].next();
+            at = u2;
+        }
+        ozl::settle_sums();
+        ozl::wait_vmcnt<0>();
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < B; i++)
+#pragma unroll
+            for (int j = 0; j < B; j++) out[i][j] = acc[i][j];
+    }
 };
-// Products of both parts where there are few tiles: three groups of waves, one for h h, h l and l h each, joined in LDS.
-struct Tile64Parts {
-    static constexpr int T = 64, TI = 2, TJ = 2, WP = 2, THREADS = 768, PER_SIMD = 3, GROUPS = 3;
-    template <bool QM, bool PM, bool>
-    using Loop = ozl::TileLoop<Half<OZ_F16>, QM, PM, 2, 2, 2, 2, 3>;
+
+// Tiles of products of the first parts (ONE) and of both. BLOCKS: bands of 16 rows and columns of a wave.
+struct Tile64 {
+    static constexpr int T = 64, BLOCKS = 2, PER_SIMD = 2;
+    template <bool QM, bool PM>
+    using One = ozl::TileLoop<Half<OZ_F16>, QM, PM, 2, 2, 2, 2, 4>;
+    template <bool QM, bool PM>
+    using Both = PairLoop<QM, PM, 2>;
 };
 struct Tile128 {
-    static constexpr int T = 128, TI = 4, TJ = 4, WP = 2, THREADS = 256, PER_SIMD = 2, GROUPS = 1;
-    template <bool QM, bool PM, bool PARTS>
-    using Loop = ozl::BigLoop<Half<OZ_F16>, QM, PM, PARTS, 4>;
+    static constexpr int T = 128, BLOCKS = 4, PER_SIMD = 2;
+    template <bool QM, bool PM>
+    using One = ozl::BigLoop<Half<OZ_F16>, QM, PM, 4>;
+    template <bool QM, bool PM>
+    using Both = PairLoop<QM, PM, 4>;
 };
 struct Tile256 {
-    static constexpr int T = 256, TI = 8, TJ = 8, WP = 2, THREADS = 256, PER_SIMD = 1, GROUPS = 1;
-    template <bool QM, bool PM, bool PARTS>
-    using Loop = ozl::BigLoop<Half<OZ_F16>, QM, PM, PARTS>;
+    static constexpr int T = 256, BLOCKS = 8, PER_SIMD = 1;
+    template <bool QM, bool PM>
+    using One = ozl::BigLoop<Half<OZ_F16>, QM, PM>;
+};
+template <class TILE, bool THREE, bool QM, bool PM>
+struct LoopOf {
+    typedef typename TILE::template One<QM, PM> type;
+};
+template <class TILE, bool QM, bool PM>
+struct LoopOf<TILE, true, QM, PM> {
+    typedef typename TILE::template Both<QM, PM> type;
 };
 
 template <Phase PHASE, class TILE, bool THREE>
-__global__ void __launch_bounds__(TILE::THREADS, TILE::PER_SIMD) newton_schulz_kernel(const Shapes m, const Ends ends, const Pass pass) {
-    constexpr int T = TILE::T, GROUPS = TILE::GROUPS, WAVES = TILE::THREADS / 64 / GROUPS;
-    constexpr bool PARTS = THREE && GROUPS == 1;
-    typedef typename TILE::template Loop<false, false, PARTS> Any;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[GROUPS * Any::LDS];
+__global__ void __launch_bounds__(256, THREE && TILE::T == 128 ? 1 : TILE::PER_SIMD) newton_schulz_kernel(const Shapes m, const Ends ends, const Pass pass) {
+    constexpr int T = TILE::T, B = TILE::BLOCKS;
+    typedef typename LoopOf<TILE, THREE, false, false>::type Any;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[Any::LDS];
     const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) % WAVES), group = __builtin_amdgcn_readfirstlane((threadIdx.x >> 6) / WAVES);
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int shape, i, tq, tp;
     if (!tile_place<PHASE, T>(m, pass, blockIdx.x, shape, i, tq, tp)) return;
     const Shape s = m.s[shape];
     const int side = side_of(s), q0 = T * tq, p0 = T * tp;
     const long long nx = (long long)s.R * s.C, nn = (long long)side * side;  // values of a plane
-    f32x4 acc[TILE::TI][TILE::TJ];
+    f32x4 acc[B][B];
     // sum over c < C of Q(q, c) P(p, c)
     auto run = [&](auto QM, auto PM, const _Float16* Q, int nq, int ldq, long long plane_q, const _Float16* P, int np, int ldp, long long plane_p, int C) {
-        typedef typename TILE::template Loop<decltype(QM)::value, decltype(PM)::value, PARTS> Loop;
+        typedef typename LoopOf<TILE, THREE, decltype(QM)::value, decltype(PM)::value>::type Loop;
         const int stages = C / ozl::BC;
-        typename Loop::OQ oq;
-        typename Loop::OP op;
-        if constexpr (GROUPS > 1) {
-            Q += group == 2 ? plane_q : 0;
-            P += group == 1 ? plane_p : 0;
+        if constexpr (THREE) {
+            typename Loop::OQ oq[2];
+            typename Loop::OP op[2];
+#pragma unroll
+            for (int k = 0; k < 2; k++) {
+                oq[k].init(Q + k * plane_q, ldq, nq, C, q0, 0, stages, lane, wave);
+                op[k].init(P + k * plane_p, ldp, np, C, p0, 0, stages, lane, wave);
+            }
+            Loop::run(lds, oq, op, stages, lane, wave, acc);
+        } else {
+            typename Loop::OQ oq;
+            typename Loop::OP op;
+            oq.init(Q, ldq, nq, C, q0, 0, stages, lane, wave);
+            op.init(P, ldp, np, C, p0, 0, stages, lane, wave);
+            Loop::template run<uint16_t>(lds, oq, op, stages, 0, lane, wave, acc);
         }
-        oq.init(Q, ldq, nq, C, q0, 0, stages, lane, wave);
-        op.init(P, ldp, np, C, p0, 0, stages, lane, wave);
-        if constexpr (PARTS) {  // h, h, l and h, l, h
-            const long long back_q = (long long)stages * oq.step, back_p = (long long)stages * op.step;
-            oq.parts(stages, -back_q, 2 * plane_q - back_q);
-            op.parts(stages, 2 * plane_p - back_p, -2 * plane_p - back_p);
-        }
-        Loop::template run<uint16_t>(lds + group * Any::LDS, oq, op, PARTS ? 3 * stages : stages, 0, lane, wave, acc);
     };
     constexpr std::false_type no{};
     constexpr std::true_type yes{};
     const _Float16* x = h_of(s, pass.from, i);
-    typedef Finish<PHASE, THREE, TILE::TI, TILE::TJ, Any::ROOM> Put;
-    const int q1 = q0 + 16 * TILE::TI * (wave / TILE::WP), p1 = p0 + 16 * TILE::TJ * (wave % TILE::WP);
+    typedef Finish<PHASE, THREE, B, B, Any::ROOM> Put;
+    const int q1 = q0 + 16 * B * (wave / 2), p1 = p0 + 16 * B * (wave % 2);
     Put put(s, pass, i, lane, q1, p1);
-    if (group == 0) put.ahead();
+    put.ahead();
     if constexpr (PHASE == GRAM) {
         if (is_tall(s)) run(yes, yes, x, s.C, s.C, nx, x, s.C, s.C, nx, s.R);
         else run(no, no, x, s.R, s.C, nx, x, s.R, s.C, nx, s.C);
@@ -372,44 +469,24 @@ __global__ void __launch_bounds__(TILE::THREADS, TILE::PER_SIMD) newton_schulz_k
         if (is_tall(s)) run(no, no, x, s.R, s.C, nx, b, side, side, nn, side);
         else run(no, yes, b, side, side, nn, x, s.C, s.C, nx, side);
     }
-    if constexpr (GROUPS > 1) {
-        constexpr int PIECES = TILE::TI * TILE::TJ;
-        f32x4* sums = reinterpret_cast<f32x4*>(lds + Any::LDS) + 64 * PIECES * wave + lane;  // behind the first group's
-        constexpr int NEXT = 64 * PIECES * WAVES;
-        if (group > 0)
-#pragma unroll
-            for (int k = 0; k < PIECES; k++) sums[NEXT * (group - 1) + 64 * k] = acc[k / TILE::TJ][k % TILE::TJ];
-        __syncthreads();
-        if (group > 0) return;
-#pragma unroll
-        for (int k = 0; k < PIECES; k++) {
-            acc[k / TILE::TJ][k % TILE::TJ] += sums[64 * k];
-            acc[k / TILE::TJ][k % TILE::TJ] += sums[NEXT + 64 * k];
-        }
-    }
     float* room = reinterpret_cast<float*>(lds) + wave * Any::ROOM;
     if constexpr (Put::S::AHEAD) put.put(ends, tq != tp, acc, room);
     else Put(s, pass, i, lane, q1, p1).put(ends, tq != tp, acc, room);
 }
 
 template <bool THREE>
-void launch_products(hipStream_t stream, Phase phase, Kind kind, const Shapes& m, const Ends& ends, const Pass& pass) {
-    const dim3 grid((unsigned)pass.places.first[m.n]);
+void launch_products(hipStream_t stream, Phase phase, int tile, const Shapes& m, const Ends& ends, const Pass& pass) {
+    const dim3 grid((unsigned)pass.places.first[m.n]), block(256);
     auto with = [&](auto TILE) {
         typedef decltype(TILE) Tile;
-        const dim3 block(Tile::THREADS);
         if (phase == GRAM) hipLaunchKernelGGL((newton_schulz_kernel<GRAM, Tile, THREE>), grid, block, 0, stream, m, ends, pass);
         else if (phase == SQUARE) hipLaunchKernelGGL((newton_schulz_kernel<SQUARE, Tile, THREE>), grid, block, 0, stream, m, ends, pass);
         else hipLaunchKernelGGL((newton_schulz_kernel<UPDATE, Tile, THREE>), grid, block, 0, stream, m, ends, pass);
     };
-    switch (kind) {
-        case K256: with(Tile256{}); break;
-        case K128: with(Tile128{}); break;
-        case K64: with(Tile64{}); break;
-        case K64_PARTS:
-            if constexpr (THREE) with(Tile64Parts{});
-            break;
-    }
+    if (tile == 64) return with(Tile64{});
+    if constexpr (!THREE)
+        if (tile == 256) return with(Tile256{});
+    with(Tile128{});
 }
 
 }  // namespace ozn
