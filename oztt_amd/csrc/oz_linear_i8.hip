@@ -178,19 +178,21 @@ __global__ void __launch_bounds__(64 * WAVES, 4) scaled_few_rows_kernel(const Sc
     else finish(a.epi, a.type, q, p0 + i, (float)v * a.p_scale[p0 + i] * a.q_scale[q]);
 }
 
-// One or two rows of X, values or integers: a wave streams rows of W, 4 KB at a time, and multiplies on the vector units, four products an
-// instruction. X is quantized by every workgroup for itself into LDS, while the first 4 KB of its waves' rows are on
+// One or two rows of X, values or integers: a wave streams rows of W, 4 KB at a time and two such ahead, and multiplies on the vector units, four products an
+// instruction. X is quantized by every workgroup for itself into LDS, while the first 8 KB of its waves' rows are on
 // the way: a launch of its own in front would cost more than that. Few rows of W: KS waves share a row's k.
-constexpr int kStreamK = 16384;  // X in a workgroup's registers, once
+constexpr int kStreamK = 16384;  // X in LDS, by each workgroup
 struct Tokens {
     const void* X;  // values of `type`, or integers with scales
     long long ldx;
     int type;
     bool int8;
 };
+template <int M>
+constexpr int kStreamGroups = M == 1 ? 4 : 3;  // of a CU, as registers allow: their first reads are all of 8192 x 8192 weights
 template <int M, int TYPE, bool INT8>
-__global__ void __launch_bounds__(64 * WAVES, 4) scaled_stream_kernel(const ScaledProduct a, const Tokens t, int ks) {
-    constexpr int U = 4, THREADS = 64 * WAVES, V = 8, PIECES = kStreamK / V / THREADS;
+__global__ void __launch_bounds__(64 * WAVES, 2 * kStreamGroups<M>) scaled_stream_kernel(const ScaledProduct a, const Tokens t, int ks) {
+    constexpr int U = 4, THREADS = 64 * WAVES, V = 8;
     extern __shared__ __attribute__((aligned(16))) int8_t xs[];  // M rows of whole KB, zeros behind K
     __shared__ unsigned tops[WAVES][M];
     __shared__ int sums[WAVES][M];
@@ -211,9 +213,20 @@ __global__ void __launch_bounds__(64 * WAVES, 4) scaled_stream_kernel(const Scal
             else w[b][u] = guarded16<false>(row, k + 16 * lane, a.K);
         }
     };
-    int turn = blockIdx.x;
-    const int8_t* row = row_of(turn);
-    ask(0, row, 0);
+    // the group to ask for next, of this row or a next one's first
+    int next_turn = blockIdx.x, next_group = 0;
+    const int8_t* next_row = row_of(next_turn);
+    auto ask_next = [&](int b) {
+        if (next_turn >= turns) return;
+        ask(b, next_row, next_group);
+        if (++next_group == groups) {
+            next_group = 0;
+            next_turn += gridDim.x;
+            next_row = row_of(next_turn);
+        }
+    };
+    ask_next(0);
+    ask_next(1);
     float scale[M];
     if constexpr (INT8) {
 #pragma unroll
@@ -223,21 +236,21 @@ __global__ void __launch_bounds__(64 * WAVES, 4) scaled_stream_kernel(const Scal
             scale[m] = a.q_scale[m];
         }
     } else {
-        float x[M][PIECES][V] = {};
+        // X is read twice, from memory and out of the caches: kept, it would take the registers of a fourth workgroup
+        auto get = [&](int m, int k, float* v) {
+            if (k + V <= a.K) load8(t.X, TYPE, m * t.ldx + k, v);
+            else load_some(t.X, TYPE, m * t.ldx + k, max(a.K - k, 0), v);
+        };
         unsigned top[M] = {};
 #pragma unroll
-        for (int m = 0; m < M; m++)
-#pragma unroll
-            for (int j = 0; j < PIECES; j++) {
-                const int k = V * (THREADS * j + threadIdx.x);
-                if (V * THREADS * j >= a.K) break;
-                if (k + V <= a.K) load8(t.X, TYPE, m * t.ldx + k, x[m][j]);
-                else load_some(t.X, TYPE, m * t.ldx + k, max(a.K - k, 0), x[m][j]);
-#pragma unroll
-                for (int e = 0; e < V; e++) top[m] = max(top[m], ozq::bits_of(x[m][j][e]));
-            }
-#pragma unroll
         for (int m = 0; m < M; m++) {
+#pragma unroll 2
+            for (int k = V * threadIdx.x; k < a.K; k += V * THREADS) {
+                float v[V];
+                get(m, k, v);
+#pragma unroll
+                for (int e = 0; e < V; e++) top[m] = max(top[m], ozq::bits_of(v[e]));
+            }
 #pragma unroll
             for (int d = 32; d > 0; d /= 2) top[m] = max(top[m], (unsigned)__shfl_xor(top[m], d));
             if (lane == 0) tops[wave][m] = top[m];
@@ -249,10 +262,11 @@ __global__ void __launch_bounds__(64 * WAVES, 4) scaled_stream_kernel(const Scal
             for (int s = 0; s < WAVES; s++) top[m] = max(top[m], tops[s][m]);
             const ozq::Scale s = ozq::scale_of(top[m]);
             scale[m] = s.scale;
-#pragma unroll
-            for (int j = 0; j < PIECES; j++) {
-                const int k = V * (THREADS * j + threadIdx.x);
-                if (k < width) *reinterpret_cast<u32x2*>(xs + m * width + k) = u32x2{ozq::pack4(x[m][j], s.inverse), ozq::pack4(x[m][j] + 4, s.inverse)};
+#pragma unroll 2
+            for (int k = V * threadIdx.x; k < width; k += V * THREADS) {
+                float v[V];
+                get(m, k, v);
+                *reinterpret_cast<u32x2*>(xs + m * width + k) = u32x2{ozq::pack4(v, s.inverse), ozq::pack4(v + 4, s.inverse)};
             }
         }
     }
@@ -274,22 +288,12 @@ __global__ void __launch_bounds__(64 * WAVES, 4) scaled_stream_kernel(const Scal
     auto put = [&](long long p, int m, int v) {
         if (p < a.np) finish(a.epi, a.type, m, p, (float)v * a.p_scale[p] * scale[m]);
     };
-    // the next group, of this row or the next one's first
-    int group = 0, next_turn = turn, next_group = 0;
-    const int8_t* next_row = row;
-    auto advance = [&]() {
-        if (++next_group == groups) {
-            next_group = 0;
-            next_turn += gridDim.x;
-            next_row = row_of(next_turn);
-        }
-    };
+    int turn = blockIdx.x, group = 0;
     auto one = [&](auto B) {
         constexpr int b = decltype(B)::value;
-        advance();
-        if (next_turn < turns) ask(b ^ 1, next_row, next_group);
         add(b, group);
-        if (next_group == 0) {  // the row's last group
+        ask_next(b);
+        if (++group == groups) {  // the row's last group
 #pragma unroll
             for (int m = 0; m < M; m++) {
 #pragma unroll
@@ -314,8 +318,8 @@ __global__ void __launch_bounds__(64 * WAVES, 4) scaled_stream_kernel(const Scal
             }
 #pragma unroll
             for (int m = 0; m < M; m++) acc[m] = 0;
+            turn += gridDim.x, group = 0;
         }
-        turn = next_turn, group = next_group;
     };
     while (turn < turns) {
         one(std::integral_constant<int, 0>{});
@@ -333,7 +337,7 @@ int waves_of_a_row(int cus, long long np, int K) {
 template <int M, int TYPE, bool INT8>
 int launch_stream(oz_dev* dev, const ScaledProduct& a, const Tokens& t) {
     const int ks = waves_of_a_row(dev->cus, a.np, a.K), rows = WAVES / ks;
-    const long long turns = (a.np + rows - 1) / rows, grid = ks > 1 ? turns : std::min<long long>(turns, 2 * dev->cus);
+    const long long turns = (a.np + rows - 1) / rows, grid = ks > 1 ? turns : std::min<long long>(turns, kStreamGroups<M> * dev->cus);
     hipLaunchKernelGGL((scaled_stream_kernel<M, TYPE, INT8>), dim3((unsigned)grid), dim3(64 * WAVES), M * ((a.K + 1023) / 1024 * 1024), dev->stream, a, t, ks);
     return oz::launch_check(dev, "scaled_stream_kernel");
 }

@@ -10,35 +10,55 @@ using namespace ozq;
 
 constexpr int THREADS = 256, V = 8;
 
-// A workgroup a row: the largest value, then the integers, from memory each time.
-template <int TYPE>
+// LANES threads a row (part of a wave, a wave or a workgroup), PIECES pieces of 8 values each, which stay in registers between the largest value and the
+// integers; PIECES = 0: rows that do not fit, read twice. Bound by memory: 8192^2 BF16 values in XXX us (201 MB; read twice, the second time
+// out of the caches, 47.7).
+template <int TYPE, int LANES, int PIECES>
 __global__ void __launch_bounds__(THREADS) quantize_kernel(long long M, int K, const void* __restrict__ X, long long ldx, int8_t* __restrict__ Q, long long ldq,
                                                            int fill, float* __restrict__ scale) {
     __shared__ unsigned part[THREADS / 64];
-    const long long row = blockIdx.x + (long long)gridDim.x * blockIdx.y;
-    if (row >= M) return;
+    const int lane = threadIdx.x % LANES;
+    const long long row = (blockIdx.x + (long long)gridDim.x * blockIdx.y) * (THREADS / LANES) + threadIdx.x / LANES;
+    const bool in = row < M;
     auto get = [&](int col, float* x) {
         if (col + V <= K) load8(X, TYPE, row * ldx + col, x);
         else load_some(X, TYPE, row * ldx + col, max(K - col, 0), x);
     };
+    float kept[PIECES ? PIECES : 1][V];
     unsigned top = 0;
-    for (int col = V * threadIdx.x; col < K; col += V * THREADS) {
-        float x[V];
-        get(col, x);
+    auto look = [&](const float* x) {
 #pragma unroll
         for (int k = 0; k < V; k++) top = max(top, bits_of(x[k]));
+    };
+    if constexpr (PIECES > 0) {
+#pragma unroll
+        for (int j = 0; j < PIECES; j++) {
+            const int col = V * (LANES * j + lane);
+#pragma unroll
+            for (int k = 0; k < V; k++) kept[j][k] = 0.0f;
+            if (in && col < K) get(col, kept[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < PIECES; j++) look(kept[j]);
+    } else if (in) {
+        for (int col = V * lane; col < K; col += V * LANES) {
+            float x[V];
+            get(col, x);
+            look(x);
+        }
     }
 #pragma unroll
-    for (int d = 32; d > 0; d /= 2) top = max(top, __shfl_xor(top, d));
-    if (!(threadIdx.x & 63)) part[threadIdx.x >> 6] = top;
-    __syncthreads();
+    for (int d = (LANES < 64 ? LANES : 64) / 2; d > 0; d /= 2) top = max(top, (unsigned)__shfl_xor(top, d));
+    if constexpr (LANES > 64) {
+        if (!(threadIdx.x & 63)) part[threadIdx.x >> 6] = top;
+        __syncthreads();
 #pragma unroll
-    for (int k = 0; k < THREADS / 64; k++) top = max(top, part[k]);
+        for (int k = 0; k < THREADS / 64; k++) top = max(top, part[k]);
+    }
+    if (!in) return;
     const Scale s = scale_of(top);
-    if (threadIdx.x == 0) scale[row] = s.scale;
-    for (int col = V * threadIdx.x; col < fill; col += V * THREADS) {
-        float x[V];
-        get(col, x);
+    if (lane == 0) scale[row] = s.scale;
+    auto put = [&](int col, const float* x) {
         const unsigned w[2] = {pack4(x, s.inverse), pack4(x + 4, s.inverse)};
         int8_t* to = Q + row * ldq + col;
         if (col + V <= fill) {
@@ -48,7 +68,41 @@ __global__ void __launch_bounds__(THREADS) quantize_kernel(long long M, int K, c
             for (int k = 0; k < V; k++)
                 if (col + k < fill) to[k] = (int8_t)(w[k / 4] >> (8 * (k % 4)));
         }
+    };
+    if constexpr (PIECES > 0) {
+#pragma unroll
+        for (int j = 0; j < PIECES; j++) put(V * (LANES * j + lane), kept[j]);
+        // the zeros behind K, where the pieces end before
+        const float none[V] = {};
+        for (int col = V * (LANES * PIECES + lane); col < fill; col += V * LANES) put(col, none);
+    } else {
+        for (int col = V * lane; col < fill; col += V * LANES) {
+            float x[V];
+            get(col, x);
+            put(col, x);
+        }
     }
+}
+
+template <int TYPE, int LANES, int PIECES>
+void launch(oz_dev* dev, long long M, int K, const void* X, long long ldx, int8_t* Q, long long ldq, int fill, float* scale) {
+    const long long groups = (M + THREADS / LANES - 1) / (THREADS / LANES), x = groups < 1 << 23 ? groups : 1 << 23;
+    hipLaunchKernelGGL((quantize_kernel<TYPE, LANES, PIECES>), dim3((unsigned)x, (unsigned)((groups + x - 1) / x)), dim3(THREADS), 0, dev->stream, M, K, X, ldx,
+                       Q, ldq, fill, scale);
+}
+
+template <int TYPE>
+void by_length(oz_dev* dev, long long M, int K, const void* X, long long ldx, int8_t* Q, long long ldq, int fill, float* scale) {
+    const auto with = [&](auto kernel) { kernel(dev, M, K, X, ldx, Q, ldq, fill, scale); };
+    if (K <= 128) with(launch<TYPE, 16, 1>);
+    else if (K <= 512) with(launch<TYPE, 64, 1>);
+    else if (K <= 2048 && M <= 1024) with(launch<TYPE, 256, 1>);  // few rows: 24 x 2048 in 3.3 us, a wave a row in 4.0; many: 4096 x 1024 5.7, 3.6
+    else if (K <= 1024) with(launch<TYPE, 64, 2>);
+    else if (K <= 2048) with(launch<TYPE, 64, 4>);
+    else if (K <= 4096) with(launch<TYPE, 256, 2>);
+    else if (K <= 8192) with(launch<TYPE, 256, 4>);
+    else if (K <= 16384) with(launch<TYPE, 256, 8>);
+    else with(launch<TYPE, 256, 0>);
 }
 
 bool misaligned(const void* p, int type) { return ((uintptr_t)p & (size_of(type) - 1)) != 0; }
@@ -56,11 +110,9 @@ bool misaligned(const void* p, int type) { return ((uintptr_t)p & (size_of(type)
 }  // namespace
 
 int ozq::launch_quantize(oz_dev* dev, int type, long long M, int K, const void* X, long long ldx, int8_t* Q, long long ldq, int fill, float* scale) {
-    const long long x = M < 1 << 23 ? M : 1 << 23;
-    const dim3 grid((unsigned)x, (unsigned)((M + x - 1) / x)), block(THREADS);
-    if (type == OZ_F32) hipLaunchKernelGGL(quantize_kernel<OZ_F32>, grid, block, 0, dev->stream, M, K, X, ldx, Q, ldq, fill, scale);
-    else if (type == OZ_BF16) hipLaunchKernelGGL(quantize_kernel<OZ_BF16>, grid, block, 0, dev->stream, M, K, X, ldx, Q, ldq, fill, scale);
-    else hipLaunchKernelGGL(quantize_kernel<OZ_F16>, grid, block, 0, dev->stream, M, K, X, ldx, Q, ldq, fill, scale);
+    if (type == OZ_F32) by_length<OZ_F32>(dev, M, K, X, ldx, Q, ldq, fill, scale);
+    else if (type == OZ_BF16) by_length<OZ_BF16>(dev, M, K, X, ldx, Q, ldq, fill, scale);
+    else by_length<OZ_F16>(dev, M, K, X, ldx, Q, ldq, fill, scale);
     return oz::launch_check(dev, "quantize_kernel");
 }
 
