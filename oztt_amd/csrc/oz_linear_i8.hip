@@ -374,6 +374,11 @@ const char* refuse(const oz_linear_i8_desc* d) {
 
 size_t up(size_t bytes) { return (bytes + 255) & ~(size_t)255; }
 
+// Few rows by the kernel of few rows: with integers for X 8 x 2048 x 2048 4.2 us (5.8 in tiles), 16 x 512 x 8192 8.5 (10.7), 4 x 4096 x 16384 15.4
+// (17.3), 4 x 8192 x 8192 13.9 (14.1). Tiles read X once for more rows of W, and long rows in more ranges: 16 x 8192 x 8192 14.1 us (17.9), 8 x
+// 8192 x 8192 14.2 (15.4), 3 x 1024 x 131000 30 (46).
+bool few_rows(int M, int N, int K) { return K <= 32768 && (M <= 4 || N <= 4096); }
+
 // How a call runs, and its workspace: the integers of X in rows of whole stages, their scales, the ranges' sums.
 struct Plan {
     bool stream;
@@ -386,7 +391,7 @@ Plan plan_of(int cus, const oz_linear_i8_desc* d) {
     Plan p{};
     p.stream = d->M <= kStreamRows && d->K <= kStreamK;
     if (p.stream || !d->M) return p;
-    p.route = route_of(cus, d->M, d->N, (d->K + 1) / 2, true, true);
+    p.route = route_of(cus, d->M, d->N, (d->K + 1) / 2, few_rows(d->M, d->N, d->K), true);
     p.width = (d->K + 2 * BC - 1) / (2 * BC) * (2 * BC);
     if (!d->x_int8) p.x = up((size_t)d->M * p.width), p.scale = up(4 * (size_t)d->M);
     return p;
@@ -450,3 +455,12 @@ int oz_linear_i8(oz_dev* dev, const oz_linear_i8_desc* d, const void* X, const f
 }
 
 }  // extern "C"
+
+// The way of a product, for tests: -2 streamed, -1 the kernel of few rows, else the tile; *splits its ranges of k.
+extern "C" int oz_rule_linear_i8(int cus, int M, int N, int K, int* splits) {
+    oz_linear_i8_desc d{};
+    d.M = M, d.N = N, d.K = K, d.x_int8 = 1;
+    const Plan p = plan_of(cus, &d);
+    if (splits) *splits = p.route.splits;
+    return p.stream ? -2 : p.route.few ? -1 : (int)p.route.tile;
+}

@@ -156,3 +156,15 @@ int ozn::iterate(oz_dev* dev, const Shapes& m, const Ends& ends, const Factors& 
         if (int st = iterate_alike(dev, p, ends, f, steps)) return st;
     return OZ_OK;
 }
+
+// The tile of a phase's products over `count` matrices of one size, and in *rest that of a last round's own launch or 0, for tests.
+extern "C" int oz_rule_newton_schulz(int cus, int phase, int rows, int cols, int count, int three, int* rest) {
+    Shapes m{};
+    m.n = 1;
+    Shape& s = m.s[0];
+    s.rows = rows, s.cols = cols, s.count = count, s.three = three;
+    s.R = (int)up(rows, kPad) * kPad, s.C = (int)up(cols, kPad) * kPad;
+    const Choice c = three ? choose(m, (Phase)phase, cus, kBoth) : choose(m, (Phase)phase, cus, kOne);
+    if (rest) *rest = c.rest.n[0] ? c.rest_tile : 0;
+    return c.tile;
+}

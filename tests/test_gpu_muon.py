@@ -132,3 +132,32 @@ def test_plan_memory_from_python(dev):
     with pytest.raises(RuntimeError, match="needed"):
         dev.muon_plan([x.tensor for x in ms], small)
     small.free()
+
+
+def test_rounds_cut_across_sizes(dev):
+    """So many tiles of several sizes that a last round's own launch takes up two of them."""
+    sizes = [(2048, 2048)] * 3 + [(1024, 4096)] * 2 + [(3000, 1024)] * 2 + [(700, 600)] * 5
+    step(dev, [Matrix(r, c, "bf16", True, "bf16", seed=i) for i, (r, c) in enumerate(sizes)])
+    sizes = [(500, 1500)] * 6 + [(1500, 400)] * 7 + [(512, 512)] * 9
+    step(dev, [Matrix(r, c, "f32", False, "f32", seed=i) for i, (r, c) in enumerate(sizes)], nesterov=False)
+
+
+def test_two_handles_at_once(dev):
+    """Two handles step two lists, each in its own workspace, with nothing between the calls."""
+    other = ozd.Device(0)
+    try:
+        lists = [[Matrix(600, 700, seed=1), Matrix(90, 300, seed=2)], [Matrix(700, 600, seed=3), Matrix(128, 128, seed=4)]]
+        wanted = [[x.step(0.02, 0.9, True) for x in l] for l in lists]
+        plans = [d.muon_plan([x.tensor for x in l]) for d, l in zip((dev, other), lists)]
+        sizes = [d.muon_workspace(p) for d, p in zip((dev, other), plans)]
+        works = [torch.zeros(n, dtype=torch.uint8, device="cuda:0") for n in sizes]
+        torch.cuda.synchronize()
+        for d, p, w, n in zip((dev, other), plans, works, sizes):
+            d.muon_step(p, 0.02, 0.9, work=Ptr(w), work_bytes=n)
+        dev.sync()
+        other.sync()
+        for l, ws in zip(lists, wanted):
+            for x, w in zip(l, ws):
+                x.check(w)
+    finally:
+        other.close()

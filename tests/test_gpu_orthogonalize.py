@@ -14,6 +14,7 @@ import pytest
 import torch
 
 from oztt_amd import device as ozd
+from tests.newton_schulz_cases import BOTH, ONE
 from tests.operator_cases import DTYPE, ROUND, Ptr, generator
 
 pytestmark = pytest.mark.gpu
@@ -183,3 +184,43 @@ def test_refusals(dev):
             call()
     dev.orthogonalize(ozd.orthogonalize_desc(8, 8, 0, "f32"), Ptr(None), Ptr(None))
     dev.sync()
+
+
+@pytest.mark.parametrize("size", sorted(set(ONE.values())), ids=str)
+def test_every_tile(dev, size):
+    print("orthogonalize", size, "bf16", flush=True)
+    G = low_rank(*size, "bf16")
+    check(run(dev, G, "bf16"), exact(G), bound_of(size, "bf16"), "bf16")
+
+
+@pytest.mark.parametrize("size", sorted(set(BOTH.values())), ids=str)
+def test_every_tile_of_both_parts(dev, size):
+    print("orthogonalize", size, "f32", flush=True)
+    G = low_rank(*size, "f32")
+    check(run(dev, G, "f32"), exact(G), bound_of(size, "f32"), "f32")
+
+
+def test_offsets_past_32_bits(dev):
+    """2^31 values and more in one matrix, wide and tall: one step, sampled, against A summed in 64 bits piece by piece."""
+    short, long = 2100, 2**20
+    for tall in (False, True):
+        print("orthogonalize", "tall" if tall else "wide", short, long, flush=True)
+        rows, cols = (long, short) if tall else (short, long)
+        G = torch.empty((1, rows, cols), dtype=torch.bfloat16, device="cuda:0").normal_(generator=generator(7))
+        got = run(dev, G, "bf16", steps=1, inplace=False)[0]
+        S, squares = torch.zeros((short, short), dtype=torch.float64, device="cuda:0"), 0.0
+        pieces = range(0, long, 2**17)
+        part = lambda i, n=2**17: (G[0, i : i + n].double().T if tall else G[0][:, i : i + n].double())  # noqa: E731
+        for i in pieces:
+            x = part(i)
+            squares += float(x.square().sum())
+            S += x @ x.T
+        norm = squares**0.5 + 1e-7
+        S /= norm**2
+        P = A * torch.eye(short, dtype=torch.float64, device="cuda:0") + B * S + C * (S @ S)
+        for i in (0, 2**19 - 64, long - 128):
+            want = P @ part(i, 128) / norm
+            o = got[i : i + 128].T if tall else got[:, i : i + 128]
+            check(o[None], want[None], 2e-3, "bf16", 0.0)
+        del G, got
+        torch.cuda.empty_cache()
