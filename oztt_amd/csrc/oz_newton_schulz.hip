@@ -12,14 +12,14 @@ namespace {
 using namespace ozn;
 
 // Tiles of one size: outputs on a side, workgroups that a CU holds, us for a stage of 64 values of c with one of them there and with all,
-// us besides for A and B and for X. Fitted to launches on 256 CUs: 8192^2's 512 and 1024 tiles of 256 x 256 (423, 409 and 863 us) and 2048 of
+// us besides for A and B and for X. Fitted to launches on 256 CUs: 8192^2's 512 and 1024 tiles of 256 x 256 (402, 398 and 863 us) and 2048 of
 // 128 x 128 (484), 9216 of 32 stages for four large blocks (695), 3 to 198 tiles of 64 x 64 of 6 to 72 stages (6.0 to 24.4); of both
 // parts 3 to 198 of 64 x 64 of 2 to 24 stages (5.2 to 16.6) and 540 of 8 and 24 (27.6), 216 of 128 x 128 of 11 (22.2) and 512 of 8 (42).
 struct Cost {
     int tile, per_cu;
     float alone, full, square, update;
 };
-constexpr Cost kOne[] = {{256, 1, 1.42f, 1.42f, 26.0f, 34.0f}, {128, 2, 0.57f, 0.86f, 10.0f, 10.0f}, {64, 2, 0.26f, 0.34f, 4.7f, 5.2f}};
+constexpr Cost kOne[] = {{256, 1, 1.42f, 1.42f, 19.0f, 34.0f}, {128, 2, 0.57f, 0.86f, 10.0f, 10.0f}, {64, 2, 0.26f, 0.34f, 4.7f, 5.2f}};
 constexpr Cost kBoth[] = {{128, 1, 1.0f, 1.0f, 13.5f, 12.0f}, {64, 2, 0.455f, 0.8f, 4.8f, 5.2f}};
 
 long long up(int n, int tile) { return (n + tile - 1) / tile; }
@@ -60,7 +60,7 @@ float estimate(const Shapes& m, Phase phase, const Cost& c, int cus, const Stret
 }
 
 // A phase in tiles of one size, and what a last, partly filled round of them would have in smaller ones by a launch of its own: 8192^2's A in
-// 512 tiles of 256 x 256 and the other 16 of 528 as 256 of 64 x 64 takes 455 us for 563. The launch costs 3 us.
+// 512 tiles of 256 x 256 and the other 16 of 528 as 256 of 64 x 64 takes 434 us for 563. The launch costs 3 us.
 struct Choice {
     int tile, rest_tile;
     Stretch main, rest;

@@ -125,7 +125,9 @@ template <int TI, int TJ, int ROOM, bool TWICE, class Ask, class Use, class Acro
 __device__ __forceinline__ void put_rows(const f32x4 (&acc)[TI][TJ], float* tile, int lane, bool twice, Ask&& ask, Use&& use, Across&& across) {
     typedef Bands<TI, TJ, ROOM> S;
     constexpr int ROW = S::ROW, RI = S::RI, RT = S::RT, BATCHES = S::NT / S::BATCH;
-    constexpr int XM = TJ * 4 >= 8 ? 7 : TJ * 4 - 1;
+    static_assert(TJ >= 2, "8 pieces of a row");
+    // a row's pieces of 4 values swizzled so that 8 rows in a row, and every eighth row, have a column on other banks
+    const auto swizzle = [](int row) { return (row ^ (row >> 3)) & 7; };
     const int r = lane & 15, g = lane >> 4, piece = 2 * (lane % (2 * TJ)), rr = lane / (2 * TJ);
     if constexpr (!S::AHEAD) ask_batch<TI, TJ, ROOM>(lane, ask, 0, std::integral_constant<int, 0>{});
     ozl::each<TI / RI>([&](auto H) {
@@ -134,7 +136,7 @@ __device__ __forceinline__ void put_rows(const f32x4 (&acc)[TI][TJ], float* tile
 #pragma unroll
         for (int i = 0; i < RI; i++)
 #pragma unroll
-            for (int j = 0; j < TJ; j++) *reinterpret_cast<f32x4*>(tile + (16 * i + r) * ROW + 4 * ((4 * j + g) ^ (r & XM))) = acc[h * RI + i][j];
+            for (int j = 0; j < TJ; j++) *reinterpret_cast<f32x4*>(tile + (16 * i + r) * ROW + 4 * ((4 * j + g) ^ swizzle(16 * i + r))) = acc[h * RI + i][j];
         __builtin_amdgcn_wave_barrier();
         ozl::each<BATCHES>([&](auto C) {
             constexpr int c = decltype(C)::value, b = h * BATCHES + c;
@@ -146,7 +148,7 @@ __device__ __forceinline__ void put_rows(const f32x4 (&acc)[TI][TJ], float* tile
                 f32x4* at[2];
 #pragma unroll
                 for (int k = 0; k < 2; k++) {
-                    at[k] = reinterpret_cast<f32x4*>(tile + row * ROW + 4 * ((piece + k) ^ (row & XM)));
+                    at[k] = reinterpret_cast<f32x4*>(tile + row * ROW + 4 * ((piece + k) ^ swizzle(row)));
                     const f32x4 x = *at[k];
 #pragma unroll
                     for (int m = 0; m < 4; m++) v[4 * k + m] = x[m];
@@ -160,16 +162,18 @@ __device__ __forceinline__ void put_rows(const f32x4 (&acc)[TI][TJ], float* tile
         });
         if constexpr (TWICE) {
             if (twice) {
-                constexpr int LANES = ROW < 64 ? ROW : 64, STEP = 8 * 64 / LANES;  // columns at a time, rows of a step
+                // 8 rows a lane, so that neighbouring lanes' 16 bytes of a column lie next to each other: whole lines (with a column a
+                // lane the 64 pieces of a store went to 64 lines: two rounds of 256 x 256 tiles of 8192^2's A 423 us for 402)
+                constexpr int CHUNKS = 2 * RI < 8 ? 2 * RI : 8, COLS = 64 / CHUNKS;
                 __builtin_amdgcn_wave_barrier();
 #pragma unroll
-                for (int c0 = 0; c0 < ROW; c0 += LANES)
+                for (int r0 = 0; r0 < 16 * RI; r0 += 8 * CHUNKS)
 #pragma unroll 2
-                    for (int r0 = 0; r0 < 16 * RI; r0 += STEP) {
-                        const int col = c0 + lane % LANES, row = r0 + 8 * (lane / LANES);
+                    for (int c0 = 0; c0 < ROW; c0 += COLS) {
+                        const int col = c0 + lane / CHUNKS, row = r0 + 8 * (lane % CHUNKS);
                         float v[8];
 #pragma unroll
-                        for (int k = 0; k < 8; k++) v[k] = tile[(row + k) * ROW + 4 * ((col >> 2) ^ ((row + k) & XM)) + (col & 3)];
+                        for (int k = 0; k < 8; k++) v[k] = tile[(row + k) * ROW + 4 * ((col >> 2) ^ swizzle(row + k)) + (col & 3)];
                         across(16 * RI * h + row, col, v);
                     }
                 __builtin_amdgcn_wave_barrier();
