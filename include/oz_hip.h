@@ -496,8 +496,9 @@ int oz_quantize_rows(oz_dev* dev, const oz_quantize_desc* d, const void* X, int8
  * INT8 matrix cores. W: N x K bytes with N scales, as oz_quantize_rows gives them. X is M x K bytes with M scales (x_int8), or M x K
  * values of `type`, which the call quantizes in the same way. The sums are exact in int32, whatever the bytes, for K up to 131071;
  * they are rounded to FP32 and multiplied by w_scale and x_scale in turn. bias (N values of `type`) and residual (M x N) may
- * be null. Rows of 8-bit operands begin at multiples of 4 bytes (addresses and leading dimensions that are none are refused),
- * what lies behind a row's K values may be anything. M may be 0. residual may be Y itself (the same leading dimension). */
+ * be null. Rows of 8-bit operands begin at multiples of 4 bytes (addresses and leading dimensions that are none are refused) and are
+ * read to the end of the 4 bytes that hold their last value; what lies behind a row's K values may be anything. A row of X without a
+ * scale gives NaN. M may be 0. residual may be Y itself (the same leading dimension). */
 typedef struct oz_linear_i8_desc {
     int M, N, K;
     int type;   /* oz_type of X and bias: OZ_BF16 or OZ_F16 */
@@ -518,7 +519,7 @@ int oz_linear_i8(oz_dev* dev, const oz_linear_i8_desc* d, const void* X, const f
  * zero or nearly so. The norm is summed in FP64, the iteration's products in FP32; X is kept in 22 bits. A BF16
  * result of more than 512 rows and columns takes products of 11 bits and is off by up to 2e-3 of its norm before it is rounded, all
  * others products of 22 bits: 1e-5 of its norm. (To both comes what rounding X leaves in directions of singular values near zero, which
- * a step makes a times larger: a^steps 2^-22 sqrt(steps) of the sum of squares' root, 1.3e-4.) X's values must stay below 16 (with the factors above they
+ * a step makes a times larger: a^steps 2^-22 sqrt(steps) of the sum of squares' root, 1.3e-4.) Singular values must stay below 8 (with the factors above they
  * stay below 1.3). A matrix of zeros gives zeros, one with a value that is not finite NaN. O may be G itself (the same type
  * and strides); matrices do not overlap each other. count may be 0. */
 typedef struct oz_orthogonalize_desc {
@@ -538,8 +539,8 @@ int oz_orthogonalize(oz_dev* dev, const oz_orthogonalize_desc* d, const void* G,
  *   m' = momentum m + (1 - momentum) g grad_scale
  *   u  = momentum m' + (1 - momentum) g grad_scale (nesterov), or m'
  *   p' = p (1 - lr weight_decay) - lr lr_scale orthogonalized(u)
- * With a master, p is the FP32 master and param receives p' rounded; without, p is param itself. Matrices are row-major and without
- * gaps. A gradient that is not finite makes its whole matrix NaN. */
+ * With a master, p is the FP32 master and param receives p' rounded; without, p is param itself. Matrices are row-major, without
+ * gaps, and do not overlap. A gradient that is not finite makes its whole matrix NaN. */
 #define OZ_MUON_SHAPES 16
 typedef struct oz_muon_tensor {
     int rows, cols; /* up to 2^20; either may be 0 */

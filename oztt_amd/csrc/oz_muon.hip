@@ -179,11 +179,13 @@ int orthogonalize(oz_dev* dev, const Shapes& m, const Ends& e, const Factors& f,
         if (pieces >> 31 || a >= 1 << 23 || b >= 1 << 23) return oz::fail(dev, OZ_ERR_ARG, "too many values in matrices");
     }
     squares.first[m.n] = (int)a, start.first[m.n] = (int)b;
+    Iteration it;
+    if (int st = prepare(dev, m, f, &it)) return st;
     hipLaunchKernelGGL(squares_kernel, dim3((unsigned)a), dim3(THREADS), 0, dev->stream, m, e, squares);
     if (int st = oz::launch_check(dev, "squares_kernel")) return st;
     hipLaunchKernelGGL(start_kernel, dim3((unsigned)b), dim3(THREADS), 0, dev->stream, m, e, start, eps, rounds);
     if (int st = oz::launch_check(dev, "start_kernel")) return st;
-    return iterate(dev, m, e, f, steps);
+    return iterate(dev, &it, e, steps);
 }
 
 constexpr int kMaxSide = 1 << 20;

@@ -108,52 +108,54 @@ bool places(const Shapes& m, Phase phase, int parent, int tile, const Stretch& t
         p->places.per[k] = (int)per;
         p->begin[k] = (int)t.begin[k];
         at += t.n[k] * (parent / tile) * (parent / tile);
-        if (per >> 22 || at >> 22 || (t.begin[k] + t.n[k]) >> 30) return false;
+        if (per >> 24 || at >> 24 || (t.begin[k] + t.n[k]) >> 24) return false;  // 2^32 threads along a dimension
     }
     p->places.first[m.n] = (int)at;
     return true;
 }
 
-int iterate_alike(oz_dev* dev, const Shapes& m, const Ends& ends, const Factors& f, int steps) {
-    if (!m.n) return OZ_OK;
-    const bool three = m.s[0].three;
-    Pass pass[3][2] = {};
-    Choice choice[3];
-    Shapes order[3];
-    for (const Phase phase : {GRAM, SQUARE, UPDATE}) {
-        order[phase] = m;
-        std::stable_sort(order[phase].s, order[phase].s + m.n, [&](const Shape& a, const Shape& b) { return stages_of(a, phase) > stages_of(b, phase); });
-        Choice& c = choice[phase];
-        c = three ? choose(order[phase], phase, dev->cus, kBoth) : choose(order[phase], phase, dev->cus, kOne);
-        if (!places(order[phase], phase, c.tile, c.tile, c.main, &pass[phase][0]) || !places(order[phase], phase, c.tile, c.rest_tile, c.rest, &pass[phase][1]))
-            return oz::fail(dev, OZ_ERR_ARG, "too many values in matrices");
-    }
-    for (int k = 0; k < steps; k++)
-        for (const Phase phase : {GRAM, SQUARE, UPDATE})
-            for (int part = 0; part < 2; part++) {
-                Pass& p = pass[phase][part];
-                if (!p.places.first[m.n]) continue;
-                p.f = f;
-                p.from = k & 1;
-                p.last = k + 1 == steps;
-                const int tile = part ? choice[phase].rest_tile : choice[phase].tile;
-                if (three) launch_products<true>(dev->stream, phase, tile, order[phase], ends, p);
-                else launch_products<false>(dev->stream, phase, tile, order[phase], ends, p);
-                if (int st = oz::launch_check(dev, "newton_schulz_kernel")) return st;
-            }
-    return OZ_OK;
-}
-
 }  // namespace
 
-int ozn::iterate(oz_dev* dev, const Shapes& m, const Ends& ends, const Factors& f, int steps) {
+int ozn::prepare(oz_dev* dev, const Shapes& m, const Factors& f, Iteration* it) {
     Shapes part[2] = {};
     for (int k = 0; k < m.n; k++) {
         Shapes& p = part[m.s[k].three];
         p.s[p.n++] = m.s[k];
     }
-    for (const Shapes& p : part)
-        if (int st = iterate_alike(dev, p, ends, f, steps)) return st;
+    for (int three = 0; three < 2; three++) {
+        Launches& l = it->of[three];
+        l = Launches{};
+        for (const Phase phase : {GRAM, SQUARE, UPDATE}) {
+            Shapes& order = l.order[phase];
+            order = part[three];
+            if (!order.n) continue;
+            std::stable_sort(order.s, order.s + order.n, [&](const Shape& a, const Shape& b) { return stages_of(a, phase) > stages_of(b, phase); });
+            const Choice c = three ? choose(order, phase, dev->cus, kBoth) : choose(order, phase, dev->cus, kOne);
+            l.tile[phase][0] = c.tile, l.tile[phase][1] = c.rest_tile;
+            if (!places(order, phase, c.tile, c.tile, c.main, &l.pass[phase][0]) || !places(order, phase, c.tile, c.rest_tile, c.rest, &l.pass[phase][1]))
+                return oz::fail(dev, OZ_ERR_ARG, "too many values in matrices");
+            for (Pass& p : l.pass[phase]) p.f = f;
+        }
+    }
+    return OZ_OK;
+}
+
+int ozn::iterate(oz_dev* dev, Iteration* it, const Ends& ends, int steps) {
+    for (int three = 0; three < 2; three++) {
+        Launches& l = it->of[three];
+        for (int k = 0; k < steps; k++)
+            for (const Phase phase : {GRAM, SQUARE, UPDATE})
+                for (int part = 0; part < 2; part++) {
+                    const Shapes& order = l.order[phase];
+                    Pass& p = l.pass[phase][part];
+                    if (!order.n || !p.places.first[order.n]) continue;
+                    p.from = k & 1;
+                    p.last = k + 1 == steps;
+                    if (three) launch_products<true>(dev->stream, phase, l.tile[phase][part], order, ends, p);
+                    else launch_products<false>(dev->stream, phase, l.tile[phase][part], order, ends, p);
+                    if (int st = oz::launch_check(dev, "newton_schulz_kernel")) return st;
+                }
+    }
     return OZ_OK;
 }
 

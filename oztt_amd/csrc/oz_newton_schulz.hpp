@@ -22,10 +22,12 @@ struct oz_dev;
 
 namespace ozn {
 
-constexpr float kScale = 4096.0f;  // X's values are at most about 1: 16 times as large ones still are FP16 numbers
+constexpr float kScale = 4096.0f;  // X.s values are at most about 1: 16 times as large ones still are FP16 numbers (8 times: B too)
 constexpr int kPad = 64;           // sides in the workspace are multiples of it, the rest zeros, which the iteration keeps
 constexpr int kShapes = OZ_MUON_SHAPES;
-constexpr int kThreeSide = 512;    // up to this shorter side the products take both parts
+// Up to this shorter side the products take both parts of X. There launches and their latency count more than products: 64^2 takes 74 us
+// for 70, 256 x 1024 130 for 98, 512^2 132 for 101, twelve of 512 x 2048 496 for 308; 1024^2 188 for 140 and twelve 933 for 466.
+constexpr int kThreeSide = 512;
 
 // `count` matrices of one size. Buffers hold them one after the other, each as one plane of R x C (h) or two (h, l).
 struct Shape {
@@ -97,7 +99,18 @@ struct Pass {
 template <bool THREE>
 void launch_products(hipStream_t stream, Phase phase, int tile, const Shapes& m, const Ends& ends, const Pass& pass);
 
+// The launches of a step, of the shapes whose products take one part of their operands and of those that take both: prepared, and
+// refused where they are too many, before anything runs.
+struct Launches {
+    Shapes order[3];  // the shapes as a phase's sequence of tiles has them
+    Pass pass[3][2];
+    int tile[3][2];
+};
+struct Iteration {
+    Launches of[2];
+};
+int prepare(oz_dev* dev, const Shapes& m, const Factors& f, Iteration* it);
 // The iteration on X0 in the shapes' x[0] (and l), the last step's results to the ends.
-int iterate(oz_dev* dev, const Shapes& m, const Ends& ends, const Factors& f, int steps);
+int iterate(oz_dev* dev, Iteration* it, const Ends& ends, int steps);
 
 }  // namespace ozn
