@@ -564,7 +564,7 @@ typedef struct oz_muon_plan {
 } oz_muon_plan;
 long long oz_muon_plan_bytes(const oz_muon_tensor* tensors, int count);
 int oz_muon_make_plan(oz_dev* dev, const oz_muon_tensor* tensors, int count, void* memory, size_t bytes, oz_muon_plan* plan);
-/* Bytes of workspace of a step: about 6 for each value of the matrices (10 with products of 22 bits) and 4 (8) of their shorter sides' squares. */
+/* Bytes of workspace of a step: about 6 for each value of the matrices (8 with products of 22 bits) and 4 (8) of their shorter sides' squares. */
 long long oz_muon_workspace(oz_dev* dev, const oz_muon_plan* plan);
 typedef struct oz_muon_options {
     double lr, momentum;

@@ -22,7 +22,7 @@ struct oz_dev;
 
 namespace ozn {
 
-constexpr float kScale = 4096.0f;  // X.s values are at most about 1: 16 times as large ones still are FP16 numbers (8 times: B too)
+constexpr float kScale = 4096.0f;  // X's values are at most about 1: 16 times as large ones still are FP16 numbers (8 times: B too)
 constexpr int kPad = 64;           // sides in the workspace are multiples of it, the rest zeros, which the iteration keeps
 constexpr int kShapes = OZ_MUON_SHAPES;
 // Up to this shorter side the products take both parts of X. There launches and their latency count more than products: 64^2 takes 74 us

@@ -99,7 +99,7 @@ __device__ __forceinline__ void put8(_Float16* h, _Float16* l, long long at, con
 
 // How a wave's sums go through LDS: RI bands of 16 rows at a time, turns of RT rows, a lane 8 values in a row; pieces of what they
 // are added to are asked for in batches.
-template <int TI, int TJ, int ROOM>
+template <bool THREE, int TI, int TJ, int ROOM>
 struct Bands {
     static constexpr int ROW = 16 * TJ;
     static constexpr int RI = TI * 16 * ROW <= ROOM ? TI : TI * 8 * ROW <= ROOM ? TI / 2 : TI / 4;
@@ -107,29 +107,30 @@ struct Bands {
     static constexpr int RT = 32 / TJ, NT = 16 * RI / RT;
     static constexpr int BATCH = NT < 8 ? NT : 8, ALL = TI / RI * NT / BATCH;  // of a turn's pieces; batches of a tile
     static_assert(NT % BATCH == 0, "whole batches");
-    // With one batch a tile's pieces are asked for before its products and wait in registers: four large blocks' update in tiles of 128 x
-    // 128 785 us, with them there 769. More do not fit: two in turn, a batch ahead.
-    static constexpr bool AHEAD = ALL == 1;
-    static constexpr int BUFFERS = AHEAD ? 1 : 2;
+    // With one batch the pieces that products of first parts are added to are asked for before them and wait in registers (four large
+    // blocks' update in tiles of 128 x 128: 693 us for 752). Products of both parts have none left over: there they cost (matrices of
+    // 700 x 1500 and others in tiles of 128 x 128: 40 us for 37). More do not fit: two in turn, a batch ahead.
+    static constexpr bool AHEAD = ALL == 1 && !THREE;
+    static constexpr int BUFFERS = ALL == 1 ? 1 : 2;
 };
 
 // The sums of a wave, as in ozl::put_sums: ask(P, t, row) loads what the t-th piece of a batch wants, use(P, t, row, v) finishes its 8
 // values (P: the batch's buffer; rows and columns are the wave's own). With TWICE use()'s values go back to LDS, and across(row, col, v)
 // gets 8 values of a column from `row` on.
-template <int TI, int TJ, int ROOM, class Ask, class P>
+template <bool THREE, int TI, int TJ, int ROOM, class Ask, class P>
 __device__ __forceinline__ void ask_batch(int lane, Ask&& ask, int b, P p) {
-    typedef Bands<TI, TJ, ROOM> S;
+    typedef Bands<THREE, TI, TJ, ROOM> S;
     ozl::each<S::BATCH>([&](auto T) { ask(p, T, (b * S::BATCH + decltype(T)::value) * S::RT + lane / (2 * TJ)); });
 }
-template <int TI, int TJ, int ROOM, bool TWICE, class Ask, class Use, class Across>
+template <bool THREE, int TI, int TJ, int ROOM, bool TWICE, class Ask, class Use, class Across>
 __device__ __forceinline__ void put_rows(const f32x4 (&acc)[TI][TJ], float* tile, int lane, bool twice, Ask&& ask, Use&& use, Across&& across) {
-    typedef Bands<TI, TJ, ROOM> S;
+    typedef Bands<THREE, TI, TJ, ROOM> S;
     constexpr int ROW = S::ROW, RI = S::RI, RT = S::RT, BATCHES = S::NT / S::BATCH;
     static_assert(TJ >= 2, "8 pieces of a row");
     // a row's pieces of 4 values swizzled so that 8 rows in a row, and every eighth row, have a column on other banks
     const auto swizzle = [](int row) { return (row ^ (row >> 3)) & 7; };
     const int r = lane & 15, g = lane >> 4, piece = 2 * (lane % (2 * TJ)), rr = lane / (2 * TJ);
-    if constexpr (!S::AHEAD) ask_batch<TI, TJ, ROOM>(lane, ask, 0, std::integral_constant<int, 0>{});
+    if constexpr (!S::AHEAD) ask_batch<THREE, TI, TJ, ROOM>(lane, ask, 0, std::integral_constant<int, 0>{});
     ozl::each<TI / RI>([&](auto H) {
         constexpr int h = decltype(H)::value;
         __builtin_amdgcn_wave_barrier();
@@ -140,7 +141,7 @@ __device__ __forceinline__ void put_rows(const f32x4 (&acc)[TI][TJ], float* tile
         __builtin_amdgcn_wave_barrier();
         ozl::each<BATCHES>([&](auto C) {
             constexpr int c = decltype(C)::value, b = h * BATCHES + c;
-            if constexpr (b + 1 < S::ALL) ask_batch<TI, TJ, ROOM>(lane, ask, b + 1, std::integral_constant<int, (b + 1) & 1>{});
+            if constexpr (b + 1 < S::ALL) ask_batch<THREE, TI, TJ, ROOM>(lane, ask, b + 1, std::integral_constant<int, (b + 1) & 1>{});
             ozl::each<S::BATCH>([&](auto T) {
                 constexpr int t = decltype(T)::value;
                 const int row = (c * S::BATCH + t) * RT + rr;
@@ -185,7 +186,7 @@ __device__ __forceinline__ void put_rows(const f32x4 (&acc)[TI][TJ], float* tile
 // What a wave's sums become: its first row and column q0 and p0, the lane's column. SQUARE adds to A, UPDATE to X.
 template <Phase PHASE, bool THREE, int TI, int TJ, int ROOM>
 struct Finish {
-    typedef Bands<TI, TJ, ROOM> S;
+    typedef Bands<THREE, TI, TJ, ROOM> S;
     const Shape s;
     const Factors f;
     const int from, last;
@@ -210,7 +211,7 @@ struct Finish {
         }
     }
     __device__ __forceinline__ void ahead() {
-        if constexpr (S::AHEAD) ask_batch<TI, TJ, ROOM>(lane, [&](auto P, auto T, int row) { ask(P, T, row); }, 0, std::integral_constant<int, 0>{});
+        if constexpr (S::AHEAD) ask_batch<THREE, TI, TJ, ROOM>(lane, [&](auto P, auto T, int row) { ask(P, T, row); }, 0, std::integral_constant<int, 0>{});
     }
     // v = factor times what it is added to, and `of` v
     template <class P, class T>
@@ -230,7 +231,7 @@ struct Finish {
         if constexpr (PHASE != UPDATE) {
             _Float16* to = PHASE == GRAM ? square_of(s, s.a, i) : square_of(s, s.b, i);
             _Float16* rest = THREE ? to + (long long)side * side : nullptr;
-            put_rows<TI, TJ, ROOM, true>(
+            put_rows<THREE, TI, TJ, ROOM, true>(
                 acc, tile, lane, mirror, get,
                 [&](auto P, auto T, int row, float* v) {
                     if constexpr (PHASE == GRAM) {
@@ -248,7 +249,7 @@ struct Finish {
             auto none = [](int, int, const float*) {};
             if (!last) {
                 _Float16 *to = h_of(s, from ^ 1, i), *rest = l_of(s, from ^ 1, i);
-                put_rows<TI, TJ, ROOM, false>(
+                put_rows<THREE, TI, TJ, ROOM, false>(
                     acc, tile, lane, false, get,
                     [&](auto P, auto T, int row, float* v) {
                         add(P, T, f.a, 1.0f, v);
@@ -258,7 +259,7 @@ struct Finish {
             } else if (e.tensors) {
                 const oz_muon_tensor t = e.tensors[s.first + i];
                 const float keep = 1.0f - e.lr * t.weight_decay, rate = e.lr * t.lr_scale * (1.0f / kScale);
-                put_rows<TI, TJ, ROOM, false>(
+                put_rows<THREE, TI, TJ, ROOM, false>(
                     acc, tile, lane, false, get,
                     [&](auto P, auto T, int row, float* v) {
                         add(P, T, f.a, 1.0f, v);
@@ -282,7 +283,7 @@ struct Finish {
                     },
                     none);
             } else {
-                put_rows<TI, TJ, ROOM, false>(
+                put_rows<THREE, TI, TJ, ROOM, false>(
                     acc, tile, lane, false, get,
                     [&](auto P, auto T, int row, float* v) {
                         add(P, T, f.a, 1.0f, v);
