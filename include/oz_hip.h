@@ -517,8 +517,8 @@ int oz_linear_i8(oz_dev* dev, const oz_linear_i8_desc* d, const void* X, const f
  * steps times X <- a X + (b A + c A^2) X, A = X X^T (from the right, with A = X^T X, where rows > cols), which moves
  * singular values s by a s + b s^3 + c s^5: with a, b, c = 3.4445, -4.7750, 2.0315 and 5 steps near 1, but for those that are
  * zero or nearly so. The norm is summed in FP64, the iteration's products in FP32; X is kept in 22 bits. A BF16
- * result of more than 512 rows and columns takes products of 11 bits and is off by up to 2e-3 of its norm before it is rounded, all
- * others products of 22 bits: 1e-5 of its norm. (To both comes what rounding X leaves in directions of singular values near zero, which
+ * result of more than 512 rows and columns takes products of 11 bits and is off by up to 2e-3 of its norm before it is rounded (by up to
+ * 1.1e-2 where values are alike and so are their roundings, as of an identity), all others products of 22 bits: 1e-5 of its norm. (To both comes what rounding X leaves in directions of singular values near zero, which
  * a step makes a times larger: a^steps 2^-22 sqrt(steps) of the sum of squares' root, 1.3e-4.) Singular values must stay below 8 (with the factors above they
  * stay below 1.3). A matrix of zeros gives zeros, one with a value that is not finite NaN. O may be G itself (the same type
  * and strides); matrices do not overlap each other. count may be 0. */

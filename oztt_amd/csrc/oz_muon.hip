@@ -159,6 +159,7 @@ size_t lay_out(Shape* s, int rows, int cols, int count, int first, bool exact, c
     if (!s->three) s->l = reinterpret_cast<_Float16*>(take(x));
     s->a = reinterpret_cast<_Float16*>(take(a));
     s->b = reinterpret_cast<_Float16*>(take(a));
+    if (!s->three) s->d = reinterpret_cast<float*>(take(4 * (size_t)count * side));
     s->sums = reinterpret_cast<double*>(take(8 * (size_t)count * s->chunks));
     return at;
 }

@@ -10,7 +10,11 @@
 // a few strong directions and many weak ones that each step makes a times larger, so what rounding does to X there
 // grows with them: with X in BF16 the result is off by 1e-2 of its norm for a Gaussian matrix and by 0.2 to 0.6 for one of
 // low rank, in FP16 by 1e-3 and 2e-2 to 7e-2. The products do not have that weakness, as B is nearly zero in the directions of small
-// singular values: with both parts in a X the result is off by 1e-4 to 2e-3 whatever the spectrum (64 to 1024 rows, against 64 bits).
+// singular values. Once most of them are near 1, B is near -2.7 times the identity, and rounding h and B to 11 bits is what shows:
+// B's diagonal is therefore kept in FP32 and multiplies both parts of X in the product's epilogue, X <- (a + diag B) X + (B - diag B) h,
+// which costs 1% (for Gaussian matrices of 513 to 1500 rows off by 1.3e-3 to 1.8e-3 without it, 4e-4 to 8.5e-4 with it). The
+// result is off by 2e-4 to 1.5e-3 whatever the spectrum (against 64 bits), by more only where values do not differ and their roundings
+// cannot average: an identity of 513 rows by up to 1.1e-2.
 // Where a side is short (the rounding errors of A and B then average over few values: up to 1e-2 at one to four rows) or the result
 // is kept in more than BF16's 8 bits, the products take both parts of both operands, h h + h l + l h: off by 1e-6.
 #pragma once
@@ -37,6 +41,7 @@ struct Shape {
     int three;       // products of both parts
     int chunks;      // of a matrix, for the sum of its squares
     _Float16 *x[2], *l, *a, *b;
+    float* d;        // products of the first parts: B's diagonals, where b has zeros
     double* sums;
 };
 struct Shapes {
@@ -69,6 +74,8 @@ __device__ __forceinline__ _Float16* l_of(const Shape& s, int b, int i) {
 }
 // A or B of a matrix
 __device__ __forceinline__ _Float16* square_of(const Shape& s, _Float16* p, int i) { return p + (long long)(1 + s.three) * i * side_of(s) * side_of(s); }
+
+__device__ __forceinline__ float* diagonal_of(const Shape& s, int i) { return s.d + (long long)i * side_of(s); }
 
 // Where the matrices come from and the results go: one array each (orthogonalize), or a list of tensors (Muon).
 struct Ends {

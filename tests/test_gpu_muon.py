@@ -88,6 +88,53 @@ def test_large(dev, size):
     step(dev, [Matrix(*size, "bf16", True, "bf16"), Matrix(*size, "f32", False, "f32", seed=2)])
 
 
+def updates(dev, G):
+    """The orthogonalized matrix in 32 bits: the negative of what a step makes of weights of zeros."""
+    x = Matrix(*G.shape, decay=0.0, scale=1.0)
+    x.param.zero_()
+    x.grad.copy_(G)
+    plan = dev.muon_plan([x.tensor])
+    n = dev.muon_workspace(plan)
+    work = torch.full((n,), 0x7F, dtype=torch.uint8, device="cuda:0")
+    torch.cuda.synchronize()
+    dev.muon_step(plan, 1.0, 0.0, True, work=Ptr(work), work_bytes=n)
+    dev.sync()
+    return -x.param.double()
+
+
+@pytest.mark.parametrize("size", [(545, 4482), (4482, 545), (1030, 1030), (2100, 1500)], ids=str)
+def test_updates_of_32_bit_weights(dev, size):
+    """With B's diagonal in FP32 products of 11 bits leave Gaussian matrices of 513 to 1500 rows off by 4e-4 to 8.5e-4 (the same roundings in 64
+    bits), with all of B in 11 bits by 1.3e-3 to 1.8e-3."""
+    print("updates", size, flush=True)
+    G = torch.randn(size, device="cuda:0", generator=generator(3))
+    want = exact(G[None], eps=1e-7)[0]
+    assert float((updates(dev, G) - want).norm() / want.norm()) <= 1.2e-3
+
+
+def off_alike(n, a, b, c, steps=5):
+    """Bound of the relative error for the identity of n rows, to first order: X = s I and s' = s p(s^2), p(q) = a + b q + c q^2. FP16 rounds h (twice
+    in A) and A by half a step, 2^-11, alike for all values; B is its diagonal, in FP32."""
+    s, e = n**-0.5, 0.0
+    for _ in range(steps):
+        q = s * s
+        p = a + b * q + c * q * q
+        e = abs((a + 3 * b * q + 5 * c * q * q) / p) * e + abs((b * q + 2 * c * q * q) / p) * 3 * 2.0**-11
+        s *= p
+    return e
+
+
+@pytest.mark.parametrize("n", [513, 600, 1024, 2048, 4096])
+def test_identity(dev, n):
+    """All singular values, and all roundings, alike."""
+    print("identity", n, flush=True)
+    eye = torch.eye(n, device="cuda:0")
+    got, want = updates(dev, eye), exact(eye[None], eps=1e-7)[0]
+    assert torch.equal(got, torch.diag(torch.diagonal(got)))
+    bound = off_alike(n, *ozd.NEWTON_SCHULZ)
+    assert bound <= 1.12e-2 and float((got - want).norm() / want.norm()) <= 1.1 * bound + 1e-5
+
+
 def test_grad_scale_decay_and_rate(dev):
     scale = torch.tensor([0.25], device="cuda:0")
     step(dev, [Matrix(80, 60, decay=0.0, scale=3.0), Matrix(60, 80, decay=0.5, scale=0.0)], lr=0.5, grad_scale=scale, steps=3, eps=1e-3)
