@@ -235,13 +235,13 @@ float estimate(const Shape& t, int cus, long long nq, long long np, long long C,
 // It is further off where c is long and tiles are few, as the estimate takes their stages for shorter than they are: without caches
 // 512 x 8192^2 96 us for 81 by 256 x 256 in 4 ranges, 256 x 8192^2 73 (estimate: 45) for 64 by 128 x 128 in 4, and of few rows 16 x
 // 8192^2 36 for 30 by 32 x 32.
-ozl::Route ozl::route_of(int cus, long long nq, long long np, long long C, bool contiguous, bool even) {
+ozl::Route ozl::route_of(int cus, long long nq, long long np, long long C, bool contiguous, bool even, int streamed) {
     Route r{};
     r.splits = 1;
     if (contiguous && (nq <= kFewRows || (!even && nq <= kFewOddRows))) {
         r.few = true;
         const long long groups = (np + few_rows_block(nq) - 1) / few_rows_block(nq);
-        while (nq > kStreamRows && r.splits < 16 && groups * r.splits * 4 <= cus && C / (r.splits * 2) >= 512) r.splits *= 2;
+        while (nq > streamed && r.splits < 16 && groups * r.splits * 4 <= cus && C / (r.splits * 2) >= 512) r.splits *= 2;
     } else {
         float best = 0.0f;
         for (int t = 0; t < TILES; t++)

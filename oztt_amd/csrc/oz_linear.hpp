@@ -112,11 +112,12 @@ struct Route {
     int splits;
     size_t parts;   // bytes of the ranges' sums
 };
-Route route_of(int cus, long long nq, long long np, long long C, bool contiguous, bool even);
+// Up to `streamed` rows have a kernel of their own, which takes no ranges.
+constexpr int kStreamRows = 2;
+Route route_of(int cus, long long nq, long long np, long long C, bool contiguous, bool even, int streamed = kStreamRows);
 int launch_tile(oz_dev* dev, int type, Tile tile, const Product& a);
 // At most 32 rows of Q, operands along c at any address; splits as in Product (1 for at most kStreamRows). A workgroup has
 // few_rows_block rows of P.
-constexpr int kStreamRows = 2;
 inline int few_rows_block(long long nq) { return nq <= 16 ? 16 : 32; }
 int launch_few_rows(oz_dev* dev, int type, const Product& a);
 // Joins the ranges of c in order.
