@@ -392,7 +392,7 @@ Plan plan_of(int cus, const oz_linear_i8_desc* d) {
     p.stream = d->M <= kStreamRows && d->K <= kStreamK;
     if (p.stream || !d->M) return p;
     // one and two rows too long to be streamed are cut into ranges as others are: 1 x 64 x 32768 9.4 us in 16 (19.7 in one), 1 x 1024 x
-    // 28672 13.2 in 4 (17.7)
+    // 28672 13.2 in 2 (17.7)
     p.route = route_of(cus, d->M, d->N, (d->K + 1) / 2, few_rows(d->M, d->N, d->K), true, 0);
     p.width = (d->K + 2 * BC - 1) / (2 * BC) * (2 * BC);
     if (!d->x_int8) p.x = up((size_t)d->M * p.width), p.scale = up(4 * (size_t)d->M);
