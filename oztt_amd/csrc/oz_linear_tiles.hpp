@@ -434,15 +434,19 @@ __global__ void __launch_bounds__(64 * WQ * WP, NSTG * 16 * BC * 2 * (TI * WQ + 
 }
 
 // c += a b with c in accumulation registers. Left to itself the compiler moves sums between the two halves of the
-// register file inside the loop (up to 184 moves for its 128 matrix instructions); written so, c stays. Nothing else
-// touches the registers while the loop runs, the same c comes up every 64 instructions, and settle_sums() stands
-// between the loop and the first use of the sums, so that no result is read early.
+// register file inside the loop (up to 184 moves for its 128 matrix instructions); written so, c stays. The compiler does not see a
+// matrix instruction here and puts no wait states around it, so the code keeps the distance itself. What depends on a result may need
+// 19 wait states (of the longest matrix instructions; these are shorter). A loop takes its sums in turn and has kLeastSums or more
+// (64 of 256 x 256 tiles, 16 of 128 x 128), so that 15 instructions of 4 cycles and more stand between two with the same c; nothing else
+// touches the registers while it runs; settle_sums(), 32 wait states, stands between the loop and the first use of the sums.
+constexpr int kLeastSums = 16;
 template <class M>
 __device__ __forceinline__ void mfma_acc(typename M::sums& c, typename M::x8 a, typename M::x8 b) {
     if constexpr (std::is_same_v<M, Half<OZ_BF16>>) asm("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
     else if constexpr (std::is_same_v<M, Half<OZ_F16>>) asm("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
     else asm("v_mfma_i32_16x16x64_i8 %0, %1, %2, %0" : "+a"(c) : "v"(a), "v"(b));
 }
+// (Not as a statement that the sums pass through: the compiler then copies them in front of it.)
 __device__ __forceinline__ void settle_sums() { asm volatile("s_nop 15\n\ts_nop 15" ::: "memory"); }
 
 // The sums of 256 x 256 outputs by 4 waves of 128 x 128, one a SIMD, each with 256 sums' registers. The fragments of the next
@@ -459,6 +463,7 @@ struct BigLoop {
     typedef Operand<PM, 32 * B, 4> OP;
     static constexpr int UNIT = 2 * BC * 32 * B, RING = 5 * UNIT, LD = OQ::N, LDS = RING, ROOM = RING / 4 / 4;
     static_assert(OQ::N == OP::N, "copies of a unit");
+    static_assert(B * B >= kLeastSums, "distance of a sum's instructions");
 
     template <class TAIL>
     __device__ static __forceinline__ void run(uint8_t* lds, OQ& oq, OP& op, int nst, int tail, int lane, int wave, Sums (&acc)[B][B]) {

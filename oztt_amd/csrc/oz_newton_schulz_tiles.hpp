@@ -391,8 +391,8 @@ struct PairLoop {
             for (int n = 0; n < 3 * B * B; n++) {
                 const int part = n / (B * B), i = n / B % B, j = n % B;
                 const T8 p = part == 1 ? xp.l[j] : xp.h[j], q = part == 2 ? xq.l[i] : xq.h[i];
-                // (written as in the large loop only where a sum comes up again 16 instructions later)
-                if constexpr (B == 4) ozl::mfma_acc<M>(acc[i][j], p, q);
+                // (written as in the large loop only where a sum comes up again late enough)
+                if constexpr (B * B >= ozl::kLeastSums) ozl::mfma_acc<M>(acc[i][j], p, q);
                 else acc[i][j] = M::mfma(p, q, acc[i][j]);
                 if (n % R == 0 && n / R < 4 * B) read(yq, yp, n / R, h, uq, up);
                 if (n % C == C - 1 && n / C < 2 * LD) {
