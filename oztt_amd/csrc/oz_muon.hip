@@ -268,7 +268,7 @@ int oz_orthogonalize(oz_dev* dev, const oz_orthogonalize_desc* d, const void* G,
     e.stride_g = or_else(d->stride_g, d->rows * e.ldg), e.stride_o = or_else(d->stride_o, d->rows * e.ldo);
     if (G == O && (e.ldg != e.ldo || (d->count > 1 && e.stride_g != e.stride_o)))
         return oz::fail(dev, OZ_ERR_ARG, "oz_orthogonalize: O is G with other strides");
-    return orthogonalize(dev, m, e, {(float)d->a, (float)d->b, (float)d->c}, d->eps, d->steps);
+    return orthogonalize(dev, m, e, factors_of(d->a, d->b, d->c, d->steps), d->eps, d->steps);
 }
 
 long long oz_muon_plan_bytes(const oz_muon_tensor* tensors, int count) {
@@ -351,7 +351,7 @@ int oz_muon_step(oz_dev* dev, const oz_muon_plan* plan, const oz_muon_options* o
     e.tensors = static_cast<const oz_muon_tensor*>(plan->memory);
     e.momentum = (float)o->momentum, e.fresh = (float)(1.0 - o->momentum), e.lr = (float)o->lr;
     e.nesterov = o->nesterov, e.grad_scale = o->grad_scale;
-    return orthogonalize(dev, m, e, {(float)o->a, (float)o->b, (float)o->c}, o->eps, o->steps);
+    return orthogonalize(dev, m, e, factors_of(o->a, o->b, o->c, o->steps), o->eps, o->steps);
 }
 
 }  // extern "C"

@@ -3,6 +3,7 @@
 #include "oz_newton_schulz_tiles.hpp"
 
 #include <algorithm>
+#include <cmath>
 
 extern template void ozn::launch_products<true>(hipStream_t, Phase, int, const Shapes&, const Ends&, const Pass&);
 template void ozn::launch_products<false>(hipStream_t, Phase, int, const Shapes&, const Ends&, const Pass&);
@@ -115,6 +116,31 @@ bool places(const Shapes& m, Phase phase, int parent, int tile, const Stretch& t
 }
 
 }  // namespace
+
+// Singular values begin within 0 to 1 and go through s <- s (a + b s^2 + c s^4). A's values are at most their largest square, B's the
+// largest |b q + c q^2| of the squares q.
+ozn::Factors ozn::factors_of(double a, double b, double c, int steps) {
+    double range = 1.0, all = 1.0;
+    for (int k = 1; k < steps && all < kMaxSingular; k++) {
+        double most = 0.0;
+        const auto look = [&](double q) {
+            if (q >= 0.0 && q <= range * range) most = std::max(most, std::sqrt(q) * std::fabs(a + b * q + c * q * q));
+        };
+        look(range * range);
+        const double root = std::sqrt(9.0 * b * b - 20.0 * a * c);  // where a + 3 b q + 5 c q^2 is 0; NaN: nowhere
+        look((-3.0 * b + root) / (10.0 * c));
+        look((-3.0 * b - root) / (10.0 * c));
+        look(-a / (3.0 * b));
+        range = std::min(most, kMaxSingular);
+        all = std::max(all, range);
+    }
+    const double q = all * all, top = -b / (2.0 * c);
+    double most = std::fabs(b * q + c * q * q);
+    if (top > 0.0 && top < q) most = std::max(most, std::fabs(b * top + c * top * top));
+    const auto scale = [](double x) { return std::exp2(std::floor(std::log2(std::min(std::max(kLargest / x, 1.0), 16384.0)))); };
+    const double of_a = scale(q), of_b = scale(most);
+    return {(float)a, (float)(b * of_b / of_a), (float)(c * of_b / (of_a * of_a)), (float)(1.0 / of_b), (float)(of_a / kScale / kScale)};
+}
 
 int ozn::prepare(oz_dev* dev, const Shapes& m, const Factors& f, Iteration* it) {
     Shapes part[2] = {};

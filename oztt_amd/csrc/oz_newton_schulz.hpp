@@ -26,7 +26,12 @@ struct oz_dev;
 
 namespace ozn {
 
-constexpr float kScale = 4096.0f;  // X's values are at most about 1: 16 times as large ones still are FP16 numbers (8 times: B too)
+constexpr float kScale = 4096.0f;  // X's values are at most about 1: 16 times as large ones still are FP16 numbers
+// A and B are kept times powers of two as well (Factors), as large as the singular values' range allows: their values are about the side's
+// reciprocal, and FP16 ends at 2^-24, so that second parts of unscaled ones had lost most of their bits (FP32 matrices of four blocks of one value, 1020 x 672: off
+// by 7.3e-5 of their norm, 5.5e-6 with the scales; with a gradient's spectrum, 4096^2, 3.7e-6 and 1.9e-6, for 3% of the time).
+constexpr double kLargest = 32768.0;  // of them, half of FP16's
+constexpr double kMaxSingular = 8.0;  // what callers promise
 constexpr int kPad = 64;           // sides in the workspace are multiples of it, the rest zeros, which the iteration keeps
 constexpr int kShapes = OZ_MUON_SHAPES;
 // Up to this shorter side the products take both parts of X. There launches and their latency count more than products: 64^2 takes 74 us
@@ -88,8 +93,9 @@ struct Ends {
     int nesterov;
     const float* grad_scale;
 };
+// The iteration's factors with the scales of what they multiply and of what becomes of it: X <- a X + update B X, B = b A + c A^2, A = gram X X^T.
 struct Factors {
-    float a, b, c;
+    float a, b, c, update, gram;
 };
 
 // The products of a step. X' goes to the ends in the last one.
@@ -105,6 +111,8 @@ struct Pass {
 // Tiles of `tile` x `tile` outputs of a phase's products, 64, 128 or (of the first parts) 256, for shapes that are alike in `three`.
 template <bool THREE>
 void launch_products(hipStream_t stream, Phase phase, int tile, const Shapes& m, const Ends& ends, const Pass& pass);
+
+Factors factors_of(double a, double b, double c, int steps);
 
 // The launches of a step, of the shapes whose products take one part of their operands and of those that take both: prepared, and
 // refused where they are too many, before anything runs.

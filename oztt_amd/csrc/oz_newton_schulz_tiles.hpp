@@ -248,14 +248,14 @@ struct Finish {
                 [&](auto P, auto T, int row, float* v) {
                     if constexpr (PHASE == GRAM) {
 #pragma unroll
-                        for (int k = 0; k < 8; k++) v[k] *= 1.0f / kScale / kScale;
+                        for (int k = 0; k < 8; k++) v[k] *= f.gram;
                     } else {
                         add(P, T, row, f.b, f.c, v);
                         if (!THREE && !mirror) {  // a tile on the diagonal
                             float* d = diagonal_of(s, i);
 #pragma unroll
                             for (int k = 0; k < 8; k++)
-                                if (q0 + row == col + k && col < side) d[col + k] = v[k], v[k] = 0.0f;
+                                if (q0 + row == col + k && col < side) d[col + k] = v[k] * f.update, v[k] = 0.0f;
                         }
                     }
                     if (q0 + row < side && col < side) put8<false>(to, rest, (long long)(q0 + row) * side + col, v);
@@ -282,7 +282,7 @@ struct Finish {
                 put_rows<THREE, TI, TJ, ROOM, false>(
                     acc, tile, lane, false, get,
                     [&](auto P, auto T, int row, float* v) {
-                        add(P, T, row, f.a, 1.0f, v);
+                        add(P, T, row, f.a, f.update, v);
                         if (q0 + row < s.R && col < s.C) put8<!THREE>(to, rest, (long long)(q0 + row) * s.C + col, v);
                     },
                     none);
@@ -292,7 +292,7 @@ struct Finish {
                 put_rows<THREE, TI, TJ, ROOM, false>(
                     acc, tile, lane, false, get,
                     [&](auto P, auto T, int row, float* v) {
-                        add(P, T, row, f.a, 1.0f, v);
+                        add(P, T, row, f.a, f.update, v);
                         const int q = q0 + row, count = q < s.rows ? min(s.cols - col, 8) : 0;
                         if (count <= 0) return;
                         const long long at = (long long)q * s.cols + col;
@@ -316,7 +316,7 @@ struct Finish {
                 put_rows<THREE, TI, TJ, ROOM, false>(
                     acc, tile, lane, false, get,
                     [&](auto P, auto T, int row, float* v) {
-                        add(P, T, row, f.a, 1.0f, v);
+                        add(P, T, row, f.a, f.update, v);
                         const int q = q0 + row, count = q < s.rows ? min(s.cols - col, 8) : 0;
                         if (count <= 0) return;
                         const long long at = (s.first + i) * ends.stride_o + q * ends.ldo + col;
