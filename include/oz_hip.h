@@ -526,6 +526,7 @@ typedef struct oz_orthogonalize_desc {
     int rows, cols, count; /* rows and cols from 1 to 2^20 */
     int type;              /* oz_type of G and O: any */
     int steps;             /* 1 to 100 */
+    int exact;             /* not 0: products of 22 bits whatever the type and size */
     double a, b, c, eps;
     long long ldg, ldo, stride_g, stride_o; /* rows and matrices apart (0: one behind the other) */
 } oz_orthogonalize_desc;
@@ -535,7 +536,7 @@ int oz_orthogonalize(oz_dev* dev, const oz_orthogonalize_desc* d, const void* G,
 
 /* ---- Muon over many matrices ------------------------------------------------------------------------
  * One step of every matrix p with gradient g, in FP32 but for the iteration's products (as above: those of 11 bits are taken where
- * both sides are over 512):
+ * both sides are over 512 and the plan does not ask for 22):
  *   m' = momentum m + (1 - momentum) g grad_scale
  *   u  = momentum m' + (1 - momentum) g grad_scale (nesterov), or m'
  *   p' = p (1 - lr weight_decay) - lr lr_scale orthogonalized(u)
@@ -553,6 +554,8 @@ typedef struct oz_muon_tensor {
 } oz_muon_tensor;
 /* The plan of a list of matrices (host array) of at most OZ_MUON_SHAPES different sizes: the list by size, copied into device
  * memory of oz_muon_plan_bytes bytes (16-byte aligned), which the caller keeps unchanged as long as it steps with the plan.
+ * Sizes with a param in FP32 have `exact` set, as a matrix in FP32 has products of 22 bits above; the caller may change it before it asks
+ * for the workspace (16-bit weights with a master are updated from products of 11 bits otherwise).
  * Waits for all work of the device (the memory may have been another stream's) and returns when the copy is done. */
 typedef struct oz_muon_shape {
     int rows, cols, count, first;
@@ -561,6 +564,7 @@ typedef struct oz_muon_plan {
     const void* memory;
     int count, shapes;
     oz_muon_shape shape[OZ_MUON_SHAPES];
+    unsigned exact; /* bit k: products of 22 bits for shape[k] */
 } oz_muon_plan;
 long long oz_muon_plan_bytes(const oz_muon_tensor* tensors, int count);
 int oz_muon_make_plan(oz_dev* dev, const oz_muon_tensor* tensors, int count, void* memory, size_t bytes, oz_muon_plan* plan);

@@ -220,17 +220,19 @@ const char* refuse(const oz_orthogonalize_desc* d) {
 }
 
 size_t shape_of(const oz_orthogonalize_desc* d, Shape* s, char* base) {
-    return lay_out(s, d->rows, d->cols, d->count, 0, d->type != OZ_BF16, base, 0);
+    return lay_out(s, d->rows, d->cols, d->count, 0, d->exact || d->type != OZ_BF16, base, 0);
 }
 
 // The plan's shapes in `base`, and the workspace's size.
 size_t shapes_of(const oz_muon_plan* p, Shapes* m, char* base) {
     size_t at = 0;
     m->n = p->shapes;
-    for (int k = 0; k < p->shapes; k++) at = lay_out(&m->s[k], p->shape[k].rows, p->shape[k].cols, p->shape[k].count, p->shape[k].first, false, base, at);
+    for (int k = 0; k < p->shapes; k++)
+        at = lay_out(&m->s[k], p->shape[k].rows, p->shape[k].cols, p->shape[k].count, p->shape[k].first, p->exact >> k & 1, base, at);
     return at;
 }
 
+static_assert(kShapes <= 32, "bits of a plan's exact");
 bool bad_plan(const oz_muon_plan* p) {
     if (!p || !p->memory || p->count < 0 || p->shapes < 0 || p->shapes > kShapes) return true;
     for (int k = 0; k < p->shapes; k++) {
@@ -312,6 +314,7 @@ int oz_muon_make_plan(oz_dev* dev, const oz_muon_tensor* tensors, int count, voi
                 if (tensors[j].rows == t.rows && tensors[j].cols == t.cols) {
                     list.push_back(tensors[j]);
                     done[j] = 1;
+                    if (tensors[j].param_type == OZ_F32) p.exact |= 1u << (p.shapes - 1);
                     s.count++;
                 }
         }

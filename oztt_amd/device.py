@@ -147,7 +147,7 @@ class LinearI8Desc(ctypes.Structure):
 
 
 class OrthogonalizeDesc(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_int) for n in ("rows", "cols", "count", "type", "steps")] + [(n, ctypes.c_double) for n in ("a", "b", "c", "eps")] + \
+    _fields_ = [(n, ctypes.c_int) for n in ("rows", "cols", "count", "type", "steps", "exact")] + [(n, ctypes.c_double) for n in ("a", "b", "c", "eps")] + \
                [(n, ctypes.c_longlong) for n in ("ldg", "ldo", "stride_g", "stride_o")]
 
 
@@ -165,7 +165,8 @@ class MuonShape(ctypes.Structure):
 
 
 class MuonPlan(ctypes.Structure):
-    _fields_ = [("memory", ctypes.c_void_p), ("count", ctypes.c_int), ("shapes", ctypes.c_int), ("shape", MuonShape * MUON_SHAPES)]
+    _fields_ = [("memory", ctypes.c_void_p), ("count", ctypes.c_int), ("shapes", ctypes.c_int), ("shape", MuonShape * MUON_SHAPES),
+                ("exact", ctypes.c_uint)]
 
 
 class MuonOptions(ctypes.Structure):
@@ -204,8 +205,10 @@ def linear_i8_desc(M, N, K, type="bf16", act="none", y_type=None, x_int8=False, 
     return LinearI8Desc(M, N, K, _number(TYPES, type), _number(TYPES, y_type or type), _number(ACTS, act), int(x_int8), ldx, ldw, ldy, ldr)
 
 
-def orthogonalize_desc(rows, cols, count=1, type="bf16", steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, ldg=0, ldo=0, stride_g=0, stride_o=0) -> OrthogonalizeDesc:
-    return OrthogonalizeDesc(rows, cols, count, _number(TYPES, type), steps, *coefficients, eps, ldg, ldo, stride_g, stride_o)
+def orthogonalize_desc(rows, cols, count=1, type="bf16", steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, ldg=0, ldo=0, stride_g=0, stride_o=0,
+                       exact=False) -> OrthogonalizeDesc:
+    """exact: products of 22 bits for large BF16 matrices too."""
+    return OrthogonalizeDesc(rows, cols, count, _number(TYPES, type), steps, int(exact), *coefficients, eps, ldg, ldo, stride_g, stride_o)
 
 
 def muon_tensor(rows, cols, param, grad, m, master=0, param_type="f32", grad_type="f32", weight_decay=0.0, lr_scale=None) -> MuonTensor:
@@ -500,9 +503,10 @@ class Device:
         arr = (MuonTensor * max(len(tensors), 1))(*tensors)
         return self._bytes(hip().oz_muon_plan_bytes(arr, len(tensors)), "oz_muon_plan_bytes")
 
-    def muon_plan(self, tensors, memory: Buffer = None, memory_bytes: int = None) -> MuonPlan:
+    def muon_plan(self, tensors, memory: Buffer = None, memory_bytes: int = None, exact: bool = None) -> MuonPlan:
         """The plan of a list of muon_tensor()s, in `memory` (muon_plan_bytes; allocated here if none is given), which lives as long as
-        the plan; memory_bytes as in adamw_plan."""
+        the plan; memory_bytes as in adamw_plan. exact: products of 22 bits for all sizes or for none of more than 512 rows and
+        columns; None: for those of FP32 weights."""
         arr = (MuonTensor * max(len(tensors), 1))(*tensors)
         need = self.muon_plan_bytes(tensors)
         memory = memory if memory is not None else self.alloc(need)
@@ -510,6 +514,8 @@ class Device:
             memory_bytes = getattr(memory, "nbytes", need)
         plan = MuonPlan()
         self._check(hip().oz_muon_make_plan(self.h, arr, len(tensors), memory.ptr, ctypes.c_size_t(memory_bytes), ctypes.byref(plan)), "oz_muon_make_plan")
+        if exact is not None:
+            plan.exact = (1 << plan.shapes) - 1 if exact else 0
         plan.buffer = memory
         return plan
 
