@@ -516,12 +516,16 @@ int oz_linear_i8(oz_dev* dev, const oz_linear_i8_desc* d, const void* X, const f
  * O = the Newton-Schulz iteration's result on each of `count` matrices G (rows x cols, row-major): with X = G / (|G|_F + eps),
  * steps times X <- a X + (b A + c A^2) X, A = X X^T (from the right, with A = X^T X, where rows > cols), which moves
  * singular values s by a s + b s^3 + c s^5: with a, b, c = 3.4445, -4.7750, 2.0315 and 5 steps near 1, but for those that are
- * zero or nearly so. The norm is summed in FP64, the iteration's products in FP32; X is kept in 22 bits. A BF16
- * result of more than 512 rows and columns takes products of 11 bits and is off by up to 2e-3 of its norm before it is rounded (by up to
- * 1.1e-2 where values are alike and so are their roundings, as of an identity), all others products of 22 bits: 1e-5 of its norm. (To both comes what rounding X leaves in directions of singular values near zero, which
- * a step makes a times larger: a^steps 2^-22 sqrt(steps) of the sum of squares' root, 1.3e-4.) Singular values must stay below 8 (with the factors above they
- * stay below 1.3). A matrix of zeros gives zeros, one with a value that is not finite NaN. O may be G itself (the same type
- * and strides); matrices do not overlap each other. count may be 0. */
+ * zero or nearly so. The norm is summed in FP64, the iteration's products in FP32; X is kept in 22 bits. A matrix of zeros gives zeros, one
+ * with a value that is not finite NaN. Singular values must stay below 8 (with the factors above they stay below 1.3). O may be G itself
+ * (the same type and strides); matrices do not overlap each other. count may be 0.
+ * How far a result may be off, of its norm, before it is rounded, with the factors above and 5 steps:
+ *   products of 22 bits: 1e-5; where values are alike, as in a block of one value, and so are the roundings of their sums, 2^-23 more
+ *     for each row and column that are alike;
+ *   products of 11 bits, which BF16 results of more than 512 rows and columns take unless `exact`, in half of the time: 2e-3; where
+ *     rows or values are alike (blocks of one value, equal rows, an identity) up to 6.2e-2, of which 1.8e-2 has been seen;
+ *   both: what rounding X leaves in directions of singular values near zero, which a step makes a times larger, a^steps 2^-22 sqrt(steps) in the
+ *     norm, 1.3e-4 (a result of n rows with singular values near 1 has a norm of sqrt(n)). */
 typedef struct oz_orthogonalize_desc {
     int rows, cols, count; /* rows and cols from 1 to 2^20 */
     int type;              /* oz_type of G and O: any */

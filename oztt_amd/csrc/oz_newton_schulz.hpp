@@ -13,10 +13,11 @@
 // singular values. Once most of them are near 1, B is near -2.7 times the identity, and rounding h and B to 11 bits is what shows:
 // B's diagonal is therefore kept in FP32 and multiplies both parts of X in the product's epilogue, X <- (a + diag B) X + (B - diag B) h,
 // which costs 1% (for Gaussian matrices of 513 to 1500 rows off by 1.3e-3 to 1.8e-3 without it, 4e-4 to 8.5e-4 with it). The
-// result is off by 2e-4 to 1.5e-3 whatever the spectrum (against 64 bits), by more only where values do not differ and their roundings
-// cannot average: an identity of 513 rows by up to 1.1e-2.
+// result is off by 2e-4 to 1.5e-3 where values differ (against 64 bits). Where rows or values do not, their roundings do not average: an identity of
+// 513 rows by up to 5e-3, equal rows and matrices of one value by 3e-3 to 8e-3, some blocks of one value by 1.8e-2; to first order by up to 6.2e-2.
 // Where a side is short (the rounding errors of A and B then average over few values: up to 1e-2 at one to four rows) or the result
-// is kept in more than BF16's 8 bits, the products take both parts of both operands, h h + h l + l h: off by 1e-6.
+// is kept in more than BF16's 8 bits, or the caller asks for it, the products take both parts of both operands, h h + h l + l h: off by 1e-6 to 4e-6,
+// and by up to 3e-4 where thousands of values are alike and so are the roundings of their FP32 sums.
 #pragma once
 #include <hip/hip_runtime.h>
 
