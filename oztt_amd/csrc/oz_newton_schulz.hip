@@ -62,7 +62,7 @@ float estimate(const Shapes& m, Phase phase, const Cost& c, int cus, const Stret
 
 // A phase in tiles of one size, and what a last, partly filled round of them would have in smaller ones by a launch of its own: 8192^2's A in
 // 512 tiles of 256 x 256 and the other 16 of 528 as 256 of 64 x 64 takes 434 us for 563. The launch costs 3 us.
-// Against every tile alone at 72 other sizes the choice is the fastest or within 2% of the whole call at 210 of 216 phases; of X in 128 x 128 tiles it cuts a last
+// Against every tile alone at 42 other sizes the choice is the fastest or within 2% of the whole call at 210 of 216 phases; of X in 128 x 128 tiles it cuts a last
 // round off that had better stayed (6000 x 2000 9%, 1700 x 6800 8%, 3300^2 7%). There are no ranges of c: a side of 64 or less has one workgroup a matrix for A, however
 // long the other one is (64 x 8192 280 us in all, 64 x 65536 1800).
 struct Choice {
