@@ -559,7 +559,7 @@ typedef struct oz_muon_tensor {
 /* The plan of a list of matrices (host array) of at most OZ_MUON_SHAPES different sizes: the list by size, copied into device
  * memory of oz_muon_plan_bytes bytes (16-byte aligned), which the caller keeps unchanged as long as it steps with the plan.
  * Sizes with a param in FP32 have `exact` set, as a matrix in FP32 has products of 22 bits above; the caller may change it before it asks
- * for the workspace (16-bit weights with a master are updated from products of 11 bits otherwise).
+ * for the workspace (16-bit weights, with a master or without, are updated from products of 11 bits otherwise).
  * Waits for all work of the device (the memory may have been another stream's) and returns when the copy is done. */
 typedef struct oz_muon_shape {
     int rows, cols, count, first;

@@ -8,8 +8,8 @@ Every HIP source is compiled with -ffp-contract=off (the splitting stages reprod
 sequence of binary32 operations) and with packed FP32 instructions disabled. The Scheme II split
 source additionally runs with FP32 denormals flushed (-fgpu-flush-denormals-to-zero), which is the
 rule of the reference's operation model. The linear layers' tiles have their loops begin at multiples of 64 bytes, whole lines
-of the instruction cache: where one began was left to chance, and the 32 x 32 tile's, of 20 instructions of each 16-cycle matrix
-instruction, was 2 to 6% slower at some places (1 x 8192 x 8192's dX 25.4 us, 27.2 and, aligned, 25.8).
+of the instruction cache: where one began was left to chance, and the 32 x 32 tile's, with some 30 other instructions to
+each matrix instruction, was 2 to 6% slower at some places (1 x 8192 x 8192's dX 25.4 us, 27.2 and, aligned, 25.8).
 """
 from __future__ import annotations
 

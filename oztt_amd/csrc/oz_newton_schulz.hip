@@ -199,3 +199,10 @@ extern "C" int oz_rule_newton_schulz(int cus, int phase, int rows, int cols, int
     if (rest) *rest = c.rest.n[0] ? c.rest_tile : 0;
     return c.tile;
 }
+
+// The scales of A and B for the iteration's factors, for tests.
+extern "C" void oz_rule_newton_schulz_scales(double a, double b, double c, int steps, double* of_a, double* of_b) {
+    const Factors f = factors_of(a, b, c, steps);
+    *of_a = (double)f.gram * kScale * kScale;
+    *of_b = 1.0 / f.update;
+}
